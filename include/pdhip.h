@@ -115,6 +115,45 @@ int pdh_row_softmax_dt(const void* x, void* y, int64_t rows, int64_t cols, int64
 int pdh_layernorm_dt(const void* x, const void* gamma, const void* beta, void* y, int64_t rows, int64_t cols,
                      int64_t ldx, int64_t ldy, float eps, int dtype, void* stream);
 
+/* Layer norm in a training step, over PDH_F32 / PDH_BF16 / PDH_F16 storage (x,
+ * gamma, beta, y and every gradient of `dtype`), computing in fp32. The
+ * forward is pdh_layernorm_dt's and also stores each row's statistics, dense
+ * fp32 [rows]:
+ *   mean = sum x / cols, rstd = 1 / sqrt(sum (x - mean)^2 / cols + eps)
+ * The backward takes them: with xh = (x - mean) rstd and u = dy gamma,
+ *   dx = rstd (u - mean(u) - xh mean(u xh)) [+ dres]
+ *   dgamma = sum over rows of dy xh, dbeta = sum over rows of dy
+ * dres (may be NULL) is the gradient that reaches x past the norm, a residual
+ * branch's. gamma, dgamma and dbeta are given together or all NULL. ws holds
+ * pdh_layernorm_bwd_workspace(rows, cols, dtype) bytes (unused without gamma): fp32
+ * partial sums, added in a fixed order, so results repeat bit for bit. Rows
+ * are strided by ld* elements (0 for an input: one row for all), columns are
+ * contiguous, at any alignment of the element type; y / dx may be x, dy or
+ * dres themselves. No rows: dgamma and
+ * dbeta are zero. The reference's gradient of this template is the carves that
+ * autodiff regenerates (autodiff.py:102-122 over zoo/zoo_common.py:56-60). */
+int pdh_layernorm_fwd(const void* x, const void* gamma, const void* beta, void* y, float* mean, float* rstd,
+                      int64_t rows, int64_t cols, int64_t ldx, int64_t ldy, float eps, int dtype, void* stream);
+size_t pdh_layernorm_bwd_workspace(int64_t rows, int64_t cols, int dtype);
+int pdh_layernorm_bwd(const void* x, const void* dy, const void* dres, const void* gamma, const float* mean,
+                      const float* rstd, void* dx, void* dgamma, void* dbeta, int64_t rows, int64_t cols, int64_t ldx,
+                      int64_t lddy, int64_t lddres, int64_t lddx, int dtype, void* ws, size_t ws_bytes, void* stream);
+
+/* Dropout whose mask is recomputed, never stored:
+ *   y = [residual +] keep ? x * 65536 / (65536 - t) : 0, t = floor(65536 p + 1/2)
+ *   keep = bits >= t, bits the 16 random bits of the element
+ * (p in [0, 1]; t = 65536 drops everything). The bits are Philox4x32-10
+ * (Salmon et al., SC 2011) at key = seed and counter = (g low, g high, step
+ * low, site), g = row * ceil(cols / 8) + col / 8: the 128 bits serve 8
+ * consecutive columns, 16 each, low halves first. rng points to {seed, step}
+ * on the device (read when the kernel runs, so a captured graph draws a new
+ * mask once the caller has moved the step on); site tells the calls of one
+ * step apart. The backward is the same call on dy without a residual. Dropped
+ * elements count for nothing whatever x holds there. y may be x or residual.
+ * No counterpart in the reference. */
+int pdh_dropout(const void* x, const void* residual, void* y, int64_t rows, int64_t cols, int64_t ldx, int64_t ldr,
+                int64_t ldy, double p, const int64_t* rng, int64_t site, int dtype, void* stream);
+
 /* Row gather: out[i, :] = table[idx[i], :] for i < n_idx, rows of row_elems
  * elements (strides ld_table / ld_out), the device form of tl.take along the
  * table's leading dim (indexing.py:192-230). The reference plans a take as a

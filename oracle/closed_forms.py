@@ -17,6 +17,11 @@ follows (paths relative to the reference repository root):
                      (autodiff.py:102-122; tiles.py:238-252): dV = P^T dO,
                      dP = dO V^T, D = rowsum(dO * O), dS = P (dP - D),
                      dQ = scale dS K, dK = scale dS^T Q
+  layernorm_bwd      the closed form of the same gradient over np_layernorm
+  philox_bits,       the published generator (Salmon et al., SC 2011) and dropout
+  dropout            under its bits; no counterpart in the reference
+  linear_xent,       the cross entropy of a linear head, lse - z[target], and its
+  linear_xent_bwd    closed-form gradient; no counterpart in the reference
   combine_partials   the flashsm combine, zoo/attention.py:40-46
 
 Inputs are upcast to float64 before any arithmetic, so a bf16 input is
@@ -142,3 +147,76 @@ def combine_partials(parts):
         sl, sr = np.exp(m - mm), np.exp(mr - mm)
         m, den, o = mm, den * sl + denr * sr, o * sl[..., None] + orr * sr[..., None]
     return m, den, o
+
+
+def layernorm_bwd(x, dy, g=None, eps=1e-5, dres=None):
+    """(dx, dgamma, dbeta) of np_layernorm over the last axis."""
+    x, dy = np.asarray(x, dtype=np.float64), np.asarray(dy, dtype=np.float64)
+    n = x.shape[-1]
+    xc = x - x.mean(-1, keepdims=True)
+    rstd = 1.0 / np.sqrt((xc * xc).mean(-1, keepdims=True) + eps)
+    xh = xc * rstd
+    u = dy if g is None else dy * np.asarray(g, dtype=np.float64)
+    dx = rstd * (u - u.mean(-1, keepdims=True) - xh * (u * xh).mean(-1, keepdims=True))
+    if dres is not None:
+        dx = dx + np.asarray(dres, dtype=np.float64)
+    flat = (dy * xh).reshape(-1, n), dy.reshape(-1, n)
+    return dx, flat[0].sum(0), flat[1].sum(0)
+
+
+def philox4x32(counter, key):
+    """Ten rounds on [n, 4] counters under a two-word key, as Python integers' words in uint64."""
+    c = [np.asarray(counter, dtype=np.uint64)[:, i].copy() for i in range(4)]
+    k0, k1 = int(key[0]), int(key[1])
+    m32, s32 = np.uint64(0xFFFFFFFF), np.uint64(32)
+    for _ in range(10):
+        p0, p1 = c[0] * np.uint64(0xD2511F53), c[2] * np.uint64(0xCD9E8D57)
+        c = [(p1 >> s32) ^ c[1] ^ np.uint64(k0), p1 & m32, (p0 >> s32) ^ c[3] ^ np.uint64(k1), p0 & m32]
+        k0, k1 = (k0 + 0x9E3779B9) & 0xFFFFFFFF, (k1 + 0xBB67AE85) & 0xFFFFFFFF
+    return np.stack(c, axis=1)
+
+
+def philox_bits(seed, step, site, rows, cols, row0=0):
+    """The 16 bits of each element of rows row0 .. row0 + rows - 1."""
+    per = -(-cols // 8)
+    g = np.uint64(row0 * per) + np.arange(rows * per, dtype=np.uint64)
+    ctr = np.stack([g & np.uint64(0xFFFFFFFF), g >> np.uint64(32), np.full_like(g, step & 0xFFFFFFFF),
+                    np.full_like(g, site)], axis=1)
+    w = philox4x32(ctr, (seed & 0xFFFFFFFF, (seed >> 32) & 0xFFFFFFFF))
+    bits = np.stack([w & np.uint64(0xFFFF), w >> np.uint64(16)], axis=2).reshape(rows, per * 8)
+    return bits[:, :cols]
+
+
+def dropout(x, p, seed, step, site=0, residual=None):
+    x = np.asarray(x, dtype=np.float64)
+    x2 = x.reshape(-1, x.shape[-1])
+    t = int(np.floor(p * 65536 + 0.5))
+    keep = philox_bits(seed, step, site, *x2.shape) >= t
+    y = np.zeros_like(x2)
+    y[keep] = x2[keep] * (65536.0 / (65536 - t) if t < 65536 else 0.0)
+    y = y.reshape(x.shape)
+    return y if residual is None else y + np.asarray(residual, dtype=np.float64)
+
+
+def linear_xent(x, w, targets):
+    """(loss, lse) of the rows; targets outside [0, vocab) have no loss."""
+    z = np.asarray(x, dtype=np.float64) @ np.asarray(w, dtype=np.float64).T
+    m = z.max(1, keepdims=True)
+    lse = np.log(np.exp(z - m).sum(1)) + m[:, 0]
+    t = np.asarray(targets)
+    live = (t >= 0) & (t < z.shape[1])
+    loss = np.where(live, lse - z[np.arange(len(t)), np.where(live, t, 0)], 0.0)
+    return loss, lse
+
+
+def linear_xent_bwd(x, w, targets, dloss):
+    """(dx, dw) of sum(dloss * loss)."""
+    x, w = np.asarray(x, dtype=np.float64), np.asarray(w, dtype=np.float64)
+    z = x @ w.T
+    p = np_softmax(z, 1)
+    t = np.asarray(targets)
+    live = (t >= 0) & (t < z.shape[1])
+    rows = np.nonzero(live)[0]
+    p[rows, t[rows]] -= 1.0
+    p *= np.where(live, np.asarray(dloss, dtype=np.float64), 0.0)[:, None]
+    return p @ w, p.T @ x

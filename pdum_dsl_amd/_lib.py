@@ -29,6 +29,10 @@ EXPORTS = (
     "pdh_layernorm",
     "pdh_row_softmax_dt",
     "pdh_layernorm_dt",
+    "pdh_layernorm_fwd",
+    "pdh_layernorm_bwd_workspace",
+    "pdh_layernorm_bwd",
+    "pdh_dropout",
     "pdh_take_rows",
     "pdh_scatter_add_rows",
     "pdh_flash_fwd",
@@ -120,6 +124,11 @@ def _declare(lib) -> None:
         "pdh_layernorm": (i32, [vp, vp, vp, vp, i64, i64, i64, i64, f32, vp]),
         "pdh_row_softmax_dt": (i32, [vp, vp, i64, i64, i64, i64, i32, vp]),
         "pdh_layernorm_dt": (i32, [vp, vp, vp, vp, i64, i64, i64, i64, f32, i32, vp]),
+        "pdh_layernorm_fwd": (i32, [vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, f32, i32, vp]),
+        "pdh_layernorm_bwd_workspace": (C.c_size_t, [i64, i64, i32]),
+        "pdh_layernorm_bwd": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, i64, i32, vp,
+                                    C.c_size_t, vp]),
+        "pdh_dropout": (i32, [vp, vp, vp, i64, i64, i64, i64, i64, C.c_double, vp, i64, i32, vp]),
         "pdh_take_rows": (i32, [vp, vp, vp, i64, i64, i64, i64, i64, i32, vp, vp]),
         "pdh_scatter_add_rows": (i32, [vp, vp, vp, i64, i64, i64, i64, i64, i32, vp, vp]),
         "pdh_flash_fwd": (i32, [vp, vp, vp, vp, vp, vp, vp, gp, i32, f32, f32, i32, i64, i64, i32, vp]),

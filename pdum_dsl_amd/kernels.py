@@ -151,6 +151,187 @@ def layernorm(
     return y if y.shape == x.shape else y.reshape(x.shape)
 
 
+def _one_device(first: torch.Tensor, *rest) -> None:
+    """Device tensors of the current device alone: a launch goes to its
+    stream, which orders nothing on another."""
+    _require_cuda(first, *rest)
+    dev = torch._C._cuda_getDevice()
+    for t in (first, *rest):
+        if t is not None and t.device.index != dev:
+            raise ValueError(f"the tensors must be on the current device cuda:{dev} (got {t.device})")
+
+
+@dataclass
+class LayernormOut:
+    y: torch.Tensor
+    mean: torch.Tensor
+    rstd: torch.Tensor
+
+
+def _norm_weights(x, **ws) -> None:
+    n = x.shape[-1]
+    for nm, t in ws.items():
+        if t is None:
+            continue
+        if t.dtype != x.dtype:
+            raise ValueError(f"{nm} must share x's element type")
+        if t.numel() != n or not t.is_contiguous():
+            raise ValueError(f"{nm} must be a contiguous vector of {n} elements")
+
+
+def layernorm_fwd(
+    x: torch.Tensor,
+    gamma: torch.Tensor | None = None,
+    beta: torch.Tensor | None = None,
+    eps: float = 1e-5,
+    out: torch.Tensor | None = None,
+) -> LayernormOut:
+    """:func:`layernorm` for a training step: the output and each row's mean
+    and rstd = 1 / sqrt(variance + eps) (fp32, x's leading shape), which
+    :func:`layernorm_bwd` takes. ``out`` (x's shape, rows of contiguous
+    columns) may be x itself."""
+    _one_device(x, gamma, beta, out)
+    if x.dtype not in _DT:
+        raise ValueError(f"layernorm_fwd stores f32, bf16 or f16 (got {x.dtype})")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("layernorm_fwd needs rows of at least one column")
+    _norm_weights(x, gamma=gamma, beta=beta)
+    if eps < 0:
+        raise ValueError("layernorm_fwd: eps must be >= 0")
+    n = x.shape[-1]
+    x2 = _rows(x)
+    y = torch.empty(x2.shape, dtype=x.dtype, device=x.device) if out is None else _out_rows(out, x)
+    stats = torch.empty((2,) + tuple(x.shape[:-1]), dtype=torch.float32, device=x.device)
+    mean, rstd = stats.unbind(0)
+    _lib.call(
+        "pdh_layernorm_fwd",
+        x2.data_ptr(), _ptr(gamma), _ptr(beta), y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), x2.shape[0], n,
+        _ld(x2), _ld(y), float(eps), _DT[x.dtype], _stream(),
+    )
+    return LayernormOut(out if out is not None else y.view(x.shape), mean, rstd)
+
+
+def _ld(x2: torch.Tensor) -> int:
+    """A 2-D tensor's row stride (a single row's is its length)."""
+    return x2.stride(0) if x2.shape[0] > 1 else x2.shape[1]
+
+
+def _out_rows(out: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
+    """A caller's output as [rows, cols], a view of it."""
+    if out.shape != x.shape or out.dtype != x.dtype or (out.shape[-1] > 1 and out.stride(-1) != 1):
+        raise ValueError("out must have x's shape and element type, and contiguous columns")
+    try:
+        o2 = out.view(-1, out.shape[-1])
+    except RuntimeError:
+        raise ValueError("out's leading dims must compose into one row stride") from None
+    if o2.shape[0] > 1 and o2.stride(0) < o2.shape[1]:
+        raise ValueError("out's rows overlap")
+    return o2
+
+
+def layernorm_bwd(
+    x: torch.Tensor,
+    dy: torch.Tensor,
+    mean: torch.Tensor,
+    rstd: torch.Tensor,
+    gamma: torch.Tensor | None = None,
+    *,
+    dres: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor | None, torch.Tensor | None]:
+    """Gradients (dx, dgamma, dbeta) of :func:`layernorm_fwd` given its mean
+    and rstd; the last two are None without ``gamma``. ``dres`` (x's shape) is
+    added to dx: the gradient that reaches x along a residual branch past the
+    norm. Element types alike, fp32 arithmetic, one rounding; deterministic."""
+    _one_device(x, dy, mean, rstd, gamma, dres)
+    if x.dtype not in _DT:
+        raise ValueError(f"layernorm_bwd stores f32, bf16 or f16 (got {x.dtype})")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("layernorm_bwd needs rows of at least one column")
+    for nm, t in (("dy", dy), ("dres", dres)):
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
+            raise ValueError(f"{nm} must have x's shape and element type")
+    for nm, t in (("mean", mean), ("rstd", rstd)):
+        if t.dtype != torch.float32 or t.shape != x.shape[:-1] or not t.is_contiguous():
+            raise ValueError(f"{nm} must be contiguous fp32 of x's leading shape")
+    _norm_weights(x, gamma=gamma)
+    n = x.shape[-1]
+    x2, dy2 = _rows(x), _rows(dy)
+    r2 = None if dres is None else _rows(dres)
+    dx = torch.empty(x2.shape, dtype=x.dtype, device=x.device)
+    ws, dgamma, dbeta, need = None, None, None, 0
+    if gamma is not None:
+        dgamma, dbeta = torch.empty_like(gamma), torch.empty_like(gamma)
+        need = _lib.lib().pdh_layernorm_bwd_workspace(x2.shape[0], n, _DT[x.dtype])
+        ws = torch.empty(need // 4, dtype=torch.float32, device=x.device)
+    _lib.call(
+        "pdh_layernorm_bwd",
+        x2.data_ptr(), dy2.data_ptr(), _ptr(r2), _ptr(gamma), mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(),
+        _ptr(dgamma), _ptr(dbeta), x2.shape[0], n, _ld(x2), _ld(dy2), 0 if r2 is None else _ld(r2), n, _DT[x.dtype],
+        _ptr(ws), need, _stream(),
+    )
+    return dx.view(x.shape), dgamma, dbeta
+
+
+def _dropout(name, x, p, rng, site, residual, out):
+    _one_device(x, rng, residual, out)
+    if x.dtype not in _DT:
+        raise ValueError(f"{name} stores f32, bf16 or f16 (got {x.dtype})")
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"{name}: the rate p = {p} must lie in [0, 1]")
+    if not 0 <= site < 1 << 32:
+        raise ValueError(f"{name}: site {site} must fit 32 bits unsigned")
+    if rng.dtype != torch.int64 or tuple(rng.shape) != (2,) or not rng.is_contiguous():
+        raise ValueError(f"{name}: rng is an int64 device tensor of two elements, the seed and the step")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"{name} needs rows of at least one column")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise ValueError("residual must have x's shape and element type")
+    n = x.shape[-1]
+    x2 = _rows(x)
+    r2 = None if residual is None else _rows(residual)
+    y = torch.empty(x2.shape, dtype=x.dtype, device=x.device) if out is None else _out_rows(out, x)
+    _lib.call(
+        "pdh_dropout",
+        x2.data_ptr(), _ptr(r2), y.data_ptr(), x2.shape[0], n, _ld(x2), 0 if r2 is None else _ld(r2), _ld(y), float(p),
+        rng.data_ptr(), site, _DT[x.dtype], _stream(),
+    )
+    return out if out is not None else y.view(x.shape)
+
+
+def dropout_fwd(
+    x: torch.Tensor,
+    p: float,
+    rng: torch.Tensor,
+    *,
+    site: int = 0,
+    residual: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """[residual +] x with each element dropped at rate ``p``, the survivors
+    scaled by 1 / (1 - p), p held to 2^-16. The mask is a function of ``rng``
+    (int64 on the device: seed and step), ``site`` (one number for each
+    dropout of a step) and the element's place in x as rows of its last axis;
+    it does not depend on the element type or the strides and is never
+    stored. ``rng`` is read when the kernel runs: move its step on between
+    training steps (``rng[1] += 1``), captured ones too, and keep it until the
+    backward has run. ``out`` may be x or residual itself."""
+    return _dropout("dropout_fwd", x, p, rng, site, residual, out)
+
+
+def dropout_bwd(
+    dy: torch.Tensor,
+    p: float,
+    rng: torch.Tensor,
+    *,
+    site: int = 0,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """The gradient of :func:`dropout_fwd` with respect to x: dy under the
+    mask that the same ``p``, ``rng`` contents, ``site`` and shape draw. (The
+    residual's gradient is dy itself.)"""
+    return _dropout("dropout_bwd", dy, p, rng, site, None, out)
+
+
 def take_rows(table: torch.Tensor, idx: torch.Tensor, out: torch.Tensor | None = None,
               bad: torch.Tensor | None = None) -> torch.Tensor:
     """out[i, ...] = table[idx[i], ...]: a gather along the table's leading
