@@ -154,6 +154,39 @@ int pdh_layernorm_bwd(const void* x, const void* dy, const void* dres, const voi
 int pdh_dropout(const void* x, const void* residual, void* y, int64_t rows, int64_t cols, int64_t ldx, int64_t ldr,
                 int64_t ldy, double p, const int64_t* rng, int64_t site, int dtype, void* stream);
 
+/* Softmax cross entropy of a linear head over a vocabulary, without the logits
+ * in memory:
+ *   z[n, v] = sum_d x[n, d] w[v, d], lse[n] = log sum_v exp z[n, v]
+ *   loss[n] = lse[n] - z[n, targets[n]]
+ * x [tokens][width], w [vocab][width] of `dtype` (rows strided by ldx / ldw,
+ * 0 allowed, features contiguous), targets int64 [tokens], loss and lse fp32
+ * [tokens]. A token whose target is ignore_index or lies outside [0, vocab)
+ * has no loss (0) and no gradient; one outside that is not ignore_index adds 1
+ * to *bad (device int, may be NULL). The backward takes the forward's lse and
+ * dloss, fp32 [tokens], the gradient of each token's loss:
+ *   dz[n, v] = dloss[n] (exp(z[n, v] - lse[n]) - [v == targets[n]])
+ *   dx = dz w [tokens][width], dw = dz^T x [vocab][width], dense, of `dtype`
+ * computing z again piece by piece of the vocabulary. Products accumulate in
+ * fp32. 16-bit types: dz of a piece is rounded to the type; PDH_F32: operands
+ * are split into three bf16 terms each, six products of them, as
+ * pdh_contract_set_f32_mode(6) does, and a token or entry that holds an
+ * infinity, a NaN or a value beyond the bf16 range comes out NaN. Nothing is
+ * atomic: results repeat bit for bit. The backward needs tokens >= 1.
+ * ws, 16-byte aligned, holds pdh_linear_xent_workspace bytes for the same
+ * x, w (looked at for alignment alone), sizes, strides and direction: packed
+ * operands where x or w is fp32 or cannot be read by 16-byte chunks, one
+ * piece's dz (at most 2^30 bytes, or 256 vocabulary entries), and partial
+ * sums. At most 2^24 tokens and entries, 2^18 features, 2^38 logits. No
+ * counterpart in the reference. */
+size_t pdh_linear_xent_workspace(const void* x, const void* w, int64_t tokens, int64_t width, int64_t vocab,
+                                 int64_t ldx, int64_t ldw, int dtype, int backward);
+int pdh_linear_xent_fwd(const void* x, const void* w, const int64_t* targets, float* loss, float* lse, int64_t tokens,
+                        int64_t width, int64_t vocab, int64_t ldx, int64_t ldw, int64_t ignore_index, int dtype,
+                        int* bad, void* ws, size_t ws_bytes, void* stream);
+int pdh_linear_xent_bwd(const void* x, const void* w, const int64_t* targets, const float* lse, const float* dloss,
+                        void* dx, void* dw, int64_t tokens, int64_t width, int64_t vocab, int64_t ldx, int64_t ldw,
+                        int64_t ignore_index, int dtype, void* ws, size_t ws_bytes, void* stream);
+
 /* Row gather: out[i, :] = table[idx[i], :] for i < n_idx, rows of row_elems
  * elements (strides ld_table / ld_out), the device form of tl.take along the
  * table's leading dim (indexing.py:192-230). The reference plans a take as a

@@ -33,6 +33,9 @@ EXPORTS = (
     "pdh_layernorm_bwd_workspace",
     "pdh_layernorm_bwd",
     "pdh_dropout",
+    "pdh_linear_xent_workspace",
+    "pdh_linear_xent_fwd",
+    "pdh_linear_xent_bwd",
     "pdh_take_rows",
     "pdh_scatter_add_rows",
     "pdh_flash_fwd",
@@ -129,6 +132,10 @@ def _declare(lib) -> None:
         "pdh_layernorm_bwd": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, i64, i32, vp,
                                     C.c_size_t, vp]),
         "pdh_dropout": (i32, [vp, vp, vp, i64, i64, i64, i64, i64, C.c_double, vp, i64, i32, vp]),
+        "pdh_linear_xent_workspace": (C.c_size_t, [vp, vp, i64, i64, i64, i64, i64, i32, i32]),
+        "pdh_linear_xent_fwd": (i32, [vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, i64, i32, vp, vp, C.c_size_t, vp]),
+        "pdh_linear_xent_bwd": (i32, [vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, i64, i32, vp, C.c_size_t,
+                                      vp]),
         "pdh_take_rows": (i32, [vp, vp, vp, i64, i64, i64, i64, i64, i32, vp, vp]),
         "pdh_scatter_add_rows": (i32, [vp, vp, vp, i64, i64, i64, i64, i64, i32, vp, vp]),
         "pdh_flash_fwd": (i32, [vp, vp, vp, vp, vp, vp, vp, gp, i32, f32, f32, i32, i64, i64, i32, vp]),

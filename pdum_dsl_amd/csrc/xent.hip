@@ -1,0 +1,775 @@
+// Softmax cross entropy of a linear head over a large vocabulary, and its
+// gradient, without the logits in memory:
+//   z[n, v] = sum_d x[n, d] w[v, d], lse[n] = log sum_v exp z[n, v]
+//   loss[n] = lse[n] - z[n, target[n]]
+//   dz[n, v] = dloss[n] (exp(z[n, v] - lse[n]) - [v = target[n]])
+//   dx = dz w, dw = dz^T x
+// Forward: one product kernel whose tiles of z stay in accumulators; each wave
+// leaves the maximum and the sum of exponentials of its vocabulary strip of
+// every token, and the target's logit where it holds it; a second kernel joins
+// the strips. Backward: the vocabulary in pieces; for each the same product again,
+// dz of the piece stored in 16 bits, then dw's rows of the piece and the
+// piece's part of dx as two more products. dx's parts over slices of the
+// vocabulary are fp32 and added in order: no atomics, results repeat.
+//
+// All three products run one tile loop (xent_tile): 32-deep k tiles, three of
+// them in LDS by direct loads, v_mfma_f32_32x32x16, accumulators m along
+// registers and n along lanes. An operand is k-contiguous or has its rows (m or
+// n) contiguous, read transposed by ds_read_b64_tr_b16, so nothing is
+// transposed in memory. The m rows are dealt to the matrix instruction's rows
+// so that a lane's 16 accumulators are 16 consecutive m: whole vocabulary runs
+// for the softmax, 32 bytes of an output row for the stores.
+//
+// dz is rounded to the storage type, as the probabilities of a 16-bit
+// attention are: a relative 2^-9 (2^-12) of each term, below the rounding of
+// the 16-bit gradients they sum to. fp16 takes it scaled by a power of two (the
+// largest |dloss| to 2^14), or a mean's 1 / tokens times a small probability
+// would fall below its range. fp32 operands are split into three bf16 terms
+// and the six cross products above 2^-24 are summed, smallest first.
+#include "common.h"
+
+#include <algorithm>
+
+namespace pdh {
+namespace {
+
+constexpr int kBK = 32;      // k depth of a tile
+constexpr int kStages = 3;   // k tiles in LDS
+constexpr uint32_t kOOB = 0x80000000u;  // past every buffer's extent: reads as zero
+constexpr int kPairs = 6;    // fp32: products of bf16 terms (term of a, term of b), smallest first
+
+// A 16-bit operand: rows of `pitch` bytes; k-contiguous (a row holds one m's or
+// n's k values) or not (a row holds one k's m or n values). fp32 operands lie
+// as three planes of bf16 terms, `plane` bytes apart.
+struct Operand {
+  const char* p;
+  int64_t pitch, plane;
+};
+
+struct TileArgs {
+  Operand a, b;
+  int m, n, k;  // extents
+  int tiles_m, tiles_n, slices;
+  int kslice;   // k columns of a slice (a multiple of kBK)
+  int group;    // n tiles that neighbouring workgroups share an m tile across
+};
+
+// The tile of workgroup `bid`: each XCD (bid % 8) takes a contiguous run of
+// tiles, ordered so that 8 x 8 neighbours share operand panels in its L2.
+struct Tile {
+  int m, n, slice;
+  bool live;
+};
+__device__ __forceinline__ Tile tile_of(const TileArgs& a) {
+  const uint32_t per = static_cast<uint32_t>(a.tiles_m) * a.tiles_n, total = per * a.slices;
+  const uint32_t chunk = (total + 7) / 8, pos = blockIdx.x >> 3;
+  uint32_t id = (blockIdx.x & 7) * chunk + pos;
+  Tile t{0, 0, 0, pos < chunk && id < total};
+  t.slice = static_cast<int>(id / per);
+  id -= t.slice * per;
+  const uint32_t gsize = static_cast<uint32_t>(a.group) * a.tiles_m, g = id / gsize, rem = id - g * gsize;
+  const uint32_t n0 = g * a.group, gn = min(static_cast<uint32_t>(a.tiles_n) - n0, static_cast<uint32_t>(a.group));
+  t.m = static_cast<int>(rem / gn);
+  t.n = static_cast<int>(n0 + rem % gn);
+  return t;
+}
+
+// Four waves, 2 x 2, each 32 TM (m) x 32 TN (n).
+template <int TM, int TN>
+struct Shape {
+  static constexpr int BM = 64 * TM, BN = 64 * TN;
+  static constexpr int LDS_A = BM * kBK * 2, LDS_B = BN * kBK * 2, STAGE = LDS_A + LDS_B;
+  static constexpr int LDS = kStages * STAGE;
+};
+
+// One operand's side of the loop. R: its rows in the tile (BM or BN); KC:
+// k-contiguous; PERM: rows dealt as described above (the m side).
+template <int R, int T, bool KC, bool PERM>
+struct Side {
+  static constexpr int BLOCKS = R * kBK * 2 / 1024 / 4;  // direct loads (1 KB) per wave and k tile
+  static constexpr int PITCH = R * 2;                    // LDS bytes of a k row (rows contiguous)
+  static constexpr int SLOTS = R / 8, KROWS = 64 / SLOTS;  // its 16-byte slots; k rows a direct load covers
+  uint32_t voff, vtail;  // the lane's byte offset in a direct load; the same in a ragged last k tile
+  uint32_t pitch;
+  int read[T][2];        // LDS offsets of the lane's fragments (without the tr read's second half)
+
+  // 16-byte slots are XOR-swizzled so that neither the b128 reads (16 lanes a cycle, the
+  // quads of one parity in each half wave) nor the tr reads (32 lanes) meet a bank twice.
+  __device__ __forceinline__ static int swz(int krow) { return R >= 128 ? 4 * (krow & 3) : 4 * ((krow >> 1) & 1); }
+
+  __device__ __forceinline__ Side(const Operand& o, int wq, int lane, int w, int ktail) {
+    pitch = static_cast<uint32_t>(o.pitch);
+    if constexpr (KC) {  // 16 rows of four 16-byte chunks a direct load
+      const int row = lane >> 2, chunk = (lane & 3) ^ ((row >> 2) & 3);
+      voff = row * pitch + (chunk << 4);
+      vtail = 8 * chunk < ktail ? voff : kOOB;
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          const int r = lane & 31, g = lane >> 5;
+          const int row_ = 32 * (wq * T + t) + (PERM ? 16 * ((r >> 2) & 1) + 4 * (r >> 3) + (r & 3) : r);
+          read[t][ks] = row_ * (kBK * 2) + (((2 * ks + g) ^ ((row_ >> 2) & 3)) << 4);
+        }
+    } else {
+      const int kr = lane / SLOTS, in_tile = (KROWS * w + kr);  // blocks are w, w + 4, ...: k rows equal mod 4
+      voff = kr * pitch + (((lane % SLOTS) ^ swz(in_tile)) << 4);
+      vtail = voff;  // k rows past the end lie past the extent
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          const int G = lane >> 4, i4 = (lane >> 2) & 3, q = 4 * (G & 1) + (lane & 3);
+          const int kr_ = 16 * ks + 8 * (G >> 1) + i4;
+          const int col = 32 * (wq * T + t) + (PERM ? 16 * (q & 1) + 4 * (q >> 1) : 4 * q);
+          read[t][ks] = kr_ * PITCH + (((col >> 3) ^ swz(kr_)) << 4) + ((col >> 2) & 1) * 8;
+        }
+    }
+  }
+
+  // Direct loads of k columns k0 .. k0 + 31 of rows r0 .. r0 + R - 1 (`rows` of them in the operand, `k` columns).
+  __device__ __forceinline__ void fetch(const Operand& o, int64_t plane, int64_t r0, int rows, int64_t k0, int64_t k,
+                                        uint32_t lds, int w) const {
+    const char* base;
+    uint32_t extent;
+    const bool last = k - k0 < kBK;
+    const int64_t nr = rows - r0 < R ? rows - r0 : R, nk = last ? k - k0 : kBK;
+    if constexpr (KC) {
+      base = o.p + plane * o.plane + r0 * o.pitch + k0 * 2;
+      extent = static_cast<uint32_t>((nr - 1) * o.pitch + ((nk * 2 + 15) & ~int64_t{15}));
+    } else {
+      base = o.p + plane * o.plane + k0 * o.pitch + r0 * 2;
+      extent = static_cast<uint32_t>((nk - 1) * o.pitch + ((nr * 2 + 15) & ~int64_t{15}));
+    }
+    const rsrc_t rs = make_rsrc(base, extent);
+    const uint32_t v = last ? vtail : voff;
+#pragma unroll
+    for (int i = 0; i < BLOCKS; ++i) {
+      const int blk = 4 * i + w;
+      dma16_at(rs, lds + blk * 1024, v, static_cast<uint32_t>(KC ? 16 * blk : KROWS * blk) * pitch);
+    }
+  }
+
+  __device__ __forceinline__ u32x4 frag(const unsigned char* tile, int t, int ks) const {
+    if constexpr (KC) {
+      return *reinterpret_cast<const u32x4*>(tile + read[t][ks]);
+    } else {
+      const u32x2 lo = ds_read_tr16(tile + read[t][ks]), hi = ds_read_tr16(tile + read[t][ks] + 4 * PITCH);
+      return u32x4{lo.x, lo.y, hi.x, hi.y};
+    }
+  }
+};
+
+// acc = the products of a tile over k columns [k0, k1): accumulator i of
+// (tm, tn) is m = m0 + 32 (wm TM + tm) + 16 (lane / 32) + i, n = n0 + 32 (wn TN + tn) + lane % 32.
+// SPLIT: the operands are planes of bf16 terms, every k tile runs kPairs times.
+// Per k tile a wave loads TM + TN direct kilobytes, reads as many operand
+// fragments twice and issues 2 TM TN products.
+template <int DT, int TM, int TN, bool KA, bool KB, bool SPLIT>
+__device__ __forceinline__ void xent_tile(const TileArgs& a, unsigned char* smem, f32x16 (&acc)[TM][TN], int m0, int n0,
+                                          int64_t k0, int64_t k1) {
+  using S = Shape<TM, TN>;
+  const int lane = threadIdx.x & 63, w = wave_id(), wm = w >> 1, wn = w & 1;
+  const int ktail = static_cast<int>((k1 - k0) % kBK);
+  const Side<S::BM, TM, KA, true> sa(a.a, wm, lane, w, ktail);
+  const Side<S::BN, TN, KB, false> sb(a.b, wn, lane, w, ktail);
+  constexpr int PER = decltype(sa)::BLOCKS + decltype(sb)::BLOCKS;
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = f32x16{};
+  const int nkt = static_cast<int>((k1 - k0 + kBK - 1) / kBK);
+  const int steps = SPLIT ? nkt * kPairs : nkt;
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(smem));
+  int fpair = 0, fkt = 0, fbuf = 0;  // the next k tile to fetch
+  auto fetch = [&]() __attribute__((always_inline)) {
+    // pairs in order of growing size: terms (0, 2) (2, 0) (1, 1) (0, 1) (1, 0) (0, 0), two bits each
+    const int64_t pa = SPLIT ? (0x0118 >> (2 * fpair)) & 3 : 0, pb = SPLIT ? (0x0052 >> (2 * fpair)) & 3 : 0;
+    const int64_t kk = k0 + static_cast<int64_t>(fkt) * kBK;
+    const uint32_t lds = lds0 + fbuf * S::STAGE;
+    sa.fetch(a.a, pa, m0, a.m, kk, k1, lds, w);
+    sb.fetch(a.b, pb, n0, a.n, kk, k1, lds + S::LDS_A, w);
+    fbuf = fbuf + 1 == kStages ? 0 : fbuf + 1;
+    if (++fkt == nkt) fkt = 0, ++fpair;
+  };
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s)
+    if (s < steps) fetch();
+  int buf = 0;
+  for (int st = 0; st < steps; ++st, buf = buf + 1 == kStages ? 0 : buf + 1) {
+    // the tile has landed when at most the next one's loads are outstanding
+    if (st + 1 < steps)
+      __builtin_amdgcn_s_waitcnt(0x0f70 | (PER & 15) | ((PER >> 4) << 14));
+    else
+      wait_vmcnt0();
+    __syncthreads();  // every wave's loads of this tile are done; everyone has finished the tile before
+    if (st + kStages - 1 < steps) fetch();
+    const unsigned char* at = smem + buf * S::STAGE;
+    const unsigned char* bt = at + S::LDS_A;
+    u32x4 af[2][TM], bf[2][TN];
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+#pragma unroll
+      for (int t = 0; t < TM; ++t) af[ks][t] = sa.frag(at, t, ks);
+#pragma unroll
+      for (int t = 0; t < TN; ++t) bf[ks][t] = sb.frag(bt, t, ks);
+    }
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = mfma32_dt<DT>(af[ks][i], bf[ks][j], acc[i][j]);
+    __builtin_amdgcn_s_setprio(0);
+  }
+}
+
+// ---------------------------------------------------------------- forward
+
+struct FwdArgs {
+  TileArgs t;  // a: w (m: vocabulary), b: x (n: tokens)
+  const int64_t* targets;
+  float2* part;  // [strips][tokens]: (max, sum of exp(z - max)) of 32 TM vocabulary entries
+  float* zt;     // [tokens]: the target's logit
+};
+
+template <int DT, int TM, int TN, bool SPLIT>
+__global__ __launch_bounds__(256, 2) void xent_fwd(FwdArgs p) {
+  using S = Shape<TM, TN>;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[S::LDS];
+  const Tile t = tile_of(p.t);
+  if (!t.live) return;
+  const int m0 = t.m * S::BM, n0 = t.n * S::BN;
+  const int lane = threadIdx.x & 63, w = wave_id(), wm = w >> 1, wn = w & 1, g = lane >> 5;
+  f32x16 acc[TM][TN];
+  xent_tile<DT, TM, TN, true, true, SPLIT>(p.t, smem, acc, m0, n0, 0, p.t.k);
+  const int vw = m0 + 32 * wm * TM, v0 = vw + 16 * g;  // the wave's strip, the lane's first entry of it
+  const int strip = 2 * t.m + wm;
+#pragma unroll
+  for (int j = 0; j < TN; ++j) {
+    const int n = n0 + 32 * (wn * TN + j) + (lane & 31);
+    const bool in = n < p.t.n;
+    const int64_t tl = (in ? p.targets[n] : -1) - v0;
+    if (vw + 32 * TM > p.t.m) {  // entries past the vocabulary weigh nothing
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (v0 + 32 * i + e >= p.t.m) acc[i][j][e] = -__builtin_inff();
+    }
+    float mx = -__builtin_inff();
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, acc[i][j][e]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    const float base = mx == -__builtin_inff() ? 0.f : mx * kLog2e;  // a strip of -inf sums to 0, not NaN
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s += fast_exp2(__builtin_fmaf(acc[i][j][e], kLog2e, -base));
+    s += __shfl_xor(s, 32, 64);
+    if (in && g == 0) p.part[static_cast<int64_t>(strip) * p.t.n + n] = make_float2(mx, s);
+    if (tl >= 0 && tl < 32 * TM && v0 + tl < p.t.m && (tl & 16) == 0) {  // this lane holds the target's logit
+      float z = 0.f;
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (tl == 32 * i + e) z = acc[i][j][e];
+      p.zt[n] = z;
+    }
+  }
+}
+
+// Joins the strips of 8 tokens, 32 lanes a token: lse and loss.
+__global__ __launch_bounds__(256) void xent_join(const float2* __restrict__ part, const float* __restrict__ zt,
+                                                 const int64_t* __restrict__ targets, int strips, int64_t n_tokens,
+                                                 int64_t vocab, int64_t ignore, float* __restrict__ loss,
+                                                 float* __restrict__ lse, int* __restrict__ bad) {
+  __shared__ float2 sh[32][8];
+  const int tok = threadIdx.x & 7, q = threadIdx.x >> 3;
+  const int64_t n = static_cast<int64_t>(blockIdx.x) * 8 + tok;
+  float m = -__builtin_inff(), s = 0.f;
+  auto add = [&](float2 o) {
+    const float mn = nan_max(m, o.x);
+    const float b = mn == -__builtin_inff() ? 0.f : mn;
+    s = s * fast_exp2((m - b) * kLog2e) + o.y * fast_exp2((o.x - b) * kLog2e);
+    m = mn;
+  };
+  if (n < n_tokens)
+    for (int i = q; i < strips; i += 32) add(part[static_cast<int64_t>(i) * n_tokens + n]);
+  sh[q][tok] = make_float2(m, s);
+  __syncthreads();
+  if (q == 0 && n < n_tokens) {
+    for (int i = 1; i < 32; ++i) add(sh[i][tok]);
+    const float l = m + logf(s);
+    const int64_t t = targets[n];
+    const bool live = t >= 0 && t < vocab && t != ignore;
+    lse[n] = l;
+    loss[n] = live ? l - zt[n] : 0.f;
+    if (!live && t != ignore && bad) atomicAdd(bad, 1);
+  }
+}
+
+// --------------------------------------------------------------- backward
+
+struct GradArgs {
+  TileArgs t;
+  const int64_t* targets;
+  const float* lse;
+  const float* g;      // [tokens]: dloss (fp16: scaled)
+  uint16_t* dz;        // [planes][tokens][ldz]
+  int64_t ldz, plane;  // elements
+  int64_t v0;          // the piece's first vocabulary entry
+  int64_t vocab, ignore;
+};
+
+// dz of a piece: a: w from the piece's first row (m: its entries), b: x.
+template <int DT, int TM, int TN, bool SPLIT>
+__global__ __launch_bounds__(256, 2) void xent_dz(GradArgs p) {
+  using S = Shape<TM, TN>;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[S::LDS];
+  const Tile t = tile_of(p.t);
+  if (!t.live) return;
+  const int m0 = t.m * S::BM, n0 = t.n * S::BN;
+  const int lane = threadIdx.x & 63, w = wave_id(), wm = w >> 1, wn = w & 1, g = lane >> 5;
+  f32x16 acc[TM][TN];
+  xent_tile<DT, TM, TN, true, true, SPLIT>(p.t, smem, acc, m0, n0, 0, p.t.k);
+  const int c0 = m0 + 32 * wm * TM + 16 * g;  // the lane's first column of dz
+#pragma unroll
+  for (int j = 0; j < TN; ++j) {
+    const int n = n0 + 32 * (wn * TN + j) + (lane & 31);
+    if (n >= p.t.n) continue;
+    const int64_t tg = p.targets[n];
+    const bool live = tg >= 0 && tg < p.vocab && tg != p.ignore;
+    const float gn = live ? p.g[n] : 0.f, l2 = p.lse[n] * kLog2e;
+    const int64_t tl = live ? tg - p.v0 - c0 : -1;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      const int c = c0 + 32 * i;
+      if (c >= p.ldz) continue;  // ldz is a multiple of 32
+      float q[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) q[e] = fast_exp2(__builtin_fmaf(acc[i][j][e], kLog2e, -l2));
+      const int64_t at = tl - 32 * i;
+      if (at >= 0 && at < 16) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (at == e) q[e] -= 1.f;
+      }
+      // an ignored token has no gradient whatever its logits are; entries past the vocabulary are zero
+#pragma unroll
+      for (int e = 0; e < 16; ++e) q[e] = live && c + e < p.t.m ? q[e] * gn : 0.f;
+      uint16_t* o = p.dz + static_cast<int64_t>(n) * p.ldz + c;
+#pragma unroll
+      for (int pl = 0; pl < (SPLIT ? 3 : 1); ++pl) {
+        u32x4 lo, hi;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (DT == PDH_BF16) {
+            lo[e] = pack2<__hip_bfloat16>(q[2 * e], q[2 * e + 1]);
+            hi[e] = pack2<__hip_bfloat16>(q[8 + 2 * e], q[9 + 2 * e]);
+          } else {
+            lo[e] = pack2<_Float16>(q[2 * e], q[2 * e + 1]);
+            hi[e] = pack2<_Float16>(q[8 + 2 * e], q[9 + 2 * e]);
+          }
+          if constexpr (SPLIT) {  // what this term leaves (exact)
+            q[2 * e] -= __uint_as_float(lo[e] << 16);
+            q[2 * e + 1] -= __uint_as_float(lo[e] & 0xffff0000u);
+            q[8 + 2 * e] -= __uint_as_float(hi[e] << 16);
+            q[9 + 2 * e] -= __uint_as_float(hi[e] & 0xffff0000u);
+          }
+        }
+        reinterpret_cast<u32x4*>(o + pl * p.plane)[0] = lo;
+        reinterpret_cast<u32x4*>(o + pl * p.plane)[1] = hi;
+      }
+    }
+  }
+}
+
+// A gradient product: a: x or w with its features contiguous (m: features),
+// b: dz, its columns (dw: n vocabulary, k tokens) or its rows (dx: n tokens, k vocabulary).
+struct ProdArgs {
+  TileArgs t;
+  void* out;           // dw rows, or fp32 parts [slices][n][ldo]
+  int64_t ldo, slice;  // elements
+  const float* scale;  // NULL: 1
+  int add;             // add to what out holds (the parts of an earlier piece)
+};
+
+template <int DT, int ODT, int TM, int TN, bool KB, bool SPLIT>
+__global__ __launch_bounds__(256, 2) void xent_prod(ProdArgs p) {
+  using S = Shape<TM, TN>;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[S::LDS];
+  const Tile t = tile_of(p.t);
+  if (!t.live) return;
+  const int m0 = t.m * S::BM, n0 = t.n * S::BN;
+  const int lane = threadIdx.x & 63, w = wave_id(), wm = w >> 1, wn = w & 1, g = lane >> 5;
+  f32x16 acc[TM][TN];
+  const int64_t k0 = static_cast<int64_t>(t.slice) * p.t.kslice;
+  const int64_t k1 = k0 + p.t.kslice < p.t.k ? k0 + p.t.kslice : p.t.k;
+  xent_tile<DT, TM, TN, false, KB, SPLIT>(p.t, smem, acc, m0, n0, k0, k1);
+  const float sc = p.scale ? *p.scale : 1.f;
+  constexpr int ES = ODT == PDH_F32 ? 4 : 2;
+#pragma unroll
+  for (int j = 0; j < TN; ++j) {
+    const int n = n0 + 32 * (wn * TN + j) + (lane & 31);
+    if (n >= p.t.n) continue;
+    char* row = static_cast<char*>(p.out) + (t.slice * p.slice + static_cast<int64_t>(n) * p.ldo) * ES;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      const int c = m0 + 32 * (wm * TM + i) + 16 * g, left = p.t.m - c;
+      if (left <= 0) continue;
+      if (left >= 16) {
+        if constexpr (ODT == PDH_F32) {
+          f32x4u* o = reinterpret_cast<f32x4u*>(row + c * 4);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            f32x4u v{acc[i][j][4 * q] * sc, acc[i][j][4 * q + 1] * sc, acc[i][j][4 * q + 2] * sc,
+                     acc[i][j][4 * q + 3] * sc};
+            if (p.add) v += o[q];
+            o[q] = v;
+          }
+        } else {
+          u32x4h* o = reinterpret_cast<u32x4h*>(row + c * 2);
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            u32x4h v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float x0 = acc[i][j][8 * q + 2 * e] * sc, x1 = acc[i][j][8 * q + 2 * e + 1] * sc;
+              v[e] = ODT == PDH_BF16 ? pack2<__hip_bfloat16>(x0, x1) : pack2<_Float16>(x0, x1);
+            }
+            o[q] = v;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 15; ++e)
+          if (e < left) {
+            float v = acc[i][j][e] * sc;
+            if (ODT == PDH_F32 && p.add) v += reinterpret_cast<float*>(row)[c + e];
+            st_dt<ODT>(row, c + e, v);
+          }
+      }
+    }
+  }
+}
+
+// dx = scale * the sum of its parts, in order.
+template <int DT>
+__global__ __launch_bounds__(256) void xent_dx(const float* __restrict__ part, void* dx, int64_t rows, int d,
+                                               int64_t ld, int64_t slice, int slices, const float* scale) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t per = ld / 4, n = i / per;
+  const int c = static_cast<int>(i - n * per) * 4;
+  if (n >= rows || c >= d) return;
+  const float* p = part + n * ld + c;
+  f32x4 s = *reinterpret_cast<const f32x4*>(p);
+  for (int q = 1; q < slices; ++q) s += *reinterpret_cast<const f32x4*>(p + q * slice);
+  if (scale) s *= *scale;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (c + e < d) st_dt<DT>(dx, n * d + c + e, s[e]);
+}
+
+// fp16's dz scale: 2^14 over the power of two above the largest |dloss| of a
+// live token. One workgroup; g[n] = dloss[n] times it, *inv its inverse.
+__global__ __launch_bounds__(1024) void xent_scale(const float* __restrict__ dloss, const int64_t* __restrict__ targets,
+                                                   int64_t n, int64_t vocab, int64_t ignore, float* __restrict__ g,
+                                                   float* __restrict__ inv) {
+  __shared__ float sh[16];
+  float mx = 0.f;
+  auto live = [&](int64_t t) { return t >= 0 && t < vocab && t != ignore; };
+  for (int64_t i = threadIdx.x; i < n; i += 1024)
+    if (live(targets[i])) mx = fmaxf(mx, fabsf(dloss[i]));
+  mx = wave_max(mx);
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = mx;
+  __syncthreads();
+  mx = sh[0];
+  for (int i = 1; i < 16; ++i) mx = fmaxf(mx, sh[i]);
+  int e = 0;
+  if (mx > 0.f && mx < __builtin_inff()) frexpf(mx, &e);  // mx < 2^e
+  const float up = ldexpf(1.f, min(14 - e, 126));
+  for (int64_t i = threadIdx.x; i < n; i += 1024) g[i] = dloss[i] * up;
+  if (threadIdx.x == 0) *inv = ldexpf(1.f, -min(14 - e, 126));
+}
+
+// An operand made fit for the direct loads: rows of `dp` (a multiple of 8)
+// 16-bit values, zero past d. fp32 rows become three planes of bf16 terms,
+// 16-bit ones of odd width, stride or alignment a padded copy.
+template <int DT>
+__global__ __launch_bounds__(256) void xent_pack(const void* __restrict__ src, int64_t ld, int64_t rows, int d, int dp,
+                                                 uint16_t* __restrict__ dst, int64_t plane) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t per = dp / 8, n = i / per;
+  const int c = static_cast<int>(i - n * per) * 8;
+  if (n >= rows) return;
+  uint16_t* o = dst + n * dp + c;
+  if constexpr (DT == PDH_F32) {
+    const float* x = static_cast<const float*>(src) + n * ld + c;
+    float v[8];
+    if (c + 8 <= d) {
+      const f32x4u a = reinterpret_cast<const f32x4u*>(x)[0], b = reinterpret_cast<const f32x4u*>(x)[1];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = a[e], v[4 + e] = b[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = c + e < d ? x[e] : 0.f;
+    }
+#pragma unroll
+    for (int pl = 0; pl < 3; ++pl) {
+      u32x4 w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        w[e] = pack2<__hip_bfloat16>(v[2 * e], v[2 * e + 1]);
+        v[2 * e] -= __uint_as_float(w[e] << 16);
+        v[2 * e + 1] -= __uint_as_float(w[e] & 0xffff0000u);
+      }
+      *reinterpret_cast<u32x4*>(o + pl * plane) = w;
+    }
+  } else {
+    const uint16_t* x = static_cast<const uint16_t*>(src) + n * ld + c;
+    u32x4 w{};
+    if (c + 8 <= d) {
+      w = *reinterpret_cast<const u32x4h*>(x);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (c + e < d) w[e >> 1] |= static_cast<uint32_t>(x[e]) << (16 * (e & 1));
+    }
+    *reinterpret_cast<u32x4*>(o) = w;
+  }
+}
+
+// ------------------------------------------------------------------- host
+
+constexpr int64_t kPieceBytes = int64_t{1} << 30;  // dz of one piece of the vocabulary
+
+int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+struct Problem {
+  int64_t n, d, v;  // tokens, width, vocabulary
+  int64_t ldx, ldw;
+  const void* x;
+  const void* w;
+  int dtype;
+  int planes() const { return dtype == PDH_F32 ? 3 : 1; }
+  int64_t dp() const { return up(d, 8); }
+  // read in place: 16-bit rows of whole 16-byte chunks, 256 of them within the loads' reach
+  static bool fit(const void* p, int64_t ld, int64_t d, int dtype) {
+    return dtype != PDH_F32 && d % 8 == 0 && ld % 8 == 0 && ld >= d && aligned16(p) && ld <= (int64_t{1} << 21);
+  }
+};
+
+// A bump allocator over the caller's workspace; without one it measures.
+struct Space {
+  char* base;
+  size_t used = 0;
+  void* take(int64_t bytes) {
+    const size_t at = used;
+    used += static_cast<size_t>(up(bytes, 1024));
+    return base ? base + at : nullptr;
+  }
+};
+
+unsigned blocks_for(int64_t threads) { return static_cast<unsigned>((threads + 255) / 256); }
+
+// The operand of rows x[rows][d]: in place, or packed into ws by a kernel.
+Operand place(const void* p, int64_t ld, int64_t rows, const Problem& q, Space& ws, bool in_place, hipStream_t s,
+              bool launch) {
+  if (in_place) return Operand{static_cast<const char*>(p), ld * 2, 0};
+  const int64_t dp = q.dp(), plane = rows * dp;
+  auto* dst = static_cast<uint16_t*>(ws.take(plane * 2 * q.planes()));
+  if (launch) {
+    const dim3 grid(blocks_for(rows * (dp / 8)));
+    if (q.dtype == PDH_F32)
+      xent_pack<PDH_F32><<<grid, 256, 0, s>>>(p, ld, rows, static_cast<int>(q.d), static_cast<int>(dp), dst, plane);
+    else
+      xent_pack<PDH_BF16><<<grid, 256, 0, s>>>(p, ld, rows, static_cast<int>(q.d), static_cast<int>(dp), dst, plane);
+  }
+  return Operand{reinterpret_cast<const char*>(dst), dp * 2, plane * 2};
+}
+
+template <int TM, int TN>
+TileArgs tiles(Operand a, Operand b, int64_t m, int64_t n, int64_t k, int64_t kslice) {
+  using S = Shape<TM, TN>;
+  TileArgs t{};
+  t.a = a, t.b = b;
+  t.m = static_cast<int>(m), t.n = static_cast<int>(n), t.k = static_cast<int>(k);
+  t.tiles_m = static_cast<int>((m + S::BM - 1) / S::BM);
+  t.tiles_n = static_cast<int>((n + S::BN - 1) / S::BN);
+  t.kslice = static_cast<int>(kslice);
+  t.slices = static_cast<int>((k + kslice - 1) / kslice);
+  t.group = t.tiles_n < 8 ? t.tiles_n : 8;
+  return t;
+}
+dim3 grid_of(const TileArgs& t) {
+  return dim3(static_cast<unsigned>((static_cast<int64_t>(t.tiles_m) * t.tiles_n * t.slices + 7) / 8 * 8));
+}
+
+constexpr int TM = 4, TN = 2;  // 256 x 128 tiles
+
+int check(const char* fn, int64_t n, int64_t d, int64_t v, int64_t ldx, int64_t ldw, int dtype) {
+  PDH_REQUIRE(dtype == PDH_F32 || dtype == PDH_BF16 || dtype == PDH_F16, PDH_EUNSUPPORTED, "%s: dtype %d", fn, dtype);
+  PDH_REQUIRE(n >= 0 && d >= 1 && v >= 1, PDH_EINVAL, "%s: need tokens >= 0, width >= 1, vocabulary >= 1 (got %lld, %lld, %lld)",
+              fn, (long long)n, (long long)d, (long long)v);
+  PDH_REQUIRE(n <= (int64_t{1} << 24) && v <= (int64_t{1} << 24) && d <= (int64_t{1} << 18), PDH_EUNSUPPORTED,
+              "%s: at most 2^24 tokens and vocabulary entries and 2^18 features", fn);
+  // every launch stays under 2^32 threads
+  PDH_REQUIRE(n * v <= (int64_t{1} << 38) && std::max(n, v) * up(d, 8) <= (int64_t{1} << 33), PDH_EUNSUPPORTED,
+              "%s: at most 2^38 logits and 2^33 elements of x or w in a call", fn);
+  PDH_REQUIRE(ldx >= 0 && ldw >= 0, PDH_EINVAL, "%s: row strides must be >= 0", fn);
+  return PDH_OK;
+}
+
+// The forward's workspace (base NULL: measured), its operands placed in it.
+struct FwdPlan {
+  Operand w, x;
+  TileArgs t;
+  float2* part;
+  float* zt;
+  int strips;
+};
+FwdPlan plan_fwd(const Problem& q, Space& ws, bool fit_x, bool fit_w, hipStream_t s, bool launch) {
+  FwdPlan p{};
+  p.w = place(q.w, q.ldw, q.v, q, ws, fit_w, s, launch);
+  p.x = place(q.x, q.ldx, q.n, q, ws, fit_x, s, launch);
+  p.t = tiles<TM, TN>(p.w, p.x, q.v, q.n, q.dp(), up(q.dp(), kBK));
+  p.strips = 2 * p.t.tiles_m;
+  p.part = static_cast<float2*>(ws.take(static_cast<int64_t>(p.strips) * q.n * 8));
+  p.zt = static_cast<float*>(ws.take(q.n * 4));
+  return p;
+}
+
+struct BwdPlan {
+  Operand w, x;
+  uint16_t* dz;
+  float* parts;
+  float* g;
+  float* inv;
+  int64_t piece;   // vocabulary entries of a piece (the last one's may be fewer)
+  int64_t kslice;  // of them in a slice of dx's product
+  int64_t slices;  // of a whole piece
+};
+BwdPlan plan_bwd(const Problem& q, Space& ws, bool fit_x, bool fit_w, hipStream_t s, bool launch) {
+  BwdPlan p{};
+  p.w = place(q.w, q.ldw, q.v, q, ws, fit_w, s, launch);
+  p.x = place(q.x, q.ldx, q.n, q, ws, fit_x, s, launch);
+  const int64_t all = up(q.v, 256), most = kPieceBytes / (q.n * 2 * q.planes()) / 256 * 256;
+  p.piece = std::min(all, std::max<int64_t>(most, 256));
+  p.dz = static_cast<uint16_t*>(ws.take(q.n * p.piece * 2 * q.planes()));
+  // dx's tiles alone would leave compute units idle: its k, the vocabulary, in slices
+  const int64_t t = ((q.d + 255) / 256) * ((q.n + 127) / 128);
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>({(1024 + t - 1) / t, p.piece / 512, 64}));
+  p.kslice = up((p.piece + want - 1) / want, kBK);
+  p.slices = (p.piece + p.kslice - 1) / p.kslice;
+  p.parts = static_cast<float*>(ws.take(p.slices * q.n * q.dp() * 4));
+  if (q.dtype == PDH_F16) {
+    p.g = static_cast<float*>(ws.take(q.n * 4));
+    p.inv = static_cast<float*>(ws.take(4));
+  }
+  return p;
+}
+
+template <int DT, bool SPLIT>
+int run_fwd(const Problem& q, const FwdPlan& p, const int64_t* targets, int64_t ignore, float* loss, float* lse, int* bad,
+            hipStream_t s) {
+  xent_fwd<DT, TM, TN, SPLIT><<<grid_of(p.t), 256, 0, s>>>(FwdArgs{p.t, targets, p.part, p.zt});
+  if (int rc = check_launch("pdh_linear_xent_fwd"); rc != PDH_OK) return rc;
+  xent_join<<<dim3(static_cast<unsigned>((q.n + 7) / 8)), 256, 0, s>>>(p.part, p.zt, targets, p.strips, q.n, q.v, ignore,
+                                                                       loss, lse, bad);
+  return check_launch("pdh_linear_xent_fwd (join)");
+}
+
+template <int DT, int ODT, bool SPLIT>
+int run_bwd(const Problem& q, const BwdPlan& p, const int64_t* targets, const float* lse, const float* dloss,
+            int64_t ignore, void* dx, void* dw, hipStream_t s) {
+  const float* g = dloss;
+  const float* scale = nullptr;
+  if constexpr (DT == PDH_F16) {
+    xent_scale<<<1, 1024, 0, s>>>(dloss, targets, q.n, q.v, ignore, p.g, p.inv);
+    g = p.g;
+    scale = p.inv;
+  }
+  const int64_t es = ODT == PDH_F32 ? 4 : 2, dp = q.dp(), slice = q.n * dp;
+  for (int64_t v0 = 0; v0 < q.v; v0 += p.piece) {
+    const int64_t nv = std::min(p.piece, q.v - v0), ldz = up(nv, 256);
+    const Operand wv{p.w.p + v0 * p.w.pitch, p.w.pitch, p.w.plane};
+    const Operand dz{reinterpret_cast<const char*>(p.dz), ldz * 2, q.n * ldz * 2};
+    GradArgs ga{tiles<TM, TN>(wv, p.x, nv, q.n, dp, up(dp, kBK)), targets, lse, g, p.dz, ldz, q.n * ldz, v0, q.v, ignore};
+    xent_dz<DT, TM, TN, SPLIT><<<grid_of(ga.t), 256, 0, s>>>(ga);
+    ProdArgs pw{tiles<TM, TN>(p.x, dz, q.d, nv, q.n, up(q.n, kBK)), static_cast<char*>(dw) + v0 * q.d * es, q.d, 0, scale, 0};
+    xent_prod<DT, ODT, TM, TN, false, SPLIT><<<grid_of(pw.t), 256, 0, s>>>(pw);
+    ProdArgs px{tiles<TM, TN>(wv, dz, q.d, q.n, nv, p.kslice), p.parts, dp, slice, nullptr, v0 > 0};
+    xent_prod<DT, PDH_F32, TM, TN, true, SPLIT><<<grid_of(px.t), 256, 0, s>>>(px);
+    if (int rc = check_launch("pdh_linear_xent_bwd"); rc != PDH_OK) return rc;
+  }
+  xent_dx<ODT><<<dim3(blocks_for(q.n * (dp / 4))), 256, 0, s>>>(p.parts, dx, q.n, static_cast<int>(q.d), dp, slice,
+                                                               static_cast<int>(p.slices), scale);
+  return check_launch("pdh_linear_xent_bwd (dx)");
+}
+
+}  // namespace
+}  // namespace pdh
+
+using namespace pdh;
+
+extern "C" size_t pdh_linear_xent_workspace(const void* x, const void* w, int64_t tokens, int64_t width, int64_t vocab,
+                                            int64_t ldx, int64_t ldw, int dtype, int backward) {
+  if (check("pdh_linear_xent_workspace", tokens, width, vocab, ldx, ldw, dtype) != PDH_OK || tokens == 0) return 0;
+  const Problem q{tokens, width, vocab, ldx, ldw, x, w, dtype};
+  const bool fx = Problem::fit(x, ldx, width, dtype), fw = Problem::fit(w, ldw, width, dtype);
+  Space ws{nullptr};
+  if (backward)
+    plan_bwd(q, ws, fx, fw, nullptr, false);
+  else
+    plan_fwd(q, ws, fx, fw, nullptr, false);
+  return ws.used;
+}
+
+extern "C" int pdh_linear_xent_fwd(const void* x, const void* w, const int64_t* targets, float* loss, float* lse,
+                                   int64_t tokens, int64_t width, int64_t vocab, int64_t ldx, int64_t ldw,
+                                   int64_t ignore_index, int dtype, int* bad, void* ws, size_t ws_bytes, void* stream) {
+  if (int rc = check("pdh_linear_xent_fwd", tokens, width, vocab, ldx, ldw, dtype); rc != PDH_OK) return rc;
+  if (tokens == 0) return PDH_OK;
+  PDH_REQUIRE(x && w && targets && loss && lse, PDH_EINVAL, "pdh_linear_xent_fwd: null pointer");
+  const Problem q{tokens, width, vocab, ldx, ldw, x, w, dtype};
+  const bool fx = Problem::fit(x, ldx, width, dtype), fw = Problem::fit(w, ldw, width, dtype);
+  Space measure{nullptr};
+  plan_fwd(q, measure, fx, fw, nullptr, false);
+  PDH_REQUIRE(ws && aligned16(ws) && ws_bytes >= measure.used, PDH_EINVAL,
+              "pdh_linear_xent_fwd: the workspace holds %zu bytes, %zu are needed, 16-byte aligned", ws ? ws_bytes : size_t{0},
+              measure.used);
+  hipStream_t s = as_stream(stream);
+  Space space{static_cast<char*>(ws)};
+  const FwdPlan p = plan_fwd(q, space, fx, fw, s, true);
+  if (dtype == PDH_F32) return run_fwd<PDH_BF16, true>(q, p, targets, ignore_index, loss, lse, bad, s);
+  if (dtype == PDH_BF16) return run_fwd<PDH_BF16, false>(q, p, targets, ignore_index, loss, lse, bad, s);
+  return run_fwd<PDH_F16, false>(q, p, targets, ignore_index, loss, lse, bad, s);
+}
+
+extern "C" int pdh_linear_xent_bwd(const void* x, const void* w, const int64_t* targets, const float* lse,
+                                   const float* dloss, void* dx, void* dw, int64_t tokens, int64_t width, int64_t vocab,
+                                   int64_t ldx, int64_t ldw, int64_t ignore_index, int dtype, void* ws, size_t ws_bytes,
+                                   void* stream) {
+  if (int rc = check("pdh_linear_xent_bwd", tokens, width, vocab, ldx, ldw, dtype); rc != PDH_OK) return rc;
+  PDH_REQUIRE(tokens > 0, PDH_EINVAL, "pdh_linear_xent_bwd: no tokens");
+  PDH_REQUIRE(x && w && targets && lse && dloss && dx && dw, PDH_EINVAL, "pdh_linear_xent_bwd: null pointer");
+  const Problem q{tokens, width, vocab, ldx, ldw, x, w, dtype};
+  const bool fx = Problem::fit(x, ldx, width, dtype), fw = Problem::fit(w, ldw, width, dtype);
+  Space measure{nullptr};
+  plan_bwd(q, measure, fx, fw, nullptr, false);
+  PDH_REQUIRE(ws && aligned16(ws) && ws_bytes >= measure.used, PDH_EINVAL,
+              "pdh_linear_xent_bwd: the workspace holds %zu bytes, %zu are needed, 16-byte aligned", ws ? ws_bytes : size_t{0},
+              measure.used);
+  hipStream_t s = as_stream(stream);
+  Space space{static_cast<char*>(ws)};
+  const BwdPlan p = plan_bwd(q, space, fx, fw, s, true);
+  if (dtype == PDH_F32) return run_bwd<PDH_BF16, PDH_F32, true>(q, p, targets, lse, dloss, ignore_index, dx, dw, s);
+  if (dtype == PDH_BF16) return run_bwd<PDH_BF16, PDH_BF16, false>(q, p, targets, lse, dloss, ignore_index, dx, dw, s);
+  return run_bwd<PDH_F16, PDH_F16, false>(q, p, targets, lse, dloss, ignore_index, dx, dw, s);
+}

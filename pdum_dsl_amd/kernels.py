@@ -332,6 +332,90 @@ def dropout_bwd(
     return _dropout("dropout_bwd", dy, p, rng, site, None, out)
 
 
+@dataclass
+class LossOut:
+    loss: torch.Tensor
+    lse: torch.Tensor
+
+
+def _head(name, x, w, targets):
+    """The checked operands of a linear head's loss: x and w as rows, the targets flat."""
+    if x.dtype not in _DT or w.dtype != x.dtype:
+        raise ValueError(f"{name}: x and w share one element type of f32, bf16 or f16 (got {x.dtype}, {w.dtype})")
+    if x.dim() < 1 or w.dim() != 2 or w.shape[1] != x.shape[-1] or x.shape[-1] < 1 or w.shape[0] < 1:
+        raise ValueError(f"{name}: x [..., width] and w [vocab, width] (got {tuple(x.shape)}, {tuple(w.shape)})")
+    if targets.dtype != torch.int64 or targets.shape != x.shape[:-1]:
+        raise ValueError(f"{name}: targets must be int64 of x's leading shape {tuple(x.shape[:-1])}")
+    return _rows(x), _rows(w), targets.reshape(-1).contiguous()
+
+
+def linear_cross_entropy(
+    x: torch.Tensor,
+    w: torch.Tensor,
+    targets: torch.Tensor,
+    *,
+    ignore_index: int = -100,
+    bad: torch.Tensor | None = None,
+) -> LossOut:
+    """Each token's softmax cross entropy under the linear head w [vocab,
+    width] (logits x w^T), the logits never in memory: loss and lse (fp32, the
+    targets' shape). A target that is ``ignore_index`` or outside [0, vocab)
+    has loss 0; the latter also count in ``bad`` (an int32 device scalar) when
+    given. fp32, bf16 or f16 operands, fp32 accumulation."""
+    _one_device(x, w, targets, bad)
+    x2, w2, t = _head("linear_cross_entropy", x, w, targets)
+    if bad is not None and (bad.dtype != torch.int32 or bad.numel() < 1):
+        raise ValueError("linear_cross_entropy: bad is an int32 device scalar")
+    n, d, v = x2.shape[0], x2.shape[1], w2.shape[0]
+    out = torch.empty((2,) + tuple(targets.shape), dtype=torch.float32, device=x.device)
+    loss, lse = out.unbind(0)
+    if n:
+        args = (n, d, v, _ld(x2), _ld(w2))
+        need = _lib.lib().pdh_linear_xent_workspace(x2.data_ptr(), w2.data_ptr(), *args, _DT[x.dtype], 0)
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+        _lib.call(
+            "pdh_linear_xent_fwd",
+            x2.data_ptr(), w2.data_ptr(), t.data_ptr(), loss.data_ptr(), lse.data_ptr(), *args, int(ignore_index),
+            _DT[x.dtype], _ptr(bad), ws.data_ptr(), need, _stream(),
+        )
+    return LossOut(loss, lse)
+
+
+def linear_cross_entropy_bwd(
+    x: torch.Tensor,
+    w: torch.Tensor,
+    targets: torch.Tensor,
+    lse: torch.Tensor,
+    dloss: torch.Tensor,
+    *,
+    ignore_index: int = -100,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Gradients (dx, dw) of sum(dloss * loss) for :func:`linear_cross_entropy`
+    given its lse; ``dloss`` (fp32, the targets' shape) is each token's weight,
+    1 / live tokens for a mean. Of x's and w's element type, rounded once from
+    fp32 sums; deterministic."""
+    _one_device(x, w, targets, lse, dloss)
+    x2, w2, t = _head("linear_cross_entropy_bwd", x, w, targets)
+    for nm, s in (("lse", lse), ("dloss", dloss)):
+        if s.dtype != torch.float32 or s.shape != targets.shape:
+            raise ValueError(f"{nm} must be fp32 of the targets' shape")
+    n, d, v = x2.shape[0], x2.shape[1], w2.shape[0]
+    if n == 0:
+        return torch.empty_like(x), torch.zeros((v, d), dtype=w.dtype, device=w.device)
+    lse, dloss = lse.contiguous(), dloss.contiguous()
+    dx = torch.empty((n, d), dtype=x.dtype, device=x.device)
+    dw = torch.empty((v, d), dtype=w.dtype, device=w.device)
+    args = (n, d, v, _ld(x2), _ld(w2))
+    need = _lib.lib().pdh_linear_xent_workspace(x2.data_ptr(), w2.data_ptr(), *args, _DT[x.dtype], 1)
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+    _lib.call(
+        "pdh_linear_xent_bwd",
+        x2.data_ptr(), w2.data_ptr(), t.data_ptr(), lse.data_ptr(), dloss.data_ptr(), dx.data_ptr(), dw.data_ptr(), *args,
+        int(ignore_index), _DT[x.dtype], ws.data_ptr(), need, _stream(),
+    )
+    return dx.view(x.shape), dw
+
+
 def take_rows(table: torch.Tensor, idx: torch.Tensor, out: torch.Tensor | None = None,
               bad: torch.Tensor | None = None) -> torch.Tensor:
     """out[i, ...] = table[idx[i], ...]: a gather along the table's leading

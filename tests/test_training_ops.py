@@ -123,3 +123,33 @@ def test_cpu_tensors_are_refused():
     ):
         with pytest.raises((ValueError, RuntimeError, AssertionError)):
             call()
+
+
+def test_linear_xent_refusals():
+    from pdum_dsl_amd import _lib
+
+    lib = _lib.lib()
+
+    def fwd(n=4, d=8, v=16, ldx=8, ldw=8, dt=1, x=FAKE, ws=FAKE, nb=1 << 30):
+        return lib.pdh_linear_xent_fwd(x, FAKE, FAKE, FAKE, FAKE, n, d, v, ldx, ldw, -100, dt, None, ws, nb, None)
+
+    def bwd(n=4, d=8, v=16, ldx=8, ldw=8, dt=1, x=FAKE, ws=FAKE, nb=1 << 30):
+        return lib.pdh_linear_xent_bwd(x, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, n, d, v, ldx, ldw, -100, dt, ws, nb, None)
+
+    for f in (fwd, bwd):
+        _refused(f(d=0), "width >= 1")
+        _refused(f(v=0), "vocabulary >= 1")
+        _refused(f(n=-1), "tokens >= 0")
+        _refused(f(ldw=-8), "row strides")
+        _refused(f(x=None), "null pointer")
+        _refused(f(ws=None), "holds 0 bytes")
+        _refused(f(nb=16), "holds 16 bytes")
+        _refused(f(ws=C.c_void_p(8)), "16-byte aligned")
+        _refused(f(dt=9), "dtype 9", _lib.PDH_EUNSUPPORTED)
+        _refused(f(d=(1 << 18) + 1), "2^18 features", _lib.PDH_EUNSUPPORTED)
+        _refused(f(n=1 << 24, v=1 << 24), "2^38 logits", _lib.PDH_EUNSUPPORTED)
+    assert fwd(n=0) == _lib.PDH_OK
+    _refused(bwd(n=0), "no tokens")
+    need = lambda x, ldx, dt: lib.pdh_linear_xent_workspace(C.c_void_p(x), FAKE, 1000, 64, 5000, ldx, 64, dt, 1)  # noqa: E731
+    assert need(256, 64, 1) < need(258, 64, 1) == need(256, 65, 1) < need(256, 64, 0)  # packed where not read in place
+    assert lib.pdh_linear_xent_workspace(FAKE, FAKE, 0, 64, 5000, 64, 64, 1, 1) == 0
