@@ -12,11 +12,12 @@
 // piece's part of dx as two more products. dx's parts over slices of the
 // vocabulary are fp32 and added in order: no atomics, results repeat.
 //
-// All three products run one tile loop (xent_tile): 32-deep k tiles, three of
-// them in LDS by direct loads, v_mfma_f32_32x32x16, accumulators m along
-// registers and n along lanes. An operand is k-contiguous or has its rows (m or
-// n) contiguous, read transposed by ds_read_b64_tr_b16, so nothing is
-// transposed in memory. The m rows are dealt to the matrix instruction's rows
+// All three products run one tile loop (xent_tile): 256 x 128 tiles, four waves
+// of 128 x 64, v_mfma_f32_32x32x16, accumulators m along registers and n along
+// lanes; 64-deep k tiles by direct loads, whole 128-byte lines of a
+// k-contiguous operand. An operand is k-contiguous or has its rows (m or n)
+// contiguous, read transposed by ds_read_b64_tr_b16, so nothing is transposed
+// in memory. The m rows are dealt to the matrix instruction's rows
 // so that a lane's 16 accumulators are 16 consecutive m: whole vocabulary runs
 // for the softmax, 32 bytes of an output row for the stores.
 //
@@ -33,8 +34,7 @@
 namespace pdh {
 namespace {
 
-constexpr int kBK = 32;      // k depth of a tile
-constexpr int kStages = 3;   // k tiles in LDS
+constexpr int kBK = 64;  // k depth of a tile: a 128-byte line of a k-contiguous operand
 constexpr uint32_t kOOB = 0x80000000u;  // past every buffer's extent: reads as zero
 constexpr int kPairs = 6;    // fp32: products of bf16 terms (term of a, term of b), smallest first
 
@@ -74,60 +74,59 @@ __device__ __forceinline__ Tile tile_of(const TileArgs& a) {
   return t;
 }
 
-// Four waves, 2 x 2, each 32 TM (m) x 32 TN (n).
-template <int TM, int TN>
-struct Shape {
-  static constexpr int BM = 64 * TM, BN = 64 * TN;
-  static constexpr int LDS_A = BM * kBK * 2, LDS_B = BN * kBK * 2, STAGE = LDS_A + LDS_B;
-  static constexpr int LDS = kStages * STAGE;
+// A workgroup: WM x WN waves of 32 TM (m) x 32 TN (n). LDS holds two k tiles
+// of a and one of b: 80 KB for 256 x 128, two workgroups a compute unit.
+template <int WM_, int WN_, int TM_, int TN_>
+struct Config {
+  static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_;
+  static constexpr int NW = WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN, THREADS = 64 * NW;
+  static constexpr int LDS_A = BM * kBK * 2, LDS_B = BN * kBK * 2, LDS = 2 * LDS_A + LDS_B;
 };
 
-// One operand's side of the loop. R: its rows in the tile (BM or BN); KC:
-// k-contiguous; PERM: rows dealt as described above (the m side).
-template <int R, int T, bool KC, bool PERM>
+// One operand's side of the loop. R: its rows in the tile (BM or BN), T: a
+// wave's 32-row blocks; KC: k-contiguous; PERM: rows dealt as described above (the m side).
+template <int R, int T, int NW, bool KC, bool PERM>
 struct Side {
-  static constexpr int BLOCKS = R * kBK * 2 / 1024 / 4;  // direct loads (1 KB) per wave and k tile
-  static constexpr int PITCH = R * 2;                    // LDS bytes of a k row (rows contiguous)
-  static constexpr int SLOTS = R / 8, KROWS = 64 / SLOTS;  // its 16-byte slots; k rows a direct load covers
+  static constexpr int BLOCKS = R * kBK * 2 / 1024 / NW;  // direct loads (1 KB) per wave and k tile
+  static constexpr int KS = kBK / 16;                     // products deep
+  static constexpr int PITCH = KC ? kBK * 2 : R * 2;      // LDS bytes of a row (rows contiguous: of a k row)
+  static constexpr int SLOTS = PITCH / 16, ROWS = 64 / SLOTS;  // its 16-byte slots; rows a direct load covers
+  static_assert(BLOCKS * 1024 * NW == R * kBK * 2 && NW % 4 == 0, "whole direct loads");
   uint32_t voff, vtail;  // the lane's byte offset in a direct load; the same in a ragged last k tile
   uint32_t pitch;
-  int read[T][2];        // LDS offsets of the lane's fragments (without the tr read's second half)
+  int read[T][KS];       // LDS offsets of the lane's fragments (without the tr read's second half)
 
   // 16-byte slots are XOR-swizzled so that neither the b128 reads (16 lanes a cycle, the
   // quads of one parity in each half wave) nor the tr reads (32 lanes) meet a bank twice.
-  __device__ __forceinline__ static int swz(int krow) { return R >= 128 ? 4 * (krow & 3) : 4 * ((krow >> 1) & 1); }
+  __device__ __forceinline__ static int swz(int row) {
+    if constexpr (KC) return (row & 7) ^ ((row >> 3) & 1);
+    return R >= 128 ? 4 * (row & 3) : 4 * ((row >> 1) & 1);
+  }
 
   __device__ __forceinline__ Side(const Operand& o, int wq, int lane, int w, int ktail) {
     pitch = static_cast<uint32_t>(o.pitch);
-    if constexpr (KC) {  // 16 rows of four 16-byte chunks a direct load
-      const int row = lane >> 2, chunk = (lane & 3) ^ ((row >> 2) & 3);
-      voff = row * pitch + (chunk << 4);
-      vtail = 8 * chunk < ktail ? voff : kOOB;
+    // this wave's direct loads are w, w + NW, ...: their rows agree as far as swz looks
+    const int row = lane / SLOTS, chunk = (lane % SLOTS) ^ swz(ROWS * w + row);
+    voff = row * pitch + (chunk << 4);
+    vtail = !KC || 8 * chunk < ktail ? voff : kOOB;  // (k rows past the end lie past the extent)
 #pragma unroll
-      for (int t = 0; t < T; ++t)
+    for (int t = 0; t < T; ++t)
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
+      for (int ks = 0; ks < KS; ++ks) {
+        if constexpr (KC) {
           const int r = lane & 31, g = lane >> 5;
-          const int row_ = 32 * (wq * T + t) + (PERM ? 16 * ((r >> 2) & 1) + 4 * (r >> 3) + (r & 3) : r);
-          read[t][ks] = row_ * (kBK * 2) + (((2 * ks + g) ^ ((row_ >> 2) & 3)) << 4);
-        }
-    } else {
-      const int kr = lane / SLOTS, in_tile = (KROWS * w + kr);  // blocks are w, w + 4, ...: k rows equal mod 4
-      voff = kr * pitch + (((lane % SLOTS) ^ swz(in_tile)) << 4);
-      vtail = voff;  // k rows past the end lie past the extent
-#pragma unroll
-      for (int t = 0; t < T; ++t)
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
+          const int at = 32 * (wq * T + t) + (PERM ? 16 * ((r >> 2) & 1) + 4 * (r >> 3) + (r & 3) : r);
+          read[t][ks] = at * PITCH + (((2 * ks + g) ^ swz(at)) << 4);
+        } else {
           const int G = lane >> 4, i4 = (lane >> 2) & 3, q = 4 * (G & 1) + (lane & 3);
-          const int kr_ = 16 * ks + 8 * (G >> 1) + i4;
+          const int kr = 16 * ks + 8 * (G >> 1) + i4;
           const int col = 32 * (wq * T + t) + (PERM ? 16 * (q & 1) + 4 * (q >> 1) : 4 * q);
-          read[t][ks] = kr_ * PITCH + (((col >> 3) ^ swz(kr_)) << 4) + ((col >> 2) & 1) * 8;
+          read[t][ks] = kr * PITCH + (((col >> 3) ^ swz(kr)) << 4) + ((col >> 2) & 1) * 8;
         }
-    }
+      }
   }
 
-  // Direct loads of k columns k0 .. k0 + 31 of rows r0 .. r0 + R - 1 (`rows` of them in the operand, `k` columns).
+  // Direct loads of k columns k0 .. k0 + 63 of rows r0 .. r0 + R - 1 (`rows` of them in the operand, `k` columns).
   __device__ __forceinline__ void fetch(const Operand& o, int64_t plane, int64_t r0, int rows, int64_t k0, int64_t k,
                                         uint32_t lds, int w) const {
     const char* base;
@@ -145,8 +144,8 @@ struct Side {
     const uint32_t v = last ? vtail : voff;
 #pragma unroll
     for (int i = 0; i < BLOCKS; ++i) {
-      const int blk = 4 * i + w;
-      dma16_at(rs, lds + blk * 1024, v, static_cast<uint32_t>(KC ? 16 * blk : KROWS * blk) * pitch);
+      const int blk = NW * i + w;
+      dma16_at(rs, lds + blk * 1024, v, static_cast<uint32_t>(ROWS * blk) * pitch);
     }
   }
 
@@ -163,17 +162,23 @@ struct Side {
 // acc = the products of a tile over k columns [k0, k1): accumulator i of
 // (tm, tn) is m = m0 + 32 (wm TM + tm) + 16 (lane / 32) + i, n = n0 + 32 (wn TN + tn) + lane % 32.
 // SPLIT: the operands are planes of bf16 terms, every k tile runs kPairs times.
-// Per k tile a wave loads TM + TN direct kilobytes, reads as many operand
-// fragments twice and issues 2 TM TN products.
-template <int DT, int TM, int TN, bool KA, bool KB, bool SPLIT>
-__device__ __forceinline__ void xent_tile(const TileArgs& a, unsigned char* smem, f32x16 (&acc)[TM][TN], int m0, int n0,
-                                          int64_t k0, int64_t k1) {
-  using S = Shape<TM, TN>;
-  const int lane = threadIdx.x & 63, w = wave_id(), wm = w >> 1, wn = w & 1;
+//
+// A k tile's b fragments go to registers first, so b needs one buffer: a
+// second barrier frees it for the next tile's loads, which, with a's, are in
+// flight under this tile's products. 64-deep tiles in two such workgroups a
+// compute unit against 32-deep ones three deep in LDS: a k-contiguous operand's
+// 64-byte rows cost every line two requests (fwd 8192 x 768 x 50257: 630 us,
+// this 544; 4096 x 4096: 1640, 1420, the matrix pipe 66% busy at the 1.62 GHz
+// that the part then holds); 256 x 256 tiles of eight waves, one workgroup a
+// unit: 610, 1450; fragments read a step ahead across the barrier: no change.
+template <int DT, typename C, bool KA, bool KB, bool SPLIT>
+__device__ __forceinline__ void xent_tile(const TileArgs& a, unsigned char* smem, f32x16 (&acc)[C::TM][C::TN], int m0,
+                                          int n0, int64_t k0, int64_t k1) {
+  constexpr int TM = C::TM, TN = C::TN, KS = kBK / 16;
+  const int lane = threadIdx.x & 63, w = wave_id(), wm = w / C::WN, wn = w % C::WN;
   const int ktail = static_cast<int>((k1 - k0) % kBK);
-  const Side<S::BM, TM, KA, true> sa(a.a, wm, lane, w, ktail);
-  const Side<S::BN, TN, KB, false> sb(a.b, wn, lane, w, ktail);
-  constexpr int PER = decltype(sa)::BLOCKS + decltype(sb)::BLOCKS;
+  const Side<C::BM, TM, C::NW, KA, true> sa(a.a, wm, lane, w, ktail);
+  const Side<C::BN, TN, C::NW, KB, false> sb(a.b, wn, lane, w, ktail);
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -181,47 +186,51 @@ __device__ __forceinline__ void xent_tile(const TileArgs& a, unsigned char* smem
   const int nkt = static_cast<int>((k1 - k0 + kBK - 1) / kBK);
   const int steps = SPLIT ? nkt * kPairs : nkt;
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(smem));
-  int fpair = 0, fkt = 0, fbuf = 0;  // the next k tile to fetch
-  auto fetch = [&]() __attribute__((always_inline)) {
+  unsigned char* const bt = smem + 2 * C::LDS_A;
+  int fpair = 0, fkt = 0;  // the k tile to fetch
+  auto fetch_a = [&](int buf) __attribute__((always_inline)) {
     // pairs in order of growing size: terms (0, 2) (2, 0) (1, 1) (0, 1) (1, 0) (0, 0), two bits each
-    const int64_t pa = SPLIT ? (0x0118 >> (2 * fpair)) & 3 : 0, pb = SPLIT ? (0x0052 >> (2 * fpair)) & 3 : 0;
-    const int64_t kk = k0 + static_cast<int64_t>(fkt) * kBK;
-    const uint32_t lds = lds0 + fbuf * S::STAGE;
-    sa.fetch(a.a, pa, m0, a.m, kk, k1, lds, w);
-    sb.fetch(a.b, pb, n0, a.n, kk, k1, lds + S::LDS_A, w);
-    fbuf = fbuf + 1 == kStages ? 0 : fbuf + 1;
+    const int64_t pa = SPLIT ? (0x0118 >> (2 * fpair)) & 3 : 0;
+    sa.fetch(a.a, pa, m0, a.m, k0 + static_cast<int64_t>(fkt) * kBK, k1, lds0 + buf * C::LDS_A, w);
+  };
+  auto fetch_b = [&]() __attribute__((always_inline)) {
+    const int64_t pb = SPLIT ? (0x0052 >> (2 * fpair)) & 3 : 0;
+    sb.fetch(a.b, pb, n0, a.n, k0 + static_cast<int64_t>(fkt) * kBK, k1, lds0 + 2 * C::LDS_A, w);
     if (++fkt == nkt) fkt = 0, ++fpair;
   };
-#pragma unroll
-  for (int s = 0; s < kStages - 1; ++s)
-    if (s < steps) fetch();
-  int buf = 0;
-  for (int st = 0; st < steps; ++st, buf = buf + 1 == kStages ? 0 : buf + 1) {
-    // the tile has landed when at most the next one's loads are outstanding
-    if (st + 1 < steps)
-      __builtin_amdgcn_s_waitcnt(0x0f70 | (PER & 15) | ((PER >> 4) << 14));
-    else
-      wait_vmcnt0();
+  fetch_a(0);
+  fetch_b();
+  for (int st = 0; st < steps; ++st) {
+    const bool more = st + 1 < steps;
+    wait_vmcnt0();
     __syncthreads();  // every wave's loads of this tile are done; everyone has finished the tile before
-    if (st + kStages - 1 < steps) fetch();
-    const unsigned char* at = smem + buf * S::STAGE;
-    const unsigned char* bt = at + S::LDS_A;
-    u32x4 af[2][TM], bf[2][TN];
+    const unsigned char* at = smem + (st & 1) * C::LDS_A;
+    u32x4 af[2][TM], bf[KS][TN];
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-#pragma unroll
-      for (int t = 0; t < TM; ++t) af[ks][t] = sa.frag(at, t, ks);
+    for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
       for (int t = 0; t < TN; ++t) bf[ks][t] = sb.frag(bt, t, ks);
-    }
-    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
+    for (int t = 0; t < TM; ++t) af[0][t] = sa.frag(at, t, 0);
+    if (more) fetch_a((st + 1) & 1);
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): b's fragments are in registers
+    __syncthreads();
+    if (more) fetch_b();
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      if (ks + 1 < KS) {
+#pragma unroll
+        for (int t = 0; t < TM; ++t) af[(ks + 1) & 1][t] = sa.frag(at, t, ks + 1);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = mfma32_dt<DT>(af[ks][i], bf[ks][j], acc[i][j]);
-    __builtin_amdgcn_s_setprio(0);
+        for (int j = 0; j < TN; ++j) acc[i][j] = mfma32_dt<DT>(af[ks & 1][i], bf[ks][j], acc[i][j]);
+      __builtin_amdgcn_s_setprio(0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   }
 }
 
@@ -234,18 +243,18 @@ struct FwdArgs {
   float* zt;     // [tokens]: the target's logit
 };
 
-template <int DT, int TM, int TN, bool SPLIT>
-__global__ __launch_bounds__(256, 2) void xent_fwd(FwdArgs p) {
-  using S = Shape<TM, TN>;
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[S::LDS];
+template <int DT, typename C, bool SPLIT>
+__global__ __launch_bounds__(C::THREADS, 2) void xent_fwd(FwdArgs p) {
+  constexpr int TM = C::TM, TN = C::TN;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[C::LDS];
   const Tile t = tile_of(p.t);
   if (!t.live) return;
-  const int m0 = t.m * S::BM, n0 = t.n * S::BN;
-  const int lane = threadIdx.x & 63, w = wave_id(), wm = w >> 1, wn = w & 1, g = lane >> 5;
+  const int m0 = t.m * C::BM, n0 = t.n * C::BN;
+  const int lane = threadIdx.x & 63, w = wave_id(), wm = w / C::WN, wn = w % C::WN, g = lane >> 5;
   f32x16 acc[TM][TN];
-  xent_tile<DT, TM, TN, true, true, SPLIT>(p.t, smem, acc, m0, n0, 0, p.t.k);
+  xent_tile<DT, C, true, true, SPLIT>(p.t, smem, acc, m0, n0, 0, p.t.k);
   const int vw = m0 + 32 * wm * TM, v0 = vw + 16 * g;  // the wave's strip, the lane's first entry of it
-  const int strip = 2 * t.m + wm;
+  const int strip = C::WM * t.m + wm;
 #pragma unroll
   for (int j = 0; j < TN; ++j) {
     const int n = n0 + 32 * (wn * TN + j) + (lane & 31);
@@ -328,16 +337,16 @@ struct GradArgs {
 };
 
 // dz of a piece: a: w from the piece's first row (m: its entries), b: x.
-template <int DT, int TM, int TN, bool SPLIT>
-__global__ __launch_bounds__(256, 2) void xent_dz(GradArgs p) {
-  using S = Shape<TM, TN>;
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[S::LDS];
+template <int DT, typename C, bool SPLIT>
+__global__ __launch_bounds__(C::THREADS, 2) void xent_dz(GradArgs p) {
+  constexpr int TM = C::TM, TN = C::TN;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[C::LDS];
   const Tile t = tile_of(p.t);
   if (!t.live) return;
-  const int m0 = t.m * S::BM, n0 = t.n * S::BN;
-  const int lane = threadIdx.x & 63, w = wave_id(), wm = w >> 1, wn = w & 1, g = lane >> 5;
+  const int m0 = t.m * C::BM, n0 = t.n * C::BN;
+  const int lane = threadIdx.x & 63, w = wave_id(), wm = w / C::WN, wn = w % C::WN, g = lane >> 5;
   f32x16 acc[TM][TN];
-  xent_tile<DT, TM, TN, true, true, SPLIT>(p.t, smem, acc, m0, n0, 0, p.t.k);
+  xent_tile<DT, C, true, true, SPLIT>(p.t, smem, acc, m0, n0, 0, p.t.k);
   const int c0 = m0 + 32 * wm * TM + 16 * g;  // the lane's first column of dz
 #pragma unroll
   for (int j = 0; j < TN; ++j) {
@@ -400,18 +409,18 @@ struct ProdArgs {
   int add;             // add to what out holds (the parts of an earlier piece)
 };
 
-template <int DT, int ODT, int TM, int TN, bool KB, bool SPLIT>
-__global__ __launch_bounds__(256, 2) void xent_prod(ProdArgs p) {
-  using S = Shape<TM, TN>;
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[S::LDS];
+template <int DT, int ODT, typename C, bool KB, bool SPLIT>
+__global__ __launch_bounds__(C::THREADS, 2) void xent_prod(ProdArgs p) {
+  constexpr int TM = C::TM, TN = C::TN;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[C::LDS];
   const Tile t = tile_of(p.t);
   if (!t.live) return;
-  const int m0 = t.m * S::BM, n0 = t.n * S::BN;
-  const int lane = threadIdx.x & 63, w = wave_id(), wm = w >> 1, wn = w & 1, g = lane >> 5;
+  const int m0 = t.m * C::BM, n0 = t.n * C::BN;
+  const int lane = threadIdx.x & 63, w = wave_id(), wm = w / C::WN, wn = w % C::WN, g = lane >> 5;
   f32x16 acc[TM][TN];
   const int64_t k0 = static_cast<int64_t>(t.slice) * p.t.kslice;
   const int64_t k1 = k0 + p.t.kslice < p.t.k ? k0 + p.t.kslice : p.t.k;
-  xent_tile<DT, TM, TN, false, KB, SPLIT>(p.t, smem, acc, m0, n0, k0, k1);
+  xent_tile<DT, C, false, KB, SPLIT>(p.t, smem, acc, m0, n0, k0, k1);
   const float sc = p.scale ? *p.scale : 1.f;
   constexpr int ES = ODT == PDH_F32 ? 4 : 2;
 #pragma unroll
@@ -594,14 +603,13 @@ Operand place(const void* p, int64_t ld, int64_t rows, const Problem& q, Space& 
   return Operand{reinterpret_cast<const char*>(dst), dp * 2, plane * 2};
 }
 
-template <int TM, int TN>
+template <typename C>
 TileArgs tiles(Operand a, Operand b, int64_t m, int64_t n, int64_t k, int64_t kslice) {
-  using S = Shape<TM, TN>;
   TileArgs t{};
   t.a = a, t.b = b;
   t.m = static_cast<int>(m), t.n = static_cast<int>(n), t.k = static_cast<int>(k);
-  t.tiles_m = static_cast<int>((m + S::BM - 1) / S::BM);
-  t.tiles_n = static_cast<int>((n + S::BN - 1) / S::BN);
+  t.tiles_m = static_cast<int>((m + C::BM - 1) / C::BM);
+  t.tiles_n = static_cast<int>((n + C::BN - 1) / C::BN);
   t.kslice = static_cast<int>(kslice);
   t.slices = static_cast<int>((k + kslice - 1) / kslice);
   t.group = t.tiles_n < 8 ? t.tiles_n : 8;
@@ -611,7 +619,7 @@ dim3 grid_of(const TileArgs& t) {
   return dim3(static_cast<unsigned>((static_cast<int64_t>(t.tiles_m) * t.tiles_n * t.slices + 7) / 8 * 8));
 }
 
-constexpr int TM = 4, TN = 2;  // 256 x 128 tiles
+using Big = Config<2, 2, 4, 2>;  // 256 x 128 tiles
 
 int check(const char* fn, int64_t n, int64_t d, int64_t v, int64_t ldx, int64_t ldw, int dtype) {
   PDH_REQUIRE(dtype == PDH_F32 || dtype == PDH_BF16 || dtype == PDH_F16, PDH_EUNSUPPORTED, "%s: dtype %d", fn, dtype);
@@ -638,8 +646,8 @@ FwdPlan plan_fwd(const Problem& q, Space& ws, bool fit_x, bool fit_w, hipStream_
   FwdPlan p{};
   p.w = place(q.w, q.ldw, q.v, q, ws, fit_w, s, launch);
   p.x = place(q.x, q.ldx, q.n, q, ws, fit_x, s, launch);
-  p.t = tiles<TM, TN>(p.w, p.x, q.v, q.n, q.dp(), up(q.dp(), kBK));
-  p.strips = 2 * p.t.tiles_m;
+  p.t = tiles<Big>(p.w, p.x, q.v, q.n, q.dp(), up(q.dp(), kBK));
+  p.strips = Big::WM * p.t.tiles_m;
   p.part = static_cast<float2*>(ws.take(static_cast<int64_t>(p.strips) * q.n * 8));
   p.zt = static_cast<float*>(ws.take(q.n * 4));
   return p;
@@ -678,7 +686,7 @@ BwdPlan plan_bwd(const Problem& q, Space& ws, bool fit_x, bool fit_w, hipStream_
 template <int DT, bool SPLIT>
 int run_fwd(const Problem& q, const FwdPlan& p, const int64_t* targets, int64_t ignore, float* loss, float* lse, int* bad,
             hipStream_t s) {
-  xent_fwd<DT, TM, TN, SPLIT><<<grid_of(p.t), 256, 0, s>>>(FwdArgs{p.t, targets, p.part, p.zt});
+  xent_fwd<DT, Big, SPLIT><<<grid_of(p.t), Big::THREADS, 0, s>>>(FwdArgs{p.t, targets, p.part, p.zt});
   if (int rc = check_launch("pdh_linear_xent_fwd"); rc != PDH_OK) return rc;
   xent_join<<<dim3(static_cast<unsigned>((q.n + 7) / 8)), 256, 0, s>>>(p.part, p.zt, targets, p.strips, q.n, q.v, ignore,
                                                                        loss, lse, bad);
@@ -700,12 +708,12 @@ int run_bwd(const Problem& q, const BwdPlan& p, const int64_t* targets, const fl
     const int64_t nv = std::min(p.piece, q.v - v0), ldz = up(nv, 256);
     const Operand wv{p.w.p + v0 * p.w.pitch, p.w.pitch, p.w.plane};
     const Operand dz{reinterpret_cast<const char*>(p.dz), ldz * 2, q.n * ldz * 2};
-    GradArgs ga{tiles<TM, TN>(wv, p.x, nv, q.n, dp, up(dp, kBK)), targets, lse, g, p.dz, ldz, q.n * ldz, v0, q.v, ignore};
-    xent_dz<DT, TM, TN, SPLIT><<<grid_of(ga.t), 256, 0, s>>>(ga);
-    ProdArgs pw{tiles<TM, TN>(p.x, dz, q.d, nv, q.n, up(q.n, kBK)), static_cast<char*>(dw) + v0 * q.d * es, q.d, 0, scale, 0};
-    xent_prod<DT, ODT, TM, TN, false, SPLIT><<<grid_of(pw.t), 256, 0, s>>>(pw);
-    ProdArgs px{tiles<TM, TN>(wv, dz, q.d, q.n, nv, p.kslice), p.parts, dp, slice, nullptr, v0 > 0};
-    xent_prod<DT, PDH_F32, TM, TN, true, SPLIT><<<grid_of(px.t), 256, 0, s>>>(px);
+    GradArgs ga{tiles<Big>(wv, p.x, nv, q.n, dp, up(dp, kBK)), targets, lse, g, p.dz, ldz, q.n * ldz, v0, q.v, ignore};
+    xent_dz<DT, Big, SPLIT><<<grid_of(ga.t), Big::THREADS, 0, s>>>(ga);
+    ProdArgs pw{tiles<Big>(p.x, dz, q.d, nv, q.n, up(q.n, kBK)), static_cast<char*>(dw) + v0 * q.d * es, q.d, 0, scale, 0};
+    xent_prod<DT, ODT, Big, false, SPLIT><<<grid_of(pw.t), Big::THREADS, 0, s>>>(pw);
+    ProdArgs px{tiles<Big>(wv, dz, q.d, q.n, nv, p.kslice), p.parts, dp, slice, nullptr, v0 > 0};
+    xent_prod<DT, PDH_F32, Big, true, SPLIT><<<grid_of(px.t), Big::THREADS, 0, s>>>(px);
     if (int rc = check_launch("pdh_linear_xent_bwd"); rc != PDH_OK) return rc;
   }
   xent_dx<ODT><<<dim3(blocks_for(q.n * (dp / 4))), 256, 0, s>>>(p.parts, dx, q.n, static_cast<int>(q.d), dp, slice,

@@ -9,11 +9,13 @@ import pytest
 
 from tests.test_lds_layout import _ways
 
-BK, OOB = 32, 1 << 31
+BK, OOB = 64, 1 << 31
 
 
-def _swz(R, krow):
-    return 4 * (krow & 3) if R >= 128 else 4 * ((krow >> 1) & 1)
+def _swz(R, kc, row):
+    if kc:
+        return (row & 7) ^ ((row >> 3) & 1)
+    return 4 * (row & 3) if R >= 128 else 4 * ((row >> 1) & 1)
 
 
 def _fill(R, kc, rows, k, k0, k1, pitch):
@@ -23,22 +25,17 @@ def _fill(R, kc, rows, k, k0, k1, pitch):
     ext = (nr - 1) * pitch + ((nk * 2 + 15) & ~15) if kc else (nk - 1) * pitch + ((nr * 2 + 15) & ~15)
     ktail = (k1 - k0) % BK
     lds = {}
-    slots = R // 8
-    krows = 64 // slots
+    slots = BK * 2 // 16 if kc else R // 8
+    nrows = 64 // slots
     for w, i in itertools.product(range(4), range(R * BK * 2 // 1024 // 4)):
         blk = 4 * i + w
         for lane in range(64):
-            if kc:
-                row = lane >> 2
-                chunk = (lane & 3) ^ ((row >> 2) & 3)
-                voff = row * pitch + 16 * chunk
-                if last and not 8 * chunk < ktail:
-                    voff = OOB
-                soff = 16 * blk * pitch
-            else:
-                kr = lane // slots
-                voff = kr * pitch + (((lane % slots) ^ _swz(R, krows * w + kr)) << 4)
-                soff = krows * blk * pitch
+            row = lane // slots
+            chunk = (lane % slots) ^ _swz(R, kc, nrows * w + row)
+            voff = row * pitch + 16 * chunk
+            if kc and last and not 8 * chunk < ktail:
+                voff = OOB
+            soff = nrows * blk * pitch
             for b in range(0, 16, 2):
                 at = voff + soff + b
                 assert blk * 1024 + lane * 16 + b not in lds
@@ -63,13 +60,13 @@ def _reads(R, T, kc, perm, wq, t, ks):
         if kc:
             r, g = lane & 31, lane >> 5
             row = 32 * (wq * T + t) + (_perm(r) if perm else r)
-            out.append(row * BK * 2 + (((2 * ks + g) ^ ((row >> 2) & 3)) << 4))
+            out.append(row * BK * 2 + (((2 * ks + g) ^ _swz(R, kc, row)) << 4))
         else:
             G, i4 = lane >> 4, (lane >> 2) & 3
             q = 4 * (G & 1) + (lane & 3)
             kr = 16 * ks + 8 * (G >> 1) + i4
             col = 32 * (wq * T + t) + (16 * (q & 1) + 4 * (q >> 1) if perm else 4 * q)
-            out.append(kr * R * 2 + (((col >> 3) ^ _swz(R, kr)) << 4) + ((col >> 2) & 1) * 8)
+            out.append(kr * R * 2 + (((col >> 3) ^ _swz(R, kc, kr)) << 4) + ((col >> 2) & 1) * 8)
     return out
 
 
@@ -96,11 +93,11 @@ def test_fragments_hold_the_rows_and_columns_the_epilogues_assume(R, T, kc, perm
     waves = R // (32 * T)
     if waves < 1:
         pytest.skip("no wave of this shape")
-    for rows, k0, k1 in ((R, 0, 64), (R - 57, 32, 64), (3, 64, 81), (R, 0, 8), (R + 40, 96, 97)):
+    for rows, k0, k1 in ((R, 0, 128), (R - 57, 64, 128), (3, 64, 81), (R, 0, 8), (R + 40, 64, 121)):
         # a k-contiguous operand's rows and a rows-contiguous one's k rows are whole 16-byte chunks of zeros past the end
         pitch = (max(k1, 128) if kc else ((rows + 7) & ~7)) * 2
         lds = _fill(R, kc, rows, 128, k0, k1, pitch)
-        for wq, t, ks in itertools.product(range(waves), range(T), range(2)):
+        for wq, t, ks in itertools.product(range(waves), range(T), range(BK // 16)):
             got = _fragment(lds, R, T, kc, perm, wq, t, ks)
             for lane in range(64):
                 r, g = lane & 31, lane >> 5
@@ -118,7 +115,7 @@ def test_fragments_hold_the_rows_and_columns_the_epilogues_assume(R, T, kc, perm
 @pytest.mark.parametrize("perm", [True, False])
 def test_no_read_meets_a_bank_twice(R, T, perm):
     for kc, width in ((True, 16), (False, 8)):
-        for wq, t, ks in itertools.product(range(R // (32 * T)), range(T), range(2)):
+        for wq, t, ks in itertools.product(range(R // (32 * T)), range(T), range(BK // 16)):
             assert _ways(_reads(R, T, kc, perm, wq, t, ks), width) == 1
 
 
