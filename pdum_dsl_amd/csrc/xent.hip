@@ -54,17 +54,27 @@ struct TileArgs {
   int group;    // n tiles that neighbouring workgroups share an m tile across
 };
 
-// The tile of workgroup `bid`: each XCD (bid % 8) takes a contiguous run of
-// tiles, ordered so that 8 x 8 neighbours share operand panels in its L2.
+// Two runs of workgroups in one launch: `first` ids, then `second`. Workgroups
+// go to the XCDs in turn (blockIdx % 8); each XCD takes a contiguous eighth of
+// either run, so that its neighbours share operand panels in its L2. Returns
+// the id in its run, or -1 for a workgroup past its end.
+__device__ __forceinline__ int run_id(uint32_t first, uint32_t second, bool& in_second) {
+  const uint32_t xcd = blockIdx.x & 7, pos = blockIdx.x >> 3, c1 = (first + 7) / 8, c2 = (second + 7) / 8;
+  in_second = pos >= c1;
+  const uint32_t id = in_second ? xcd * c2 + (pos - c1) : xcd * c1 + pos;
+  return (in_second ? pos - c1 < c2 && id < second : id < first) ? static_cast<int>(id) : -1;
+}
+dim3 run_grid(int64_t first, int64_t second) {
+  return dim3(static_cast<unsigned>(((first + 7) / 8 + (second + 7) / 8) * 8));
+}
+
+// Tile `id`: slices outermost, then groups of n tiles, m, the group's n tiles.
 struct Tile {
   int m, n, slice;
-  bool live;
 };
-__device__ __forceinline__ Tile tile_of(const TileArgs& a) {
-  const uint32_t per = static_cast<uint32_t>(a.tiles_m) * a.tiles_n, total = per * a.slices;
-  const uint32_t chunk = (total + 7) / 8, pos = blockIdx.x >> 3;
-  uint32_t id = (blockIdx.x & 7) * chunk + pos;
-  Tile t{0, 0, 0, pos < chunk && id < total};
+__device__ __forceinline__ Tile tile_of(const TileArgs& a, uint32_t id) {
+  const uint32_t per = static_cast<uint32_t>(a.tiles_m) * a.tiles_n;
+  Tile t;
   t.slice = static_cast<int>(id / per);
   id -= t.slice * per;
   const uint32_t gsize = static_cast<uint32_t>(a.group) * a.tiles_m, g = id / gsize, rem = id - g * gsize;
@@ -234,38 +244,127 @@ __device__ __forceinline__ void xent_tile(const TileArgs& a, unsigned char* smem
   }
 }
 
+// Stores a wave's 32 n rows (n tile j) of its 32 TM m columns, ES bytes each:
+// every lane has a row's 16-column runs (`v`: as stored), which would make
+// stores of 16 bytes in 64 places; through the wave's own part of LDS each
+// instruction stores whole lines instead. `left` columns are inside the output,
+// `rows` of the rows. add: fp32 only, to what is there. The caller has passed a
+// barrier since the tile loop.
+template <int ES, int TM>
+constexpr int put_pitch() {
+  return TM * 32 * ES + 16;  // 16 bytes on: rows start at different banks
+}
+template <int ES, int TM>
+__device__ __forceinline__ void put_rows(unsigned char* lds, const u32x4 (&v)[TM][ES], char* out, int64_t ld_b, int rows,
+                                         int left, bool add) {
+  constexpr int P = put_pitch<ES, TM>(), CH = TM * 32 * ES / 16, VE = 16 / ES;
+  const int lane = threadIdx.x & 63;
+  unsigned char* mine = lds + (lane & 31) * P + (lane >> 5) * 16 * ES;
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int q = 0; q < ES; ++q) *reinterpret_cast<u32x4*>(mine + i * 32 * ES + q * 16) = v[i][q];
+  __builtin_amdgcn_wave_barrier();  // the wave's own rows: LDS keeps its order, no workgroup barrier
+#pragma unroll
+  for (int it = 0; it < 32 * CH / 64; ++it) {
+    const int idx = it * 64 + lane, row = idx / CH, ch = idx % CH;
+    const u32x4 w = *reinterpret_cast<const u32x4*>(lds + row * P + ch * 16);
+    char* o = out + row * ld_b + ch * 16;
+    if (row >= rows) continue;
+    if ((ch + 1) * VE <= left) {
+      if constexpr (ES == 4) {
+        f32x4 x = __builtin_bit_cast(f32x4, w);
+        if (add) x += *reinterpret_cast<const f32x4u*>(o);
+        *reinterpret_cast<f32x4u*>(o) = x;
+      } else {
+        *reinterpret_cast<u32x4h*>(o) = w;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < VE - 1; ++e)
+        if (ch * VE + e < left) {
+          if constexpr (ES == 4) {
+            float* f = reinterpret_cast<float*>(o) + e;
+            *f = add ? *f + __uint_as_float(w[e]) : __uint_as_float(w[e]);
+          } else {
+            reinterpret_cast<uint16_t*>(o)[e] = static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)));
+          }
+        }
+    }
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ u32x4 pack8(const float* q) {
+  u32x4 w;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    w[e] = DT == PDH_BF16 ? pack2<__hip_bfloat16>(q[2 * e], q[2 * e + 1]) : pack2<_Float16>(q[2 * e], q[2 * e + 1]);
+  return w;
+}
+
+using Big = Config<2, 2, 4, 2>;    // 256 x 128 tiles
+using Small = Config<2, 2, 2, 1>;  // 128 x 64: a quarter of one
+constexpr int kStrip = 128;        // vocabulary entries of a forward's strip
+
+// The logits' tiles, [0, big) whole and the rest quartered (`small` of them),
+// so that the last round of workgroups is a short one.
+struct LogitTiles {
+  TileArgs t;  // a: w (m: vocabulary), b: x (n: tokens)
+  int big, small;
+};
+template <typename F, typename G>
+__device__ __forceinline__ void logit_tile(const LogitTiles& l, F&& whole, G&& quarter) {
+  bool second;
+  const int id = run_id(l.big, l.small, second);
+  if (id < 0) return;
+  const Tile t = tile_of(l.t, second ? l.big + id / 4 : id);
+  const int m0 = t.m * Big::BM, n0 = t.n * Big::BN;
+  if (!second) {
+    whole(m0, n0);
+  } else {
+    const int mq = m0 + (id & 1) * Small::BM, nq = n0 + ((id >> 1) & 1) * Small::BN;
+    if (mq < l.t.m && nq < l.t.n) quarter(mq, nq);
+  }
+}
+
 // ---------------------------------------------------------------- forward
 
 struct FwdArgs {
-  TileArgs t;  // a: w (m: vocabulary), b: x (n: tokens)
+  LogitTiles l;
   const int64_t* targets;
-  float2* part;  // [strips][tokens]: (max, sum of exp(z - max)) of 32 TM vocabulary entries
+  float2* part;  // [strips][tokens]: (max, sum of exp(z - max)) of kStrip vocabulary entries
   float* zt;     // [tokens]: the target's logit
 };
 
+// Joins (m, s) and (om, os), sums of exponentials below their maxima.
+__device__ __forceinline__ void join(float& m, float& s, float om, float os) {
+  const float mn = nan_max(m, om);
+  const float b = mn == -__builtin_inff() ? 0.f : mn;  // nothing but -inf so far sums to 0, not NaN
+  s = s * fast_exp2((m - b) * kLog2e) + os * fast_exp2((om - b) * kLog2e);
+  m = mn;
+}
+
 template <int DT, typename C, bool SPLIT>
-__global__ __launch_bounds__(C::THREADS, 2) void xent_fwd(FwdArgs p) {
+__device__ __forceinline__ void fwd_tile(const FwdArgs& p, unsigned char* smem, int m0, int n0) {
   constexpr int TM = C::TM, TN = C::TN;
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[C::LDS];
-  const Tile t = tile_of(p.t);
-  if (!t.live) return;
-  const int m0 = t.m * C::BM, n0 = t.n * C::BN;
   const int lane = threadIdx.x & 63, w = wave_id(), wm = w / C::WN, wn = w % C::WN, g = lane >> 5;
   f32x16 acc[TM][TN];
-  xent_tile<DT, C, true, true, SPLIT>(p.t, smem, acc, m0, n0, 0, p.t.k);
-  const int vw = m0 + 32 * wm * TM, v0 = vw + 16 * g;  // the wave's strip, the lane's first entry of it
-  const int strip = C::WM * t.m + wm;
+  xent_tile<DT, C, true, true, SPLIT>(p.l.t, smem, acc, m0, n0, 0, p.l.t.k);
+  const int vocab = p.l.t.m, tokens = p.l.t.n;
+  const int vw = m0 + 32 * wm * TM, v0 = vw + 16 * g;  // the wave's entries, the lane's first
+  float mxs[TN], sums[TN];
 #pragma unroll
   for (int j = 0; j < TN; ++j) {
     const int n = n0 + 32 * (wn * TN + j) + (lane & 31);
-    const bool in = n < p.t.n;
-    const int64_t tl = (in ? p.targets[n] : -1) - v0;
-    if (vw + 32 * TM > p.t.m) {  // entries past the vocabulary weigh nothing
+    const int64_t tl = (n < tokens ? p.targets[n] : -1) - v0;
+    if (vw + 32 * TM > vocab) {  // entries past the vocabulary weigh nothing
 #pragma unroll
       for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          if (v0 + 32 * i + e >= p.t.m) acc[i][j][e] = -__builtin_inff();
+          if (v0 + 32 * i + e >= vocab) acc[i][j][e] = -__builtin_inff();
     }
     float mx = -__builtin_inff();
 #pragma unroll
@@ -273,15 +372,15 @@ __global__ __launch_bounds__(C::THREADS, 2) void xent_fwd(FwdArgs p) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) mx = fmaxf(mx, acc[i][j][e]);
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    const float base = mx == -__builtin_inff() ? 0.f : mx * kLog2e;  // a strip of -inf sums to 0, not NaN
+    const float base = mx == -__builtin_inff() ? 0.f : mx * kLog2e;
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
       for (int e = 0; e < 16; ++e) s += fast_exp2(__builtin_fmaf(acc[i][j][e], kLog2e, -base));
     s += __shfl_xor(s, 32, 64);
-    if (in && g == 0) p.part[static_cast<int64_t>(strip) * p.t.n + n] = make_float2(mx, s);
-    if (tl >= 0 && tl < 32 * TM && v0 + tl < p.t.m && (tl & 16) == 0) {  // this lane holds the target's logit
+    mxs[j] = mx, sums[j] = s;
+    if (tl >= 0 && tl < 32 * TM && v0 + tl < vocab && (tl & 16) == 0) {  // this lane holds the target's logit
       float z = 0.f;
 #pragma unroll
       for (int i = 0; i < TM; ++i)
@@ -291,6 +390,35 @@ __global__ __launch_bounds__(C::THREADS, 2) void xent_fwd(FwdArgs p) {
       p.zt[n] = z;
     }
   }
+  if constexpr (32 * TM < kStrip) {  // the strip's two waves meet in LDS
+    static_assert(64 * TM == kStrip && C::WM == 2, "two waves a strip");
+    __syncthreads();  // the tile loop's last reads are over
+    float2* sh = reinterpret_cast<float2*>(smem);
+    if (wm == 1 && g == 0)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) sh[(wn * TN + j) * 32 + lane] = make_float2(mxs[j], sums[j]);
+    __syncthreads();
+    if (wm == 1) return;
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const float2 o = sh[(wn * TN + j) * 32 + (lane & 31)];
+      join(mxs[j], sums[j], o.x, o.y);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < TN; ++j) {
+    const int n = n0 + 32 * (wn * TN + j) + (lane & 31);
+    if (n < tokens && g == 0 && vw < vocab)
+      p.part[static_cast<int64_t>(vw / kStrip) * tokens + n] = make_float2(mxs[j], sums[j]);
+  }
+}
+
+template <int DT, bool SPLIT>
+__global__ __launch_bounds__(256, 2) void xent_fwd(FwdArgs p) {
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[Big::LDS];
+  logit_tile(
+      p.l, [&](int m0, int n0) { fwd_tile<DT, Big, SPLIT>(p, smem, m0, n0); },
+      [&](int m0, int n0) { fwd_tile<DT, Small, SPLIT>(p, smem, m0, n0); });
 }
 
 // Joins the strips of 8 tokens, 32 lanes a token: lse and loss.
@@ -302,12 +430,7 @@ __global__ __launch_bounds__(256) void xent_join(const float2* __restrict__ part
   const int tok = threadIdx.x & 7, q = threadIdx.x >> 3;
   const int64_t n = static_cast<int64_t>(blockIdx.x) * 8 + tok;
   float m = -__builtin_inff(), s = 0.f;
-  auto add = [&](float2 o) {
-    const float mn = nan_max(m, o.x);
-    const float b = mn == -__builtin_inff() ? 0.f : mn;
-    s = s * fast_exp2((m - b) * kLog2e) + o.y * fast_exp2((o.x - b) * kLog2e);
-    m = mn;
-  };
+  auto add = [&](float2 o) { join(m, s, o.x, o.y); };
   if (n < n_tokens)
     for (int i = q; i < strips; i += 32) add(part[static_cast<int64_t>(i) * n_tokens + n]);
   sh[q][tok] = make_float2(m, s);
@@ -326,7 +449,7 @@ __global__ __launch_bounds__(256) void xent_join(const float2* __restrict__ part
 // --------------------------------------------------------------- backward
 
 struct GradArgs {
-  TileArgs t;
+  LogitTiles l;        // a: w from the piece's first row (m: its entries)
   const int64_t* targets;
   const float* lse;
   const float* g;      // [tokens]: dloss (fp16: scaled)
@@ -336,136 +459,130 @@ struct GradArgs {
   int64_t vocab, ignore;
 };
 
-// dz of a piece: a: w from the piece's first row (m: its entries), b: x.
 template <int DT, typename C, bool SPLIT>
-__global__ __launch_bounds__(C::THREADS, 2) void xent_dz(GradArgs p) {
+__device__ __forceinline__ void dz_tile(const GradArgs& p, unsigned char* smem, int m0, int n0) {
   constexpr int TM = C::TM, TN = C::TN;
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[C::LDS];
-  const Tile t = tile_of(p.t);
-  if (!t.live) return;
-  const int m0 = t.m * C::BM, n0 = t.n * C::BN;
   const int lane = threadIdx.x & 63, w = wave_id(), wm = w / C::WN, wn = w % C::WN, g = lane >> 5;
   f32x16 acc[TM][TN];
-  xent_tile<DT, C, true, true, SPLIT>(p.t, smem, acc, m0, n0, 0, p.t.k);
-  const int c0 = m0 + 32 * wm * TM + 16 * g;  // the lane's first column of dz
+  xent_tile<DT, C, true, true, SPLIT>(p.l.t, smem, acc, m0, n0, 0, p.l.t.k);
+  __syncthreads();  // the tile loop's last reads are over: LDS serves the stores
+  unsigned char* lds = smem + w * 32 * put_pitch<2, TM>();
+  static_assert(C::NW * 32 * put_pitch<2, TM>() <= C::LDS, "the stores' rows fit");
+  const int cw = m0 + 32 * wm * TM;  // the wave's first column of dz
 #pragma unroll
   for (int j = 0; j < TN; ++j) {
-    const int n = n0 + 32 * (wn * TN + j) + (lane & 31);
-    if (n >= p.t.n) continue;
-    const int64_t tg = p.targets[n];
+    const int nw = n0 + 32 * (wn * TN + j), n = nw + (lane & 31);
+    const int64_t tg = n < p.l.t.n ? p.targets[n] : -1;
     const bool live = tg >= 0 && tg < p.vocab && tg != p.ignore;
-    const float gn = live ? p.g[n] : 0.f, l2 = p.lse[n] * kLog2e;
-    const int64_t tl = live ? tg - p.v0 - c0 : -1;
+    const float gn = live ? p.g[n] : 0.f, l2 = live ? p.lse[n] * kLog2e : 0.f;
+    const int64_t tl = live ? tg - p.v0 - (cw + 16 * g) : -1;
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
-      const int c = c0 + 32 * i;
-      if (c >= p.ldz) continue;  // ldz is a multiple of 32
-      float q[16];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) q[e] = fast_exp2(__builtin_fmaf(acc[i][j][e], kLog2e, -l2));
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = fast_exp2(__builtin_fmaf(acc[i][j][e], kLog2e, -l2));
       const int64_t at = tl - 32 * i;
       if (at >= 0 && at < 16) {
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          if (at == e) q[e] -= 1.f;
+          if (at == e) acc[i][j][e] -= 1.f;
       }
       // an ignored token has no gradient whatever its logits are; entries past the vocabulary are zero
+      const int c = cw + 32 * i + 16 * g;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) q[e] = live && c + e < p.t.m ? q[e] * gn : 0.f;
-      uint16_t* o = p.dz + static_cast<int64_t>(n) * p.ldz + c;
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = live && c + e < p.l.t.m ? acc[i][j][e] * gn : 0.f;
+    }
 #pragma unroll
-      for (int pl = 0; pl < (SPLIT ? 3 : 1); ++pl) {
-        u32x4 lo, hi;
+    for (int pl = 0; pl < (SPLIT ? 3 : 1); ++pl) {
+      u32x4 v[TM][2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if constexpr (DT == PDH_BF16) {
-            lo[e] = pack2<__hip_bfloat16>(q[2 * e], q[2 * e + 1]);
-            hi[e] = pack2<__hip_bfloat16>(q[8 + 2 * e], q[9 + 2 * e]);
-          } else {
-            lo[e] = pack2<_Float16>(q[2 * e], q[2 * e + 1]);
-            hi[e] = pack2<_Float16>(q[8 + 2 * e], q[9 + 2 * e]);
-          }
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          float x[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = acc[i][j][8 * q + e];
+          v[i][q] = pack8<DT>(x);
           if constexpr (SPLIT) {  // what this term leaves (exact)
-            q[2 * e] -= __uint_as_float(lo[e] << 16);
-            q[2 * e + 1] -= __uint_as_float(lo[e] & 0xffff0000u);
-            q[8 + 2 * e] -= __uint_as_float(hi[e] << 16);
-            q[9 + 2 * e] -= __uint_as_float(hi[e] & 0xffff0000u);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              acc[i][j][8 * q + e] -= __uint_as_float(e & 1 ? v[i][q][e >> 1] & 0xffff0000u : v[i][q][e >> 1] << 16);
           }
         }
-        reinterpret_cast<u32x4*>(o + pl * p.plane)[0] = lo;
-        reinterpret_cast<u32x4*>(o + pl * p.plane)[1] = hi;
-      }
+      put_rows<2, TM>(lds, v, reinterpret_cast<char*>(p.dz + pl * p.plane + static_cast<int64_t>(nw) * p.ldz + cw),
+                      p.ldz * 2, p.l.t.n - nw, static_cast<int>(p.ldz) - cw, false);
     }
   }
 }
 
-// A gradient product: a: x or w with its features contiguous (m: features),
-// b: dz, its columns (dw: n vocabulary, k tokens) or its rows (dx: n tokens, k vocabulary).
+template <int DT, bool SPLIT>
+__global__ __launch_bounds__(256, 2) void xent_dz(GradArgs p) {
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[Big::LDS];
+  logit_tile(
+      p.l, [&](int m0, int n0) { dz_tile<DT, Big, SPLIT>(p, smem, m0, n0); },
+      [&](int m0, int n0) { dz_tile<DT, Small, SPLIT>(p, smem, m0, n0); });
+}
+
+// The gradient products, both in one launch so that their tiles fill the chip
+// together: a: x or w with its features contiguous (m: features), b: dz, by its
+// columns (dw: n vocabulary, k tokens) or rows (dx: n tokens, k vocabulary).
 struct ProdArgs {
-  TileArgs t;
-  void* out;           // dw rows, or fp32 parts [slices][n][ldo]
-  int64_t ldo, slice;  // elements
-  const float* scale;  // NULL: 1
-  int add;             // add to what out holds (the parts of an earlier piece)
+  TileArgs w, x;
+  int tiles_w, tiles_x;  // with slices
+  int x_first;           // the longer tiles go first
+  void* dw;
+  float* parts;          // dx's, [slices][tokens][ldp]
+  int64_t lddw, ldp, slice;
+  const float* scale;    // of dw; NULL: 1
+  int add;               // dx's parts of an earlier piece are there
 };
 
 template <int DT, int ODT, typename C, bool KB, bool SPLIT>
-__global__ __launch_bounds__(C::THREADS, 2) void xent_prod(ProdArgs p) {
-  constexpr int TM = C::TM, TN = C::TN;
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[C::LDS];
-  const Tile t = tile_of(p.t);
-  if (!t.live) return;
+__device__ __forceinline__ void prod_tile(const TileArgs& a, int id, unsigned char* smem, char* out, int64_t ld,
+                                          int64_t slice, const float* scale, bool add) {
+  constexpr int TM = C::TM, TN = C::TN, ES = ODT == PDH_F32 ? 4 : 2;
+  const Tile t = tile_of(a, id);
   const int m0 = t.m * C::BM, n0 = t.n * C::BN;
-  const int lane = threadIdx.x & 63, w = wave_id(), wm = w / C::WN, wn = w % C::WN, g = lane >> 5;
+  const int w = wave_id(), wm = w / C::WN, wn = w % C::WN;
   f32x16 acc[TM][TN];
-  const int64_t k0 = static_cast<int64_t>(t.slice) * p.t.kslice;
-  const int64_t k1 = k0 + p.t.kslice < p.t.k ? k0 + p.t.kslice : p.t.k;
-  xent_tile<DT, C, false, KB, SPLIT>(p.t, smem, acc, m0, n0, k0, k1);
-  const float sc = p.scale ? *p.scale : 1.f;
-  constexpr int ES = ODT == PDH_F32 ? 4 : 2;
+  const int64_t k0 = static_cast<int64_t>(t.slice) * a.kslice, k1 = k0 + a.kslice < a.k ? k0 + a.kslice : a.k;
+  xent_tile<DT, C, false, KB, SPLIT>(a, smem, acc, m0, n0, k0, k1);
+  __syncthreads();  // the tile loop's last reads are over: LDS serves the stores
+  unsigned char* lds = smem + w * 32 * put_pitch<ES, TM>();
+  static_assert(C::NW * 32 * put_pitch<ES, TM>() <= C::LDS, "the stores' rows fit");
+  const float sc = scale ? *scale : 1.f;
+  const int cw = m0 + 32 * wm * TM;
 #pragma unroll
   for (int j = 0; j < TN; ++j) {
-    const int n = n0 + 32 * (wn * TN + j) + (lane & 31);
-    if (n >= p.t.n) continue;
-    char* row = static_cast<char*>(p.out) + (t.slice * p.slice + static_cast<int64_t>(n) * p.ldo) * ES;
+    const int nw = n0 + 32 * (wn * TN + j);
+    u32x4 v[TM][ES];
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      const int c = m0 + 32 * (wm * TM + i) + 16 * g, left = p.t.m - c;
-      if (left <= 0) continue;
-      if (left >= 16) {
-        if constexpr (ODT == PDH_F32) {
-          f32x4u* o = reinterpret_cast<f32x4u*>(row + c * 4);
+    for (int i = 0; i < TM; ++i)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            f32x4u v{acc[i][j][4 * q] * sc, acc[i][j][4 * q + 1] * sc, acc[i][j][4 * q + 2] * sc,
-                     acc[i][j][4 * q + 3] * sc};
-            if (p.add) v += o[q];
-            o[q] = v;
-          }
-        } else {
-          u32x4h* o = reinterpret_cast<u32x4h*>(row + c * 2);
+      for (int q = 0; q < ES; ++q) {
+        float x[8];
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            u32x4h v;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float x0 = acc[i][j][8 * q + 2 * e] * sc, x1 = acc[i][j][8 * q + 2 * e + 1] * sc;
-              v[e] = ODT == PDH_BF16 ? pack2<__hip_bfloat16>(x0, x1) : pack2<_Float16>(x0, x1);
-            }
-            o[q] = v;
-          }
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 15; ++e)
-          if (e < left) {
-            float v = acc[i][j][e] * sc;
-            if (ODT == PDH_F32 && p.add) v += reinterpret_cast<float*>(row)[c + e];
-            st_dt<ODT>(row, c + e, v);
-          }
+        for (int e = 0; e < 16 / ES; ++e) x[e] = acc[i][j][16 / ES * q + e] * sc;
+        if constexpr (ES == 4)
+          v[i][q] = u32x4{__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])};
+        else
+          v[i][q] = pack8<ODT>(x);
       }
-    }
+    put_rows<ES, TM>(lds, v, out + (t.slice * slice + static_cast<int64_t>(nw) * ld + cw) * ES, ld * ES, a.n - nw,
+                     a.m - cw, add);
   }
+}
+
+template <int DT, int ODT, bool SPLIT>
+__global__ __launch_bounds__(256, 2) void xent_prod(ProdArgs p) {
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[Big::LDS];
+  bool second;
+  const int id = run_id(p.x_first ? p.tiles_x : p.tiles_w, p.x_first ? p.tiles_w : p.tiles_x, second);
+  if (id < 0) return;
+  if (second != static_cast<bool>(p.x_first))
+    prod_tile<DT, PDH_F32, Big, true, SPLIT>(p.x, id, smem, reinterpret_cast<char*>(p.parts), p.ldp, p.slice, nullptr,
+                                             p.add);
+  else
+    prod_tile<DT, ODT, Big, false, SPLIT>(p.w, id, smem, static_cast<char*>(p.dw), p.lddw, 0, p.scale, false);
 }
 
 // dx = scale * the sum of its parts, in order.
@@ -615,11 +732,57 @@ TileArgs tiles(Operand a, Operand b, int64_t m, int64_t n, int64_t k, int64_t ks
   t.group = t.tiles_n < 8 ? t.tiles_n : 8;
   return t;
 }
-dim3 grid_of(const TileArgs& t) {
-  return dim3(static_cast<unsigned>((static_cast<int64_t>(t.tiles_m) * t.tiles_n * t.slices + 7) / 8 * 8));
+int64_t count(const TileArgs& t) { return static_cast<int64_t>(t.tiles_m) * t.tiles_n * t.slices; }
+
+// Workgroups of these kernels that run at a time.
+int64_t slots() {
+  static thread_local int cus = 0;
+  if (!cus) cus = pdh_device_cus();
+  return 2 * (cus ? cus : 256);
 }
 
-using Big = Config<2, 2, 4, 2>;  // 256 x 128 tiles
+// The logits' tiles past the last whole round run as quarters where those take less time: a
+// quarter takes 0.33 of a tile's time.
+LogitTiles logit_tiles(const TileArgs& t) {
+  const int64_t all = count(t), s = slots(), left = all % s;
+  const bool quarter = left > 0 && 0.33 * static_cast<double>((4 * left + s - 1) / s) < 1.0;
+  const int64_t big = quarter ? all - left : all;
+  return LogitTiles{t, static_cast<int>(big), static_cast<int>(quarter ? 4 * left : 0)};
+}
+
+// The time at which `s` slots end n1 jobs of d1 and then n2 of d2 <= d1, each
+// slot taking the next job when it is free.
+double makespan(int64_t n1, double d1, int64_t n2, double d2, int64_t s) {
+  const int64_t q = n1 / s, r = n1 % s;  // r slots are free at (q + 1) d1, the rest at q d1
+  const double early = q * d1, late = early + (r ? d1 : 0.0);
+  if (n2 == 0) return r ? late : early;
+  double best = 1e300;
+  for (int64_t i = 1; best == 1e300; ++i) {
+    for (const double t : {early + i * d2, late + i * d2}) {
+      const int64_t fit = (s - r) * static_cast<int64_t>((t - early) / d2 + 1e-9) +
+                          r * std::max<int64_t>(0, static_cast<int64_t>((t - late) / d2 + 1e-9));
+      if (t >= late && fit >= n2) best = std::min(best, t);
+    }
+  }
+  return best;
+}
+
+// The slices of dx's product, a piece's vocabulary, that end both gradient
+// products soonest, in k tiles' time: a tile's own cost is its k tiles and
+// about 5 for its start and stores, a slice's the traffic of its part, added
+// and read again (9e-7 k tiles an element at 4.5 TB/s, 2 us a k tile).
+int64_t pick_slices(int64_t tiles_w, int64_t tiles_x, int64_t n, int64_t piece, int64_t dp, int terms) {
+  const double dw = static_cast<double>(terms) * ((n + kBK - 1) / kBK) + 5;
+  double best = 1e300;
+  int64_t at = 1;
+  for (int64_t s = 1; s <= 64 && s * 256 <= std::max<int64_t>(piece, 256); ++s) {
+    const double dx = static_cast<double>(terms) * ((piece + s * kBK - 1) / (s * kBK)) + 5;
+    const double t = (dx > dw ? makespan(tiles_x * s, dx, tiles_w, dw, slots())
+                              : makespan(tiles_w, dw, tiles_x * s, dx, slots())) + 9e-7 * s * n * dp;
+    if (t < best) best = t, at = s;
+  }
+  return at;
+}
 
 int check(const char* fn, int64_t n, int64_t d, int64_t v, int64_t ldx, int64_t ldw, int dtype) {
   PDH_REQUIRE(dtype == PDH_F32 || dtype == PDH_BF16 || dtype == PDH_F16, PDH_EUNSUPPORTED, "%s: dtype %d", fn, dtype);
@@ -647,7 +810,7 @@ FwdPlan plan_fwd(const Problem& q, Space& ws, bool fit_x, bool fit_w, hipStream_
   p.w = place(q.w, q.ldw, q.v, q, ws, fit_w, s, launch);
   p.x = place(q.x, q.ldx, q.n, q, ws, fit_x, s, launch);
   p.t = tiles<Big>(p.w, p.x, q.v, q.n, q.dp(), up(q.dp(), kBK));
-  p.strips = Big::WM * p.t.tiles_m;
+  p.strips = static_cast<int>((q.v + kStrip - 1) / kStrip);
   p.part = static_cast<float2*>(ws.take(static_cast<int64_t>(p.strips) * q.n * 8));
   p.zt = static_cast<float*>(ws.take(q.n * 4));
   return p;
@@ -670,9 +833,9 @@ BwdPlan plan_bwd(const Problem& q, Space& ws, bool fit_x, bool fit_w, hipStream_
   const int64_t all = up(q.v, 256), most = kPieceBytes / (q.n * 2 * q.planes()) / 256 * 256;
   p.piece = std::min(all, std::max<int64_t>(most, 256));
   p.dz = static_cast<uint16_t*>(ws.take(q.n * p.piece * 2 * q.planes()));
-  // dx's tiles alone would leave compute units idle: its k, the vocabulary, in slices
-  const int64_t t = ((q.d + 255) / 256) * ((q.n + 127) / 128);
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>({(1024 + t - 1) / t, p.piece / 512, 64}));
+  const int64_t mt = (q.d + Big::BM - 1) / Big::BM;
+  const int64_t want = pick_slices(mt * ((p.piece + Big::BN - 1) / Big::BN), mt * ((q.n + Big::BN - 1) / Big::BN), q.n,
+                                   p.piece, q.dp(), q.dtype == PDH_F32 ? kPairs : 1);
   p.kslice = up((p.piece + want - 1) / want, kBK);
   p.slices = (p.piece + p.kslice - 1) / p.kslice;
   p.parts = static_cast<float*>(ws.take(p.slices * q.n * q.dp() * 4));
@@ -686,7 +849,8 @@ BwdPlan plan_bwd(const Problem& q, Space& ws, bool fit_x, bool fit_w, hipStream_
 template <int DT, bool SPLIT>
 int run_fwd(const Problem& q, const FwdPlan& p, const int64_t* targets, int64_t ignore, float* loss, float* lse, int* bad,
             hipStream_t s) {
-  xent_fwd<DT, Big, SPLIT><<<grid_of(p.t), Big::THREADS, 0, s>>>(FwdArgs{p.t, targets, p.part, p.zt});
+  const LogitTiles l = logit_tiles(p.t);
+  xent_fwd<DT, SPLIT><<<run_grid(l.big, l.small), 256, 0, s>>>(FwdArgs{l, targets, p.part, p.zt});
   if (int rc = check_launch("pdh_linear_xent_fwd"); rc != PDH_OK) return rc;
   xent_join<<<dim3(static_cast<unsigned>((q.n + 7) / 8)), 256, 0, s>>>(p.part, p.zt, targets, p.strips, q.n, q.v, ignore,
                                                                        loss, lse, bad);
@@ -708,12 +872,18 @@ int run_bwd(const Problem& q, const BwdPlan& p, const int64_t* targets, const fl
     const int64_t nv = std::min(p.piece, q.v - v0), ldz = up(nv, 256);
     const Operand wv{p.w.p + v0 * p.w.pitch, p.w.pitch, p.w.plane};
     const Operand dz{reinterpret_cast<const char*>(p.dz), ldz * 2, q.n * ldz * 2};
-    GradArgs ga{tiles<Big>(wv, p.x, nv, q.n, dp, up(dp, kBK)), targets, lse, g, p.dz, ldz, q.n * ldz, v0, q.v, ignore};
-    xent_dz<DT, Big, SPLIT><<<grid_of(ga.t), Big::THREADS, 0, s>>>(ga);
-    ProdArgs pw{tiles<Big>(p.x, dz, q.d, nv, q.n, up(q.n, kBK)), static_cast<char*>(dw) + v0 * q.d * es, q.d, 0, scale, 0};
-    xent_prod<DT, ODT, Big, false, SPLIT><<<grid_of(pw.t), Big::THREADS, 0, s>>>(pw);
-    ProdArgs px{tiles<Big>(wv, dz, q.d, q.n, nv, p.kslice), p.parts, dp, slice, nullptr, v0 > 0};
-    xent_prod<DT, PDH_F32, Big, true, SPLIT><<<grid_of(px.t), Big::THREADS, 0, s>>>(px);
+    const GradArgs ga{logit_tiles(tiles<Big>(wv, p.x, nv, q.n, dp, up(dp, kBK))), targets, lse, g, p.dz, ldz, q.n * ldz,
+                      v0, q.v, ignore};
+    xent_dz<DT, SPLIT><<<run_grid(ga.l.big, ga.l.small), 256, 0, s>>>(ga);
+    ProdArgs pr{};
+    pr.w = tiles<Big>(p.x, dz, q.d, nv, q.n, up(q.n, kBK));
+    pr.x = tiles<Big>(wv, dz, q.d, q.n, nv, p.kslice);
+    pr.tiles_w = static_cast<int>(count(pr.w)), pr.tiles_x = static_cast<int>(count(pr.x));
+    pr.x_first = p.kslice > q.n;
+    pr.dw = static_cast<char*>(dw) + v0 * q.d * es;
+    pr.parts = p.parts, pr.lddw = q.d, pr.ldp = dp, pr.slice = slice;
+    pr.scale = scale, pr.add = v0 > 0;
+    xent_prod<DT, ODT, SPLIT><<<run_grid(pr.tiles_w, pr.tiles_x), 256, 0, s>>>(pr);
     if (int rc = check_launch("pdh_linear_xent_bwd"); rc != PDH_OK) return rc;
   }
   xent_dx<ODT><<<dim3(blocks_for(q.n * (dp / 4))), 256, 0, s>>>(p.parts, dx, q.n, static_cast<int>(q.d), dp, slice,

@@ -132,19 +132,45 @@ def test_the_pairs_of_terms_grow():
     assert list(zip(pa, pb)) == [(0, 2), (2, 0), (1, 1), (0, 1), (1, 0), (0, 0)]
 
 
+def _run_ids(first, second):
+    c1, c2 = (first + 7) // 8, (second + 7) // 8
+    for bid in range((c1 + c2) * 8):
+        xcd, pos = bid & 7, bid >> 3
+        in2 = pos >= c1
+        i = xcd * c2 + pos - c1 if in2 else xcd * c1 + pos
+        if (pos - c1 < c2 and i < second) if in2 else i < first:
+            yield in2, i
+
+
+def _tile(tm, tn, i):
+    s, i = divmod(i, tm * tn)
+    group = min(8, tn)
+    g, rem = divmod(i, group * tm)
+    gn = min(tn - g * group, group)
+    return s, rem // gn, g * group + rem % gn
+
+
 def test_every_tile_is_taken_once():
+    for first, second in itertools.product((0, 1, 7, 8, 9, 513), (0, 1, 30, 64)):
+        ids = list(_run_ids(first, second))
+        assert sorted(ids) == [(False, i) for i in range(first)] + [(True, i) for i in range(second)]
     for tm, tn, sl in itertools.product((1, 3, 20, 197), (1, 2, 7, 8, 9, 33), (1, 5)):
-        group, per = min(8, tn), tm * tn
-        total = per * sl
-        chunk = (total + 7) // 8
-        seen = set()
-        for bid in range((total + 7) // 8 * 8):
-            pos = bid >> 3
-            i = (bid & 7) * chunk + pos
-            if not (pos < chunk and i < total):
-                continue
-            s, i = divmod(i, per)
-            g, rem = divmod(i, group * tm)
-            gn = min(tn - g * group, group)
-            seen.add((s, rem // gn, g * group + rem % gn))
-        assert seen == set(itertools.product(range(sl), range(tm), range(tn)))
+        assert {_tile(tm, tn, i) for i in range(tm * tn * sl)} == set(
+            itertools.product(range(sl), range(tm), range(tn)))
+
+
+@pytest.mark.parametrize("es,tm", [(2, 4), (4, 4), (2, 2)])
+def test_stored_rows_leave_lds_as_they_came(es, tm):
+    """put_rows: each lane's sixteen-column runs come back as whole rows."""
+    pitch, ch = tm * 32 * es + 16, tm * 32 * es // 16
+    lds = {}
+    for lane, i, q in itertools.product(range(64), range(tm), range(es)):
+        at = (lane & 31) * pitch + (lane >> 5) * 16 * es + i * 32 * es + 16 * q
+        assert at not in lds and at + 16 <= 32 * pitch
+        lds[at] = (lane & 31, 32 * i + 16 * (lane >> 5) + 16 // es * q)  # row, first column
+    seen = set()
+    for it, lane in itertools.product(range(32 * ch // 64), range(64)):
+        row, c = divmod(it * 64 + lane, ch)
+        assert lds[row * pitch + 16 * c] == (row, c * 16 // es)
+        seen.add((row, c))
+    assert len(seen) == 32 * ch
