@@ -285,21 +285,39 @@ __global__ __launch_bounds__(64 * W * R) void norm_bwd(NormGradArgs a) {
 }
 
 // dgamma / dbeta = the sums over `n` partial rows [n][2][cols], in a fixed
-// order: 32 columns of one of the two a workgroup, 8 lanes a column.
+// order: 16 columns of one of the two a workgroup, 64 lanes a column with
+// eight loads in flight each (768 columns, 512 parts: 4 us against 20 with 8
+// lanes a column on 48 workgroups, a chain of loads).
 template <int DT>
-__global__ __launch_bounds__(256) void norm_weights(const float* __restrict__ part, int n, int64_t cols, void* dgamma,
-                                                    void* dbeta) {
-  __shared__ float sh[8][32];
-  const int c32 = threadIdx.x & 31, q = threadIdx.x >> 5;
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + c32;
+__global__ __launch_bounds__(1024) void norm_weights(const float* __restrict__ part, int n, int64_t cols, void* dgamma,
+                                                     void* dbeta) {
+  __shared__ float sh[64][17];
+  const int c16 = threadIdx.x & 15, q = threadIdx.x >> 4;
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * 16 + c16;
   const int which = blockIdx.y;
   float s = 0.f;
-  if (c < cols)
-    for (int i = q; i < n; i += 8) s += part[(static_cast<int64_t>(i) * 2 + which) * cols + c];
-  sh[q][c32] = s;
+  if (c < cols) {
+    const float* p = part + which * cols + c;
+    for (int i = q; i < n; i += 512) {
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = i + 64 * j < n ? p[static_cast<int64_t>(i + 64 * j) * 2 * cols] : 0.f;
+      s += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+    }
+  }
+  sh[q][c16] = s;
   __syncthreads();
-  if (q == 0 && c < cols) {
-    for (int i = 1; i < 8; ++i) s += sh[i][c32];
+  if (threadIdx.x < 256) {  // four lanes' sums each, then the sixteen
+    const int r = threadIdx.x >> 4;
+    s = (sh[4 * r][c16] + sh[4 * r + 1][c16]) + (sh[4 * r + 2][c16] + sh[4 * r + 3][c16]);
+  }
+  __syncthreads();
+  if (threadIdx.x < 256) sh[threadIdx.x >> 4][c16] = s;
+  __syncthreads();
+  if (threadIdx.x < 16 && c < cols) {
+    s = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s += sh[r][c16];
     st_dt<DT>(which ? dbeta : dgamma, c, s);
   }
 }
@@ -459,7 +477,7 @@ int run_bwd(const NormGradArgs& a, void* dgamma, void* dbeta, hipStream_t s) {
     if (int rc = check_launch("pdh_layernorm_bwd"); rc != PDH_OK) return rc;
   }
   if (dgamma) {
-    norm_weights<DT><<<dim3(static_cast<unsigned>((a.cols + 31) / 32), 2), 256, 0, s>>>(
+    norm_weights<DT><<<dim3(static_cast<unsigned>((a.cols + 15) / 16), 2), 1024, 0, s>>>(
         a.part, static_cast<int>(parts), a.cols, dgamma, dbeta);
     return check_launch("pdh_layernorm_bwd (weights)");
   }

@@ -278,7 +278,7 @@ __device__ __forceinline__ void put_rows(unsigned char* lds, const u32x4 (&v)[TM
         if (add) x += *reinterpret_cast<const f32x4u*>(o);
         *reinterpret_cast<f32x4u*>(o) = x;
       } else {
-        *reinterpret_cast<u32x4h*>(o) = w;
+        __builtin_nontemporal_store(__builtin_bit_cast(u32x4h, w), reinterpret_cast<u32x4h*>(o));
       }
     } else {
 #pragma unroll

@@ -151,14 +151,19 @@ def layernorm(
     return y if y.shape == x.shape else y.reshape(x.shape)
 
 
-def _one_device(first: torch.Tensor, *rest) -> None:
-    """Device tensors of the current device alone: a launch goes to its
-    stream, which orders nothing on another."""
-    _require_cuda(first, *rest)
-    dev = torch._C._cuda_getDevice()
-    for t in (first, *rest):
-        if t is not None and t.device.index != dev:
+def _one_device(*ts) -> None:
+    """Device tensors (None aside) of the current device alone: a launch goes
+    to its stream, which orders nothing on another."""
+    dev = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -1
+    for t in ts:
+        if t is not None and (t.get_device() != dev or dev < 0):
+            _require_cuda(t)
             raise ValueError(f"the tensors must be on the current device cuda:{dev} (got {t.device})")
+
+
+def _like(x: torch.Tensor) -> torch.Tensor:
+    """A dense tensor of x's shape and type (empty_like is the cheaper call, 1.2 us against 2.3)."""
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
 @dataclass
@@ -168,15 +173,23 @@ class LayernormOut:
     rstd: torch.Tensor
 
 
-def _norm_weights(x, **ws) -> None:
-    n = x.shape[-1]
-    for nm, t in ws.items():
-        if t is None:
-            continue
-        if t.dtype != x.dtype:
-            raise ValueError(f"{nm} must share x's element type")
-        if t.numel() != n or not t.is_contiguous():
-            raise ValueError(f"{nm} must be a contiguous vector of {n} elements")
+def _rows_of(name: str, x: torch.Tensor):
+    """x as rows of its last axis, their element type's code, number, length and stride."""
+    code = _DT.get(x.dtype)
+    if code is None:
+        raise ValueError(f"{name} stores f32, bf16 or f16 (got {x.dtype})")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"{name} needs rows of at least one column")
+    x2 = _rows(x)
+    m, n = x2.shape
+    return x2, code, m, n, x2.stride(0) if m > 1 else n
+
+
+def _norm_weight(name: str, t: torch.Tensor, x: torch.Tensor, n: int) -> None:
+    if t.dtype != x.dtype:
+        raise ValueError(f"{name} must share x's element type")
+    if t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous vector of {n} elements")
 
 
 def layernorm_fwd(
@@ -191,42 +204,36 @@ def layernorm_fwd(
     :func:`layernorm_bwd` takes. ``out`` (x's shape, rows of contiguous
     columns) may be x itself."""
     _one_device(x, gamma, beta, out)
-    if x.dtype not in _DT:
-        raise ValueError(f"layernorm_fwd stores f32, bf16 or f16 (got {x.dtype})")
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError("layernorm_fwd needs rows of at least one column")
-    _norm_weights(x, gamma=gamma, beta=beta)
-    if eps < 0:
+    x2, code, m, n, ld = _rows_of("layernorm_fwd", x)
+    if gamma is not None:
+        _norm_weight("gamma", gamma, x, n)
+    if beta is not None:
+        _norm_weight("beta", beta, x, n)
+    if not eps >= 0:
         raise ValueError("layernorm_fwd: eps must be >= 0")
-    n = x.shape[-1]
-    x2 = _rows(x)
-    y = torch.empty(x2.shape, dtype=x.dtype, device=x.device) if out is None else _out_rows(out, x)
-    stats = torch.empty((2,) + tuple(x.shape[:-1]), dtype=torch.float32, device=x.device)
-    mean, rstd = stats.unbind(0)
-    _lib.call(
-        "pdh_layernorm_fwd",
-        x2.data_ptr(), _ptr(gamma), _ptr(beta), y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), x2.shape[0], n,
-        _ld(x2), _ld(y), float(eps), _DT[x.dtype], _stream(),
-    )
-    return LayernormOut(out if out is not None else y.view(x.shape), mean, rstd)
+    lead = x.shape[:-1]
+    if out is None:
+        y, ldy = _like(x), n
+    else:
+        y, ldy = out, _out_stride(out, x, m, n)
+    mean = x.new_empty(lead, dtype=torch.float32)
+    rstd = torch.empty_like(mean)
+    _lib.call("pdh_layernorm_fwd", x2.data_ptr(), _ptr(gamma), _ptr(beta), y.data_ptr(), mean.data_ptr(),
+              rstd.data_ptr(), m, n, ld, ldy, eps, code, _stream())
+    return LayernormOut(y, mean, rstd)
 
 
-def _ld(x2: torch.Tensor) -> int:
-    """A 2-D tensor's row stride (a single row's is its length)."""
-    return x2.stride(0) if x2.shape[0] > 1 else x2.shape[1]
-
-
-def _out_rows(out: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
-    """A caller's output as [rows, cols], a view of it."""
-    if out.shape != x.shape or out.dtype != x.dtype or (out.shape[-1] > 1 and out.stride(-1) != 1):
+def _out_stride(out: torch.Tensor, x: torch.Tensor, m: int, n: int) -> int:
+    """The row stride of a caller's output, written in place as rows of its last axis."""
+    if out.shape != x.shape or out.dtype != x.dtype or (n > 1 and out.stride(-1) != 1):
         raise ValueError("out must have x's shape and element type, and contiguous columns")
     try:
-        o2 = out.view(-1, out.shape[-1])
+        o2 = out.view(-1, n)
     except RuntimeError:
         raise ValueError("out's leading dims must compose into one row stride") from None
-    if o2.shape[0] > 1 and o2.stride(0) < o2.shape[1]:
+    if m > 1 and o2.stride(0) < n:
         raise ValueError("out's rows overlap")
-    return o2
+    return o2.stride(0) if m > 1 else n
 
 
 def layernorm_bwd(
@@ -243,59 +250,60 @@ def layernorm_bwd(
     added to dx: the gradient that reaches x along a residual branch past the
     norm. Element types alike, fp32 arithmetic, one rounding; deterministic."""
     _one_device(x, dy, mean, rstd, gamma, dres)
-    if x.dtype not in _DT:
-        raise ValueError(f"layernorm_bwd stores f32, bf16 or f16 (got {x.dtype})")
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError("layernorm_bwd needs rows of at least one column")
-    for nm, t in (("dy", dy), ("dres", dres)):
-        if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
-            raise ValueError(f"{nm} must have x's shape and element type")
+    x2, code, m, n, ld = _rows_of("layernorm_bwd", x)
+    if dy.shape != x.shape or dy.dtype != x.dtype:
+        raise ValueError("dy must have x's shape and element type")
+    lead = x.shape[:-1]
     for nm, t in (("mean", mean), ("rstd", rstd)):
-        if t.dtype != torch.float32 or t.shape != x.shape[:-1] or not t.is_contiguous():
+        if t.dtype != torch.float32 or t.shape != lead or not t.is_contiguous():
             raise ValueError(f"{nm} must be contiguous fp32 of x's leading shape")
-    _norm_weights(x, gamma=gamma)
-    n = x.shape[-1]
-    x2, dy2 = _rows(x), _rows(dy)
-    r2 = None if dres is None else _rows(dres)
-    dx = torch.empty(x2.shape, dtype=x.dtype, device=x.device)
+    dy2 = _rows(dy)
+    r2, ldr = None, 0
+    if dres is not None:
+        if dres.shape != x.shape or dres.dtype != x.dtype:
+            raise ValueError("dres must have x's shape and element type")
+        r2 = _rows(dres)
+        ldr = r2.stride(0) if m > 1 else n
+    dx = _like(x)
     ws, dgamma, dbeta, need = None, None, None, 0
     if gamma is not None:
+        _norm_weight("gamma", gamma, x, n)
         dgamma, dbeta = torch.empty_like(gamma), torch.empty_like(gamma)
-        need = _lib.lib().pdh_layernorm_bwd_workspace(x2.shape[0], n, _DT[x.dtype])
-        ws = torch.empty(need // 4, dtype=torch.float32, device=x.device)
-    _lib.call(
-        "pdh_layernorm_bwd",
-        x2.data_ptr(), dy2.data_ptr(), _ptr(r2), _ptr(gamma), mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(),
-        _ptr(dgamma), _ptr(dbeta), x2.shape[0], n, _ld(x2), _ld(dy2), 0 if r2 is None else _ld(r2), n, _DT[x.dtype],
-        _ptr(ws), need, _stream(),
-    )
-    return dx.view(x.shape), dgamma, dbeta
+        need = _norm_workspace(m, n, code)
+        ws = x.new_empty(need // 4, dtype=torch.float32)
+    _lib.call("pdh_layernorm_bwd", x2.data_ptr(), dy2.data_ptr(), _ptr(r2), _ptr(gamma), mean.data_ptr(),
+              rstd.data_ptr(), dx.data_ptr(), _ptr(dgamma), _ptr(dbeta), m, n, ld, dy2.stride(0) if m > 1 else n, ldr,
+              n, code, _ptr(ws), need, _stream())
+    return dx, dgamma, dbeta
+
+
+@functools.lru_cache(maxsize=4096)
+def _norm_workspace(rows: int, cols: int, code: int) -> int:
+    return _lib.lib().pdh_layernorm_bwd_workspace(rows, cols, code)
 
 
 def _dropout(name, x, p, rng, site, residual, out):
     _one_device(x, rng, residual, out)
-    if x.dtype not in _DT:
-        raise ValueError(f"{name} stores f32, bf16 or f16 (got {x.dtype})")
+    x2, code, m, n, ld = _rows_of(name, x)
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"{name}: the rate p = {p} must lie in [0, 1]")
     if not 0 <= site < 1 << 32:
         raise ValueError(f"{name}: site {site} must fit 32 bits unsigned")
-    if rng.dtype != torch.int64 or tuple(rng.shape) != (2,) or not rng.is_contiguous():
+    if rng.dtype != torch.int64 or rng.shape != (2,) or not rng.is_contiguous():
         raise ValueError(f"{name}: rng is an int64 device tensor of two elements, the seed and the step")
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"{name} needs rows of at least one column")
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
-        raise ValueError("residual must have x's shape and element type")
-    n = x.shape[-1]
-    x2 = _rows(x)
-    r2 = None if residual is None else _rows(residual)
-    y = torch.empty(x2.shape, dtype=x.dtype, device=x.device) if out is None else _out_rows(out, x)
-    _lib.call(
-        "pdh_dropout",
-        x2.data_ptr(), _ptr(r2), y.data_ptr(), x2.shape[0], n, _ld(x2), 0 if r2 is None else _ld(r2), _ld(y), float(p),
-        rng.data_ptr(), site, _DT[x.dtype], _stream(),
-    )
-    return out if out is not None else y.view(x.shape)
+    r2, ldr = None, 0
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            raise ValueError("residual must have x's shape and element type")
+        r2 = _rows(residual)
+        ldr = r2.stride(0) if m > 1 else n
+    if out is None:
+        y, ldy = _like(x), n
+    else:
+        y, ldy = out, _out_stride(out, x, m, n)
+    _lib.call("pdh_dropout", x2.data_ptr(), _ptr(r2), y.data_ptr(), m, n, ld, ldr, ldy, p, rng.data_ptr(), site, code,
+              _stream())
+    return y
 
 
 def dropout_fwd(
@@ -339,14 +347,17 @@ class LossOut:
 
 
 def _head(name, x, w, targets):
-    """The checked operands of a linear head's loss: x and w as rows, the targets flat."""
-    if x.dtype not in _DT or w.dtype != x.dtype:
-        raise ValueError(f"{name}: x and w share one element type of f32, bf16 or f16 (got {x.dtype}, {w.dtype})")
-    if x.dim() < 1 or w.dim() != 2 or w.shape[1] != x.shape[-1] or x.shape[-1] < 1 or w.shape[0] < 1:
+    """The checked operands of a linear head's loss: x and w as rows, the targets flat, the sizes."""
+    if w.dtype != x.dtype:
+        raise ValueError(f"{name}: x and w share one element type (got {x.dtype}, {w.dtype})")
+    x2, code, n, d, ldx = _rows_of(name, x)
+    if w.dim() != 2 or w.shape[1] != d or w.shape[0] < 1:
         raise ValueError(f"{name}: x [..., width] and w [vocab, width] (got {tuple(x.shape)}, {tuple(w.shape)})")
     if targets.dtype != torch.int64 or targets.shape != x.shape[:-1]:
         raise ValueError(f"{name}: targets must be int64 of x's leading shape {tuple(x.shape[:-1])}")
-    return _rows(x), _rows(w), targets.reshape(-1).contiguous()
+    w2 = _rows(w)
+    v = w2.shape[0]
+    return x2, w2, targets.contiguous(), code, (n, d, v, ldx, w2.stride(0) if v > 1 else d)
 
 
 def linear_cross_entropy(
@@ -363,22 +374,27 @@ def linear_cross_entropy(
     has loss 0; the latter also count in ``bad`` (an int32 device scalar) when
     given. fp32, bf16 or f16 operands, fp32 accumulation."""
     _one_device(x, w, targets, bad)
-    x2, w2, t = _head("linear_cross_entropy", x, w, targets)
+    x2, w2, t, code, sizes = _head("linear_cross_entropy", x, w, targets)
     if bad is not None and (bad.dtype != torch.int32 or bad.numel() < 1):
         raise ValueError("linear_cross_entropy: bad is an int32 device scalar")
-    n, d, v = x2.shape[0], x2.shape[1], w2.shape[0]
-    out = torch.empty((2,) + tuple(targets.shape), dtype=torch.float32, device=x.device)
-    loss, lse = out.unbind(0)
-    if n:
-        args = (n, d, v, _ld(x2), _ld(w2))
-        need = _lib.lib().pdh_linear_xent_workspace(x2.data_ptr(), w2.data_ptr(), *args, _DT[x.dtype], 0)
-        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-        _lib.call(
-            "pdh_linear_xent_fwd",
-            x2.data_ptr(), w2.data_ptr(), t.data_ptr(), loss.data_ptr(), lse.data_ptr(), *args, int(ignore_index),
-            _DT[x.dtype], _ptr(bad), ws.data_ptr(), need, _stream(),
-        )
+    loss = x.new_empty(targets.shape, dtype=torch.float32)
+    lse = torch.empty_like(loss)
+    if sizes[0]:
+        px, pw = x2.data_ptr(), w2.data_ptr()
+        need = _head_workspace(px & 15, pw & 15, *sizes, code, 0)
+        ws = x.new_empty(need, dtype=torch.uint8)
+        _lib.call("pdh_linear_xent_fwd", px, pw, t.data_ptr(), loss.data_ptr(), lse.data_ptr(), *sizes,
+                  ignore_index, code, _ptr(bad), ws.data_ptr(), need, _stream())
     return LossOut(loss, lse)
+
+
+@functools.lru_cache(maxsize=4096)
+def _head_workspace(px: int, pw: int, *args) -> int:
+    """pdh_linear_xent_workspace by the operands' alignment (it looks at nothing else of them)."""
+    need = _lib.lib().pdh_linear_xent_workspace(256 + px, 256 + pw, *args)
+    if need == 0:
+        _lib.check("pdh_linear_xent_workspace", _lib.PDH_EUNSUPPORTED)
+    return need
 
 
 def linear_cross_entropy_bwd(
@@ -393,27 +409,24 @@ def linear_cross_entropy_bwd(
     """Gradients (dx, dw) of sum(dloss * loss) for :func:`linear_cross_entropy`
     given its lse; ``dloss`` (fp32, the targets' shape) is each token's weight,
     1 / live tokens for a mean. Of x's and w's element type, rounded once from
-    fp32 sums; deterministic."""
+    fp32 sums; deterministic. An ignored token's dx is zero; its x is still
+    multiplied by zeros into dw, so it has to be finite."""
     _one_device(x, w, targets, lse, dloss)
-    x2, w2, t = _head("linear_cross_entropy_bwd", x, w, targets)
+    x2, w2, t, code, sizes = _head("linear_cross_entropy_bwd", x, w, targets)
     for nm, s in (("lse", lse), ("dloss", dloss)):
         if s.dtype != torch.float32 or s.shape != targets.shape:
             raise ValueError(f"{nm} must be fp32 of the targets' shape")
-    n, d, v = x2.shape[0], x2.shape[1], w2.shape[0]
-    if n == 0:
-        return torch.empty_like(x), torch.zeros((v, d), dtype=w.dtype, device=w.device)
+    dx = _like(x)
+    if sizes[0] == 0:
+        return dx, torch.zeros(w.shape, dtype=w.dtype, device=w.device)
     lse, dloss = lse.contiguous(), dloss.contiguous()
-    dx = torch.empty((n, d), dtype=x.dtype, device=x.device)
-    dw = torch.empty((v, d), dtype=w.dtype, device=w.device)
-    args = (n, d, v, _ld(x2), _ld(w2))
-    need = _lib.lib().pdh_linear_xent_workspace(x2.data_ptr(), w2.data_ptr(), *args, _DT[x.dtype], 1)
-    ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-    _lib.call(
-        "pdh_linear_xent_bwd",
-        x2.data_ptr(), w2.data_ptr(), t.data_ptr(), lse.data_ptr(), dloss.data_ptr(), dx.data_ptr(), dw.data_ptr(), *args,
-        int(ignore_index), _DT[x.dtype], ws.data_ptr(), need, _stream(),
-    )
-    return dx.view(x.shape), dw
+    dw = _like(w)
+    px, pw = x2.data_ptr(), w2.data_ptr()
+    need = _head_workspace(px & 15, pw & 15, *sizes, code, 1)
+    ws = x.new_empty(need, dtype=torch.uint8)
+    _lib.call("pdh_linear_xent_bwd", px, pw, t.data_ptr(), lse.data_ptr(), dloss.data_ptr(), dx.data_ptr(),
+              dw.data_ptr(), *sizes, ignore_index, code, ws.data_ptr(), need, _stream())
+    return dx, dw
 
 
 def take_rows(table: torch.Tensor, idx: torch.Tensor, out: torch.Tensor | None = None,
