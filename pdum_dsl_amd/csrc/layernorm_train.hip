@@ -14,11 +14,17 @@
 // so rows of odd lengths and strides run the same path. Sums of a row: DPP rotations in
 // 16-lane rows, four readlanes, LDS between waves.
 //
-// The backward's grid is fixed (kBwdGroups workgroups): each walks its rows
-// with the next row's loads in flight, keeps its columns' sums of dy xh and dy
-// in registers and writes them once, fp32, to the workspace; a second kernel
-// adds the workgroups' partial sums in order. No atomics: results repeat bit
-// for bit.
+// The backward's grid is fixed, a workgroup of eight waves (16 for the longest
+// rows) on every compute unit: each walks its rows with the next row's loads in
+// flight, keeps its columns' sums of dy xh and dy in registers and writes them
+// once, fp32, to the workspace; a second kernel adds the workgroups' partial
+// sums in order. No atomics: results repeat bit for bit. Two workgroups a unit
+// hide no more latency and double the partial sums: 4096 x 4096 bf16 41.5 us
+// against 34.8, 2048 x 8192 50 against 36.
+//
+// Outputs leave past the caches: forward 8192 x 4096 fp32 47.6 -> 39.7 us (6.8
+// TB/s), 32768 x 768 bf16 21.8 -> 19.0. Loads past them gain in the backward
+// (8192 x 4096 fp32 82.7 -> 78.9) and cost in the forward (39.7 -> 49).
 //
 // Rows of over 16384 columns, or of fewer than a chunk, take one workgroup a
 // row in several passes, and column sums by a kernel of their own.
@@ -29,7 +35,7 @@ namespace {
 
 constexpr int kVals = 16;         // values of a row a lane holds
 constexpr int kMaxCols = 16384;   // 16 waves x 64 lanes x kVals
-constexpr int kBwdGroups = 512;   // workgroups of the backward (partial sums of the weights' gradients)
+constexpr int kBwdGroups = 256;   // workgroups of the backward: a compute unit each, and their partial sums
 constexpr int64_t kFwdRows = int64_t{1} << 21;  // rows of one forward launch
 constexpr int kLongGroups = 1 << 16;  // workgroups of the long rows' backward
 constexpr int kSlices = 64;       // row slices of the long rows' column sums
@@ -103,14 +109,21 @@ struct Share {
     }
   }
   __device__ __forceinline__ bool mine(int j) const { return j % V >= skip[j / V]; }
+  // STREAM: past the caches, for a row that this launch reads once
+  template <bool STREAM>
   __device__ __forceinline__ void load(const char* row, u32x4 (&w)[CH]) const {
 #pragma unroll
-    for (int i = 0; i < CH; ++i) w[i] = *reinterpret_cast<const u32x4h*>(row + c[i] * es<DT>());
+    for (int i = 0; i < CH; ++i) {
+      const u32x4h* p = reinterpret_cast<const u32x4h*>(row + c[i] * es<DT>());
+      w[i] = STREAM ? __builtin_bit_cast(u32x4, __builtin_nontemporal_load(p)) : __builtin_bit_cast(u32x4, *p);
+    }
   }
   __device__ __forceinline__ void store(char* row, const float (&v)[kVals]) const {
 #pragma unroll
     for (int i = 0; i < CH; ++i)
-      if (skip[i] < V) *reinterpret_cast<u32x4h*>(row + c[i] * es<DT>()) = pack_chunk<DT>(v + i * V);
+      if (skip[i] < V)
+        __builtin_nontemporal_store(__builtin_bit_cast(u32x4h, pack_chunk<DT>(v + i * V)),
+                                    reinterpret_cast<u32x4h*>(row + c[i] * es<DT>()));
   }
 };
 
@@ -163,9 +176,9 @@ __global__ __launch_bounds__(64 * W * R) void norm_fwd(NormArgs a) {
   if (W == 1 && row >= a.rows) return;  // W > 1 has R = 1: the grid is the rows
   const S sh_of(wave, lane, a.cols);
   u32x4 raw[S::CH], gw[S::CH], bw[S::CH];
-  sh_of.load(static_cast<const char*>(a.x) + row * a.ldx * es<DT>(), raw);
-  if (a.gamma) sh_of.load(static_cast<const char*>(a.gamma), gw);
-  if (a.beta) sh_of.load(static_cast<const char*>(a.beta), bw);
+  sh_of.template load<false>(static_cast<const char*>(a.x) + row * a.ldx * es<DT>(), raw);
+  if (a.gamma) sh_of.template load<false>(static_cast<const char*>(a.gamma), gw);
+  if (a.beta) sh_of.template load<false>(static_cast<const char*>(a.beta), bw);
   float v[kVals], s = 0.f, ss = 0.f;
 #pragma unroll
   for (int j = 0; j < kVals; ++j) {
@@ -213,7 +226,7 @@ __global__ __launch_bounds__(64 * W * R) void norm_bwd(NormGradArgs a) {
   using S = Share<DT, W>;
   constexpr int CH = S::CH, V = S::V;
   // two reductions' worth, used in turn: a wave writes one while a slow one still reads the other
-  __shared__ float sh[2][2 * W];
+  __shared__ float sh[R][2][2 * W];
   __shared__ float acc_sh[AFFINE && R > 1 ? R * 64 * W * kVals : 1];
   const int lane = threadIdx.x & 63, w = wave_id(), wave = w % W, slot = w / W;
   const int64_t step = static_cast<int64_t>(gridDim.x) * R;
@@ -222,11 +235,11 @@ __global__ __launch_bounds__(64 * W * R) void norm_bwd(NormGradArgs a) {
   const S own(wave, lane, a.cols);
   u32x4 gw[CH], xw[CH], yw[CH], rw[CH];
   float ag[kVals] = {}, ab[kVals] = {}, mean = 0.f, rstd = 0.f;
-  if (AFFINE) own.load(static_cast<const char*>(a.gamma), gw);
+  if (AFFINE) own.template load<false>(static_cast<const char*>(a.gamma), gw);
   auto fetch = [&](int64_t r) __attribute__((always_inline)) {
-    own.load(static_cast<const char*>(a.x) + r * a.ldx * es<DT>(), xw);
-    own.load(static_cast<const char*>(a.dy) + r * a.lddy * es<DT>(), yw);
-    if (a.dres) own.load(static_cast<const char*>(a.dres) + r * a.lddres * es<DT>(), rw);
+    own.template load<true>(static_cast<const char*>(a.x) + r * a.ldx * es<DT>(), xw);
+    own.template load<true>(static_cast<const char*>(a.dy) + r * a.lddy * es<DT>(), yw);
+    if (a.dres) own.template load<true>(static_cast<const char*>(a.dres) + r * a.lddres * es<DT>(), rw);
     mean = a.mean[r];
     rstd = a.rstd[r];
   };
@@ -234,8 +247,11 @@ __global__ __launch_bounds__(64 * W * R) void norm_bwd(NormGradArgs a) {
   constexpr bool AHEAD = W < 16;
   if (AHEAD && row < a.rows) fetch(row);
   int turn = 0;
-  for (; row < a.rows; row += step, turn ^= 1) {
-    if (!AHEAD) fetch(row);
+  // with more than one wave a row the slots meet at barriers: all run the first one's rounds
+  for (int64_t first = static_cast<int64_t>(blockIdx.x) * R; first < a.rows; first += step, row += step, turn ^= 1) {
+    const bool live = R == 1 || row < a.rows;
+    if (W == 1 && !live) break;
+    if (!AHEAD && live) fetch(row);
     float xh[kVals], u[kVals], o[kVals], su = 0.f, sux = 0.f;
     const float rs = rstd;
 #pragma unroll
@@ -244,7 +260,7 @@ __global__ __launch_bounds__(64 * W * R) void norm_bwd(NormGradArgs a) {
       xh[j] = (elem<DT>(xw[j / V], j % V) - mean) * rs;
       u[j] = AFFINE ? d * elem<DT>(gw[j / V], j % V) : d;
       o[j] = a.dres ? elem<DT>(rw[j / V], j % V) : 0.f;
-      if (AFFINE) {  // another lane's values are left out of the store below
+      if (AFFINE && live) {  // another lane's values are left out of the store below
         ag[j] += d * xh[j];
         ab[j] += d;
       }
@@ -253,11 +269,11 @@ __global__ __launch_bounds__(64 * W * R) void norm_bwd(NormGradArgs a) {
     }
     const int64_t next = row + step;
     if (AHEAD && next < a.rows) fetch(next);
-    row_add2<W>(su, sux, sh[turn], wave, lane);
+    row_add2<W>(su, sux, sh[slot][turn], wave, lane);
     const float c1 = su * inv_n, c2 = sux * inv_n;
 #pragma unroll
     for (int j = 0; j < kVals; ++j) o[j] += rs * (u[j] - c1 - xh[j] * c2);
-    own.store(static_cast<char*>(a.dx) + row * a.lddx * es<DT>(), o);
+    if (live) own.store(static_cast<char*>(a.dx) + row * a.lddx * es<DT>(), o);
   }
   if constexpr (AFFINE) {
     float* part = a.part + static_cast<int64_t>(blockIdx.x) * 2 * a.cols;
@@ -286,7 +302,7 @@ __global__ __launch_bounds__(64 * W * R) void norm_bwd(NormGradArgs a) {
 
 // dgamma / dbeta = the sums over `n` partial rows [n][2][cols], in a fixed
 // order: 16 columns of one of the two a workgroup, 64 lanes a column with
-// eight loads in flight each (768 columns, 512 parts: 4 us against 20 with 8
+// four loads in flight each (768 columns, 512 parts: 4 us against 20 with 8
 // lanes a column on 48 workgroups, a chain of loads).
 template <int DT>
 __global__ __launch_bounds__(1024) void norm_weights(const float* __restrict__ part, int n, int64_t cols, void* dgamma,
@@ -298,11 +314,11 @@ __global__ __launch_bounds__(1024) void norm_weights(const float* __restrict__ p
   float s = 0.f;
   if (c < cols) {
     const float* p = part + which * cols + c;
-    for (int i = q; i < n; i += 512) {
-      float v[8];
+    for (int i = q; i < n; i += 256) {
+      float v[4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = i + 64 * j < n ? p[static_cast<int64_t>(i + 64 * j) * 2 * cols] : 0.f;
-      s += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+      for (int j = 0; j < 4; ++j) v[j] = i + 64 * j < n ? p[static_cast<int64_t>(i + 64 * j) * 2 * cols] : 0.f;
+      s += (v[0] + v[1]) + (v[2] + v[3]);
     }
   }
   sh[q][c16] = s;
@@ -442,7 +458,7 @@ void launch_fwd(const NormArgs& all, hipStream_t s) {
 }
 
 bool long_rows(int64_t cols, int dtype) { return cols > kMaxCols || cols < (dtype == PDH_F32 ? 4 : 8); }
-int bwd_rows(int64_t cols) { return cols <= 1024 ? 4 : 1; }  // rows a workgroup takes at a time
+int bwd_rows(int64_t cols) { return cols <= 1024 ? 8 : cols <= 4096 ? 2 : 1; }  // rows a workgroup takes at a time
 
 // Partial rows of the weights' gradients.
 int64_t bwd_parts(int64_t rows, int64_t cols, int dtype) {
@@ -457,9 +473,9 @@ void launch_bwd(const NormGradArgs& a, unsigned groups, hipStream_t s) {
     norm_bwd_long<DT><<<dim3(static_cast<unsigned>(a.rows < kLongGroups ? a.rows : kLongGroups)), 1024, 0, s>>>(a);
     if (AFFINE) norm_cols_long<DT><<<dim3((a.cols + 63) / 64, groups), 256, 0, s>>>(a);
   } else if (a.cols <= 1024)
-    norm_bwd<DT, 1, 4, AFFINE><<<dim3(groups), 256, 0, s>>>(a);
+    norm_bwd<DT, 1, 8, AFFINE><<<dim3(groups), 512, 0, s>>>(a);
   else if (a.cols <= 4096)
-    norm_bwd<DT, 4, 1, AFFINE><<<dim3(groups), 256, 0, s>>>(a);
+    norm_bwd<DT, 4, 2, AFFINE><<<dim3(groups), 512, 0, s>>>(a);
   else if (a.cols <= 8192)
     norm_bwd<DT, 8, 1, AFFINE><<<dim3(groups), 512, 0, s>>>(a);
   else
