@@ -36,7 +36,9 @@ namespace {
 
 constexpr int kBK = 64;  // k depth of a tile: a 128-byte line of a k-contiguous operand
 constexpr uint32_t kOOB = 0x80000000u;  // past every buffer's extent: reads as zero
-constexpr int kPairs = 6;    // fp32: products of bf16 terms (term of a, term of b), smallest first
+// fp32: the products of bf16 terms, in order of growing size: terms (0, 2) (2, 0)
+// (1, 1) (0, 1) (1, 0) (0, 0) of (a, b), two bits each
+constexpr int kPairs = 6, kPairA = 0x0118, kPairB = 0x0052;
 
 // A 16-bit operand: rows of `pitch` bytes; k-contiguous (a row holds one m's or
 // n's k values) or not (a row holds one k's m or n values). fp32 operands lie
@@ -84,13 +86,15 @@ __device__ __forceinline__ Tile tile_of(const TileArgs& a, uint32_t id) {
   return t;
 }
 
-// A workgroup: WM x WN waves of 32 TM (m) x 32 TN (n). LDS holds two k tiles
-// of a and one of b: 80 KB for 256 x 128, two workgroups a compute unit.
-template <int WM_, int WN_, int TM_, int TN_>
+// A workgroup: WM x WN waves of 32 TM (m) x 32 TN (n). NS 0: LDS holds two k
+// tiles of a and one of b (80 KB for 256 x 128, two workgroups a compute unit);
+// otherwise NS k tiles of both.
+template <int WM_, int WN_, int TM_, int TN_, int NS_>
 struct Config {
-  static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_;
+  static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_, NS = NS_;
   static constexpr int NW = WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN, THREADS = 64 * NW;
-  static constexpr int LDS_A = BM * kBK * 2, LDS_B = BN * kBK * 2, LDS = 2 * LDS_A + LDS_B;
+  static constexpr int LDS_A = BM * kBK * 2, LDS_B = BN * kBK * 2;
+  static constexpr int LDS = NS ? NS * (LDS_A + LDS_B) : 2 * LDS_A + LDS_B;
 };
 
 // One operand's side of the loop. R: its rows in the tile (BM or BN), T: a
@@ -104,7 +108,7 @@ struct Side {
   static_assert(BLOCKS * 1024 * NW == R * kBK * 2 && NW % 4 == 0, "whole direct loads");
   uint32_t voff, vtail;  // the lane's byte offset in a direct load; the same in a ragged last k tile
   uint32_t pitch;
-  int read[T][KS];       // LDS offsets of the lane's fragments (without the tr read's second half)
+  int read[KC ? KS : T];  // LDS offsets of the lane's fragments: block 0's, or step 0's, without the tr read's second half
 
   // 16-byte slots are XOR-swizzled so that neither the b128 reads (16 lanes a cycle, the
   // quads of one parity in each half wave) nor the tr reads (32 lanes) meet a bank twice.
@@ -119,21 +123,20 @@ struct Side {
     const int row = lane / SLOTS, chunk = (lane % SLOTS) ^ swz(ROWS * w + row);
     voff = row * pitch + (chunk << 4);
     vtail = !KC || 8 * chunk < ktail ? voff : kOOB;  // (k rows past the end lie past the extent)
+    if constexpr (KC) {  // a block is 32 rows on: the same swizzle
+      const int r = lane & 31, g = lane >> 5;
+      const int at = 32 * wq * T + (PERM ? 16 * ((r >> 2) & 1) + 4 * (r >> 3) + (r & 3) : r);
 #pragma unroll
-    for (int t = 0; t < T; ++t)
+      for (int ks = 0; ks < KS; ++ks) read[ks] = at * PITCH + (((2 * ks + g) ^ swz(at)) << 4);
+    } else {  // a step is 16 k rows on: the same swizzle
+      const int G = lane >> 4, i4 = (lane >> 2) & 3, q = 4 * (G & 1) + (lane & 3);
+      const int kr = 8 * (G >> 1) + i4;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        if constexpr (KC) {
-          const int r = lane & 31, g = lane >> 5;
-          const int at = 32 * (wq * T + t) + (PERM ? 16 * ((r >> 2) & 1) + 4 * (r >> 3) + (r & 3) : r);
-          read[t][ks] = at * PITCH + (((2 * ks + g) ^ swz(at)) << 4);
-        } else {
-          const int G = lane >> 4, i4 = (lane >> 2) & 3, q = 4 * (G & 1) + (lane & 3);
-          const int kr = 16 * ks + 8 * (G >> 1) + i4;
-          const int col = 32 * (wq * T + t) + (PERM ? 16 * (q & 1) + 4 * (q >> 1) : 4 * q);
-          read[t][ks] = kr * PITCH + (((col >> 3) ^ swz(kr)) << 4) + ((col >> 2) & 1) * 8;
-        }
+      for (int t = 0; t < T; ++t) {
+        const int col = 32 * (wq * T + t) + (PERM ? 16 * (q & 1) + 4 * (q >> 1) : 4 * q);
+        read[t] = kr * PITCH + (((col >> 3) ^ swz(kr)) << 4) + ((col >> 2) & 1) * 8;
       }
+    }
   }
 
   // Direct loads of k columns k0 .. k0 + 63 of rows r0 .. r0 + R - 1 (`rows` of them in the operand, `k` columns).
@@ -161,9 +164,10 @@ struct Side {
 
   __device__ __forceinline__ u32x4 frag(const unsigned char* tile, int t, int ks) const {
     if constexpr (KC) {
-      return *reinterpret_cast<const u32x4*>(tile + read[t][ks]);
+      return *reinterpret_cast<const u32x4*>(tile + read[ks] + 32 * t * PITCH);
     } else {
-      const u32x2 lo = ds_read_tr16(tile + read[t][ks]), hi = ds_read_tr16(tile + read[t][ks] + 4 * PITCH);
+      const unsigned char* p = tile + read[t] + 16 * ks * PITCH;
+      const u32x2 lo = ds_read_tr16(p), hi = ds_read_tr16(p + 4 * PITCH);
       return u32x4{lo.x, lo.y, hi.x, hi.y};
     }
   }
@@ -181,6 +185,9 @@ struct Side {
 // this 544; 4096 x 4096: 1640, 1420, the matrix pipe 66% busy at the 1.62 GHz
 // that the part then holds); 256 x 256 tiles of eight waves, one workgroup a
 // unit: 610, 1450; fragments read a step ahead across the barrier: no change.
+// Workgroups that walk over their tiles, the next one's first loads under the
+// last products, fall out of step, and neighbours no longer find each other's
+// panels in L2: 1420 -> 1515, 560 -> 593 (so does any other staggering).
 template <int DT, typename C, bool KA, bool KB, bool SPLIT>
 __device__ __forceinline__ void xent_tile(const TileArgs& a, unsigned char* smem, f32x16 (&acc)[C::TM][C::TN], int m0,
                                           int n0, int64_t k0, int64_t k1) {
@@ -199,12 +206,11 @@ __device__ __forceinline__ void xent_tile(const TileArgs& a, unsigned char* smem
   unsigned char* const bt = smem + 2 * C::LDS_A;
   int fpair = 0, fkt = 0;  // the k tile to fetch
   auto fetch_a = [&](int buf) __attribute__((always_inline)) {
-    // pairs in order of growing size: terms (0, 2) (2, 0) (1, 1) (0, 1) (1, 0) (0, 0), two bits each
-    const int64_t pa = SPLIT ? (0x0118 >> (2 * fpair)) & 3 : 0;
+    const int64_t pa = SPLIT ? (kPairA >> (2 * fpair)) & 3 : 0;
     sa.fetch(a.a, pa, m0, a.m, k0 + static_cast<int64_t>(fkt) * kBK, k1, lds0 + buf * C::LDS_A, w);
   };
   auto fetch_b = [&]() __attribute__((always_inline)) {
-    const int64_t pb = SPLIT ? (0x0052 >> (2 * fpair)) & 3 : 0;
+    const int64_t pb = SPLIT ? (kPairB >> (2 * fpair)) & 3 : 0;
     sb.fetch(a.b, pb, n0, a.n, k0 + static_cast<int64_t>(fkt) * kBK, k1, lds0 + 2 * C::LDS_A, w);
     if (++fkt == nkt) fkt = 0, ++fpair;
   };
@@ -244,53 +250,121 @@ __device__ __forceinline__ void xent_tile(const TileArgs& a, unsigned char* smem
   }
 }
 
+// One tile by k tiles that are C::NS deep in LDS: for tiles whose products take
+// less than a load's latency. acc as above.
+template <int DT, typename C, bool KA, bool KB, bool SPLIT>
+__device__ __forceinline__ void deep_tile(const TileArgs& a, unsigned char* smem, f32x16 (&acc)[C::TM][C::TN], int m0,
+                                          int n0, int64_t k0, int64_t k1) {
+  constexpr int TM = C::TM, TN = C::TN, KS = kBK / 16, NS = C::NS, STAGE = C::LDS_A + C::LDS_B;
+  const int lane = threadIdx.x & 63, w = wave_id(), wm = w / C::WN, wn = w % C::WN;
+  const int ktail = static_cast<int>((k1 - k0) % kBK);
+  const Side<C::BM, TM, C::NW, KA, true> sa(a.a, wm, lane, w, ktail);
+  const Side<C::BN, TN, C::NW, KB, false> sb(a.b, wn, lane, w, ktail);
+  constexpr int PER = decltype(sa)::BLOCKS + decltype(sb)::BLOCKS;
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = f32x16{};
+  const int nkt = static_cast<int>((k1 - k0 + kBK - 1) / kBK);
+  const int steps = SPLIT ? nkt * kPairs : nkt;
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(smem));
+  int fpair = 0, fkt = 0, fbuf = 0, buf = 0;
+  auto fetch = [&]() __attribute__((always_inline)) {
+    const int64_t pa = SPLIT ? (kPairA >> (2 * fpair)) & 3 : 0, pb = SPLIT ? (kPairB >> (2 * fpair)) & 3 : 0;
+    const int64_t kk = k0 + static_cast<int64_t>(fkt) * kBK;
+    sa.fetch(a.a, pa, m0, a.m, kk, k1, lds0 + fbuf * STAGE, w);
+    sb.fetch(a.b, pb, n0, a.n, kk, k1, lds0 + fbuf * STAGE + C::LDS_A, w);
+    fbuf = fbuf + 1 == NS ? 0 : fbuf + 1;
+    if (++fkt == nkt) fkt = 0, ++fpair;
+  };
+#pragma unroll
+  for (int i = 0; i < NS - 1; ++i)
+    if (i < steps) fetch();
+  for (int st = 0; st < steps; ++st, buf = buf + 1 == NS ? 0 : buf + 1) {
+    if (st + NS - 2 < steps)  // all but the NS - 2 later tiles' loads have landed
+      __builtin_amdgcn_s_waitcnt(0x0f70 | (((NS - 2) * PER) & 15) | ((((NS - 2) * PER) >> 4) << 14));
+    else
+      wait_vmcnt0();
+    __syncthreads();  // every wave's loads of this tile are done; everyone has finished the tile before
+    if (st + NS - 1 < steps) fetch();
+    const unsigned char* at = smem + buf * STAGE;
+    u32x4 af[KS][TM], bf[KS][TN];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+      for (int t = 0; t < TM; ++t) af[ks][t] = sa.frag(at, t, ks);
+#pragma unroll
+      for (int t = 0; t < TN; ++t) bf[ks][t] = sb.frag(at + C::LDS_A, t, ks);
+    }
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = mfma32_dt<DT>(af[ks][i], bf[ks][j], acc[i][j]);
+  }
+}
+
 // Stores a wave's 32 n rows (n tile j) of its 32 TM m columns, ES bytes each:
 // every lane has a row's 16-column runs (`v`: as stored), which would make
-// stores of 16 bytes in 64 places; through the wave's own part of LDS each
-// instruction stores whole lines instead. `left` columns are inside the output,
-// `rows` of the rows. add: fp32 only, to what is there. The caller has passed a
-// barrier since the tile loop.
+// stores of 16 bytes in 64 places; through 8 KB of LDS of the wave's own (4 KB
+// for 16-bit rows of 64) each instruction stores whole lines instead, the rows'
+// 16-byte slots XOR-swizzled so that neither side meets a bank twice. `left`
+// columns are inside the output, `rows` of the rows. add: fp32 only, to what is
+// there. Every wave has left the tile loop.
 template <int ES, int TM>
-constexpr int put_pitch() {
-  return TM * 32 * ES + 16;  // 16 bytes on: rows start at different banks
+constexpr int put_rows_at_once() {
+  return ES == 4 ? 16 : 32;
+}
+template <int ES, int TM>
+constexpr int put_bytes() {
+  return put_rows_at_once<ES, TM>() * TM * 32 * ES;
 }
 template <int ES, int TM>
 __device__ __forceinline__ void put_rows(unsigned char* lds, const u32x4 (&v)[TM][ES], char* out, int64_t ld_b, int rows,
                                          int left, bool add) {
-  constexpr int P = put_pitch<ES, TM>(), CH = TM * 32 * ES / 16, VE = 16 / ES;
-  const int lane = threadIdx.x & 63;
-  unsigned char* mine = lds + (lane & 31) * P + (lane >> 5) * 16 * ES;
-  __builtin_amdgcn_wave_barrier();
+  constexpr int P = TM * 32 * ES, CH = P / 16, VE = 16 / ES, PASS = put_rows_at_once<ES, TM>();
+  constexpr int SW = CH < 16 ? CH - 1 : 15;
+  const int lane = threadIdx.x & 63, mine = lane & 31;
 #pragma unroll
-  for (int i = 0; i < TM; ++i)
+  for (int r0 = 0; r0 < 32; r0 += PASS) {
+    __builtin_amdgcn_wave_barrier();  // the wave's own rows: LDS keeps its order, no workgroup barrier
+    if (PASS == 32 || (mine >= r0 && mine < r0 + PASS)) {
 #pragma unroll
-    for (int q = 0; q < ES; ++q) *reinterpret_cast<u32x4*>(mine + i * 32 * ES + q * 16) = v[i][q];
-  __builtin_amdgcn_wave_barrier();  // the wave's own rows: LDS keeps its order, no workgroup barrier
+      for (int i = 0; i < TM; ++i)
 #pragma unroll
-  for (int it = 0; it < 32 * CH / 64; ++it) {
-    const int idx = it * 64 + lane, row = idx / CH, ch = idx % CH;
-    const u32x4 w = *reinterpret_cast<const u32x4*>(lds + row * P + ch * 16);
-    char* o = out + row * ld_b + ch * 16;
-    if (row >= rows) continue;
-    if ((ch + 1) * VE <= left) {
-      if constexpr (ES == 4) {
-        f32x4 x = __builtin_bit_cast(f32x4, w);
-        if (add) x += *reinterpret_cast<const f32x4u*>(o);
-        *reinterpret_cast<f32x4u*>(o) = x;
-      } else {
-        __builtin_nontemporal_store(__builtin_bit_cast(u32x4h, w), reinterpret_cast<u32x4h*>(o));
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < VE - 1; ++e)
-        if (ch * VE + e < left) {
-          if constexpr (ES == 4) {
-            float* f = reinterpret_cast<float*>(o) + e;
-            *f = add ? *f + __uint_as_float(w[e]) : __uint_as_float(w[e]);
-          } else {
-            reinterpret_cast<uint16_t*>(o)[e] = static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)));
-          }
+        for (int q = 0; q < ES; ++q) {
+          const int ch = (i * 32 + 16 * (lane >> 5)) * ES / 16 + q;
+          *reinterpret_cast<u32x4*>(lds + (mine - r0) * P + ((ch ^ (mine & SW)) << 4)) = v[i][q];
         }
+    }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int it = 0; it < PASS * CH / 64; ++it) {
+      const int idx = it * 64 + lane, r = idx / CH, ch = idx % CH, row = r0 + r;
+      const u32x4 w = *reinterpret_cast<const u32x4*>(lds + r * P + ((ch ^ (row & SW)) << 4));
+      char* o = out + row * ld_b + ch * 16;
+      if (row >= rows) continue;
+      if ((ch + 1) * VE <= left) {
+        if constexpr (ES == 4) {
+          f32x4 x = __builtin_bit_cast(f32x4, w);
+          if (add) x += *reinterpret_cast<const f32x4u*>(o);
+          *reinterpret_cast<f32x4u*>(o) = x;
+        } else {
+          __builtin_nontemporal_store(__builtin_bit_cast(u32x4h, w), reinterpret_cast<u32x4h*>(o));
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < VE - 1; ++e)
+          if (ch * VE + e < left) {
+            if constexpr (ES == 4) {
+              float* f = reinterpret_cast<float*>(o) + e;
+              *f = add ? *f + __uint_as_float(w[e]) : __uint_as_float(w[e]);
+            } else {
+              reinterpret_cast<uint16_t*>(o)[e] = static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)));
+            }
+          }
+      }
     }
   }
 }
@@ -304,8 +378,11 @@ __device__ __forceinline__ u32x4 pack8(const float* q) {
   return w;
 }
 
-using Big = Config<2, 2, 4, 2>;    // 256 x 128 tiles
-using Small = Config<2, 2, 2, 1>;  // 128 x 64: a quarter of one
+using Big = Config<2, 2, 4, 2, 0>;    // 256 x 128 tiles
+using Small = Config<2, 2, 2, 1, 3>;  // 128 x 64: a quarter of one
+static_assert(Small::LDS <= Big::LDS, "one kernel runs both");
+static_assert(4 * put_bytes<2, 4>() <= Big::LDS_A && 4 * put_bytes<4, 4>() <= Big::LDS_A && 4 * put_bytes<2, 2>() <= Small::LDS,
+              "the stores' rows fit");
 constexpr int kStrip = 128;        // vocabulary entries of a forward's strip
 
 // The logits' tiles, [0, big) whole and the rest quartered (`small` of them),
@@ -314,18 +391,25 @@ struct LogitTiles {
   TileArgs t;  // a: w (m: vocabulary), b: x (n: tokens)
   int big, small;
 };
-template <typename F, typename G>
-__device__ __forceinline__ void logit_tile(const LogitTiles& l, F&& whole, G&& quarter) {
+template <int DT, bool SPLIT, typename P, typename F>
+__device__ __forceinline__ void logit_tile(const LogitTiles& l, unsigned char* smem, const P& p, const F& epilogue) {
   bool second;
   const int id = run_id(l.big, l.small, second);
   if (id < 0) return;
   const Tile t = tile_of(l.t, second ? l.big + id / 4 : id);
-  const int m0 = t.m * Big::BM, n0 = t.n * Big::BN;
+  int m0 = t.m * Big::BM, n0 = t.n * Big::BN;
   if (!second) {
-    whole(m0, n0);
+    f32x16 acc[Big::TM][Big::TN];
+    const auto info = epilogue.template info<Big>(p, n0);
+    xent_tile<DT, Big, true, true, SPLIT>(l.t, smem, acc, m0, n0, 0, l.t.k);
+    epilogue.template store<Big>(p, acc, info, m0, n0, smem);
   } else {
-    const int mq = m0 + (id & 1) * Small::BM, nq = n0 + ((id >> 1) & 1) * Small::BN;
-    if (mq < l.t.m && nq < l.t.n) quarter(mq, nq);
+    m0 += (id & 1) * Small::BM, n0 += ((id >> 1) & 1) * Small::BN;
+    if (m0 >= l.t.m || n0 >= l.t.n) return;
+    f32x16 acc[Small::TM][Small::TN];
+    const auto info = epilogue.template info<Small>(p, n0);
+    deep_tile<DT, Small, true, true, SPLIT>(l.t, smem, acc, m0, n0, 0, l.t.k);
+    epilogue.template store<Small>(p, acc, info, m0, n0, smem);
   }
 }
 
@@ -346,79 +430,97 @@ __device__ __forceinline__ void join(float& m, float& s, float om, float os) {
   m = mn;
 }
 
-template <int DT, typename C, bool SPLIT>
-__device__ __forceinline__ void fwd_tile(const FwdArgs& p, unsigned char* smem, int m0, int n0) {
-  constexpr int TM = C::TM, TN = C::TN;
-  const int lane = threadIdx.x & 63, w = wave_id(), wm = w / C::WN, wn = w % C::WN, g = lane >> 5;
-  f32x16 acc[TM][TN];
-  xent_tile<DT, C, true, true, SPLIT>(p.l.t, smem, acc, m0, n0, 0, p.l.t.k);
-  const int vocab = p.l.t.m, tokens = p.l.t.n;
-  const int vw = m0 + 32 * wm * TM, v0 = vw + 16 * g;  // the wave's entries, the lane's first
-  float mxs[TN], sums[TN];
+// What the epilogue needs of a lane's tokens, read before the products.
+template <int TN>
+struct FwdInfo {
+  int target[TN];  // -1: none
+};
+
+struct FwdEpilogue {
+  template <typename C>
+  __device__ __forceinline__ FwdInfo<C::TN> info(const FwdArgs& p, int n0) const {
+    FwdInfo<C::TN> f;
 #pragma unroll
-  for (int j = 0; j < TN; ++j) {
-    const int n = n0 + 32 * (wn * TN + j) + (lane & 31);
-    const int64_t tl = (n < tokens ? p.targets[n] : -1) - v0;
-    if (vw + 32 * TM > vocab) {  // entries past the vocabulary weigh nothing
-#pragma unroll
-      for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (v0 + 32 * i + e >= vocab) acc[i][j][e] = -__builtin_inff();
+    for (int j = 0; j < C::TN; ++j) {
+      const int n = n0 + 32 * ((wave_id() % C::WN) * C::TN + j) + (threadIdx.x & 31);
+      const int64_t t = n < p.l.t.n ? p.targets[n] : -1;
+      f.target[j] = t >= 0 && t < p.l.t.m ? static_cast<int>(t) : -1;
     }
-    float mx = -__builtin_inff();
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, acc[i][j][e]);
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    const float base = mx == -__builtin_inff() ? 0.f : mx * kLog2e;
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) s += fast_exp2(__builtin_fmaf(acc[i][j][e], kLog2e, -base));
-    s += __shfl_xor(s, 32, 64);
-    mxs[j] = mx, sums[j] = s;
-    if (tl >= 0 && tl < 32 * TM && v0 + tl < vocab && (tl & 16) == 0) {  // this lane holds the target's logit
-      float z = 0.f;
-#pragma unroll
-      for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (tl == 32 * i + e) z = acc[i][j][e];
-      p.zt[n] = z;
-    }
+    return f;
   }
-  if constexpr (32 * TM < kStrip) {  // the strip's two waves meet in LDS
-    static_assert(64 * TM == kStrip && C::WM == 2, "two waves a strip");
-    __syncthreads();  // the tile loop's last reads are over
-    float2* sh = reinterpret_cast<float2*>(smem);
-    if (wm == 1 && g == 0)
-#pragma unroll
-      for (int j = 0; j < TN; ++j) sh[(wn * TN + j) * 32 + lane] = make_float2(mxs[j], sums[j]);
-    __syncthreads();
-    if (wm == 1) return;
+  template <typename C>
+  __device__ __forceinline__ void store(const FwdArgs& p, f32x16 (&acc)[C::TM][C::TN], const FwdInfo<C::TN>& f, int m0,
+                                        int n0, unsigned char* lds) const {
+    constexpr int TM = C::TM, TN = C::TN;
+    const int lane = threadIdx.x & 63, w = wave_id(), wm = w / C::WN, wn = w % C::WN, g = lane >> 5;
+    const int vocab = p.l.t.m, tokens = p.l.t.n;
+    const int vw = m0 + 32 * wm * TM, v0 = vw + 16 * g;  // the wave's entries, the lane's first
+    float mxs[TN], sums[TN], zs[TN];
+    bool hit[TN];
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
-      const float2 o = sh[(wn * TN + j) * 32 + (lane & 31)];
-      join(mxs[j], sums[j], o.x, o.y);
+      if (vw + 32 * TM > vocab) {  // entries past the vocabulary weigh nothing
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (v0 + 32 * i + e >= vocab) acc[i][j][e] = -__builtin_inff();
+      }
+      float mx = -__builtin_inff();
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, acc[i][j][e]);
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const float base = mx == -__builtin_inff() ? 0.f : mx * kLog2e;
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s += fast_exp2(__builtin_fmaf(acc[i][j][e], kLog2e, -base));
+      s += __shfl_xor(s, 32, 64);
+      mxs[j] = mx, sums[j] = s;
+      const int tl = f.target[j] - v0;
+      hit[j] = f.target[j] >= 0 && tl >= 0 && tl < 32 * TM && (tl & 16) == 0;
+      zs[j] = 0.f;
+      if (hit[j]) {  // this lane holds the target's logit
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (tl == 32 * i + e) zs[j] = acc[i][j][e];
+      }
+    }
+    if constexpr (32 * TM < kStrip) {  // the strip's two waves meet in LDS
+      static_assert(64 * TM == kStrip && C::WM == 2, "two waves a strip");
+      __syncthreads();  // the tile loop's last reads are over
+      float2* sh = reinterpret_cast<float2*>(lds);
+      if (wm == 1 && g == 0)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) sh[(wn * TN + j) * 32 + lane] = make_float2(mxs[j], sums[j]);
+      __syncthreads();
+      if (wm == 0) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          const float2 o = sh[(wn * TN + j) * 32 + (lane & 31)];
+          join(mxs[j], sums[j], o.x, o.y);
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int n = n0 + 32 * (wn * TN + j) + (lane & 31);
+      if (n < tokens && g == 0 && vw < vocab && (32 * TM == kStrip || wm == 0))
+        p.part[static_cast<int64_t>(vw / kStrip) * tokens + n] = make_float2(mxs[j], sums[j]);
+      if (hit[j]) p.zt[n] = zs[j];
     }
   }
-#pragma unroll
-  for (int j = 0; j < TN; ++j) {
-    const int n = n0 + 32 * (wn * TN + j) + (lane & 31);
-    if (n < tokens && g == 0 && vw < vocab)
-      p.part[static_cast<int64_t>(vw / kStrip) * tokens + n] = make_float2(mxs[j], sums[j]);
-  }
-}
+};
 
 template <int DT, bool SPLIT>
 __global__ __launch_bounds__(256, 2) void xent_fwd(FwdArgs p) {
   __shared__ __attribute__((aligned(1024))) unsigned char smem[Big::LDS];
-  logit_tile(
-      p.l, [&](int m0, int n0) { fwd_tile<DT, Big, SPLIT>(p, smem, m0, n0); },
-      [&](int m0, int n0) { fwd_tile<DT, Small, SPLIT>(p, smem, m0, n0); });
+  logit_tile<DT, SPLIT>(p.l, smem, p, FwdEpilogue{});
 }
 
 // Joins the strips of 8 tokens, 32 lanes a token: lse and loss.
@@ -459,67 +561,88 @@ struct GradArgs {
   int64_t vocab, ignore;
 };
 
-template <int DT, typename C, bool SPLIT>
-__device__ __forceinline__ void dz_tile(const GradArgs& p, unsigned char* smem, int m0, int n0) {
-  constexpr int TM = C::TM, TN = C::TN;
-  const int lane = threadIdx.x & 63, w = wave_id(), wm = w / C::WN, wn = w % C::WN, g = lane >> 5;
-  f32x16 acc[TM][TN];
-  xent_tile<DT, C, true, true, SPLIT>(p.l.t, smem, acc, m0, n0, 0, p.l.t.k);
-  __syncthreads();  // the tile loop's last reads are over: LDS serves the stores
-  unsigned char* lds = smem + w * 32 * put_pitch<2, TM>();
-  static_assert(C::NW * 32 * put_pitch<2, TM>() <= C::LDS, "the stores' rows fit");
-  const int cw = m0 + 32 * wm * TM;  // the wave's first column of dz
+constexpr int kNoToken = INT32_MIN;
+template <int TN>
+struct DzInfo {
+  int target[TN];  // from the piece's first entry; kNoToken: an ignored token
+  float g[TN], lse2[TN];
+};
+
+template <int DT, bool SPLIT>
+struct DzEpilogue {
+  template <typename C>
+  __device__ __forceinline__ DzInfo<C::TN> info(const GradArgs& p, int n0) const {
+    DzInfo<C::TN> f;
 #pragma unroll
-  for (int j = 0; j < TN; ++j) {
-    const int nw = n0 + 32 * (wn * TN + j), n = nw + (lane & 31);
-    const int64_t tg = n < p.l.t.n ? p.targets[n] : -1;
-    const bool live = tg >= 0 && tg < p.vocab && tg != p.ignore;
-    const float gn = live ? p.g[n] : 0.f, l2 = live ? p.lse[n] * kLog2e : 0.f;
-    const int64_t tl = live ? tg - p.v0 - (cw + 16 * g) : -1;
-#pragma unroll
-    for (int i = 0; i < TM; ++i) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = fast_exp2(__builtin_fmaf(acc[i][j][e], kLog2e, -l2));
-      const int64_t at = tl - 32 * i;
-      if (at >= 0 && at < 16) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (at == e) acc[i][j][e] -= 1.f;
-      }
-      // an ignored token has no gradient whatever its logits are; entries past the vocabulary are zero
-      const int c = cw + 32 * i + 16 * g;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = live && c + e < p.l.t.m ? acc[i][j][e] * gn : 0.f;
+    for (int j = 0; j < C::TN; ++j) {
+      const int n = n0 + 32 * ((wave_id() % C::WN) * C::TN + j) + (threadIdx.x & 31);
+      const int64_t t = n < p.l.t.n ? p.targets[n] : -1;
+      const bool live = t >= 0 && t < p.vocab && t != p.ignore;
+      f.target[j] = live ? static_cast<int>(t - p.v0) : kNoToken;
+      f.g[j] = live ? p.g[n] : 0.f;
+      f.lse2[j] = live ? p.lse[n] * kLog2e : 0.f;
     }
+    return f;
+  }
+  template <typename C>
+  __device__ __forceinline__ void store(const GradArgs& p, f32x16 (&acc)[C::TM][C::TN], const DzInfo<C::TN>& f, int m0,
+                                        int n0, unsigned char* lds) const {
+    constexpr int TM = C::TM, TN = C::TN;
+    const int lane = threadIdx.x & 63, w = wave_id(), wm = w / C::WN, wn = w % C::WN, g = lane >> 5;
+    const int cw = m0 + 32 * wm * TM;  // the wave's first column of dz
 #pragma unroll
-    for (int pl = 0; pl < (SPLIT ? 3 : 1); ++pl) {
-      u32x4 v[TM][2];
+    for (int j = 0; j < TN; ++j) {
+      const bool live = f.target[j] != kNoToken;
+      const int tl = live ? f.target[j] - (cw + 16 * g) : -1;
 #pragma unroll
-      for (int i = 0; i < TM; ++i)
+      for (int i = 0; i < TM; ++i) {
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          float x[8];
+        for (int e = 0; e < 16; ++e) acc[i][j][e] = fast_exp2(__builtin_fmaf(acc[i][j][e], kLog2e, -f.lse2[j]));
+        const int at = tl - 32 * i;
+        if (at >= 0 && at < 16) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = acc[i][j][8 * q + e];
-          v[i][q] = pack8<DT>(x);
-          if constexpr (SPLIT) {  // what this term leaves (exact)
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              acc[i][j][8 * q + e] -= __uint_as_float(e & 1 ? v[i][q][e >> 1] & 0xffff0000u : v[i][q][e >> 1] << 16);
-          }
+          for (int e = 0; e < 16; ++e)
+            if (at == e) acc[i][j][e] -= 1.f;
         }
-      put_rows<2, TM>(lds, v, reinterpret_cast<char*>(p.dz + pl * p.plane + static_cast<int64_t>(nw) * p.ldz + cw),
-                      p.ldz * 2, p.l.t.n - nw, static_cast<int>(p.ldz) - cw, false);
+        // an ignored token has no gradient whatever its logits are; entries past the vocabulary are zero
+        const int c = cw + 32 * i + 16 * g;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][j][e] = live && c + e < p.l.t.m ? acc[i][j][e] * f.g[j] : 0.f;
+      }
+    }
+    __syncthreads();  // the tile loop's last reads are over: LDS serves the stores
+    lds += w * put_bytes<2, TM>();
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int nw = n0 + 32 * (wn * TN + j);
+#pragma unroll
+      for (int pl = 0; pl < (SPLIT ? 3 : 1); ++pl) {
+        u32x4 v[TM][2];
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = acc[i][j][8 * q + e];
+            v[i][q] = pack8<DT>(x);
+            if constexpr (SPLIT) {  // what this term leaves (exact)
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                acc[i][j][8 * q + e] -= __uint_as_float(e & 1 ? v[i][q][e >> 1] & 0xffff0000u : v[i][q][e >> 1] << 16);
+            }
+          }
+        put_rows<2, TM>(lds, v, reinterpret_cast<char*>(p.dz + pl * p.plane + static_cast<int64_t>(nw) * p.ldz + cw),
+                        p.ldz * 2, p.l.t.n - nw, static_cast<int>(p.ldz) - cw, false);
+      }
     }
   }
-}
+};
 
 template <int DT, bool SPLIT>
 __global__ __launch_bounds__(256, 2) void xent_dz(GradArgs p) {
   __shared__ __attribute__((aligned(1024))) unsigned char smem[Big::LDS];
-  logit_tile(
-      p.l, [&](int m0, int n0) { dz_tile<DT, Big, SPLIT>(p, smem, m0, n0); },
-      [&](int m0, int n0) { dz_tile<DT, Small, SPLIT>(p, smem, m0, n0); });
+  logit_tile<DT, SPLIT>(p.l, smem, p, DzEpilogue<DT, SPLIT>{});
 }
 
 // The gradient products, both in one launch so that their tiles fill the chip
@@ -547,8 +670,7 @@ __device__ __forceinline__ void prod_tile(const TileArgs& a, int id, unsigned ch
   const int64_t k0 = static_cast<int64_t>(t.slice) * a.kslice, k1 = k0 + a.kslice < a.k ? k0 + a.kslice : a.k;
   xent_tile<DT, C, false, KB, SPLIT>(a, smem, acc, m0, n0, k0, k1);
   __syncthreads();  // the tile loop's last reads are over: LDS serves the stores
-  unsigned char* lds = smem + w * 32 * put_pitch<ES, TM>();
-  static_assert(C::NW * 32 * put_pitch<ES, TM>() <= C::LDS, "the stores' rows fit");
+  unsigned char* lds = smem + w * put_bytes<ES, TM>();
   const float sc = scale ? *scale : 1.f;
   const int cw = m0 + 32 * wm * TM;
 #pragma unroll
@@ -594,8 +716,16 @@ __global__ __launch_bounds__(256) void xent_dx(const float* __restrict__ part, v
   const int c = static_cast<int>(i - n * per) * 4;
   if (n >= rows || c >= d) return;
   const float* p = part + n * ld + c;
-  f32x4 s = *reinterpret_cast<const f32x4*>(p);
-  for (int q = 1; q < slices; ++q) s += *reinterpret_cast<const f32x4*>(p + q * slice);
+  f32x4 s{};
+  for (int q0 = 0; q0 < slices; q0 += 8) {  // eight loads in flight, added in order
+    f32x4 v[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (q0 + q < slices) v[q] = *reinterpret_cast<const f32x4*>(p + (q0 + q) * slice);
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (q0 + q < slices) s += v[q];
+  }
   if (scale) s *= *scale;
 #pragma unroll
   for (int e = 0; e < 4; ++e)

@@ -54,19 +54,19 @@ def _perm(r):
 
 
 def _reads(R, T, kc, perm, wq, t, ks):
-    """The lanes' LDS addresses (b128, or the first tr read's) of a fragment."""
+    """The lanes' LDS addresses (b128, or the first tr read's) of a fragment: block 0's 32 t rows on, or step 0's 16 ks k rows on."""
     out = []
     for lane in range(64):
         if kc:
             r, g = lane & 31, lane >> 5
-            row = 32 * (wq * T + t) + (_perm(r) if perm else r)
-            out.append(row * BK * 2 + (((2 * ks + g) ^ _swz(R, kc, row)) << 4))
+            row = 32 * wq * T + (_perm(r) if perm else r)
+            out.append(row * BK * 2 + (((2 * ks + g) ^ _swz(R, kc, row)) << 4) + 32 * t * BK * 2)
         else:
             G, i4 = lane >> 4, (lane >> 2) & 3
             q = 4 * (G & 1) + (lane & 3)
-            kr = 16 * ks + 8 * (G >> 1) + i4
+            kr = 8 * (G >> 1) + i4
             col = 32 * (wq * T + t) + (16 * (q & 1) + 4 * (q >> 1) if perm else 4 * q)
-            out.append(kr * R * 2 + (((col >> 3) ^ _swz(R, kc, kr)) << 4) + ((col >> 2) & 1) * 8)
+            out.append(kr * R * 2 + (((col >> 3) ^ _swz(R, kc, kr)) << 4) + ((col >> 2) & 1) * 8 + 16 * ks * R * 2)
     return out
 
 
@@ -161,16 +161,34 @@ def test_every_tile_is_taken_once():
 
 @pytest.mark.parametrize("es,tm", [(2, 4), (4, 4), (2, 2)])
 def test_stored_rows_leave_lds_as_they_came(es, tm):
-    """put_rows: each lane's sixteen-column runs come back as whole rows."""
-    pitch, ch = tm * 32 * es + 16, tm * 32 * es // 16
-    lds = {}
-    for lane, i, q in itertools.product(range(64), range(tm), range(es)):
-        at = (lane & 31) * pitch + (lane >> 5) * 16 * es + i * 32 * es + 16 * q
-        assert at not in lds and at + 16 <= 32 * pitch
-        lds[at] = (lane & 31, 32 * i + 16 * (lane >> 5) + 16 // es * q)  # row, first column
+    """put_rows: each lane's sixteen-column runs come back as whole rows, from a part of LDS no larger than its own,
+    without bank conflicts."""
+    pitch, ch = tm * 32 * es, tm * 32 * es // 16
+    at_once, sw = (16 if es == 4 else 32), (ch - 1 if ch < 16 else 15)
+    assert 4 * at_once * pitch <= 32768
     seen = set()
-    for it, lane in itertools.product(range(32 * ch // 64), range(64)):
-        row, c = divmod(it * 64 + lane, ch)
-        assert lds[row * pitch + 16 * c] == (row, c * 16 // es)
-        seen.add((row, c))
+    for r0 in range(0, 32, at_once):
+        lds = {}
+        for i, q in itertools.product(range(tm), range(es)):
+            offs = {}
+            for lane in range(64):
+                mine = lane & 31
+                if not r0 <= mine < r0 + at_once:
+                    continue
+                c = (i * 32 + 16 * (lane >> 5)) * es // 16 + q
+                at = (mine - r0) * pitch + ((c ^ (mine & sw)) << 4)
+                assert at not in lds and at + 16 <= at_once * pitch
+                lds[at] = (mine, 32 * i + 16 * (lane >> 5) + 16 // es * q)  # row, first column
+                offs[lane] = at
+            if len(offs) == 64 and ch >= 16:
+                assert _ways([offs[lane] for lane in range(64)], 16) == 1
+        for it in range(at_once * ch // 64):
+            offs = []
+            for lane in range(64):
+                r, c = divmod(it * 64 + lane, ch)
+                row = r0 + r
+                offs.append(r * pitch + ((c ^ (row & sw)) << 4))
+                assert lds[offs[-1]] == (row, c * 16 // es)
+                seen.add((row, c))
+            assert ch < 16 or _ways(offs, 16) == 1
     assert len(seen) == 32 * ch
