@@ -734,47 +734,57 @@ __global__ __launch_bounds__(256) void xent_dx(const float* __restrict__ part, v
 
 // fp16's dz scale: 2^14 over the power of two above the largest |dloss| of a
 // live token. One workgroup; g[n] = dloss[n] times it, *inv its inverse.
-__global__ __launch_bounds__(1024) void xent_scale(const float* __restrict__ dloss, const int64_t* __restrict__ targets,
-                                                   int64_t n, int64_t vocab, int64_t ignore, float* __restrict__ g,
-                                                   float* __restrict__ inv) {
-  __shared__ float sh[16];
+struct ScaleArgs {
+  const float* dloss;  // NULL: none to do
+  const int64_t* targets;
+  int64_t n, vocab, ignore;
+  float* g;
+  float* inv;
+};
+__device__ __forceinline__ void scale_dloss(const ScaleArgs& p) {
+  __shared__ float sh[4];
   float mx = 0.f;
-  auto live = [&](int64_t t) { return t >= 0 && t < vocab && t != ignore; };
-  for (int64_t i = threadIdx.x; i < n; i += 1024)
-    if (live(targets[i])) mx = fmaxf(mx, fabsf(dloss[i]));
+  for (int64_t i = threadIdx.x; i < p.n; i += 256) {
+    const int64_t t = p.targets[i];
+    if (t >= 0 && t < p.vocab && t != p.ignore) mx = fmaxf(mx, fabsf(p.dloss[i]));
+  }
   mx = wave_max(mx);
   if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = mx;
   __syncthreads();
-  mx = sh[0];
-  for (int i = 1; i < 16; ++i) mx = fmaxf(mx, sh[i]);
+  mx = fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
   int e = 0;
   if (mx > 0.f && mx < __builtin_inff()) frexpf(mx, &e);  // mx < 2^e
   const float up = ldexpf(1.f, min(14 - e, 126));
-  for (int64_t i = threadIdx.x; i < n; i += 1024) g[i] = dloss[i] * up;
-  if (threadIdx.x == 0) *inv = ldexpf(1.f, -min(14 - e, 126));
+  for (int64_t i = threadIdx.x; i < p.n; i += 256) p.g[i] = p.dloss[i] * up;
+  if (threadIdx.x == 0) *p.inv = ldexpf(1.f, -min(14 - e, 126));
 }
 
 // An operand made fit for the direct loads: rows of `dp` (a multiple of 8)
 // 16-bit values, zero past d. fp32 rows become three planes of bf16 terms,
 // 16-bit ones of odd width, stride or alignment a padded copy.
+struct PackArgs {
+  const void* src;  // NULL: read in place
+  int64_t ld, rows;
+  int d, dp;
+  uint16_t* dst;
+  int64_t plane;
+};
 template <int DT>
-__global__ __launch_bounds__(256) void xent_pack(const void* __restrict__ src, int64_t ld, int64_t rows, int d, int dp,
-                                                 uint16_t* __restrict__ dst, int64_t plane) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int64_t per = dp / 8, n = i / per;
+__device__ __forceinline__ void pack_rows(const PackArgs& p, int64_t i) {
+  const int64_t per = p.dp / 8, n = i / per;
   const int c = static_cast<int>(i - n * per) * 8;
-  if (n >= rows) return;
-  uint16_t* o = dst + n * dp + c;
+  if (n >= p.rows) return;
+  uint16_t* o = p.dst + n * p.dp + c;
   if constexpr (DT == PDH_F32) {
-    const float* x = static_cast<const float*>(src) + n * ld + c;
+    const float* x = static_cast<const float*>(p.src) + n * p.ld + c;
     float v[8];
-    if (c + 8 <= d) {
+    if (c + 8 <= p.d) {
       const f32x4u a = reinterpret_cast<const f32x4u*>(x)[0], b = reinterpret_cast<const f32x4u*>(x)[1];
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = a[e], v[4 + e] = b[e];
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = c + e < d ? x[e] : 0.f;
+      for (int e = 0; e < 8; ++e) v[e] = c + e < p.d ? x[e] : 0.f;
     }
 #pragma unroll
     for (int pl = 0; pl < 3; ++pl) {
@@ -785,20 +795,37 @@ __global__ __launch_bounds__(256) void xent_pack(const void* __restrict__ src, i
         v[2 * e] -= __uint_as_float(w[e] << 16);
         v[2 * e + 1] -= __uint_as_float(w[e] & 0xffff0000u);
       }
-      *reinterpret_cast<u32x4*>(o + pl * plane) = w;
+      *reinterpret_cast<u32x4*>(o + pl * p.plane) = w;
     }
   } else {
-    const uint16_t* x = static_cast<const uint16_t*>(src) + n * ld + c;
+    const uint16_t* x = static_cast<const uint16_t*>(p.src) + n * p.ld + c;
     u32x4 w{};
-    if (c + 8 <= d) {
+    if (c + 8 <= p.d) {
       w = *reinterpret_cast<const u32x4h*>(x);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (c + e < d) w[e >> 1] |= static_cast<uint32_t>(x[e]) << (16 * (e & 1));
+        if (c + e < p.d) w[e >> 1] |= static_cast<uint32_t>(x[e]) << (16 * (e & 1));
     }
     *reinterpret_cast<u32x4*>(o) = w;
   }
+}
+
+// What the products wait for, in one launch: w's and x's workgroups, then fp16's scale in one more.
+struct PrepArgs {
+  PackArgs w, x;
+  ScaleArgs scale;
+  uint32_t blocks_w, blocks_x;
+};
+template <int DT>
+__global__ __launch_bounds__(256) void xent_prep(PrepArgs p) {
+  const uint32_t b = blockIdx.x;
+  if (b < p.blocks_w)
+    pack_rows<DT>(p.w, static_cast<int64_t>(b) * 256 + threadIdx.x);
+  else if (b < p.blocks_w + p.blocks_x)
+    pack_rows<DT>(p.x, static_cast<int64_t>(b - p.blocks_w) * 256 + threadIdx.x);
+  else
+    scale_dloss(p.scale);
 }
 
 // ------------------------------------------------------------------- host
@@ -834,20 +861,28 @@ struct Space {
 
 unsigned blocks_for(int64_t threads) { return static_cast<unsigned>((threads + 255) / 256); }
 
-// The operand of rows x[rows][d]: in place, or packed into ws by a kernel.
-Operand place(const void* p, int64_t ld, int64_t rows, const Problem& q, Space& ws, bool in_place, hipStream_t s,
-              bool launch) {
+// The operand of rows p[rows][d]: in place, or in ws, where `pack` says how it comes there.
+Operand place(const void* p, int64_t ld, int64_t rows, const Problem& q, Space& ws, bool in_place, PackArgs& pack) {
+  pack = PackArgs{};
   if (in_place) return Operand{static_cast<const char*>(p), ld * 2, 0};
   const int64_t dp = q.dp(), plane = rows * dp;
   auto* dst = static_cast<uint16_t*>(ws.take(plane * 2 * q.planes()));
-  if (launch) {
-    const dim3 grid(blocks_for(rows * (dp / 8)));
-    if (q.dtype == PDH_F32)
-      xent_pack<PDH_F32><<<grid, 256, 0, s>>>(p, ld, rows, static_cast<int>(q.d), static_cast<int>(dp), dst, plane);
-    else
-      xent_pack<PDH_BF16><<<grid, 256, 0, s>>>(p, ld, rows, static_cast<int>(q.d), static_cast<int>(dp), dst, plane);
-  }
+  pack = PackArgs{p, ld, rows, static_cast<int>(q.d), static_cast<int>(dp), dst, plane};
   return Operand{reinterpret_cast<const char*>(dst), dp * 2, plane * 2};
+}
+
+// Launches what there is to prepare.
+int prepare(const char* fn, const Problem& q, PackArgs w, PackArgs x, const ScaleArgs& scale, hipStream_t s) {
+  PrepArgs p{w, x, scale, 0, 0};
+  if (w.src) p.blocks_w = blocks_for(w.rows * (w.dp / 8));
+  if (x.src) p.blocks_x = blocks_for(x.rows * (x.dp / 8));
+  const unsigned blocks = p.blocks_w + p.blocks_x + (scale.dloss ? 1 : 0);
+  if (blocks == 0) return PDH_OK;
+  if (q.dtype == PDH_F32)
+    xent_prep<PDH_F32><<<dim3(blocks), 256, 0, s>>>(p);
+  else
+    xent_prep<PDH_BF16><<<dim3(blocks), 256, 0, s>>>(p);  // 16-bit rows are copied as they are
+  return check_launch(fn);
 }
 
 template <typename C>
@@ -920,7 +955,7 @@ int check(const char* fn, int64_t n, int64_t d, int64_t v, int64_t ldx, int64_t 
               fn, (long long)n, (long long)d, (long long)v);
   PDH_REQUIRE(n <= (int64_t{1} << 24) && v <= (int64_t{1} << 24) && d <= (int64_t{1} << 18), PDH_EUNSUPPORTED,
               "%s: at most 2^24 tokens and vocabulary entries and 2^18 features", fn);
-  // every launch stays under 2^32 threads
+  // every launch stays under 2^32 threads (packing: one for 8 elements of x and of w)
   PDH_REQUIRE(n * v <= (int64_t{1} << 38) && std::max(n, v) * up(d, 8) <= (int64_t{1} << 33), PDH_EUNSUPPORTED,
               "%s: at most 2^38 logits and 2^33 elements of x or w in a call", fn);
   PDH_REQUIRE(ldx >= 0 && ldw >= 0, PDH_EINVAL, "%s: row strides must be >= 0", fn);
@@ -930,15 +965,16 @@ int check(const char* fn, int64_t n, int64_t d, int64_t v, int64_t ldx, int64_t 
 // The forward's workspace (base NULL: measured), its operands placed in it.
 struct FwdPlan {
   Operand w, x;
+  PackArgs pack_w, pack_x;
   TileArgs t;
   float2* part;
   float* zt;
   int strips;
 };
-FwdPlan plan_fwd(const Problem& q, Space& ws, bool fit_x, bool fit_w, hipStream_t s, bool launch) {
+FwdPlan plan_fwd(const Problem& q, Space& ws, bool fit_x, bool fit_w) {
   FwdPlan p{};
-  p.w = place(q.w, q.ldw, q.v, q, ws, fit_w, s, launch);
-  p.x = place(q.x, q.ldx, q.n, q, ws, fit_x, s, launch);
+  p.w = place(q.w, q.ldw, q.v, q, ws, fit_w, p.pack_w);
+  p.x = place(q.x, q.ldx, q.n, q, ws, fit_x, p.pack_x);
   p.t = tiles<Big>(p.w, p.x, q.v, q.n, q.dp(), up(q.dp(), kBK));
   p.strips = static_cast<int>((q.v + kStrip - 1) / kStrip);
   p.part = static_cast<float2*>(ws.take(static_cast<int64_t>(p.strips) * q.n * 8));
@@ -948,6 +984,7 @@ FwdPlan plan_fwd(const Problem& q, Space& ws, bool fit_x, bool fit_w, hipStream_
 
 struct BwdPlan {
   Operand w, x;
+  PackArgs pack_w, pack_x;
   uint16_t* dz;
   float* parts;
   float* g;
@@ -956,10 +993,10 @@ struct BwdPlan {
   int64_t kslice;  // of them in a slice of dx's product
   int64_t slices;  // of a whole piece
 };
-BwdPlan plan_bwd(const Problem& q, Space& ws, bool fit_x, bool fit_w, hipStream_t s, bool launch) {
+BwdPlan plan_bwd(const Problem& q, Space& ws, bool fit_x, bool fit_w) {
   BwdPlan p{};
-  p.w = place(q.w, q.ldw, q.v, q, ws, fit_w, s, launch);
-  p.x = place(q.x, q.ldx, q.n, q, ws, fit_x, s, launch);
+  p.w = place(q.w, q.ldw, q.v, q, ws, fit_w, p.pack_w);
+  p.x = place(q.x, q.ldx, q.n, q, ws, fit_x, p.pack_x);
   const int64_t all = up(q.v, 256), most = kPieceBytes / (q.n * 2 * q.planes()) / 256 * 256;
   p.piece = std::min(all, std::max<int64_t>(most, 256));
   p.dz = static_cast<uint16_t*>(ws.take(q.n * p.piece * 2 * q.planes()));
@@ -979,6 +1016,7 @@ BwdPlan plan_bwd(const Problem& q, Space& ws, bool fit_x, bool fit_w, hipStream_
 template <int DT, bool SPLIT>
 int run_fwd(const Problem& q, const FwdPlan& p, const int64_t* targets, int64_t ignore, float* loss, float* lse, int* bad,
             hipStream_t s) {
+  if (int rc = prepare("pdh_linear_xent_fwd (pack)", q, p.pack_w, p.pack_x, ScaleArgs{}, s); rc != PDH_OK) return rc;
   const LogitTiles l = logit_tiles(p.t);
   xent_fwd<DT, SPLIT><<<run_grid(l.big, l.small), 256, 0, s>>>(FwdArgs{l, targets, p.part, p.zt});
   if (int rc = check_launch("pdh_linear_xent_fwd"); rc != PDH_OK) return rc;
@@ -992,11 +1030,13 @@ int run_bwd(const Problem& q, const BwdPlan& p, const int64_t* targets, const fl
             int64_t ignore, void* dx, void* dw, hipStream_t s) {
   const float* g = dloss;
   const float* scale = nullptr;
+  ScaleArgs sa{};
   if constexpr (DT == PDH_F16) {
-    xent_scale<<<1, 1024, 0, s>>>(dloss, targets, q.n, q.v, ignore, p.g, p.inv);
+    sa = ScaleArgs{dloss, targets, q.n, q.v, ignore, p.g, p.inv};
     g = p.g;
     scale = p.inv;
   }
+  if (int rc = prepare("pdh_linear_xent_bwd (pack)", q, p.pack_w, p.pack_x, sa, s); rc != PDH_OK) return rc;
   const int64_t es = ODT == PDH_F32 ? 4 : 2, dp = q.dp(), slice = q.n * dp;
   for (int64_t v0 = 0; v0 < q.v; v0 += p.piece) {
     const int64_t nv = std::min(p.piece, q.v - v0), ldz = up(nv, 256);
@@ -1033,9 +1073,9 @@ extern "C" size_t pdh_linear_xent_workspace(const void* x, const void* w, int64_
   const bool fx = Problem::fit(x, ldx, width, dtype), fw = Problem::fit(w, ldw, width, dtype);
   Space ws{nullptr};
   if (backward)
-    plan_bwd(q, ws, fx, fw, nullptr, false);
+    plan_bwd(q, ws, fx, fw);
   else
-    plan_fwd(q, ws, fx, fw, nullptr, false);
+    plan_fwd(q, ws, fx, fw);
   return ws.used;
 }
 
@@ -1048,13 +1088,13 @@ extern "C" int pdh_linear_xent_fwd(const void* x, const void* w, const int64_t* 
   const Problem q{tokens, width, vocab, ldx, ldw, x, w, dtype};
   const bool fx = Problem::fit(x, ldx, width, dtype), fw = Problem::fit(w, ldw, width, dtype);
   Space measure{nullptr};
-  plan_fwd(q, measure, fx, fw, nullptr, false);
+  plan_fwd(q, measure, fx, fw);
   PDH_REQUIRE(ws && aligned16(ws) && ws_bytes >= measure.used, PDH_EINVAL,
               "pdh_linear_xent_fwd: the workspace holds %zu bytes, %zu are needed, 16-byte aligned", ws ? ws_bytes : size_t{0},
               measure.used);
   hipStream_t s = as_stream(stream);
   Space space{static_cast<char*>(ws)};
-  const FwdPlan p = plan_fwd(q, space, fx, fw, s, true);
+  const FwdPlan p = plan_fwd(q, space, fx, fw);
   if (dtype == PDH_F32) return run_fwd<PDH_BF16, true>(q, p, targets, ignore_index, loss, lse, bad, s);
   if (dtype == PDH_BF16) return run_fwd<PDH_BF16, false>(q, p, targets, ignore_index, loss, lse, bad, s);
   return run_fwd<PDH_F16, false>(q, p, targets, ignore_index, loss, lse, bad, s);
@@ -1070,13 +1110,13 @@ extern "C" int pdh_linear_xent_bwd(const void* x, const void* w, const int64_t* 
   const Problem q{tokens, width, vocab, ldx, ldw, x, w, dtype};
   const bool fx = Problem::fit(x, ldx, width, dtype), fw = Problem::fit(w, ldw, width, dtype);
   Space measure{nullptr};
-  plan_bwd(q, measure, fx, fw, nullptr, false);
+  plan_bwd(q, measure, fx, fw);
   PDH_REQUIRE(ws && aligned16(ws) && ws_bytes >= measure.used, PDH_EINVAL,
               "pdh_linear_xent_bwd: the workspace holds %zu bytes, %zu are needed, 16-byte aligned", ws ? ws_bytes : size_t{0},
               measure.used);
   hipStream_t s = as_stream(stream);
   Space space{static_cast<char*>(ws)};
-  const BwdPlan p = plan_bwd(q, space, fx, fw, s, true);
+  const BwdPlan p = plan_bwd(q, space, fx, fw);
   if (dtype == PDH_F32) return run_bwd<PDH_BF16, PDH_F32, true>(q, p, targets, lse, dloss, ignore_index, dx, dw, s);
   if (dtype == PDH_BF16) return run_bwd<PDH_BF16, PDH_BF16, false>(q, p, targets, lse, dloss, ignore_index, dx, dw, s);
   return run_bwd<PDH_F16, PDH_F16, false>(q, p, targets, lse, dloss, ignore_index, dx, dw, s);
