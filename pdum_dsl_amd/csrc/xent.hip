@@ -22,10 +22,13 @@
 // for the softmax, 32 bytes of an output row for the stores.
 //
 // dz is rounded to the storage type, as the probabilities of a 16-bit
-// attention are: a relative 2^-9 (2^-12) of each term, below the rounding of
-// the 16-bit gradients they sum to. fp16 takes it scaled by a power of two (the
-// largest |dloss| to 2^14), or a mean's 1 / tokens times a small probability
-// would fall below its range. fp32 operands are split into three bf16 terms
+// attention are: a relative 2^-8 (2^-11) of each term at most, independent from
+// term to term, as the rounding of the 16-bit gradients they sum to. It is taken
+// over the largest |dloss|, which the products' fp32 results are multiplied by:
+// a mean's equal weights 1 / tokens would give every target's entry the same
+// rounding error, which no sum averages out (0.38% of the gradient at 7780
+// live tokens, 0.17% so, what the output's own rounding leaves); fp16 takes it
+// times 2^14 on top, or small probabilities would fall below its range. fp32 operands are split into three bf16 terms
 // and the six cross products above 2^-24 are summed, smallest first.
 #include "common.h"
 
@@ -554,7 +557,7 @@ struct GradArgs {
   LogitTiles l;        // a: w from the piece's first row (m: its entries)
   const int64_t* targets;
   const float* lse;
-  const float* g;      // [tokens]: dloss (fp16: scaled)
+  const float* g;      // [tokens]: dloss (16-bit: scaled)
   uint16_t* dz;        // [planes][tokens][ldz]
   int64_t ldz, plane;  // elements
   int64_t v0;          // the piece's first vocabulary entry
@@ -732,12 +735,13 @@ __global__ __launch_bounds__(256) void xent_dx(const float* __restrict__ part, v
     if (c + e < d) st_dt<DT>(dx, n * d + c + e, s[e]);
 }
 
-// fp16's dz scale: 2^14 over the power of two above the largest |dloss| of a
-// live token. One workgroup; g[n] = dloss[n] times it, *inv its inverse.
+// 16-bit dz's scale: g[n] = dloss[n] `up` over the largest |dloss| of a live
+// token, *inv the factor that undoes it. One workgroup.
 struct ScaleArgs {
   const float* dloss;  // NULL: none to do
   const int64_t* targets;
   int64_t n, vocab, ignore;
+  float up;
   float* g;
   float* inv;
 };
@@ -752,11 +756,9 @@ __device__ __forceinline__ void scale_dloss(const ScaleArgs& p) {
   if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = mx;
   __syncthreads();
   mx = fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
-  int e = 0;
-  if (mx > 0.f && mx < __builtin_inff()) frexpf(mx, &e);  // mx < 2^e
-  const float up = ldexpf(1.f, min(14 - e, 126));
-  for (int64_t i = threadIdx.x; i < p.n; i += 256) p.g[i] = p.dloss[i] * up;
-  if (threadIdx.x == 0) *p.inv = ldexpf(1.f, -min(14 - e, 126));
+  if (!(mx > 0.f && mx < __builtin_inff())) mx = 1.f;
+  for (int64_t i = threadIdx.x; i < p.n; i += 256) p.g[i] = p.dloss[i] / mx * p.up;
+  if (threadIdx.x == 0) *p.inv = mx / p.up;
 }
 
 // An operand made fit for the direct loads: rows of `dp` (a multiple of 8)
@@ -811,7 +813,7 @@ __device__ __forceinline__ void pack_rows(const PackArgs& p, int64_t i) {
   }
 }
 
-// What the products wait for, in one launch: w's and x's workgroups, then fp16's scale in one more.
+// What the products wait for, in one launch: w's and x's workgroups, then dz's scale in one more.
 struct PrepArgs {
   PackArgs w, x;
   ScaleArgs scale;
@@ -1006,7 +1008,7 @@ BwdPlan plan_bwd(const Problem& q, Space& ws, bool fit_x, bool fit_w) {
   p.kslice = up((p.piece + want - 1) / want, kBK);
   p.slices = (p.piece + p.kslice - 1) / p.kslice;
   p.parts = static_cast<float*>(ws.take(p.slices * q.n * q.dp() * 4));
-  if (q.dtype == PDH_F16) {
+  if (q.dtype != PDH_F32) {
     p.g = static_cast<float*>(ws.take(q.n * 4));
     p.inv = static_cast<float*>(ws.take(4));
   }
@@ -1031,8 +1033,8 @@ int run_bwd(const Problem& q, const BwdPlan& p, const int64_t* targets, const fl
   const float* g = dloss;
   const float* scale = nullptr;
   ScaleArgs sa{};
-  if constexpr (DT == PDH_F16) {
-    sa = ScaleArgs{dloss, targets, q.n, q.v, ignore, p.g, p.inv};
+  if constexpr (!SPLIT) {
+    sa = ScaleArgs{dloss, targets, q.n, q.v, ignore, DT == PDH_F16 ? 16384.f : 1.f, p.g, p.inv};
     g = p.g;
     scale = p.inv;
   }

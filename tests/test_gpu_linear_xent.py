@@ -318,3 +318,25 @@ def test_loss_refusals_and_no_tokens():
     f = K.linear_cross_entropy(e, w, t[:0])
     dx, dw = K.linear_cross_entropy_bwd(e, w, t[:0], f.lse, f.lse)
     assert f.loss.shape == (0,) and dx.shape == (0, 8) and dw.shape == w.shape and not dw.any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_equal_weights_leave_no_common_rounding_error(dtype):
+    """A mean's weights all lie half a step between two 16-bit values: held to
+    them, every target's entry of dz would err by the same eps / 2, which no sum
+    averages out. dz's other terms are small here, so the gradients' error is the
+    rounding of the outputs, and half as much again at most."""
+    from pdum_dsl_amd import kernels as K
+
+    rng = np.random.default_rng(12)
+    n, d, v = 400, 256, 3000
+    x, w = _draw(rng, (n, d), dtype), _draw(rng, (v, d), dtype, 2.0 * d**-0.5)
+    ht = rng.integers(0, v, n)
+    t = torch.as_tensor(ht).cuda()
+    weight = (1.0 + HALF[dtype]) * 2.0**-8
+    dloss = torch.full((n,), weight, device="cuda")
+    f = K.linear_cross_entropy(x, w, t)
+    got = K.linear_cross_entropy_bwd(x, w, t, f.lse, dloss)
+    for a, want in zip(got, cf.linear_xent_bwd(_h(x), _h(w), ht, np.full(n, weight))):
+        rounded = _h(torch.as_tensor(want).to(dtype))
+        assert np.linalg.norm(_h(a) - want) <= 1.5 * np.linalg.norm(rounded - want)
