@@ -167,11 +167,12 @@ int pdh_dropout(const void* x, const void* residual, void* y, int64_t rows, int6
  *   dz[n, v] = dloss[n] (exp(z[n, v] - lse[n]) - [v == targets[n]])
  *   dx = dz w [tokens][width], dw = dz^T x [vocab][width], dense, of `dtype`
  * computing z again piece by piece of the vocabulary. Products accumulate in
- * fp32. 16-bit types: dz of a piece, over the largest |dloss|, is rounded to the
+ * fp32. dz of a piece is taken over the largest |dloss|; 16-bit types: rounded to the
  * type; PDH_F32: operands
  * are split into three bf16 terms each, six products of them, as
- * pdh_contract_set_f32_mode(6) does, and a token or entry that holds an
- * infinity, a NaN or a value beyond the bf16 range comes out NaN. Nothing is
+ * pdh_contract_set_f32_mode(6) does (values under 2^-100 keep fewer digits),
+ * and a token or entry that holds an infinity, a NaN or a value beyond the
+ * bf16 range comes out NaN. Nothing is
  * atomic: results repeat bit for bit. The backward needs tokens >= 1.
  * ws, 16-byte aligned, holds pdh_linear_xent_workspace bytes for the same
  * x, w (looked at for alignment alone), sizes, strides and direction: packed

@@ -28,7 +28,8 @@
 // a mean's equal weights 1 / tokens would give every target's entry the same
 // rounding error, which no sum averages out (0.38% of the gradient at 7780
 // live tokens, 0.17% so, what the output's own rounding leaves); fp16 takes it
-// times 2^14 on top, or small probabilities would fall below its range. fp32 operands are split into three bf16 terms
+// times 2^14 on top, or small probabilities would fall below its range, and
+// fp32's terms stay clear of subnormal values for weights of any size. fp32 operands are split into three bf16 terms
 // and the six cross products above 2^-24 are summed, smallest first.
 #include "common.h"
 
@@ -557,7 +558,7 @@ struct GradArgs {
   LogitTiles l;        // a: w from the piece's first row (m: its entries)
   const int64_t* targets;
   const float* lse;
-  const float* g;      // [tokens]: dloss (16-bit: scaled)
+  const float* g;      // [tokens]: dloss, scaled
   uint16_t* dz;        // [planes][tokens][ldz]
   int64_t ldz, plane;  // elements
   int64_t v0;          // the piece's first vocabulary entry
@@ -658,7 +659,7 @@ struct ProdArgs {
   void* dw;
   float* parts;          // dx's, [slices][tokens][ldp]
   int64_t lddw, ldp, slice;
-  const float* scale;    // of dw; NULL: 1
+  const float* scale;    // of dw
   int add;               // dx's parts of an earlier piece are there
 };
 
@@ -729,13 +730,13 @@ __global__ __launch_bounds__(256) void xent_dx(const float* __restrict__ part, v
     for (int q = 0; q < 8; ++q)
       if (q0 + q < slices) s += v[q];
   }
-  if (scale) s *= *scale;
+  s *= *scale;
 #pragma unroll
   for (int e = 0; e < 4; ++e)
     if (c + e < d) st_dt<DT>(dx, n * d + c + e, s[e]);
 }
 
-// 16-bit dz's scale: g[n] = dloss[n] `up` over the largest |dloss| of a live
+// dz's scale: g[n] = dloss[n] `up` over the largest |dloss| of a live
 // token, *inv the factor that undoes it. One workgroup.
 struct ScaleArgs {
   const float* dloss;  // NULL: none to do
@@ -832,7 +833,10 @@ __global__ __launch_bounds__(256) void xent_prep(PrepArgs p) {
 
 // ------------------------------------------------------------------- host
 
-constexpr int64_t kPieceBytes = int64_t{1} << 30;  // dz of one piece of the vocabulary
+// dz of one piece of the vocabulary (backward 8192 x 768 x 50257 bf16: 1986 us
+// in one piece of 823 MB, 1999 in pieces of 512 MiB, 2088 of 256, 2094 of 128),
+// and dx's parts
+constexpr int64_t kPieceBytes = int64_t{1} << 30, kPartBytes = int64_t{1} << 31;
 
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
@@ -942,7 +946,8 @@ int64_t pick_slices(int64_t tiles_w, int64_t tiles_x, int64_t n, int64_t piece, 
   const double dw = static_cast<double>(terms) * ((n + kBK - 1) / kBK) + 5;
   double best = 1e300;
   int64_t at = 1;
-  for (int64_t s = 1; s <= 64 && s * 256 <= std::max<int64_t>(piece, 256); ++s) {
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>({64, piece / 256, kPartBytes / (n * dp * 4)}));
+  for (int64_t s = 1; s <= most; ++s) {
     const double dx = static_cast<double>(terms) * ((piece + s * kBK - 1) / (s * kBK)) + 5;
     const double t = (dx > dw ? makespan(tiles_x * s, dx, tiles_w, dw, slots())
                               : makespan(tiles_w, dw, tiles_x * s, dx, slots())) + 9e-7 * s * n * dp;
@@ -1000,7 +1005,8 @@ BwdPlan plan_bwd(const Problem& q, Space& ws, bool fit_x, bool fit_w) {
   p.w = place(q.w, q.ldw, q.v, q, ws, fit_w, p.pack_w);
   p.x = place(q.x, q.ldx, q.n, q, ws, fit_x, p.pack_x);
   const int64_t all = up(q.v, 256), most = kPieceBytes / (q.n * 2 * q.planes()) / 256 * 256;
-  p.piece = std::min(all, std::max<int64_t>(most, 256));
+  // (2^22 entries keep 128 rows of dz within the loads' 32-bit offsets)
+  p.piece = std::min(std::min(all, int64_t{1} << 22), std::max<int64_t>(most, 256));
   p.dz = static_cast<uint16_t*>(ws.take(q.n * p.piece * 2 * q.planes()));
   const int64_t mt = (q.d + Big::BM - 1) / Big::BM;
   const int64_t want = pick_slices(mt * ((p.piece + Big::BN - 1) / Big::BN), mt * ((q.n + Big::BN - 1) / Big::BN), q.n,
@@ -1008,10 +1014,8 @@ BwdPlan plan_bwd(const Problem& q, Space& ws, bool fit_x, bool fit_w) {
   p.kslice = up((p.piece + want - 1) / want, kBK);
   p.slices = (p.piece + p.kslice - 1) / p.kslice;
   p.parts = static_cast<float*>(ws.take(p.slices * q.n * q.dp() * 4));
-  if (q.dtype != PDH_F32) {
-    p.g = static_cast<float*>(ws.take(q.n * 4));
-    p.inv = static_cast<float*>(ws.take(4));
-  }
+  p.g = static_cast<float*>(ws.take(q.n * 4));
+  p.inv = static_cast<float*>(ws.take(4));
   return p;
 }
 
@@ -1030,21 +1034,14 @@ int run_fwd(const Problem& q, const FwdPlan& p, const int64_t* targets, int64_t 
 template <int DT, int ODT, bool SPLIT>
 int run_bwd(const Problem& q, const BwdPlan& p, const int64_t* targets, const float* lse, const float* dloss,
             int64_t ignore, void* dx, void* dw, hipStream_t s) {
-  const float* g = dloss;
-  const float* scale = nullptr;
-  ScaleArgs sa{};
-  if constexpr (!SPLIT) {
-    sa = ScaleArgs{dloss, targets, q.n, q.v, ignore, DT == PDH_F16 ? 16384.f : 1.f, p.g, p.inv};
-    g = p.g;
-    scale = p.inv;
-  }
+  const ScaleArgs sa{dloss, targets, q.n, q.v, ignore, DT == PDH_F16 ? 16384.f : 1.f, p.g, p.inv};
   if (int rc = prepare("pdh_linear_xent_bwd (pack)", q, p.pack_w, p.pack_x, sa, s); rc != PDH_OK) return rc;
   const int64_t es = ODT == PDH_F32 ? 4 : 2, dp = q.dp(), slice = q.n * dp;
   for (int64_t v0 = 0; v0 < q.v; v0 += p.piece) {
     const int64_t nv = std::min(p.piece, q.v - v0), ldz = up(nv, 256);
     const Operand wv{p.w.p + v0 * p.w.pitch, p.w.pitch, p.w.plane};
     const Operand dz{reinterpret_cast<const char*>(p.dz), ldz * 2, q.n * ldz * 2};
-    const GradArgs ga{logit_tiles(tiles<Big>(wv, p.x, nv, q.n, dp, up(dp, kBK))), targets, lse, g, p.dz, ldz, q.n * ldz,
+    const GradArgs ga{logit_tiles(tiles<Big>(wv, p.x, nv, q.n, dp, up(dp, kBK))), targets, lse, p.g, p.dz, ldz, q.n * ldz,
                       v0, q.v, ignore};
     xent_dz<DT, SPLIT><<<run_grid(ga.l.big, ga.l.small), 256, 0, s>>>(ga);
     ProdArgs pr{};
@@ -1054,12 +1051,12 @@ int run_bwd(const Problem& q, const BwdPlan& p, const int64_t* targets, const fl
     pr.x_first = p.kslice > q.n;
     pr.dw = static_cast<char*>(dw) + v0 * q.d * es;
     pr.parts = p.parts, pr.lddw = q.d, pr.ldp = dp, pr.slice = slice;
-    pr.scale = scale, pr.add = v0 > 0;
+    pr.scale = p.inv, pr.add = v0 > 0;
     xent_prod<DT, ODT, SPLIT><<<run_grid(pr.tiles_w, pr.tiles_x), 256, 0, s>>>(pr);
     if (int rc = check_launch("pdh_linear_xent_bwd"); rc != PDH_OK) return rc;
   }
   xent_dx<ODT><<<dim3(blocks_for(q.n * (dp / 4))), 256, 0, s>>>(p.parts, dx, q.n, static_cast<int>(q.d), dp, slice,
-                                                               static_cast<int>(p.slices), scale);
+                                                               static_cast<int>(p.slices), p.inv);
   return check_launch("pdh_linear_xent_bwd (dx)");
 }
 

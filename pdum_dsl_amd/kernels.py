@@ -219,7 +219,7 @@ def layernorm_fwd(
     mean = x.new_empty(lead, dtype=torch.float32)
     rstd = torch.empty_like(mean)
     _lib.call("pdh_layernorm_fwd", x2.data_ptr(), _ptr(gamma), _ptr(beta), y.data_ptr(), mean.data_ptr(),
-              rstd.data_ptr(), m, n, ld, ldy, eps, code, _stream())
+              rstd.data_ptr(), m, n, ld, ldy, float(eps), code, _stream())
     return LayernormOut(y, mean, rstd)
 
 
@@ -301,8 +301,8 @@ def _dropout(name, x, p, rng, site, residual, out):
         y, ldy = _like(x), n
     else:
         y, ldy = out, _out_stride(out, x, m, n)
-    _lib.call("pdh_dropout", x2.data_ptr(), _ptr(r2), y.data_ptr(), m, n, ld, ldr, ldy, p, rng.data_ptr(), site, code,
-              _stream())
+    _lib.call("pdh_dropout", x2.data_ptr(), _ptr(r2), y.data_ptr(), m, n, ld, ldr, ldy, float(p), rng.data_ptr(),
+              int(site), code, _stream())
     return y
 
 
@@ -384,7 +384,7 @@ def linear_cross_entropy(
         need = _head_workspace(px & 15, pw & 15, *sizes, code, 0)
         ws = x.new_empty(need, dtype=torch.uint8)
         _lib.call("pdh_linear_xent_fwd", px, pw, t.data_ptr(), loss.data_ptr(), lse.data_ptr(), *sizes,
-                  ignore_index, code, _ptr(bad), ws.data_ptr(), need, _stream())
+                  int(ignore_index), code, _ptr(bad), ws.data_ptr(), need, _stream())
     return LossOut(loss, lse)
 
 
@@ -425,7 +425,7 @@ def linear_cross_entropy_bwd(
     need = _head_workspace(px & 15, pw & 15, *sizes, code, 1)
     ws = x.new_empty(need, dtype=torch.uint8)
     _lib.call("pdh_linear_xent_bwd", px, pw, t.data_ptr(), lse.data_ptr(), dloss.data_ptr(), dx.data_ptr(),
-              dw.data_ptr(), *sizes, ignore_index, code, ws.data_ptr(), need, _stream())
+              dw.data_ptr(), *sizes, int(ignore_index), code, ws.data_ptr(), need, _stream())
     return dx, dw
 
 

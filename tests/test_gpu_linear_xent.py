@@ -340,3 +340,77 @@ def test_equal_weights_leave_no_common_rounding_error(dtype):
     for a, want in zip(got, cf.linear_xent_bwd(_h(x), _h(w), ht, np.full(n, weight))):
         rounded = _h(torch.as_tensor(want).to(dtype))
         assert np.linalg.norm(_h(a) - want) <= 1.5 * np.linalg.norm(rounded - want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,d,v", [(5, 64, 17), (131, 72, 300), (1, 40, 1), (70, 33, 129)])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_nothing_beside_the_operands_is_read(n, d, v, dtype, shift):
+    """x, w and the workspace lie in memory full of NaN (what a tile reads past
+    its operand has to count as zero), at whole chunks and one element on: the
+    results are those of operands that stand alone, and nothing is written
+    beside the outputs."""
+    from pdum_dsl_amd import _lib
+    from pdum_dsl_amd import kernels as K
+
+    rng = np.random.default_rng(n + d + v)
+    x, w = _draw(rng, (n, d), dtype), _draw(rng, (v, d), dtype, 0.3)
+    t = torch.as_tensor(rng.integers(0, v, n)).cuda()
+    dloss = torch.as_tensor(rng.standard_normal(n), dtype=torch.float32).cuda()
+    f = K.linear_cross_entropy(x, w, t)
+    want = K.linear_cross_entropy_bwd(x, w, t, f.lse, dloss)
+
+    def within(a):
+        big = torch.full((a.shape[0] + 1024, a.shape[1] + 64), float("nan"), dtype=dtype, device="cuda")
+        view = big[512:512 + a.shape[0], 16 + shift:16 + shift + a.shape[1]]
+        view.copy_(a)
+        return view
+
+    bx, bw = within(x), within(w)
+    f2 = K.linear_cross_entropy(bx, bw, t)
+    assert torch.equal(f.loss, f2.loss) and torch.equal(f.lse, f2.lse)
+    lib, code, sizes = _lib.lib(), K._DT[dtype], (n, d, v, bx.stride(0), bw.stride(0))
+    need = lib.pdh_linear_xent_workspace(bx.data_ptr(), bw.data_ptr(), *sizes, code, 1)
+    ws = torch.full((need + 4096,), 255, dtype=torch.uint8, device="cuda")
+    out = [torch.full((a.shape[0] + 2, a.shape[1]), 7.0, dtype=dtype, device="cuda") for a in want]
+    _lib.call("pdh_linear_xent_bwd", bx.data_ptr(), bw.data_ptr(), t.data_ptr(), f.lse.data_ptr(), dloss.data_ptr(),
+              out[0][1:].data_ptr(), out[1][1:].data_ptr(), *sizes, -100, code, ws.data_ptr(), need, K._stream())
+    torch.cuda.synchronize()
+    for a, b in zip(out, want):
+        assert torch.equal(a[1:-1], b) and (a[0] == 7).all() and (a[-1] == 7).all()
+    assert (ws[need:] == 255).all()
+
+
+def test_one_token_alone_and_numpy_scalars():
+    from pdum_dsl_amd import kernels as K
+
+    x, w = torch.randn(48, device="cuda"), torch.randn((30, 48), device="cuda")
+    t = torch.tensor(7, device="cuda")
+    f = K.linear_cross_entropy(x, w, t, ignore_index=np.int64(-100))
+    dx, dw = K.linear_cross_entropy_bwd(x, w, t, f.lse, torch.ones((), device="cuda"), ignore_index=np.int32(-100))
+    g = K.linear_cross_entropy(x[None], w, t[None])
+    assert f.loss.shape == () and dx.shape == (48,) and dw.shape == (30, 48) and torch.equal(f.loss, g.loss[0])
+    r = torch.tensor([1, 2], device="cuda")
+    assert torch.equal(K.dropout_fwd(x, np.float32(0.5), r, site=np.int64(1)), K.dropout_fwd(x, 0.5, r, site=1))
+    assert torch.equal(K.layernorm_fwd(x, eps=np.float64(1e-5)).y, K.layernorm_fwd(x[None]).y[0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", [1e-30, 1e30])
+def test_weights_of_any_size(dtype, size):
+    """dloss as small or large as fp32 allows: dx and dw are those of weights near one, times it (in fp32's range,
+    and in bf16's; fp16's output range ends first)."""
+    from pdum_dsl_amd import kernels as K
+
+    rng = np.random.default_rng(9)
+    x, w = _draw(rng, (60, 64), dtype), _draw(rng, (200, 64), dtype, 0.3)
+    t = torch.as_tensor(rng.integers(0, 200, 60)).cuda()
+    weight = torch.as_tensor(rng.random(60) + 0.5, dtype=torch.float32).cuda()
+    f = K.linear_cross_entropy(x, w, t)
+    one = K.linear_cross_entropy_bwd(x, w, t, f.lse, weight)
+    got = K.linear_cross_entropy_bwd(x, w, t, f.lse, weight * size)
+    if dtype == torch.float16:
+        assert all((g == 0).all() if size < 1 else torch.isinf(g[o.abs() > 1e-3]).all() for g, o in zip(got, one))
+        return
+    for g, o in zip(got, one):  # each rounded once from sums over weights that differ in their last place
+        assert ((g.double() / size - o.double()).abs() <= 4 * HALF[dtype] * o.double().abs() + 1e-6 * o.double().abs().max()).all()
