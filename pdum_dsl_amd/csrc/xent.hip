@@ -527,22 +527,38 @@ __global__ __launch_bounds__(256, 2) void xent_fwd(FwdArgs p) {
   logit_tile<DT, SPLIT>(p.l, smem, p, FwdEpilogue{});
 }
 
-// Joins the strips of 8 tokens, 32 lanes a token: lse and loss.
-__global__ __launch_bounds__(256) void xent_join(const float2* __restrict__ part, const float* __restrict__ zt,
-                                                 const int64_t* __restrict__ targets, int strips, int64_t n_tokens,
-                                                 int64_t vocab, int64_t ignore, float* __restrict__ loss,
-                                                 float* __restrict__ lse, int* __restrict__ bad) {
-  __shared__ float2 sh[32][8];
-  const int tok = threadIdx.x & 7, q = threadIdx.x >> 3;
-  const int64_t n = static_cast<int64_t>(blockIdx.x) * 8 + tok;
+// Joins the strips of 16 tokens, 64 lanes a token with eight loads in flight
+// each: lse and loss (8192 tokens, 393 strips: 8 us; 32 lanes a token and a
+// load at a time, 13).
+__global__ __launch_bounds__(1024) void xent_join(const float2* __restrict__ part, const float* __restrict__ zt,
+                                                  const int64_t* __restrict__ targets, int strips, int64_t n_tokens,
+                                                  int64_t vocab, int64_t ignore, float* __restrict__ loss,
+                                                  float* __restrict__ lse, int* __restrict__ bad) {
+  __shared__ float2 sh[64][16];
+  const int tok = threadIdx.x & 15, q = threadIdx.x >> 4;
+  const int64_t n = static_cast<int64_t>(blockIdx.x) * 16 + tok;
   float m = -__builtin_inff(), s = 0.f;
-  auto add = [&](float2 o) { join(m, s, o.x, o.y); };
-  if (n < n_tokens)
-    for (int i = q; i < strips; i += 32) add(part[static_cast<int64_t>(i) * n_tokens + n]);
+  if (n < n_tokens) {
+    for (int i0 = q; i0 < strips; i0 += 512) {
+      float2 v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        v[u] = i0 + 64 * u < strips ? part[static_cast<int64_t>(i0 + 64 * u) * n_tokens + n]
+                                    : make_float2(-__builtin_inff(), 0.f);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) join(m, s, v[u].x, v[u].y);
+    }
+  }
   sh[q][tok] = make_float2(m, s);
   __syncthreads();
+  if (q < 8) {
+    for (int i = q + 8; i < 64; i += 8) join(m, s, sh[i][tok].x, sh[i][tok].y);
+  }
+  __syncthreads();
+  if (q < 8) sh[q][tok] = make_float2(m, s);
+  __syncthreads();
   if (q == 0 && n < n_tokens) {
-    for (int i = 1; i < 32; ++i) add(sh[i][tok]);
+    for (int i = 1; i < 8; ++i) join(m, s, sh[i][tok].x, sh[i][tok].y);
     const float l = m + logf(s);
     const int64_t t = targets[n];
     const bool live = t >= 0 && t < vocab && t != ignore;
@@ -558,7 +574,9 @@ struct GradArgs {
   LogitTiles l;        // a: w from the piece's first row (m: its entries)
   const int64_t* targets;
   const float* lse;
-  const float* g;      // [tokens]: dloss, scaled
+  const float* dloss;
+  const float* most;   // dz is taken over it,
+  float raise;         // times this power of two
   uint16_t* dz;        // [planes][tokens][ldz]
   int64_t ldz, plane;  // elements
   int64_t v0;          // the piece's first vocabulary entry
@@ -583,7 +601,7 @@ struct DzEpilogue {
       const int64_t t = n < p.l.t.n ? p.targets[n] : -1;
       const bool live = t >= 0 && t < p.vocab && t != p.ignore;
       f.target[j] = live ? static_cast<int>(t - p.v0) : kNoToken;
-      f.g[j] = live ? p.g[n] : 0.f;
+      f.g[j] = live ? p.dloss[n] / *p.most * p.raise : 0.f;
       f.lse2[j] = live ? p.lse[n] * kLog2e : 0.f;
     }
     return f;
@@ -659,13 +677,14 @@ struct ProdArgs {
   void* dw;
   float* parts;          // dx's, [slices][tokens][ldp]
   int64_t lddw, ldp, slice;
-  const float* scale;    // of dw
+  const float* most;     // dw is times it,
+  float down;            // and this
   int add;               // dx's parts of an earlier piece are there
 };
 
 template <int DT, int ODT, typename C, bool KB, bool SPLIT>
 __device__ __forceinline__ void prod_tile(const TileArgs& a, int id, unsigned char* smem, char* out, int64_t ld,
-                                          int64_t slice, const float* scale, bool add) {
+                                          int64_t slice, float sc, bool add) {
   constexpr int TM = C::TM, TN = C::TN, ES = ODT == PDH_F32 ? 4 : 2;
   const Tile t = tile_of(a, id);
   const int m0 = t.m * C::BM, n0 = t.n * C::BN;
@@ -675,7 +694,6 @@ __device__ __forceinline__ void prod_tile(const TileArgs& a, int id, unsigned ch
   xent_tile<DT, C, false, KB, SPLIT>(a, smem, acc, m0, n0, k0, k1);
   __syncthreads();  // the tile loop's last reads are over: LDS serves the stores
   unsigned char* lds = smem + w * put_bytes<ES, TM>();
-  const float sc = scale ? *scale : 1.f;
   const int cw = m0 + 32 * wm * TM;
 #pragma unroll
   for (int j = 0; j < TN; ++j) {
@@ -705,16 +723,18 @@ __global__ __launch_bounds__(256, 2) void xent_prod(ProdArgs p) {
   const int id = run_id(p.x_first ? p.tiles_x : p.tiles_w, p.x_first ? p.tiles_w : p.tiles_x, second);
   if (id < 0) return;
   if (second != static_cast<bool>(p.x_first))
-    prod_tile<DT, PDH_F32, Big, true, SPLIT>(p.x, id, smem, reinterpret_cast<char*>(p.parts), p.ldp, p.slice, nullptr,
+    prod_tile<DT, PDH_F32, Big, true, SPLIT>(p.x, id, smem, reinterpret_cast<char*>(p.parts), p.ldp, p.slice, 1.f,
                                              p.add);
   else
-    prod_tile<DT, ODT, Big, false, SPLIT>(p.w, id, smem, static_cast<char*>(p.dw), p.lddw, 0, p.scale, false);
+    prod_tile<DT, ODT, Big, false, SPLIT>(p.w, id, smem, static_cast<char*>(p.dw), p.lddw, 0, *p.most * p.down,
+                                              false);
 }
 
-// dx = scale * the sum of its parts, in order.
+// dx = *most * down * the sum of its parts, in order.
 template <int DT>
 __global__ __launch_bounds__(256) void xent_dx(const float* __restrict__ part, void* dx, int64_t rows, int d,
-                                               int64_t ld, int64_t slice, int slices, const float* scale) {
+                                               int64_t ld, int64_t slice, int slices, const float* __restrict__ most,
+                                               float down) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   const int64_t per = ld / 4, n = i / per;
   const int c = static_cast<int>(i - n * per) * 4;
@@ -730,36 +750,43 @@ __global__ __launch_bounds__(256) void xent_dx(const float* __restrict__ part, v
     for (int q = 0; q < 8; ++q)
       if (q0 + q < slices) s += v[q];
   }
-  s *= *scale;
+  s *= *most * down;
 #pragma unroll
   for (int e = 0; e < 4; ++e)
     if (c + e < d) st_dt<DT>(dx, n * d + c + e, s[e]);
 }
 
-// dz's scale: g[n] = dloss[n] `up` over the largest |dloss| of a live
-// token, *inv the factor that undoes it. One workgroup.
-struct ScaleArgs {
+// *most = the largest finite |dloss| of a live token, 1 where there is none
+// (or it is infinite): dz is taken over it. One workgroup, sixteen tokens' loads
+// in flight a lane (8192 tokens: 7 us; one at a time, 36).
+struct MostArgs {
   const float* dloss;  // NULL: none to do
   const int64_t* targets;
   int64_t n, vocab, ignore;
-  float up;
-  float* g;
-  float* inv;
+  float* most;
 };
-__device__ __forceinline__ void scale_dloss(const ScaleArgs& p) {
+__device__ __forceinline__ void most_dloss(const MostArgs& p) {
   __shared__ float sh[4];
+  constexpr int U = 16;
   float mx = 0.f;
-  for (int64_t i = threadIdx.x; i < p.n; i += 256) {
-    const int64_t t = p.targets[i];
-    if (t >= 0 && t < p.vocab && t != p.ignore) mx = fmaxf(mx, fabsf(p.dloss[i]));
+  for (int64_t i0 = threadIdx.x; i0 < p.n; i0 += 256 * U) {
+    int64_t t[U];
+    float d[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t i = i0 + 256 * u < p.n ? i0 + 256 * u : i0;
+      t[u] = p.targets[i];
+      d[u] = p.dloss[i];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (t[u] >= 0 && t[u] < p.vocab && t[u] != p.ignore) mx = fmaxf(mx, fabsf(d[u]));
   }
   mx = wave_max(mx);
   if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = mx;
   __syncthreads();
   mx = fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
-  if (!(mx > 0.f && mx < __builtin_inff())) mx = 1.f;
-  for (int64_t i = threadIdx.x; i < p.n; i += 256) p.g[i] = p.dloss[i] / mx * p.up;
-  if (threadIdx.x == 0) *p.inv = mx / p.up;
+  if (threadIdx.x == 0) *p.most = mx > 0.f && mx < __builtin_inff() ? mx : 1.f;
 }
 
 // An operand made fit for the direct loads: rows of `dp` (a multiple of 8)
@@ -814,10 +841,10 @@ __device__ __forceinline__ void pack_rows(const PackArgs& p, int64_t i) {
   }
 }
 
-// What the products wait for, in one launch: w's and x's workgroups, then dz's scale in one more.
+// What the products wait for, in one launch: w's and x's workgroups, then dloss's largest value in one more.
 struct PrepArgs {
   PackArgs w, x;
-  ScaleArgs scale;
+  MostArgs most;
   uint32_t blocks_w, blocks_x;
 };
 template <int DT>
@@ -828,7 +855,7 @@ __global__ __launch_bounds__(256) void xent_prep(PrepArgs p) {
   else if (b < p.blocks_w + p.blocks_x)
     pack_rows<DT>(p.x, static_cast<int64_t>(b - p.blocks_w) * 256 + threadIdx.x);
   else
-    scale_dloss(p.scale);
+    most_dloss(p.most);
 }
 
 // ------------------------------------------------------------------- host
@@ -878,11 +905,11 @@ Operand place(const void* p, int64_t ld, int64_t rows, const Problem& q, Space& 
 }
 
 // Launches what there is to prepare.
-int prepare(const char* fn, const Problem& q, PackArgs w, PackArgs x, const ScaleArgs& scale, hipStream_t s) {
-  PrepArgs p{w, x, scale, 0, 0};
+int prepare(const char* fn, const Problem& q, PackArgs w, PackArgs x, const MostArgs& most, hipStream_t s) {
+  PrepArgs p{w, x, most, 0, 0};
   if (w.src) p.blocks_w = blocks_for(w.rows * (w.dp / 8));
   if (x.src) p.blocks_x = blocks_for(x.rows * (x.dp / 8));
-  const unsigned blocks = p.blocks_w + p.blocks_x + (scale.dloss ? 1 : 0);
+  const unsigned blocks = p.blocks_w + p.blocks_x + (most.dloss ? 1 : 0);
   if (blocks == 0) return PDH_OK;
   if (q.dtype == PDH_F32)
     xent_prep<PDH_F32><<<dim3(blocks), 256, 0, s>>>(p);
@@ -994,8 +1021,7 @@ struct BwdPlan {
   PackArgs pack_w, pack_x;
   uint16_t* dz;
   float* parts;
-  float* g;
-  float* inv;
+  float* most;
   int64_t piece;   // vocabulary entries of a piece (the last one's may be fewer)
   int64_t kslice;  // of them in a slice of dx's product
   int64_t slices;  // of a whole piece
@@ -1014,19 +1040,18 @@ BwdPlan plan_bwd(const Problem& q, Space& ws, bool fit_x, bool fit_w) {
   p.kslice = up((p.piece + want - 1) / want, kBK);
   p.slices = (p.piece + p.kslice - 1) / p.kslice;
   p.parts = static_cast<float*>(ws.take(p.slices * q.n * q.dp() * 4));
-  p.g = static_cast<float*>(ws.take(q.n * 4));
-  p.inv = static_cast<float*>(ws.take(4));
+  p.most = static_cast<float*>(ws.take(4));
   return p;
 }
 
 template <int DT, bool SPLIT>
 int run_fwd(const Problem& q, const FwdPlan& p, const int64_t* targets, int64_t ignore, float* loss, float* lse, int* bad,
             hipStream_t s) {
-  if (int rc = prepare("pdh_linear_xent_fwd (pack)", q, p.pack_w, p.pack_x, ScaleArgs{}, s); rc != PDH_OK) return rc;
+  if (int rc = prepare("pdh_linear_xent_fwd (pack)", q, p.pack_w, p.pack_x, MostArgs{}, s); rc != PDH_OK) return rc;
   const LogitTiles l = logit_tiles(p.t);
   xent_fwd<DT, SPLIT><<<run_grid(l.big, l.small), 256, 0, s>>>(FwdArgs{l, targets, p.part, p.zt});
   if (int rc = check_launch("pdh_linear_xent_fwd"); rc != PDH_OK) return rc;
-  xent_join<<<dim3(static_cast<unsigned>((q.n + 7) / 8)), 256, 0, s>>>(p.part, p.zt, targets, p.strips, q.n, q.v, ignore,
+  xent_join<<<dim3(static_cast<unsigned>((q.n + 15) / 16)), 1024, 0, s>>>(p.part, p.zt, targets, p.strips, q.n, q.v, ignore,
                                                                        loss, lse, bad);
   return check_launch("pdh_linear_xent_fwd (join)");
 }
@@ -1034,15 +1059,16 @@ int run_fwd(const Problem& q, const FwdPlan& p, const int64_t* targets, int64_t 
 template <int DT, int ODT, bool SPLIT>
 int run_bwd(const Problem& q, const BwdPlan& p, const int64_t* targets, const float* lse, const float* dloss,
             int64_t ignore, void* dx, void* dw, hipStream_t s) {
-  const ScaleArgs sa{dloss, targets, q.n, q.v, ignore, DT == PDH_F16 ? 16384.f : 1.f, p.g, p.inv};
-  if (int rc = prepare("pdh_linear_xent_bwd (pack)", q, p.pack_w, p.pack_x, sa, s); rc != PDH_OK) return rc;
+  const MostArgs most{dloss, targets, q.n, q.v, ignore, p.most};
+  const float raise = DT == PDH_F16 ? 16384.f : 1.f;
+  if (int rc = prepare("pdh_linear_xent_bwd (pack)", q, p.pack_w, p.pack_x, most, s); rc != PDH_OK) return rc;
   const int64_t es = ODT == PDH_F32 ? 4 : 2, dp = q.dp(), slice = q.n * dp;
   for (int64_t v0 = 0; v0 < q.v; v0 += p.piece) {
     const int64_t nv = std::min(p.piece, q.v - v0), ldz = up(nv, 256);
     const Operand wv{p.w.p + v0 * p.w.pitch, p.w.pitch, p.w.plane};
     const Operand dz{reinterpret_cast<const char*>(p.dz), ldz * 2, q.n * ldz * 2};
-    const GradArgs ga{logit_tiles(tiles<Big>(wv, p.x, nv, q.n, dp, up(dp, kBK))), targets, lse, p.g, p.dz, ldz, q.n * ldz,
-                      v0, q.v, ignore};
+    const GradArgs ga{logit_tiles(tiles<Big>(wv, p.x, nv, q.n, dp, up(dp, kBK))), targets, lse, dloss, p.most, raise,
+                      p.dz, ldz, q.n * ldz, v0, q.v, ignore};
     xent_dz<DT, SPLIT><<<run_grid(ga.l.big, ga.l.small), 256, 0, s>>>(ga);
     ProdArgs pr{};
     pr.w = tiles<Big>(p.x, dz, q.d, nv, q.n, up(q.n, kBK));
@@ -1051,12 +1077,12 @@ int run_bwd(const Problem& q, const BwdPlan& p, const int64_t* targets, const fl
     pr.x_first = p.kslice > q.n;
     pr.dw = static_cast<char*>(dw) + v0 * q.d * es;
     pr.parts = p.parts, pr.lddw = q.d, pr.ldp = dp, pr.slice = slice;
-    pr.scale = p.inv, pr.add = v0 > 0;
+    pr.most = p.most, pr.down = 1.f / raise, pr.add = v0 > 0;
     xent_prod<DT, ODT, SPLIT><<<run_grid(pr.tiles_w, pr.tiles_x), 256, 0, s>>>(pr);
     if (int rc = check_launch("pdh_linear_xent_bwd"); rc != PDH_OK) return rc;
   }
   xent_dx<ODT><<<dim3(blocks_for(q.n * (dp / 4))), 256, 0, s>>>(p.parts, dx, q.n, static_cast<int>(q.d), dp, slice,
-                                                               static_cast<int>(p.slices), p.inv);
+                                                               static_cast<int>(p.slices), p.most, 1.f / raise);
   return check_launch("pdh_linear_xent_bwd (dx)");
 }
 
