@@ -10,7 +10,8 @@
 // the strips. Backward: the vocabulary in pieces; for each the same product again,
 // dz of the piece stored in 16 bits, then dw's rows of the piece and the
 // piece's part of dx as two more products. dx's parts over slices of the
-// vocabulary are fp32 and added in order: no atomics, results repeat.
+// vocabulary (and dw's over slices of the tokens, where its tiles are few) are
+// fp32 and added in order: no atomics, results repeat.
 //
 // All three products run one tile loop (xent_tile): 256 x 128 tiles, four waves
 // of 128 x 64, v_mfma_f32_32x32x16, accumulators m along registers and n along
@@ -384,8 +385,12 @@ __device__ __forceinline__ u32x4 pack8(const float* q) {
 
 using Big = Config<2, 2, 4, 2, 0>;    // 256 x 128 tiles
 using Small = Config<2, 2, 2, 1, 3>;  // 128 x 64: a quarter of one
+// The gradient products of widths that would leave half a 256-feature tile empty.
+using Half = Config<1, 4, 4, 2, 0>;      // 128 x 256
+using Quarter = Config<1, 4, 2, 2, 0>;   // 64 x 256
 static_assert(Small::LDS <= Big::LDS, "one kernel runs both");
-static_assert(4 * put_bytes<2, 4>() <= Big::LDS_A && 4 * put_bytes<4, 4>() <= Big::LDS_A && 4 * put_bytes<2, 2>() <= Small::LDS,
+static_assert(4 * put_bytes<2, 4>() <= Big::LDS_A && 4 * put_bytes<4, 4>() <= Big::LDS_A && 4 * put_bytes<2, 2>() <= Small::LDS &&
+                  4 * put_bytes<4, 4>() <= Half::LDS && 4 * put_bytes<4, 2>() <= Quarter::LDS,
               "the stores' rows fit");
 constexpr int kStrip = 128;        // vocabulary entries of a forward's strip
 
@@ -674,9 +679,9 @@ struct ProdArgs {
   TileArgs w, x;
   int tiles_w, tiles_x;  // with slices
   int x_first;           // the longer tiles go first
-  void* dw;
+  void* dw;              // or its parts, [slices][vocabulary][ldp] (w.slices > 1)
   float* parts;          // dx's, [slices][tokens][ldp]
-  int64_t lddw, ldp, slice;
+  int64_t lddw, ldp, slice_w, slice;
   const float* most;     // dw is times it,
   float down;            // and this
   int add;               // dx's parts of an earlier piece are there
@@ -716,23 +721,23 @@ __device__ __forceinline__ void prod_tile(const TileArgs& a, int id, unsigned ch
   }
 }
 
-template <int DT, int ODT, bool SPLIT>
+template <int DT, int ODT, typename C, bool SPLIT>
 __global__ __launch_bounds__(256, 2) void xent_prod(ProdArgs p) {
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[Big::LDS];
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[C::LDS];
   bool second;
   const int id = run_id(p.x_first ? p.tiles_x : p.tiles_w, p.x_first ? p.tiles_w : p.tiles_x, second);
   if (id < 0) return;
   if (second != static_cast<bool>(p.x_first))
-    prod_tile<DT, PDH_F32, Big, true, SPLIT>(p.x, id, smem, reinterpret_cast<char*>(p.parts), p.ldp, p.slice, 1.f,
-                                             p.add);
+    prod_tile<DT, PDH_F32, C, true, SPLIT>(p.x, id, smem, reinterpret_cast<char*>(p.parts), p.ldp, p.slice, 1.f, p.add);
+  else if (p.w.slices > 1)
+    prod_tile<DT, PDH_F32, C, false, SPLIT>(p.w, id, smem, static_cast<char*>(p.dw), p.ldp, p.slice_w, 1.f, false);
   else
-    prod_tile<DT, ODT, Big, false, SPLIT>(p.w, id, smem, static_cast<char*>(p.dw), p.lddw, 0, *p.most * p.down,
-                                              false);
+    prod_tile<DT, ODT, C, false, SPLIT>(p.w, id, smem, static_cast<char*>(p.dw), p.lddw, 0, *p.most * p.down, false);
 }
 
-// dx = *most * down * the sum of its parts, in order.
+// A gradient = *most * down * the sum of its parts, in order.
 template <int DT>
-__global__ __launch_bounds__(256) void xent_dx(const float* __restrict__ part, void* dx, int64_t rows, int d,
+__global__ __launch_bounds__(256) void xent_sum(const float* __restrict__ part, void* dx, int64_t rows, int d,
                                                int64_t ld, int64_t slice, int slices, const float* __restrict__ most,
                                                float down) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
@@ -965,22 +970,53 @@ double makespan(int64_t n1, double d1, int64_t n2, double d2, int64_t s) {
   return best;
 }
 
-// The slices of dx's product, a piece's vocabulary, that end both gradient
-// products soonest, in k tiles' time: a tile's own cost is its k tiles and
-// about 5 for its start and stores, a slice's the traffic of its part, added
-// and read again (9e-7 k tiles an element at 4.5 TB/s, 2 us a k tile).
-int64_t pick_slices(int64_t tiles_w, int64_t tiles_x, int64_t n, int64_t piece, int64_t dp, int terms) {
-  const double dw = static_cast<double>(terms) * ((n + kBK - 1) / kBK) + 5;
+// The gradient products' tiles: 256 features where the width fills them, 128
+// where half of the last one would be empty, 64 for widths up to that.
+// Backward at 16384 tokens x 20000 entries, us, always 256 and dw in one part /
+// the choice and dw's parts below: bf16 width 64 574 / 448, 128 627 / 522 (and
+// 256, with parts alone, 739 / 677), 640 1478 / 1402; fp32 width 32 4040 / 1817.
+enum class Prod { kBig, kHalf, kQuarter };
+Prod pick_prod(int64_t d) { return d <= 64 ? Prod::kQuarter : (d + 127) / 128 % 2 ? Prod::kHalf : Prod::kBig; }
+
+// k columns of a slice, and slices, of the two gradient products.
+struct Slices {
+  int64_t kw, w, kx, x;
+};
+
+// Those that end both products soonest, in k tiles' time: a tile's own cost is
+// its k tiles and about 5 for its start and stores, a slice's the traffic of its
+// part, added and read again (9e-7 k tiles an element at 4.5 TB/s, 2 us a k
+// tile); dw's parts are one more launch, and there are some only where its tiles
+// leave compute units without one. Backward with dw in one part / in those, us:
+// 16000 x 700 x 1500 fp16 340 / 187, 30000 x 1100 x 1000 bf16 657 / 337,
+// 5000 x 4096 x 300 bf16 157 / 116, 4000 x 384 x 6000 fp32 608 / 402.
+Slices pick_slices(const Problem& q, int64_t piece) {
+  const Prod kind = pick_prod(q.d);
+  const int64_t bm = kind == Prod::kBig ? Big::BM : kind == Prod::kHalf ? Half::BM : Quarter::BM;
+  const int64_t bn = kind == Prod::kBig ? Big::BN : Half::BN, mt = (q.d + bm - 1) / bm, dp = q.dp();
+  const int64_t tw = mt * ((piece + bn - 1) / bn), tx = mt * ((q.n + bn - 1) / bn), free = slots();
+  const double terms = (q.dtype == PDH_F32 ? kPairs : 1) * (kind == Prod::kQuarter ? 0.6 : 1.0);
+  static constexpr int kTry[] = {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 28, 32, 40, 48, 56, 64};
+  const int64_t most_w = tw < free ? std::min<int64_t>(q.n / 512, kPartBytes / (piece * dp * 4)) : 1;
+  const int64_t most_x = std::min<int64_t>(piece / 256, kPartBytes / (q.n * dp * 4));
   double best = 1e300;
-  int64_t at = 1;
-  const int64_t most = std::max<int64_t>(1, std::min<int64_t>({64, piece / 256, kPartBytes / (n * dp * 4)}));
-  for (int64_t s = 1; s <= most; ++s) {
-    const double dx = static_cast<double>(terms) * ((piece + s * kBK - 1) / (s * kBK)) + 5;
-    const double t = (dx > dw ? makespan(tiles_x * s, dx, tiles_w, dw, slots())
-                              : makespan(tiles_w, dw, tiles_x * s, dx, slots())) + 9e-7 * s * n * dp;
-    if (t < best) best = t, at = s;
+  int64_t bw = 1, bx = 1;
+  for (const int64_t w : kTry) {
+    if (w > 1 && w > most_w) break;
+    const double dw = terms * ((q.n + w * kBK - 1) / (w * kBK)) + 5;
+    const double cost_w = w > 1 ? 9e-7 * w * piece * dp + 2.5 : 0;
+    for (const int64_t x : kTry) {
+      if (x > 1 && x > most_x) break;
+      const double dx = terms * ((piece + x * kBK - 1) / (x * kBK)) + 5;
+      const double t = cost_w + 9e-7 * x * q.n * dp + (dx > dw ? makespan(tx * x, dx, tw * w, dw, free)
+                                                               : makespan(tw * w, dw, tx * x, dx, free));
+      if (t < best) best = t, bw = w, bx = x;
+    }
   }
-  return at;
+  Slices r;
+  r.kw = up((q.n + bw - 1) / bw, kBK), r.w = (q.n + r.kw - 1) / r.kw;
+  r.kx = up((piece + bx - 1) / bx, kBK), r.x = (piece + r.kx - 1) / r.kx;
+  return r;
 }
 
 int check(const char* fn, int64_t n, int64_t d, int64_t v, int64_t ldx, int64_t ldw, int dtype) {
@@ -996,7 +1032,8 @@ int check(const char* fn, int64_t n, int64_t d, int64_t v, int64_t ldx, int64_t 
   return PDH_OK;
 }
 
-// The forward's workspace (base NULL: measured), its operands placed in it.
+// The forward's workspace (base NULL: measured) and its operands' places. Plans
+// touch no memory: the caller checks what they used before it launches.
 struct FwdPlan {
   Operand w, x;
   PackArgs pack_w, pack_x;
@@ -1022,24 +1059,21 @@ struct BwdPlan {
   uint16_t* dz;
   float* parts;
   float* most;
+  float* parts_w;  // dw's parts of a piece, where there are any
   int64_t piece;   // vocabulary entries of a piece (the last one's may be fewer)
-  int64_t kslice;  // of them in a slice of dx's product
-  int64_t slices;  // of a whole piece
+  Slices slices;   // of a whole piece
 };
 BwdPlan plan_bwd(const Problem& q, Space& ws, bool fit_x, bool fit_w) {
   BwdPlan p{};
   p.w = place(q.w, q.ldw, q.v, q, ws, fit_w, p.pack_w);
   p.x = place(q.x, q.ldx, q.n, q, ws, fit_x, p.pack_x);
   const int64_t all = up(q.v, 256), most = kPieceBytes / (q.n * 2 * q.planes()) / 256 * 256;
-  // (2^22 entries keep 128 rows of dz within the loads' 32-bit offsets)
+  // (2^22 entries keep a tile's rows of dz within the loads' 32-bit offsets: that many only of 128 tokens or fewer)
   p.piece = std::min(std::min(all, int64_t{1} << 22), std::max<int64_t>(most, 256));
   p.dz = static_cast<uint16_t*>(ws.take(q.n * p.piece * 2 * q.planes()));
-  const int64_t mt = (q.d + Big::BM - 1) / Big::BM;
-  const int64_t want = pick_slices(mt * ((p.piece + Big::BN - 1) / Big::BN), mt * ((q.n + Big::BN - 1) / Big::BN), q.n,
-                                   p.piece, q.dp(), q.dtype == PDH_F32 ? kPairs : 1);
-  p.kslice = up((p.piece + want - 1) / want, kBK);
-  p.slices = (p.piece + p.kslice - 1) / p.kslice;
-  p.parts = static_cast<float*>(ws.take(p.slices * q.n * q.dp() * 4));
+  p.slices = pick_slices(q, p.piece);
+  p.parts = static_cast<float*>(ws.take(p.slices.x * q.n * q.dp() * 4));
+  if (p.slices.w > 1) p.parts_w = static_cast<float*>(ws.take(p.slices.w * p.piece * q.dp() * 4));
   p.most = static_cast<float*>(ws.take(4));
   return p;
 }
@@ -1056,13 +1090,34 @@ int run_fwd(const Problem& q, const FwdPlan& p, const int64_t* targets, int64_t 
   return check_launch("pdh_linear_xent_fwd (join)");
 }
 
+// Both gradient products of a piece: entries v0 .. v0 + nv - 1.
+template <int DT, int ODT, typename C, bool SPLIT>
+void run_prod(const Problem& q, const BwdPlan& p, const Operand& wv, const Operand& dz, int64_t v0, int64_t nv,
+              float down, void* dw, hipStream_t s) {
+  const int64_t dp = q.dp();
+  void* rows = static_cast<char*>(dw) + v0 * q.d * (ODT == PDH_F32 ? 4 : 2);
+  const bool split = p.slices.w > 1;
+  ProdArgs a{};
+  a.w = tiles<C>(p.x, dz, q.d, nv, q.n, p.slices.kw);
+  a.x = tiles<C>(wv, dz, q.d, q.n, nv, p.slices.kx);
+  a.tiles_w = static_cast<int>(count(a.w)), a.tiles_x = static_cast<int>(count(a.x));
+  a.x_first = p.slices.kx > p.slices.kw;
+  a.dw = split ? p.parts_w : rows;
+  a.parts = p.parts, a.lddw = q.d, a.ldp = dp, a.slice_w = nv * dp, a.slice = q.n * dp;
+  a.most = p.most, a.down = down, a.add = v0 > 0;
+  xent_prod<DT, ODT, C, SPLIT><<<run_grid(a.tiles_w, a.tiles_x), 256, 0, s>>>(a);
+  if (split)
+    xent_sum<ODT><<<dim3(blocks_for(nv * (dp / 4))), 256, 0, s>>>(p.parts_w, rows, nv, static_cast<int>(q.d), dp,
+                                                                 nv * dp, static_cast<int>(p.slices.w), p.most, down);
+}
+
 template <int DT, int ODT, bool SPLIT>
 int run_bwd(const Problem& q, const BwdPlan& p, const int64_t* targets, const float* lse, const float* dloss,
             int64_t ignore, void* dx, void* dw, hipStream_t s) {
   const MostArgs most{dloss, targets, q.n, q.v, ignore, p.most};
   const float raise = DT == PDH_F16 ? 16384.f : 1.f;
   if (int rc = prepare("pdh_linear_xent_bwd (pack)", q, p.pack_w, p.pack_x, most, s); rc != PDH_OK) return rc;
-  const int64_t es = ODT == PDH_F32 ? 4 : 2, dp = q.dp(), slice = q.n * dp;
+  const int64_t dp = q.dp();
   for (int64_t v0 = 0; v0 < q.v; v0 += p.piece) {
     const int64_t nv = std::min(p.piece, q.v - v0), ldz = up(nv, 256);
     const Operand wv{p.w.p + v0 * p.w.pitch, p.w.pitch, p.w.plane};
@@ -1070,19 +1125,17 @@ int run_bwd(const Problem& q, const BwdPlan& p, const int64_t* targets, const fl
     const GradArgs ga{logit_tiles(tiles<Big>(wv, p.x, nv, q.n, dp, up(dp, kBK))), targets, lse, dloss, p.most, raise,
                       p.dz, ldz, q.n * ldz, v0, q.v, ignore};
     xent_dz<DT, SPLIT><<<run_grid(ga.l.big, ga.l.small), 256, 0, s>>>(ga);
-    ProdArgs pr{};
-    pr.w = tiles<Big>(p.x, dz, q.d, nv, q.n, up(q.n, kBK));
-    pr.x = tiles<Big>(wv, dz, q.d, q.n, nv, p.kslice);
-    pr.tiles_w = static_cast<int>(count(pr.w)), pr.tiles_x = static_cast<int>(count(pr.x));
-    pr.x_first = p.kslice > q.n;
-    pr.dw = static_cast<char*>(dw) + v0 * q.d * es;
-    pr.parts = p.parts, pr.lddw = q.d, pr.ldp = dp, pr.slice = slice;
-    pr.most = p.most, pr.down = 1.f / raise, pr.add = v0 > 0;
-    xent_prod<DT, ODT, SPLIT><<<run_grid(pr.tiles_w, pr.tiles_x), 256, 0, s>>>(pr);
+    const Prod kind = pick_prod(q.d);
+    if (kind == Prod::kBig)
+      run_prod<DT, ODT, Big, SPLIT>(q, p, wv, dz, v0, nv, 1.f / raise, dw, s);
+    else if (kind == Prod::kHalf)
+      run_prod<DT, ODT, Half, SPLIT>(q, p, wv, dz, v0, nv, 1.f / raise, dw, s);
+    else
+      run_prod<DT, ODT, Quarter, SPLIT>(q, p, wv, dz, v0, nv, 1.f / raise, dw, s);
     if (int rc = check_launch("pdh_linear_xent_bwd"); rc != PDH_OK) return rc;
   }
-  xent_dx<ODT><<<dim3(blocks_for(q.n * (dp / 4))), 256, 0, s>>>(p.parts, dx, q.n, static_cast<int>(q.d), dp, slice,
-                                                               static_cast<int>(p.slices), p.most, 1.f / raise);
+  xent_sum<ODT><<<dim3(blocks_for(q.n * (dp / 4))), 256, 0, s>>>(p.parts, dx, q.n, static_cast<int>(q.d), dp, q.n * dp,
+                                                                static_cast<int>(p.slices.x), p.most, 1.f / raise);
   return check_launch("pdh_linear_xent_bwd (dx)");
 }
 
@@ -1112,14 +1165,12 @@ extern "C" int pdh_linear_xent_fwd(const void* x, const void* w, const int64_t* 
   PDH_REQUIRE(x && w && targets && loss && lse, PDH_EINVAL, "pdh_linear_xent_fwd: null pointer");
   const Problem q{tokens, width, vocab, ldx, ldw, x, w, dtype};
   const bool fx = Problem::fit(x, ldx, width, dtype), fw = Problem::fit(w, ldw, width, dtype);
-  Space measure{nullptr};
-  plan_fwd(q, measure, fx, fw);
-  PDH_REQUIRE(ws && aligned16(ws) && ws_bytes >= measure.used, PDH_EINVAL,
-              "pdh_linear_xent_fwd: the workspace holds %zu bytes, %zu are needed, 16-byte aligned", ws ? ws_bytes : size_t{0},
-              measure.used);
-  hipStream_t s = as_stream(stream);
   Space space{static_cast<char*>(ws)};
   const FwdPlan p = plan_fwd(q, space, fx, fw);
+  PDH_REQUIRE(ws && aligned16(ws) && ws_bytes >= space.used, PDH_EINVAL,
+              "pdh_linear_xent_fwd: the workspace holds %zu bytes, %zu are needed, 16-byte aligned", ws ? ws_bytes : size_t{0},
+              space.used);
+  hipStream_t s = as_stream(stream);
   if (dtype == PDH_F32) return run_fwd<PDH_BF16, true>(q, p, targets, ignore_index, loss, lse, bad, s);
   if (dtype == PDH_BF16) return run_fwd<PDH_BF16, false>(q, p, targets, ignore_index, loss, lse, bad, s);
   return run_fwd<PDH_F16, false>(q, p, targets, ignore_index, loss, lse, bad, s);
@@ -1134,14 +1185,12 @@ extern "C" int pdh_linear_xent_bwd(const void* x, const void* w, const int64_t* 
   PDH_REQUIRE(x && w && targets && lse && dloss && dx && dw, PDH_EINVAL, "pdh_linear_xent_bwd: null pointer");
   const Problem q{tokens, width, vocab, ldx, ldw, x, w, dtype};
   const bool fx = Problem::fit(x, ldx, width, dtype), fw = Problem::fit(w, ldw, width, dtype);
-  Space measure{nullptr};
-  plan_bwd(q, measure, fx, fw);
-  PDH_REQUIRE(ws && aligned16(ws) && ws_bytes >= measure.used, PDH_EINVAL,
-              "pdh_linear_xent_bwd: the workspace holds %zu bytes, %zu are needed, 16-byte aligned", ws ? ws_bytes : size_t{0},
-              measure.used);
-  hipStream_t s = as_stream(stream);
   Space space{static_cast<char*>(ws)};
   const BwdPlan p = plan_bwd(q, space, fx, fw);
+  PDH_REQUIRE(ws && aligned16(ws) && ws_bytes >= space.used, PDH_EINVAL,
+              "pdh_linear_xent_bwd: the workspace holds %zu bytes, %zu are needed, 16-byte aligned", ws ? ws_bytes : size_t{0},
+              space.used);
+  hipStream_t s = as_stream(stream);
   if (dtype == PDH_F32) return run_bwd<PDH_BF16, PDH_F32, true>(q, p, targets, lse, dloss, ignore_index, dx, dw, s);
   if (dtype == PDH_BF16) return run_bwd<PDH_BF16, PDH_BF16, false>(q, p, targets, lse, dloss, ignore_index, dx, dw, s);
   return run_bwd<PDH_F16, PDH_F16, false>(q, p, targets, lse, dloss, ignore_index, dx, dw, s);

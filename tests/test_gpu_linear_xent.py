@@ -110,6 +110,24 @@ def test_loss_and_gradient(shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(2100, 64, 300), (3001, 100, 203), (1600, 200, 700), (4500, 8, 9), (1030, 391, 260)])
+def test_many_tokens_over_a_small_vocabulary(shape, dtype):
+    """dw's product in parts over the tokens, in each width's tiles; the same bits again."""
+    from pdum_dsl_amd import kernels as K
+
+    n, d, v = shape
+    rng = np.random.default_rng(n + d + v)
+    x, w = _draw(rng, (n, d), dtype), _draw(rng, (v, d), dtype, 2.0 * d**-0.5)
+    t = torch.as_tensor(rng.integers(0, v, n)).cuda()
+    dloss = torch.as_tensor(rng.standard_normal(n) / n, dtype=torch.float32).cuda()
+    f = K.linear_cross_entropy(x, w, t)
+    g = K.linear_cross_entropy_bwd(x, w, t, f.lse, dloss)
+    _check(x, w, t, dloss, f, g, dtype)
+    for a, b in zip(g, K.linear_cross_entropy_bwd(x, w, t, f.lse, dloss)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_ignored_and_bad_targets(dtype):
     """Ignored tokens have no loss and no gradient, targets outside the
     vocabulary likewise and are counted; ignore_index may be an entry."""

@@ -86,7 +86,7 @@ def _fragment(lds, R, T, kc, perm, wq, t, ks):
     return out
 
 
-@pytest.mark.parametrize("R,T", [(256, 4), (128, 2), (128, 4), (64, 1), (64, 2)])
+@pytest.mark.parametrize("R,T", [(256, 4), (256, 2), (128, 2), (128, 4), (64, 1), (64, 2)])
 @pytest.mark.parametrize("kc", [True, False])
 @pytest.mark.parametrize("perm", [True, False])
 def test_fragments_hold_the_rows_and_columns_the_epilogues_assume(R, T, kc, perm):
@@ -111,7 +111,7 @@ def test_fragments_hold_the_rows_and_columns_the_epilogues_assume(R, T, kc, perm
                         assert kc and v == (row, k) and k < (k1 + 7) & ~7  # (rows past the last feed no output)
 
 
-@pytest.mark.parametrize("R,T", [(256, 4), (128, 2), (64, 1)])
+@pytest.mark.parametrize("R,T", [(256, 4), (256, 2), (128, 2), (128, 4), (64, 1), (64, 2)])
 @pytest.mark.parametrize("perm", [True, False])
 def test_no_read_meets_a_bank_twice(R, T, perm):
     for kc, width in ((True, 16), (False, 8)):
