@@ -470,8 +470,9 @@ int64_t bwd_parts(int64_t rows, int64_t cols, int dtype) {
 template <int DT, bool AFFINE>
 void launch_bwd(const NormGradArgs& a, unsigned groups, hipStream_t s) {
   if (long_rows(a.cols, DT)) {
-    norm_bwd_long<DT><<<dim3(static_cast<unsigned>(a.rows < kLongGroups ? a.rows : kLongGroups)), 1024, 0, s>>>(a);
+    // the column sums first: dx may take x's or dy's place
     if (AFFINE) norm_cols_long<DT><<<dim3((a.cols + 63) / 64, groups), 256, 0, s>>>(a);
+    norm_bwd_long<DT><<<dim3(static_cast<unsigned>(a.rows < kLongGroups ? a.rows : kLongGroups)), 1024, 0, s>>>(a);
   } else if (a.cols <= 1024)
     norm_bwd<DT, 1, 8, AFFINE><<<dim3(groups), 512, 0, s>>>(a);
   else if (a.cols <= 4096)

@@ -159,6 +159,28 @@ def test_layernorm_in_place_and_repeatable():
     assert K.layernorm_fwd(z, g, out=z).y is z and torch.equal(z, f.y)
 
 
+@pytest.mark.parametrize("where", ["x", "dy", "dres"])
+@pytest.mark.parametrize("cols", [3, 100, 1500, 5000, 9001, 16401])
+def test_layernorm_gradient_in_the_place_of_an_input(cols, where):
+    """The C entry point's dx may be x, dy or dres: as into a tensor of its own, bit for bit."""
+    from pdum_dsl_amd import _lib
+    from pdum_dsl_amd import kernels as K
+
+    rows = 37
+    ins = {k: torch.randn((rows, cols), device="cuda").bfloat16() for k in ("x", "dy", "dres")}
+    g = torch.randn(cols, device="cuda").bfloat16()
+    f = K.layernorm_fwd(ins["x"], g)
+    want = K.layernorm_bwd(ins["x"], ins["dy"], f.mean, f.rstd, g, dres=ins["dres"])
+    dg, db = torch.empty_like(g), torch.empty_like(g)
+    need = _lib.lib().pdh_layernorm_bwd_workspace(rows, cols, _lib.PDH_BF16)
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    _lib.call("pdh_layernorm_bwd", ins["x"].data_ptr(), ins["dy"].data_ptr(), ins["dres"].data_ptr(), g.data_ptr(),
+              f.mean.data_ptr(), f.rstd.data_ptr(), ins[where].data_ptr(), dg.data_ptr(), db.data_ptr(), rows, cols,
+              cols, cols, cols, cols, _lib.PDH_BF16, ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+    for a, b in zip((ins[where], dg, db), want):
+        assert torch.equal(a, b)
+
+
 def test_layernorm_gradient_matches_differences():
     """The device's gradient against central differences of the float64
     forward along random directions."""
