@@ -166,7 +166,8 @@ int pdh_dropout(const void* x, const void* residual, void* y, int64_t rows, int6
  * dloss, fp32 [tokens], the gradient of each token's loss:
  *   dz[n, v] = dloss[n] (exp(z[n, v] - lse[n]) - [v == targets[n]])
  *   dx = dz w [tokens][width], dw = dz^T x [vocab][width], dense, of `dtype`
- * computing z again piece by piece of the vocabulary. Products accumulate in
+ * computing z again piece by piece of the vocabulary. A token without a gradient
+ * counts for nothing in dw whatever x holds there. Products accumulate in
  * fp32. dz of a piece is taken over the largest |dloss|; 16-bit types: rounded to the
  * type; PDH_F32: operands
  * are split into three bf16 terms each, six products of them, as
@@ -176,8 +177,8 @@ int pdh_dropout(const void* x, const void* residual, void* y, int64_t rows, int6
  * atomic: results repeat bit for bit. The backward needs tokens >= 1.
  * ws, 16-byte aligned, holds pdh_linear_xent_workspace bytes for the same
  * x, w (looked at for alignment alone), sizes, strides and direction: packed
- * operands where x or w is fp32 or cannot be read by 16-byte chunks, one
- * piece's dz (at most 2^30 bytes, or 256 vocabulary entries), and partial
+ * operands where x or w is fp32 or cannot be read by 16-byte chunks (x always
+ * in the backward), one piece's dz (at most 2^30 bytes, or 256 vocabulary entries), and partial
  * sums. At most 2^24 tokens and entries, 2^18 features, 2^38 logits. No
  * counterpart in the reference. */
 size_t pdh_linear_xent_workspace(const void* x, const void* w, int64_t tokens, int64_t width, int64_t vocab,

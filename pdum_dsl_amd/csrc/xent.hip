@@ -796,13 +796,18 @@ __device__ __forceinline__ void most_dloss(const MostArgs& p) {
 
 // An operand made fit for the direct loads: rows of `dp` (a multiple of 8)
 // 16-bit values, zero past d. fp32 rows become three planes of bf16 terms,
-// 16-bit ones of odd width, stride or alignment a padded copy.
+// 16-bit ones of odd width, stride or alignment a padded copy. The backward's
+// tokens are always copied: an ignored one's row comes out zero, so that what a
+// padded batch holds there (infinities, NaN) never meets dw's products (8192 x
+// 768 x 50257 bf16 1931 us either way, 4096 x 4096 x 50257 4394 -> 4423).
 struct PackArgs {
   const void* src;  // NULL: read in place
   int64_t ld, rows;
   int d, dp;
   uint16_t* dst;
   int64_t plane;
+  const int64_t* targets;  // NULL: every row; or a row without a target in [0, vocab) is zero
+  int64_t vocab, ignore;
 };
 template <int DT>
 __device__ __forceinline__ void pack_rows(const PackArgs& p, int64_t i) {
@@ -810,6 +815,14 @@ __device__ __forceinline__ void pack_rows(const PackArgs& p, int64_t i) {
   const int c = static_cast<int>(i - n * per) * 8;
   if (n >= p.rows) return;
   uint16_t* o = p.dst + n * p.dp + c;
+  if (p.targets) {
+    const int64_t t = p.targets[n];
+    if (t < 0 || t >= p.vocab || t == p.ignore) {
+#pragma unroll
+      for (int pl = 0; pl < (DT == PDH_F32 ? 3 : 1); ++pl) *reinterpret_cast<u32x4*>(o + pl * p.plane) = u32x4{};
+      return;
+    }
+  }
   if constexpr (DT == PDH_F32) {
     const float* x = static_cast<const float*>(p.src) + n * p.ld + c;
     float v[8];
@@ -905,7 +918,7 @@ Operand place(const void* p, int64_t ld, int64_t rows, const Problem& q, Space& 
   if (in_place) return Operand{static_cast<const char*>(p), ld * 2, 0};
   const int64_t dp = q.dp(), plane = rows * dp;
   auto* dst = static_cast<uint16_t*>(ws.take(plane * 2 * q.planes()));
-  pack = PackArgs{p, ld, rows, static_cast<int>(q.d), static_cast<int>(dp), dst, plane};
+  pack = PackArgs{p, ld, rows, static_cast<int>(q.d), static_cast<int>(dp), dst, plane, nullptr, 0, 0};
   return Operand{reinterpret_cast<const char*>(dst), dp * 2, plane * 2};
 }
 
@@ -1063,10 +1076,10 @@ struct BwdPlan {
   int64_t piece;   // vocabulary entries of a piece (the last one's may be fewer)
   Slices slices;   // of a whole piece
 };
-BwdPlan plan_bwd(const Problem& q, Space& ws, bool fit_x, bool fit_w) {
+BwdPlan plan_bwd(const Problem& q, Space& ws, bool fit_w) {
   BwdPlan p{};
   p.w = place(q.w, q.ldw, q.v, q, ws, fit_w, p.pack_w);
-  p.x = place(q.x, q.ldx, q.n, q, ws, fit_x, p.pack_x);
+  p.x = place(q.x, q.ldx, q.n, q, ws, false, p.pack_x);
   const int64_t all = up(q.v, 256), most = kPieceBytes / (q.n * 2 * q.planes()) / 256 * 256;
   // (2^22 entries keep a tile's rows of dz within the loads' 32-bit offsets: that many only of 128 tokens or fewer)
   p.piece = std::min(std::min(all, int64_t{1} << 22), std::max<int64_t>(most, 256));
@@ -1116,7 +1129,9 @@ int run_bwd(const Problem& q, const BwdPlan& p, const int64_t* targets, const fl
             int64_t ignore, void* dx, void* dw, hipStream_t s) {
   const MostArgs most{dloss, targets, q.n, q.v, ignore, p.most};
   const float raise = DT == PDH_F16 ? 16384.f : 1.f;
-  if (int rc = prepare("pdh_linear_xent_bwd (pack)", q, p.pack_w, p.pack_x, most, s); rc != PDH_OK) return rc;
+  PackArgs live = p.pack_x;
+  live.targets = targets, live.vocab = q.v, live.ignore = ignore;
+  if (int rc = prepare("pdh_linear_xent_bwd (pack)", q, p.pack_w, live, most, s); rc != PDH_OK) return rc;
   const int64_t dp = q.dp();
   for (int64_t v0 = 0; v0 < q.v; v0 += p.piece) {
     const int64_t nv = std::min(p.piece, q.v - v0), ldz = up(nv, 256);
@@ -1151,7 +1166,7 @@ extern "C" size_t pdh_linear_xent_workspace(const void* x, const void* w, int64_
   const bool fx = Problem::fit(x, ldx, width, dtype), fw = Problem::fit(w, ldw, width, dtype);
   Space ws{nullptr};
   if (backward)
-    plan_bwd(q, ws, fx, fw);
+    plan_bwd(q, ws, fw);
   else
     plan_fwd(q, ws, fx, fw);
   return ws.used;
@@ -1184,9 +1199,9 @@ extern "C" int pdh_linear_xent_bwd(const void* x, const void* w, const int64_t* 
   PDH_REQUIRE(tokens > 0, PDH_EINVAL, "pdh_linear_xent_bwd: no tokens");
   PDH_REQUIRE(x && w && targets && lse && dloss && dx && dw, PDH_EINVAL, "pdh_linear_xent_bwd: null pointer");
   const Problem q{tokens, width, vocab, ldx, ldw, x, w, dtype};
-  const bool fx = Problem::fit(x, ldx, width, dtype), fw = Problem::fit(w, ldw, width, dtype);
+  const bool fw = Problem::fit(w, ldw, width, dtype);
   Space space{static_cast<char*>(ws)};
-  const BwdPlan p = plan_bwd(q, space, fx, fw);
+  const BwdPlan p = plan_bwd(q, space, fw);
   PDH_REQUIRE(ws && aligned16(ws) && ws_bytes >= space.used, PDH_EINVAL,
               "pdh_linear_xent_bwd: the workspace holds %zu bytes, %zu are needed, 16-byte aligned", ws ? ws_bytes : size_t{0},
               space.used);

@@ -409,8 +409,8 @@ def linear_cross_entropy_bwd(
     """Gradients (dx, dw) of sum(dloss * loss) for :func:`linear_cross_entropy`
     given its lse; ``dloss`` (fp32, the targets' shape) is each token's weight,
     1 / live tokens for a mean. Of x's and w's element type, rounded once from
-    fp32 sums; deterministic. An ignored token's dx is zero; its x is still
-    multiplied by zeros into dw, so it has to be finite."""
+    fp32 sums; deterministic. An ignored token's dx is zero and its x counts
+    for nothing in dw, infinities and NaN included."""
     _one_device(x, w, targets, lse, dloss)
     x2, w2, t, code, sizes = _head("linear_cross_entropy_bwd", x, w, targets)
     for nm, s in (("lse", lse), ("dloss", dloss)):

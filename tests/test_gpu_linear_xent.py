@@ -225,6 +225,33 @@ def test_non_finite_tokens_stay_their_own(dtype):
     assert torch.isfinite(dx[keep]).all() and not torch.isfinite(dx[[3, 6]]).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n, d, v", [(40, 64, 300), (1100, 72, 333), (33, 51, 130)])
+def test_ignored_tokens_may_hold_anything(n, d, v, dtype):
+    """Rows of a padded batch hold NaN and infinities, as do their lse and
+    dloss: the live tokens' loss and every gradient are those of finite rows."""
+    from pdum_dsl_amd import kernels as K
+
+    rng = np.random.default_rng(n)
+    x, w = _draw(rng, (n, d), dtype), _draw(rng, (v, d), dtype, 0.3)
+    ht = rng.integers(0, v, n)
+    ht[-n // 4:] = -100
+    ht[2] = v + 7
+    t = torch.as_tensor(ht).cuda()
+    dloss = torch.as_tensor(rng.standard_normal(n) / n, dtype=torch.float32).cuda()
+    f = K.linear_cross_entropy(x, w, t)
+    want = K.linear_cross_entropy_bwd(x, w, t, f.lse, dloss)
+    dead = torch.as_tensor((ht < 0) | (ht >= v)).cuda()
+    y, nan = x.clone(), float("nan")
+    y[dead] = nan
+    y[2] = float("inf")
+    g = K.linear_cross_entropy(y, w, t)
+    assert torch.equal(g.loss, f.loss) and torch.equal(g.lse[~dead], f.lse[~dead])
+    got = K.linear_cross_entropy_bwd(y, w, t, g.lse, torch.where(dead, nan, dloss))
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
 def test_the_gradient_matches_differences():
     """Along random directions, central differences of the float64 loss."""
     from pdum_dsl_amd import kernels as K

@@ -150,6 +150,7 @@ def test_linear_xent_refusals():
         _refused(f(n=1 << 24, v=1 << 24), "2^38 logits", _lib.PDH_EUNSUPPORTED)
     assert fwd(n=0) == _lib.PDH_OK
     _refused(bwd(n=0), "no tokens")
-    need = lambda x, ldx, dt: lib.pdh_linear_xent_workspace(C.c_void_p(x), FAKE, 1000, 64, 5000, ldx, 64, dt, 1)  # noqa: E731
+    need = lambda x, ldx, dt, bwd=0: lib.pdh_linear_xent_workspace(C.c_void_p(x), FAKE, 1000, 64, 5000, ldx, 64, dt, bwd)  # noqa: E731
     assert need(256, 64, 1) < need(258, 64, 1) == need(256, 65, 1) < need(256, 64, 0)  # packed where not read in place
+    assert need(256, 64, 1, 1) == need(258, 64, 1, 1) < need(256, 64, 0, 1)  # the backward always packs x
     assert lib.pdh_linear_xent_workspace(FAKE, FAKE, 0, 64, 5000, 64, 64, 1, 1) == 0
