@@ -307,6 +307,51 @@ def test_several_pieces_of_the_vocabulary():
         assert ((got.double() - want).abs() <= lim).all()
 
 
+@pytest.mark.parametrize("n, d, v, dtype", [(3000, 200, 70001, torch.float32), (9000, 100, 70001, torch.bfloat16),
+                                            (5000, 500, 120001, torch.float16)])
+def test_pieces_in_every_width_of_tile(n, d, v, dtype):
+    """Two pieces whose dw is in parts over the tokens (the first two shapes) or
+    whole, ignored tokens among them. Against the formulas given the device's lse:
+    the bounds above without lse's error."""
+    from pdum_dsl_amd import kernels as K
+
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    x = torch.randn((n, d), generator=gen, device="cuda").to(dtype)
+    w = (0.2 * torch.randn((v, d), generator=gen, device="cuda")).to(dtype)
+    t = torch.randint(0, v, (n,), generator=gen, device="cuda")
+    t[::5] = -100
+    g = torch.rand(n, generator=gen, device="cuda") / n
+    f = K.linear_cross_entropy(x, w, t)
+    dx, dw = K.linear_cross_entropy_bwd(x, w, t, f.lse, g)
+    live = (t >= 0).double()[:, None]
+    hx, gd, lse = x.double(), g.double()[:, None] * live, f.lse.double()[:, None]
+    m = lambda k: 6 * U * (4 * -(-k // 16) * (6 if dtype == torch.float32 else 1)) ** 0.5  # noqa: E731
+    tiny = 2.0**-25 * 2.0 ** (np.floor(np.log2(g.max().item())) + 1 - 14) if dtype == torch.float16 else 0.0
+    wx, ex, qx = (torch.zeros((n, d), dtype=torch.float64, device="cuda") for _ in range(3))
+    ok = True
+    for lo in range(0, v, 10000):
+        wc = w[lo:lo + 10000].double()
+        z = hx @ wc.T
+        ep = m(d) * (z.abs() + 4 * ((hx**2) @ (wc**2).T).sqrt()) + 4 * U * (z.abs() + lse.abs() + 1)
+        p = torch.exp(z - lse)
+        dz = p.clone()
+        hit = (t >= lo) & (t < lo + wc.shape[0])
+        dz[hit.nonzero()[:, 0], t[hit] - lo] -= 1.0
+        dz *= gd
+        e = HALF[dtype] * dz.abs() + gd * (p * ep + 2 * U) + tiny * live
+        wx += dz @ wc
+        ex += e @ wc.abs()
+        qx += (dz**2) @ (wc**2)
+        want = dz.T @ hx
+        err = e.T @ hx.abs() + m(n) * (want.abs() + 4 * ((dz**2).T @ (hx**2)).sqrt())
+        lim = err + HALF[dtype] * (want.abs() + err) + (2.0**-25 if dtype == torch.float16 else 0.0)
+        ok = ok and bool(((dw[lo:lo + 10000].double() - want).abs() <= lim).all())
+    assert ok
+    err = ex + m(v) * (wx.abs() + 4 * qx.sqrt())
+    lim = err + HALF[dtype] * (wx.abs() + err) + (2.0**-25 if dtype == torch.float16 else 0.0)
+    assert ((dx.double() - wx).abs() <= lim).all()
+
+
 def test_loss_repeats_and_replays_in_a_graph():
     from pdum_dsl_amd import kernels as K
 
