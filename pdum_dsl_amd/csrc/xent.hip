@@ -616,7 +616,8 @@ struct DzEpilogue {
       const bool live = t >= 0 && t < p.vocab && t != p.ignore;
       f.target[j] = live ? static_cast<int>(t - p.v0) : kNoToken;
       f.g[j] = live ? p.dloss[n] / *p.most * p.raise : 0.f;
-      f.lse2[j] = live ? p.lse[n] * kLog2e : 0.f;
+      // an ignored token's x is zeros: 0 = exp2(-inf) times 0
+      f.lse2[j] = live ? p.lse[n] * kLog2e : __builtin_inff();
     }
     return f;
   }
@@ -640,11 +641,18 @@ struct DzEpilogue {
           for (int e = 0; e < 16; ++e)
             if (at == e) acc[i][j][e] -= 1.f;
         }
-        // an ignored token has no gradient whatever its logits are; entries past the vocabulary are zero
-        const int c = cw + 32 * i + 16 * g;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) acc[i][j][e] = live && c + e < p.l.t.m ? acc[i][j][e] * f.g[j] : 0.f;
+        for (int e = 0; e < 16; ++e) acc[i][j][e] *= f.g[j];
       }
+    }
+    if (cw + 32 * TM > p.l.t.m) {  // entries past the vocabulary are zero
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (cw + 32 * i + 16 * g + e >= p.l.t.m) acc[i][j][e] = 0.f;
     }
     __syncthreads();  // the tile loop's last reads are over: LDS serves the stores
     lds += w * put_bytes<2, TM>();
