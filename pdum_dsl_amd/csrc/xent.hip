@@ -33,12 +33,12 @@
 // fp32's terms stay clear of subnormal values for weights of any size. fp32 operands are split into three bf16 terms
 // and the six cross products above 2^-24 are summed, smallest first.
 //
-// Bound by the matrix pipe at the clock that the power limit leaves it (46-68%
-// busy at 1.65-1.9 GHz in every large product). Forward and backward in us, and
+// Bound by the matrix pipe at the clock that the power limit leaves it (49-68%
+// busy at 1.55-1.9 GHz in every large product). Forward and backward in us, and
 // the rate of the products run (z's again among the backward's): 8192 x 768 x
-// 50257 bf16 553 (1143 TF/s) and 1931 (983), 4096 x 4096 x 50257 1390 (1213) and
-// 4400 (1150), 1024 x 768 x 50257 fp32 445 (1066, of bf16 products) and 1400
-// (1015); a library's bf16 product of 16384 cubed runs at 1338, of 8192 cubed at
+// 50257 bf16 554 (1141 TF/s) and 1903 (997), 4096 x 4096 x 50257 1390 (1213) and
+// 4390 (1153), 1024 x 768 x 50257 fp32 445 (1066, of bf16 products) and 1385
+// (1027); a library's bf16 product of 16384 cubed runs at 1338, of 8192 cubed at
 // 1088. Small ones are bound by steps of 0.5 us a 64-deep k tile on few
 // compute units (100 x 768 x 5003: 9 us of product, 4 of join).
 #include "common.h"
