@@ -1008,7 +1008,9 @@ double makespan(int64_t n1, double d1, int64_t n2, double d2, int64_t s) {
 enum class Prod { kBig, kHalf, kQuarter };
 Prod pick_prod(int64_t d) { return d <= 64 ? Prod::kQuarter : (d + 127) / 128 % 2 ? Prod::kHalf : Prod::kBig; }
 
-// k columns of a slice, and slices, of the two gradient products.
+// k columns of a slice, and slices, of the two gradient products of the first
+// piece: the parts that are summed are those that its launch writes (a later
+// piece, no longer, adds to them).
 struct Slices {
   int64_t kw, w, kx, x;
 };
@@ -1045,7 +1047,9 @@ Slices pick_slices(const Problem& q, int64_t piece) {
   }
   Slices r;
   r.kw = up((q.n + bw - 1) / bw, kBK), r.w = (q.n + r.kw - 1) / r.kw;
-  r.kx = up((piece + bx - 1) / bx, kBK), r.x = (piece + r.kx - 1) / r.kx;
+  // a piece of the whole vocabulary is rounded up to tiles, past which no slice may lie
+  const int64_t first = std::min(piece, q.v);
+  r.kx = up((piece + bx - 1) / bx, kBK), r.x = (first + r.kx - 1) / r.kx;
   return r;
 }
 
@@ -1091,7 +1095,7 @@ struct BwdPlan {
   float* most;
   float* parts_w;  // dw's parts of a piece, where there are any
   int64_t piece;   // vocabulary entries of a piece (the last one's may be fewer)
-  Slices slices;   // of a whole piece
+  Slices slices;
 };
 BwdPlan plan_bwd(const Problem& q, Space& ws, bool fit_w) {
   BwdPlan p{};
