@@ -778,8 +778,9 @@ __global__ __launch_bounds__(256) void xent_sum(const float* __restrict__ part, 
     if (c + e < d) st_dt<DT>(dx, n * d + c + e, s[e]);
 }
 
-// *most = the largest finite |dloss| of a live token, 1 where there is none
-// (or it is infinite): dz is taken over it. One workgroup, sixteen tokens' loads
+// *most = the largest finite |dloss| of a live token, 1 where there is none:
+// dz is taken over it. (Over an infinite one, or over 1 beside it, fp16's dz of
+// every other token would leave its range.) One workgroup, sixteen tokens' loads
 // in flight a lane (8192 tokens: 7 us; one at a time, 36).
 struct MostArgs {
   const float* dloss;  // NULL: none to do
@@ -802,13 +803,13 @@ __device__ __forceinline__ void most_dloss(const MostArgs& p) {
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (t[u] >= 0 && t[u] < p.vocab && t[u] != p.ignore) mx = fmaxf(mx, fabsf(d[u]));
+      if (t[u] >= 0 && t[u] < p.vocab && t[u] != p.ignore && fabsf(d[u]) < __builtin_inff()) mx = fmaxf(mx, fabsf(d[u]));
   }
   mx = wave_max(mx);
   if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = mx;
   __syncthreads();
   mx = fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
-  if (threadIdx.x == 0) *p.most = mx > 0.f && mx < __builtin_inff() ? mx : 1.f;
+  if (threadIdx.x == 0) *p.most = mx > 0.f ? mx : 1.f;
 }
 
 // An operand made fit for the direct loads: rows of `dp` (a multiple of 8)
