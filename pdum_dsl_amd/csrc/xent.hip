@@ -968,10 +968,13 @@ TileArgs tiles(Operand a, Operand b, int64_t m, int64_t n, int64_t k, int64_t ks
 }
 int64_t count(const TileArgs& t) { return static_cast<int64_t>(t.tiles_m) * t.tiles_n * t.slices; }
 
-// Workgroups of these kernels that run at a time.
+// Workgroups of these kernels that run at a time on the current device, on which
+// the plan, and so the workspace and the order of the sums, depends.
 int64_t slots() {
-  static thread_local int cus = 0;
-  if (!cus) cus = pdh_device_cus();
+  static thread_local int of = -1, cus = 0;
+  int dev = -1;
+  if (hipGetDevice(&dev) != hipSuccess) dev = -1;
+  if (dev != of || !cus) of = dev, cus = pdh_device_cus();
   return 2 * (cus ? cus : 256);
 }
 

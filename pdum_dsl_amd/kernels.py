@@ -388,9 +388,14 @@ def linear_cross_entropy(
     return LossOut(loss, lse)
 
 
-@functools.lru_cache(maxsize=4096)
 def _head_workspace(px: int, pw: int, *args) -> int:
-    """pdh_linear_xent_workspace by the operands' alignment (it looks at nothing else of them)."""
+    """pdh_linear_xent_workspace by the operands' alignment (it looks at nothing else of them) on the
+    current device (whose compute units the plan counts)."""
+    return _head_workspace_on(torch._C._cuda_getDevice(), px, pw, *args)
+
+
+@functools.lru_cache(maxsize=4096)
+def _head_workspace_on(device: int, px: int, pw: int, *args) -> int:
     need = _lib.lib().pdh_linear_xent_workspace(256 + px, 256 + pw, *args)
     if need == 0:
         _lib.check("pdh_linear_xent_workspace", _lib.PDH_EUNSUPPORTED)
