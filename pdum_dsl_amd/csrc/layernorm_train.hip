@@ -22,12 +22,20 @@
 // hide no more latency and double the partial sums: 4096 x 4096 bf16 41.5 us
 // against 34.8, 2048 x 8192 50 against 36.
 //
-// Outputs leave past the caches: forward 8192 x 4096 fp32 47.6 -> 39.7 us (6.8
-// TB/s), 32768 x 768 bf16 21.8 -> 19.0. Loads past them gain in the backward
-// (8192 x 4096 fp32 82.7 -> 78.9) and cost in the forward (39.7 -> 49).
+// 8192 x 4096 fp32, the kernels' times in us: forward 38 (7.0 TB/s) on the same
+// tensors again and again, which the caches hold in part, 50 (5.4) on six sets of
+// tensors in turn; backward 71 (5.7) either way, 62 (6.4) right after the forward.
+// In turn, 32768 x 768 bf16: 22 and 30; 8192 x 768: 7.3 and 11.9.
+// Outputs leave past the caches (in the caches' place, forward in a step 66
+// against 51, 8192 x 768 bf16 8.4 against 7.0). Loads go past them in the backward
+// (through them, 75 against 71 in turn, but 64 against 71 on the same tensors) and
+// through them in the forward (past them, 49 against 38 on the same tensors, and
+// the backward after it 71 against 62).
 //
 // Rows of over 16384 columns, or of fewer than a chunk, take one workgroup a
-// row in several passes, and column sums by a kernel of their own.
+// row in several passes of single elements, and column sums by a kernel of their
+// own: right for any width, and far from the bytes' rate (forward and backward,
+// 2048 x 20000 bf16 122 and 198 us, fp32 152 and 244; 65536 x 3 fp32 263 and 299).
 #include "common.h"
 
 namespace pdh {
@@ -302,8 +310,9 @@ __global__ __launch_bounds__(64 * W * R) void norm_bwd(NormGradArgs a) {
 
 // dgamma / dbeta = the sums over `n` partial rows [n][2][cols], in a fixed
 // order: 16 columns of one of the two a workgroup, 64 lanes a column with
-// four loads in flight each (768 columns, 512 parts: 4 us against 20 with 8
-// lanes a column on 48 workgroups, a chain of loads).
+// four loads in flight each (768 columns, 256 parts: 3.5-4 us; 512 parts, of an
+// earlier grid, took 4 so and 20 with 8 lanes a column on 48 workgroups, a chain
+// of loads).
 template <int DT>
 __global__ __launch_bounds__(1024) void norm_weights(const float* __restrict__ part, int n, int64_t cols, void* dgamma,
                                                      void* dbeta) {

@@ -8,7 +8,8 @@
 // leaves the maximum and the sum of exponentials of its vocabulary strip of
 // every token, and the target's logit where it holds it; a second kernel joins
 // the strips. Backward: the vocabulary in pieces; for each the same product again,
-// dz of the piece stored in 16 bits, then dw's rows of the piece and the
+// dz of the piece stored in 16 bits (2 bytes a token and entry, fp32's three terms
+// 6; 1 GiB at the most, or 256 entries), then dw's rows of the piece and the
 // piece's part of dx as two more products. dx's parts over slices of the
 // vocabulary (and dw's over slices of the tokens, where its tiles are few) are
 // fp32 and added in order: no atomics, results repeat.
@@ -29,7 +30,8 @@
 // a mean's equal weights 1 / tokens would give every target's entry the same
 // rounding error, which no sum averages out (0.38% of the gradient at 7780
 // live tokens, 0.17% so, what the output's own rounding leaves); fp16 takes it
-// times 2^14 on top, or small probabilities would fall below its range, and
+// times 2^14 on top, or small probabilities would fall below its range (its spacing
+// is then 2^-38 of that weight at the finest), and
 // fp32's terms stay clear of subnormal values for weights of any size. fp32 operands are split into three bf16 terms
 // and the six cross products above 2^-24 are summed, smallest first.
 //

@@ -320,9 +320,9 @@ def dropout_fwd(
     (int64 on the device: seed and step), ``site`` (one number for each
     dropout of a step) and the element's place in x as rows of its last axis;
     it does not depend on the element type or the strides and is never
-    stored. ``rng`` is read when the kernel runs: move its step on between
-    training steps (``rng[1] += 1``), captured ones too, and keep it until the
-    backward has run. ``out`` may be x or residual itself."""
+    stored; of the step the low 32 bits count. ``rng`` is read when the kernel
+    runs: move its step on between training steps (``rng[1] += 1``), captured
+    ones too, and keep it until the backward has run. ``out`` may be x or residual itself."""
     return _dropout("dropout_fwd", x, p, rng, site, residual, out)
 
 
@@ -415,7 +415,11 @@ def linear_cross_entropy_bwd(
     given its lse; ``dloss`` (fp32, the targets' shape) is each token's weight,
     1 / live tokens for a mean. Of x's and w's element type, rounded once from
     fp32 sums; deterministic. An ignored token's dx is zero and its x counts
-    for nothing in dw, infinities and NaN included."""
+    for nothing in dw, infinities and NaN included. Beside the outputs the
+    call holds a piece's gradient of the logits (2 bytes for a token and
+    entry, 6 in fp32; 1 GiB, or 256 entries, at the most), partial sums of
+    dx and dw (2 GiB each at the most, or one fp32 dx) and a copy of x (of
+    w too where it is fp32 or its rows are not 16-byte chunks)."""
     _one_device(x, w, targets, lse, dloss)
     x2, w2, t, code, sizes = _head("linear_cross_entropy_bwd", x, w, targets)
     for nm, s in (("lse", lse), ("dloss", dloss)):
