@@ -260,7 +260,9 @@ def _own(s):
     from pdum_dsl_amd import kernels as K
 
     case = s["case"]
-    cache = K.PagedCache(s["k"], s["v"], s["k_scale"], s["v_scale"], TORCH[case["dtype"]])
+    if "cache" not in s:  # a program keeps its cache from step to step
+        s["cache"] = K.PagedCache(s["k"], s["v"], s["k_scale"], s["v_scale"], TORCH[case["dtype"]])
+    cache = s["cache"]
     if case["kind"] == "attend":
         return K.paged_attention(s["q"], cache, s["table"], s["starts"], s["lengths"], window=case["window"] or None,
                                  sinks=case["sinks"])
