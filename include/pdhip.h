@@ -318,6 +318,86 @@ int pdh_scan(const void* x, void* y, int64_t outer, int64_t n, int64_t inner, in
 int pdh_attn_decode_noalloc(const void* q, const void* k, const void* v, void* o, float* lse_out,
                             const pdh_attn_geom* geom, int dtype, float scale, int nsplit, void* stream);
 
+/* ---- paged caches: keys and values of many sequences, in pages.
+ *
+ * Pools [pages][heads][page_rows][features], features contiguous (64 or 128):
+ * token s of sequence i lies in page table[i][s / page_rows], row s % page_rows
+ * (page_rows a power of two, 16 to 4096). bits 16: elements of dtype
+ * (PDH_BF16 / PDH_F16). bits 4: e2m1 codes (0 .5 1 1.5 2 3 4 6 and a sign), two
+ * a byte, the even feature in the low half; features 32 g .. 32 g + 31 of a row
+ * are worth the code times 2^(byte - 127), byte g of the row's scales (255:
+ * NaN); dtype is the type that they are computed with. */
+typedef struct pdh_paged_cache {
+  void *k, *v;
+  void *k_scale, *v_scale;                 /* bits 4: [pages][heads][page_rows][features / 32]; else unused */
+  int64_t pages, heads, page_rows, features;
+  int64_t k_sp, k_sh, k_sr;                /* strides of a page, a head, a row: elements (bits 4: bytes), multiples */
+  int64_t v_sp, v_sh, v_sr;                /* of 16 bytes; rows less than 2^16 apart */
+  int64_t ks_sp, ks_sh, ks_sr, vs_sp, vs_sh, vs_sr; /* the scales', bytes */
+  int32_t dtype, bits;
+} pdh_paged_cache;
+
+/* The sequences of one call, device memory that the kernels read when they
+ * run: sequence i's new tokens are rows starts[i] .. starts[i + 1] - 1 (starts
+ * ascend) and the last of its lengths[i] tokens: row r has position
+ * lengths[i] - (starts[i + 1] - r). Values out of range reach no memory: a
+ * row outside [0, rows) is not there, a token before 0, past the table or on a
+ * page outside the pool has no place. */
+typedef struct pdh_paged_batch {
+  const int32_t* table;   /* [seqs][width], rows ld_table apart; width * page_rows <= 2^30 */
+  const int32_t* starts;  /* [seqs + 1] */
+  const int32_t* lengths; /* [seqs] */
+  int64_t seqs, rows, width, ld_table;
+} pdh_paged_batch;
+
+/* Store k and v [rows][heads][features] (strides *_st of a row, *_sh of a
+ * head, multiples of 8 elements, 16-byte aligned) at their tokens' places, and
+ * write q [rows][heads_q][features] to q_out (which may be q; both NULL with
+ * heads_q = 0). Where rotary (fp32 [positions][rotated], rows ld_rotary apart;
+ * cosines, then sines) is given, k and q are turned by their positions first:
+ * for i < rotated / 2 with (a, b) = features (i, i + rotated / 2), or (2 i, 2 i
+ * + 1) if interleaved, (a cos - b sin, b cos + a sin), in fp32, every product
+ * and sum rounded; rotated a multiple of 16. One rounding to dtype; or to 4
+ * bits: the scale's exponent is the least e in [-126, 125] (PDH_F16: 13) with
+ * max |y| <= 7 2^e of the group, codes are the nearest of y / 2^e (ties to even
+ * codes, past 6 to 6), a group with an infinity or a NaN gets byte 255.
+ * A token without a place, or past the rotary's positions, is stored nowhere,
+ * its row of q_out is zero, and it adds 1 to *bad (device int, may be NULL).
+ * Rows of no sequence are written zero to q_out where zero_rest != 0, else
+ * not at all. Tokens that share a place leave any of them, or a mixture. No
+ * counterpart in the reference. */
+int pdh_paged_append(const void* k, const void* v, const void* q, void* q_out, int64_t heads_q, int64_t k_st,
+                     int64_t k_sh, int64_t v_st, int64_t v_sh, int64_t q_st, int64_t q_sh, int64_t qo_st,
+                     int64_t qo_sh, const pdh_paged_cache* cache, const pdh_paged_batch* batch, const float* rotary,
+                     int64_t positions, int64_t rotated, int64_t ld_rotary, int interleaved, int zero_rest, int* bad,
+                     void* stream);
+
+/* The values that the cache holds of the batch's tokens, in dtype, to k_out
+ * and v_out [rows][heads][features]; tokens without a place are zero, rows of
+ * no sequence too where zero_rest != 0. No counterpart in the reference. */
+int pdh_paged_rows(void* k_out, void* v_out, int64_t ko_st, int64_t ko_sh, int64_t vo_st, int64_t vo_sh,
+                   const pdh_paged_cache* cache, const pdh_paged_batch* batch, int zero_rest, void* stream);
+
+/* Attention of the batch's rows over their sequences' caches: q, o
+ * [rows][heads_q][features] of dtype, query head h reads head h / (heads_q /
+ * heads), lse (may be NULL) fp32 [rows][heads_q]. A row at position p sees the
+ * tokens s <= p with s > p - window or s < sinks (window >= 1; 2^30 and more:
+ * all):
+ *   x = scale q . k_s, o = sum softmax(x) v_s, lse = log sum exp x   (scale > 0)
+ * fp32 scores, statistics and sums; the weights are rounded to dtype as
+ * factors. Tokens that a row does not see count for nothing in it whatever the
+ * pools hold. A row that sees nothing, or scores of -inf alone: o = 0, lse =
+ * -inf; rows of no sequence likewise where zero_rest != 0, else they are not
+ * written. ws, 16-byte aligned, holds pdh_paged_attention_workspace bytes for
+ * the same sizes (partial states of rows whose keys several workgroups share).
+ * Nothing is atomic: results repeat bit for bit. No counterpart in the
+ * reference. */
+size_t pdh_paged_attention_workspace(const pdh_paged_cache* cache, const pdh_paged_batch* batch, int64_t heads_q,
+                                     int64_t window, int64_t sinks);
+int pdh_paged_attention(const void* q, void* o, float* lse, int64_t heads_q, int64_t q_st, int64_t q_sh, int64_t o_st,
+                        int64_t o_sh, const pdh_paged_cache* cache, const pdh_paged_batch* batch, int64_t window,
+                        int64_t sinks, float scale, int zero_rest, void* ws, size_t ws_bytes, void* stream);
+
 /* ------------------------------------------------------------------------
  * Elementwise programs. The pointwise chains of the map-chain template and
  * of a contraction's epilogue are lowered to a small register program, run

@@ -45,6 +45,10 @@ EXPORTS = (
     "pdh_attn_decode_workspace",
     "pdh_attn_decode",
     "pdh_attn_decode_noalloc",
+    "pdh_paged_append",
+    "pdh_paged_rows",
+    "pdh_paged_attention_workspace",
+    "pdh_paged_attention",
     "pdh_map_chain",
     "pdh_contract",
     "pdh_contract_strided",
@@ -86,6 +90,26 @@ class AttnGeom(C.Structure):
     ]
 
 
+class PagedCacheC(C.Structure):
+    """pdh_paged_cache: a paged cache's pools, sizes and strides."""
+
+    _fields_ = [(n, C.c_void_p) for n in "k v k_scale v_scale".split()] + [
+        (n, C.c_int64)
+        for n in (
+            "pages heads page_rows features "
+            "k_sp k_sh k_sr v_sp v_sh v_sr ks_sp ks_sh ks_sr vs_sp vs_sh vs_sr"
+        ).split()
+    ] + [("dtype", C.c_int32), ("bits", C.c_int32)]
+
+
+class PagedBatch(C.Structure):
+    """pdh_paged_batch: the sequences of one call."""
+
+    _fields_ = [(n, C.c_void_p) for n in "table starts lengths".split()] + [
+        (n, C.c_int64) for n in "seqs rows width ld_table".split()
+    ]
+
+
 # elementwise programs (pdh_ew_program): limits and opcodes, as include/pdhip.h
 EW_MAX_INSNS, EW_MAX_REGS, EW_MAX_OPERANDS, EW_MAX_DIMS = 64, 16, 8, 4
 EW_OPS = (
@@ -119,6 +143,7 @@ def _declare(lib) -> None:
     vp, i64, i32, f32 = C.c_void_p, C.c_int64, C.c_int, C.c_float
     fp = C.POINTER(C.c_float)
     gp = C.POINTER(AttnGeom)
+    cp, bp = C.POINTER(PagedCacheC), C.POINTER(PagedBatch)
     sigs = {
         "pdh_version": (i32, []),
         "pdh_last_error": (C.c_size_t, [C.c_char_p, C.c_size_t]),
@@ -146,6 +171,12 @@ def _declare(lib) -> None:
         "pdh_attn_decode_workspace": (C.c_size_t, [gp, i32]),
         "pdh_attn_decode": (i32, [vp, vp, vp, vp, vp, gp, i32, f32, i32, vp, C.c_size_t, vp]),
         "pdh_attn_decode_noalloc": (i32, [vp, vp, vp, vp, vp, gp, i32, f32, i32, vp]),
+        "pdh_paged_append": (i32, [vp, vp, vp, vp, i64, i64, i64, i64, i64, i64, i64, i64, i64, cp, bp, vp, i64, i64,
+                                   i64, i32, i32, vp, vp]),
+        "pdh_paged_rows": (i32, [vp, vp, i64, i64, i64, i64, cp, bp, i32, vp]),
+        "pdh_paged_attention_workspace": (C.c_size_t, [cp, bp, i64, i64, i64]),
+        "pdh_paged_attention": (i32, [vp, vp, vp, i64, i64, i64, i64, i64, cp, bp, i64, i64, f32, i32, vp, C.c_size_t,
+                                      vp]),
         "pdh_map_chain": (i32, [C.POINTER(EwProgram), C.POINTER(vp), vp, i32, vp]),
         "pdh_contract": (i32, [vp, vp, i64, i64, i64, i64, i64, C.POINTER(EwProgram), C.POINTER(vp), vp, i32, vp]),
         "pdh_contract_strided": (

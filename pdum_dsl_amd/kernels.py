@@ -778,6 +778,282 @@ def attn_decode_static(
     )
 
 
+# ------------------------------------------------------------- paged caches
+
+
+@dataclass(frozen=True)
+class PagedCache:
+    """Keys and values of many sequences in pages of ``page_rows`` tokens
+    (a power of two, 16 to 4096): a sequence's tokens lie in the pages that its row of a
+    table names, wherever those are in the pool.
+
+    16 bits: ``k`` and ``v`` are [pages, heads, page_rows, features], bf16 or
+    f16, any strides that are multiples of 8 elements, features contiguous.
+    4 bits: ``k`` and ``v`` are uint8 [pages, heads, page_rows, features / 2]
+    (strides multiples of 16) and ``k_scale`` / ``v_scale`` uint8 [pages,
+    heads, page_rows, features / 32]: e2m1 codes, the even feature in the low
+    half of a byte, times 2^(scale - 127) (255: NaN). ``dtype`` is the 16-bit
+    type that they are computed with. features 64 or 128.
+
+    The object describes the tensors, whose contents the calls read and write;
+    they stay in place while it lives."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor | None = None
+    v_scale: torch.Tensor | None = None
+    dtype: torch.dtype | None = None
+
+    @functools.cached_property
+    def c(self) -> _lib.PagedCacheC:
+        """pdh_paged_cache, checked."""
+        k, v, ks, vs = self.k, self.v, self.k_scale, self.v_scale
+        bits = 4 if k.dtype == torch.uint8 else 16
+        dtype = self.dtype or (torch.bfloat16 if bits == 4 else k.dtype)
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"PagedCache: the values are bf16 or f16 (got {dtype})")
+        if v.dtype != k.dtype or (bits == 16 and k.dtype != dtype):
+            raise ValueError(f"PagedCache: k and v are both {dtype}, or both uint8 codes (got {k.dtype}, {v.dtype})")
+        if k.dim() != 4 or v.shape != k.shape or k.numel() == 0:
+            raise ValueError(f"PagedCache: k and v are [pages, heads, page_rows, features], not empty (got "
+                             f"{tuple(k.shape)}, {tuple(v.shape)})")
+        pages, heads, rows, d = k.shape
+        d = 2 * d if bits == 4 else d
+        if k.stride(3) != 1 or v.stride(3) != 1:
+            raise ValueError("PagedCache: features must be contiguous")
+        if (bits == 4) != (ks is not None) or (bits == 4) != (vs is not None):
+            raise ValueError("PagedCache: a 4-bit cache has k_scale and v_scale, a 16-bit one neither")
+
+        def apart(t):  # the strides of pages, heads and rows; those of a single one count for nothing
+            return [st if n > 1 else 0 for st, n in zip(t.stride()[:3], t.shape[:3])]
+
+        scales = [0] * 6
+        if bits == 4:
+            want = (pages, heads, rows, d // 32)
+            for nm, t in (("k_scale", ks), ("v_scale", vs)):
+                if t.dtype != torch.uint8 or tuple(t.shape) != want or t.stride(3) != 1:
+                    raise ValueError(f"PagedCache: {nm} must be uint8 {want} with contiguous groups")
+            scales = apart(ks) + apart(vs)
+        devices = {t.device for t in (k, v, ks, vs) if t is not None}
+        if len(devices) != 1:
+            raise ValueError("PagedCache: the tensors must be on one device")
+        return _lib.PagedCacheC(_ptr(k), _ptr(v), _ptr(ks), _ptr(vs), pages, heads, rows, d, *apart(k), *apart(v),
+                                *scales, _DT[dtype], bits)
+
+    @functools.cached_property
+    def _call(self):
+        """What a call needs of the cache: the struct, device, value type, heads, features."""
+        c = self.c
+        return (C.byref(c), self.k.get_device(), torch.bfloat16 if c.dtype == PDH_BF16 else torch.float16, c.heads,
+                c.features)
+
+
+def paged_cache(pages: int, heads: int, page_rows: int, features: int, dtype: torch.dtype = torch.bfloat16, *,
+                bits: int = 16, device: str | torch.device = "cuda") -> PagedCache:
+    """A zeroed :class:`PagedCache` of its own tensors."""
+    if bits not in (16, 4):
+        raise ValueError(f"paged_cache: 16 or 4 bits (got {bits})")
+    shape = (pages, heads, page_rows)
+    if bits == 16:
+        return PagedCache(torch.zeros(shape + (features,), dtype=dtype, device=device),
+                          torch.zeros(shape + (features,), dtype=dtype, device=device), dtype=dtype)
+    make = lambda n: torch.zeros(shape + (n,), dtype=torch.uint8, device=device)  # noqa: E731
+    return PagedCache(make(features // 2), make(features // 2), make(features // 32), make(features // 32), dtype)
+
+
+def rotary_table(positions: int, rotated: int, base: float = 10000.0, *,
+                 device: str | torch.device = "cuda") -> torch.Tensor:
+    """fp32 [positions, rotated]: the cosines, then the sines, of position p's
+    angles p base^(-2 i / rotated), i < rotated / 2, computed in 64 bits (an
+    fp32 angle is off by 2^-24 p radians)."""
+    i = torch.arange(0, rotated, 2, dtype=torch.float64, device=device)
+    angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * base ** (-i / rotated)
+    return torch.cat((angle.cos(), angle.sin()), 1).float()
+
+
+def _paged(name, cache, table, starts, lengths, rows, others):
+    """The checked batch of a call on a paged cache."""
+    dev = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -1
+    if cache._call[1] != dev or dev < 0:
+        _one_device(cache.k)
+    _one_device(table, starts, lengths, *others)
+    if table.dtype != torch.int32 or starts.dtype != torch.int32 or lengths.dtype != torch.int32:
+        raise ValueError(f"{name}: table, starts and lengths are int32")
+    seqs = lengths.shape[0] if lengths.dim() == 1 else -1
+    if seqs < 0 or starts.shape != (seqs + 1,) or table.dim() != 2 or table.shape[0] != seqs:
+        raise ValueError(f"{name}: table [sequences, pages], starts [sequences + 1], lengths [sequences] (got "
+                         f"{tuple(table.shape)}, {tuple(starts.shape)}, {tuple(lengths.shape)})")
+    width = table.shape[1]
+    if not (starts.is_contiguous() and lengths.is_contiguous()) or (width > 1 and table.stride(1) != 1):
+        raise ValueError(f"{name}: starts, lengths and the table's rows must be contiguous")
+    return _lib.PagedBatch(table.data_ptr(), starts.data_ptr(), lengths.data_ptr(), seqs, rows, width,
+                           table.stride(0) if seqs > 1 else width)
+
+
+def _tokens(name, nm, t, dtype, heads, features, rows=None):
+    """A [rows, heads, features] tensor's row and head strides, checked."""
+    if t.dtype != dtype or t.dim() != 3 or t.shape[2] != features or (heads is not None and t.shape[1] != heads) or (
+            rows is not None and t.shape[0] != rows):
+        raise ValueError(f"{name}: {nm} must be {dtype} [{'rows' if rows is None else rows}, "
+                         f"{'heads' if heads is None else heads}, {features}] (got {t.dtype} {tuple(t.shape)})")
+    st = t.stride()
+    if st[2] != 1:
+        raise ValueError(f"{name}: {nm}'s features must be contiguous")
+    return (st[0] if t.shape[0] > 1 else 0), (st[1] if t.shape[1] > 1 else 0)
+
+
+def _written(name, nm, t):
+    """An output that a call writes by rows of heads: no two of them may lie in one place."""
+    n, h, d = t.shape
+    sr, sh = t.stride(0), t.stride(1)
+    inner, outer = ((h, sh), (n, sr)) if sr >= sh or n <= 1 else ((n, sr), (h, sh))
+    if (inner[0] > 1 and inner[1] < d) or (outer[0] > 1 and outer[1] < (inner[0] - 1) * inner[1] + d):
+        raise ValueError(f"{name}: {nm}'s rows overlap")
+
+
+def paged_append(
+    k: torch.Tensor,
+    v: torch.Tensor,
+    cache: PagedCache,
+    table: torch.Tensor,
+    starts: torch.Tensor,
+    lengths: torch.Tensor,
+    *,
+    q: torch.Tensor | None = None,
+    rotary: torch.Tensor | None = None,
+    interleaved: bool = False,
+    out: torch.Tensor | None = None,
+    bad: torch.Tensor | None = None,
+) -> torch.Tensor | None:
+    """Store the new tokens' keys and values ``k`` / ``v`` [rows, heads,
+    features] in the cache, the keys rotated by their positions, and return
+    ``q`` [rows, query heads, features] rotated alike (None without q).
+
+    Sequence i's new tokens are rows starts[i] .. starts[i + 1] - 1 and the
+    last of its lengths[i] tokens (these counted), at the places that row i
+    of ``table`` [sequences, pages] names; ``starts`` ascend; all three are int32 on the
+    device, read when the kernel runs. ``rotary`` (:func:`rotary_table`, fp32
+    [positions, rotated], rotated a multiple of 16) turns features i and i +
+    rotated / 2, or 2 i and 2 i + 1 where ``interleaved``; the rest stay as
+    they are. fp32 arithmetic, rounded once to the cache's type or to its 4
+    bits (a group's scale is the least power of two of which it holds no
+    value over 7; each value goes to the nearest code, ties to the even one; a
+    group with an infinity or a NaN reads as NaN).
+
+    A token without a place (a position below 0, past the rotary table or the
+    page table, or a page outside the pool) is dropped, its row of the result
+    is zero, and it counts in ``bad`` (an int32 device scalar) when given.
+    Rows of no sequence are stored nowhere; their rows of the result are zero,
+    or stay as they are in ``out`` (which may be q itself). Two tokens with one
+    place leave either of them, or parts of both, there."""
+    cc, _, dtype, heads, d = cache._call
+    rows = k.shape[0] if k.dim() == 3 else 0
+    b = _paged("paged_append", cache, table, starts, lengths, rows, (k, v, q, rotary, out, bad))
+    ks = _tokens("paged_append", "k", k, dtype, heads, d)
+    vs = _tokens("paged_append", "v", v, dtype, heads, d, rows)
+    hq, qs, os = 0, (0, 0), (0, 0)
+    if q is not None:
+        qs = _tokens("paged_append", "q", q, dtype, None, d, rows)
+        hq = q.shape[1]
+        if hq < 1:
+            raise ValueError("paged_append: q has no heads")
+        zero = out is None
+        if zero:
+            out = q.new_empty(q.shape)
+        os = _tokens("paged_append", "out", out, dtype, hq, d, rows)
+        if not zero:
+            _written("paged_append", "out", out)
+            if out.data_ptr() == q.data_ptr() and os != qs:
+                raise ValueError("paged_append: out in q's place must have q's strides")
+    elif out is not None:
+        raise ValueError("paged_append: out is q's, and there is no q")
+    else:
+        zero = False
+    positions, rotated, ldr = 0, 0, 0
+    if rotary is not None:
+        if rotary.dtype != torch.float32 or rotary.dim() != 2 or rotary.stride(1) != 1:
+            raise ValueError("paged_append: rotary must be fp32 [positions, rotated] with contiguous rows")
+        positions, rotated = rotary.shape
+        ldr = rotary.stride(0) if positions > 1 else rotated
+    if bad is not None and (bad.dtype != torch.int32 or bad.numel() < 1):
+        raise ValueError("paged_append: bad is an int32 device scalar")
+    _lib.call("pdh_paged_append", k.data_ptr(), v.data_ptr(), _ptr(q), _ptr(out), hq, *ks, *vs, *qs, *os, cc, C.byref(b),
+              _ptr(rotary), positions, rotated, ldr, int(interleaved), int(zero), _ptr(bad), _stream())
+    return out
+
+
+def paged_rows(
+    cache: PagedCache,
+    table: torch.Tensor,
+    starts: torch.Tensor,
+    lengths: torch.Tensor,
+    rows: int,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """What the cache holds: keys and values [rows, heads, features], in its
+    16-bit type, of the tokens that :func:`paged_append` stores for the same
+    ``table``, ``starts`` and ``lengths`` (starts that ascend by the lengths:
+    everything). Tokens without a place and rows of no sequence are zero."""
+    cc, _, dtype, heads, d = cache._call
+    if rows < 0:
+        raise ValueError("paged_rows: rows must be >= 0")
+    b = _paged("paged_rows", cache, table, starts, lengths, int(rows), ())
+    k = torch.empty((rows, heads, d), dtype=dtype, device=cache.k.device)
+    v = torch.empty_like(k)
+    _lib.call("pdh_paged_rows", k.data_ptr(), v.data_ptr(), heads * d, d, heads * d, d, cc, C.byref(b), 1, _stream())
+    return k, v
+
+
+def paged_attention(
+    q: torch.Tensor,
+    cache: PagedCache,
+    table: torch.Tensor,
+    starts: torch.Tensor,
+    lengths: torch.Tensor,
+    *,
+    window: int | None = None,
+    sinks: int = 0,
+    scale: float | None = None,
+    want_lse: bool = True,
+    out: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """Causal attention of each sequence's last tokens over its cache: ``q``
+    [rows, query heads, features] (a multiple of the cache's heads: query head
+    h reads head h // (query heads / heads)), sequence i's rows starts[i] ..
+    starts[i + 1] - 1 at its last positions of lengths[i], as
+    :func:`paged_append` takes them. Row p sees token s <= p; with ``window``
+    only the last ``window`` of those (its own counted) and the first
+    ``sinks`` of the sequence. One token a sequence, a whole prompt, or both
+    in one call. Returns (o, lse): q's shape and type; fp32 [rows, query
+    heads], None without ``want_lse``.
+
+    What a row does not see has no part in it, whatever the cache holds there;
+    tokens on pages outside the pool or past the table are not seen. A row
+    that sees nothing (or only scores of -inf) has o = 0 and lse = -inf. Rows
+    of no sequence likewise; ``out`` (q's shape and type) they leave as it is.
+    The 4 bits are exact in the 16-bit type but for f16 under 2^-24."""
+    cc, _, dtype, heads, d = cache._call
+    b = _paged("paged_attention", cache, table, starts, lengths, q.shape[0] if q.dim() == 3 else 0, (q, out))
+    qs = _tokens("paged_attention", "q", q, dtype, None, d)
+    rows, hq = q.shape[:2]
+    if hq < 1 or hq % heads:
+        raise ValueError(f"paged_attention: query heads ({hq}) must be a multiple of the cache's heads ({heads})")
+    window = I64_MAX if window is None else int(window)
+    if window < 1 or sinks < 0:
+        raise ValueError(f"paged_attention: window >= 1 and sinks >= 0 (got {window}, {sinks})")
+    sc = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    zero = out is None
+    o = q.new_empty(q.shape) if zero else out
+    os = _tokens("paged_attention", "out", o, dtype, hq, d, rows)
+    if not zero:
+        _written("paged_attention", "out", o)
+    lse = q.new_empty((rows, hq), dtype=torch.float32) if want_lse else None
+    need = _lib.lib().pdh_paged_attention_workspace(cc, C.byref(b), hq, window, int(sinks))
+    ws = q.new_empty((need + 3) // 4, dtype=torch.float32) if need else None
+    _lib.call("pdh_paged_attention", q.data_ptr(), o.data_ptr(), _ptr(lse), hq, *qs, *os, cc, C.byref(b), window,
+              int(sinks), sc, int(zero), _ptr(ws), need, _stream())
+    return o, lse
+
+
 # ------------------------------------------------- elementwise programs
 
 
