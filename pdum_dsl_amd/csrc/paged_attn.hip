@@ -5,6 +5,7 @@
 //
 // Row kernel: a wave per (row, query head), keys 64 at a time, one a lane; the online softmax's maximum and sum are the
 // wave's, o's features lie across its lanes. It touches no key that the row does not see.
+#include "attn_common.h"
 #include "paged.h"
 
 #include <cmath>
@@ -106,6 +107,17 @@ __device__ void row_sweep(const PagedAttn& a, int seq, int hk, const uint16_t* q
   }
 }
 
+// A finished row: o's features lane + 64 j, m in units of log2.
+template <typename T, int D>
+__device__ __forceinline__ void write_row(const PagedAttn& a, int row, int h, float m, float l, const float (&o)[D / 64]) {
+  const int lane = threadIdx.x & 63;
+  const float inv = l == 0.f ? 0.f : 1.0f / l;  // nothing seen, or scores of -inf alone
+  uint16_t* out = a.o + row * a.o_st + h * a.o_sh;
+#pragma unroll
+  for (int j = 0; j < D / 64; ++j) out[lane + 64 * j] = Elem<T>::from_f32(o[j] * inv);
+  if (lane == 0 && a.lse) a.lse[static_cast<int64_t>(row) * a.heads_q + h] = l == 0.f ? -kInf : (m + __log2f(l)) * kLn2;
+}
+
 template <typename T, int D, int BITS>
 __global__ __launch_bounds__(256) void paged_attn_rows(PagedAttn a) {
   const int lane = threadIdx.x & 63;
@@ -124,11 +136,466 @@ __global__ __launch_bounds__(256) void paged_attn_rows(PagedAttn a) {
   if (owned)
     row_sweep<T, D, BITS>(a, seq, h / a.group, a.q + row * a.q_st + h * a.q_sh, s.len - s.n + (row - s.row0), 0,
                           kMaxTokens, m, l, o);
-  const float inv = l == 0.f ? 0.f : 1.0f / l;
-  uint16_t* out = a.o + row * a.o_st + h * a.o_sh;
+  write_row<T, D>(a, row, h, m, l, o);
+}
+
+// ------------------------------------------------------------------ few rows a sequence
+//
+// Decode: the work is reading the caches once. A sequence's rows times the group of query heads that share a key/value head,
+// flattened (row * group + head), are cut into blocks of 16, the columns of v_mfma_f32_16x16x32: every cached byte that a
+// block reads serves all of them. Keys go by blocks of 32 on the absolute grid, so that a block lies in at most two pages,
+// whose numbers are wave-uniform scalars, fetched two blocks ahead.
+//
+// Shares. Sequences differ in length, and the lengths are device memory. Every workgroup sums up all sequences' work (blocks of
+// keys x blocks of rows x heads), takes the same share of the line they form, and sweeps what lies in it: a part of one
+// (sequence, head, row block), several whole ones, a part of another. A whole one is written out at once; of a cut one each
+// workgroup leaves its state (m, l, o) and paged_decode_merge, one workgroup for each, joins them.
+//
+// A block of keys (S^T = K Q^T, O^T += V^T P^T as in decode.hip): K straight from its loads as the A operand, V through a
+// tile of the wave's own in LDS, read back transposed. The next block's loads are in flight while one is computed. A 4-bit row
+// is loaded as codes: a lane takes features D/4 g .. + D/4 of its row (one load, one scale), which k-step s contracts by
+// eights, and q is laid out to match; V is widened to 16 bits on its way into LDS.
+
+// Workgroups a compute unit holds at once: by registers (16 bits), by LDS (4).
+template <int BITS>
+constexpr int kDecWgs = BITS == 16 ? 2 : 4;
+
+template <int D, int BITS>
+struct DecCfg {
+  static constexpr int KS = D / 32;        // k-steps of the score product
+  static constexpr int ET = D / 16;        // 16-feature tiles of the output product
+  static constexpr int CPR = D / 8;        // 16-byte chunks a 16-bit row
+  static constexpr int RPI = 64 / CPR;     // rows a 16-bit value load
+  static constexpr int VL = 32 / RPI;      // 16-bit value loads a block
+  static constexpr int VROW = D * 2 + 32;  // LDS bytes a value row (32 of padding: conflict-free transposed reads)
+  static constexpr int VTILE = 32 * VROW;
+  static constexpr int RS = 2 + D;  // floats of a row's state: m, l, o
+  static constexpr int RED = 4 * 16 * RS * 4;
+  static constexpr int LDS = 4 * VTILE > RED ? 4 * VTILE : RED;
+  // an item of fewer blocks of keys is not cut: a workgroup's four waves take a block each
+  static constexpr int LEAST = 4;
+};
+
+// One block of 32 keys in flight.
+template <int D, int BITS>
+struct DecBlk;
+template <int D>
+struct DecBlk<D, 16> {
+  u32x4 k[2 * D / 32], v[32 / (64 / (D / 8))];
+};
+template <int D>
+struct DecBlk<D, 4> {
+  typedef uint32_t codes __attribute__((ext_vector_type(D / 32)));
+  codes k[2], v[2];
+  uint32_t ks[2], vs[2];  // scale bytes
+};
+
+// Device memory that no kernel in flight writes, read through the scalar cache where the address is uniform.
+__device__ __forceinline__ int32_t uniform_i32(const int32_t* p) {
+  typedef const __attribute__((address_space(4))) int32_t c_i32;
+  return *(c_i32*)(p);
+}
+
+// A sequence's work: blocks of rows and of keys. Visible keys lie in blocks [0, sb) (the first tokens) and [wb, eb).
+struct SeqPlan {
+  int row0, n, pos0;  // first row, rows, the first row's position
+  int nb, sb, wb, blocks;
+  __device__ __forceinline__ int key_block(int v) const { return v < sb ? v : v - sb + wb; }
+};
+
+template <int ROWS, int KEYS>
+__device__ __forceinline__ SeqPlan plan_of(const PagedAttn& a, int i) {
+  Seq s{0, 0, 0};
+  if (i < a.b.seqs) {
+    s = seq_at(a.b, i);
+  } else if (a.zero_rest) {  // the rows behind the last sequence: no keys
+    const int r0 = a.b.seqs ? clamp_row(a.b.starts[i], static_cast<int>(a.b.rows)) : 0;
+    s = Seq{r0, static_cast<int>(a.b.rows) - r0, 0};
+  }
+  SeqPlan p;
+  p.row0 = s.row0;
+  p.n = s.n;
+  p.pos0 = s.len - s.n;
+  const int end = s.len < a.reach ? s.len : a.reach;
+  const int eb = (end + KEYS - 1) / KEYS;
+  const int lo = p.pos0 - a.window + 1;
+  p.wb = lo > 0 ? lo / KEYS : 0;
+  p.wb = p.wb < eb ? p.wb : eb;
+  const int sink = a.sinks < end ? a.sinks : end;
+  p.sb = (sink + KEYS - 1) / KEYS;
+  p.sb = p.sb < p.wb ? p.sb : p.wb;
+  p.blocks = p.sb + eb - p.wb;
+  p.blocks = p.blocks > 0 ? p.blocks : 1;  // one that sees nothing
+  p.nb = static_cast<int>((static_cast<int64_t>(s.n) * a.group + ROWS - 1) / ROWS);
+  return p;
+}
+
+struct DecMeta {
+  int last, seq, rb, head;  // the last workgroup of the item that starts in this one's share and ends in another's; -1: none
+};
+
+template <typename T, int D, int BITS>
+__global__ __launch_bounds__(256, kDecWgs<BITS>) void paged_decode(PagedAttn a, DecMeta* meta, float* ws) {
+  using C = DecCfg<D, BITS>;
+  constexpr int KS = C::KS, ET = C::ET, RS = C::RS;
+  __shared__ __attribute__((aligned(1024))) unsigned char dsm[C::LDS];
+  __shared__ int64_t scan[8];
+  const int tid = threadIdx.x, lane = tid & 63, w = wave_id();
+  const int col = lane & 15, g = lane >> 4;
+  const int hkv = static_cast<int>(a.c.heads), R = a.group;
+
+  // ---- this workgroup's share [at, end) of the line of (sequence, head, row block, key block)
+  const int nseq = static_cast<int>(a.b.seqs) + 1;
+  const int each = (nseq + 255) / 256;
+  int64_t mine = 0;
+  for (int j = 0; j < each; ++j) {
+    const int i = tid * each + j;
+    if (i < nseq) {
+      const SeqPlan p = plan_of<16, 32>(a, i);
+      mine += static_cast<int64_t>(p.nb) * p.blocks * hkv;
+    }
+  }
+  int64_t incl = mine;
 #pragma unroll
-  for (int j = 0; j < D / 64; ++j) out[lane + 64 * j] = Elem<T>::from_f32(o[j] * inv);
-  if (lane == 0 && a.lse) a.lse[static_cast<int64_t>(row) * a.heads_q + h] = l == 0.f ? -kInf : (m + __log2f(l)) * kLn2;
+  for (int off = 1; off < 64; off <<= 1) {
+    const int64_t o = (static_cast<int64_t>(__shfl_up(static_cast<int>(incl >> 32), off, kWave)) << 32) |
+                      static_cast<uint32_t>(__shfl_up(static_cast<int>(incl), off, kWave));
+    incl += lane >= off ? o : 0;
+  }
+  if (lane == 63) scan[w] = incl;
+  __syncthreads();
+  int64_t total = 0, before = incl - mine;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    before += i < w ? scan[i] : 0;
+    total += scan[i];
+  }
+  int64_t per = (total + gridDim.x - 1) / gridDim.x;
+  per = (per + C::LEAST - 1) / C::LEAST * C::LEAST;
+  int64_t at = per * blockIdx.x;
+  int64_t left = total - at < per ? total - at : per;
+  if (left <= 0) {
+    if (tid == 0) meta[blockIdx.x] = DecMeta{-1, 0, 0, 0};
+    return;
+  }
+  __syncthreads();
+  if (before <= at && at < before + mine) {
+    scan[0] = tid * each;
+    scan[1] = at - before;
+  }
+  __syncthreads();
+  int seq = __builtin_amdgcn_readfirstlane(static_cast<int>(scan[0]));
+  int64_t in_seq = scan[1];
+  SeqPlan sp;
+  for (;; ++seq) {
+    sp = plan_of<16, 32>(a, seq);
+    const int64_t cost = static_cast<int64_t>(sp.nb) * sp.blocks * hkv;
+    if (in_seq < cost) break;
+    in_seq -= cost;
+  }
+  int item = __builtin_amdgcn_readfirstlane(static_cast<int>(in_seq / sp.blocks));  // heads x row blocks < 2^31 (host)
+  int kb = __builtin_amdgcn_readfirstlane(static_cast<int>(in_seq % sp.blocks));
+  DecMeta cut{-1, 0, 0, 0};
+
+  unsigned char* vt = dsm + w * C::VTILE;
+  // transposed value reads: lane 4k + c of group g addresses row 4 g + k, features 4 c .. +3 (+ 16 t)
+  const int trb = (4 * g + (col >> 2)) * C::VROW + (col & 3) * 8;
+  constexpr int ES = BITS == 16 ? 2 : 1;  // bytes of a stride's unit
+  const uint32_t kst = static_cast<uint32_t>(a.c.k_sr) * ES, vst = static_cast<uint32_t>(a.c.v_sr) * ES;
+  const int vrow = BITS == 16 ? lane / C::CPR : lane / 4, vch = BITS == 16 ? lane % C::CPR : lane % 4;
+
+  while (left > 0) {
+    const int rb = item % sp.nb, head = item / sp.nb;
+    const int todo = static_cast<int>(sp.blocks - kb < left ? sp.blocks - kb : left);
+    const int k_end = kb + todo;
+
+    // ---- the block's rows: column c is flattened row 16 rb + c
+    const int nq = sp.n * static_cast<int64_t>(R) - 16 * static_cast<int64_t>(rb) < 16
+                       ? static_cast<int>(sp.n * static_cast<int64_t>(R) - 16 * static_cast<int64_t>(rb))
+                       : 16;
+    const int f0 = rb * 16, fc = f0 + (col < nq ? col : 0);
+    const int pos = sp.pos0 + fc / R;
+    const int pos_lo = sp.pos0 + f0 / R, pos_hi = sp.pos0 + (f0 + nq - 1) / R;
+    u32x4 qb[KS];
+    {
+      const uint16_t* qr = a.q + (sp.row0 + fc / R) * a.q_st + (head * R + fc % R) * a.q_sh;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const u32x4 v = *reinterpret_cast<const u32x4*>(qr + (BITS == 16 ? s * 32 + g * 8 : g * (D / 4) + s * 8));
+        qb[s] = col < nq ? v : u32x4{0u, 0u, 0u, 0u};
+      }
+    }
+
+    struct Pages {
+      int p[2];  // of the two halves of a block; -1: none
+    };
+    auto pages = [&](int v) {
+      Pages r;
+      const int key0 = sp.key_block(v) * 32;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int e = (key0 + 16 * h) >> a.shift;
+        const int p = e < a.b.width ? uniform_i32(a.b.table + seq * a.b.ld_table + e) : -1;
+        r.p[h] = static_cast<uint32_t>(p) < static_cast<uint64_t>(a.c.pages) ? p : -1;
+      }
+      return r;
+    };
+    // A half without a page reads page 0: what it holds is masked.
+    auto load = [&](int v, const Pages& pg, DecBlk<D, BITS>& r) {
+      const int key0 = sp.key_block(v) * 32;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int64_t p = pg.p[h] < 0 ? 0 : pg.p[h];
+        const int in = (key0 + 16 * h) & ((1 << a.shift) - 1);
+        const char* kp = static_cast<const char*>(a.c.k) + (p * a.c.k_sp + head * a.c.k_sh + in * a.c.k_sr) * ES;
+        const char* vp = static_cast<const char*>(a.c.v) + (p * a.c.v_sp + head * a.c.v_sh + in * a.c.v_sr) * ES;
+        if constexpr (BITS == 16) {
+#pragma unroll
+          for (int s = 0; s < KS; ++s) r.k[h * KS + s] = gload<u32x4>(kp, col * kst + g * 16 + s * 64);
+#pragma unroll
+          for (int j = 0; j < C::VL / 2; ++j)
+            r.v[h * (C::VL / 2) + j] = gload<u32x4>(vp, (j * C::RPI + vrow) * vst + vch * 16);
+        } else {
+          typedef typename DecBlk<D, 4>::codes codes;
+          const char* ksp = static_cast<const char*>(a.c.k_scale) + p * a.c.ks_sp + head * a.c.ks_sh + in * a.c.ks_sr;
+          const char* vsp = static_cast<const char*>(a.c.v_scale) + p * a.c.vs_sp + head * a.c.vs_sh + in * a.c.vs_sr;
+          r.k[h] = gload<codes>(kp, col * kst + g * (D / 8));
+          r.ks[h] = gload<uint8_t>(ksp, col * static_cast<uint32_t>(a.c.ks_sr) + g * (D / 4) / 32);
+          r.v[h] = gload<codes>(vp, vrow * vst + vch * (D / 8));
+          r.vs[h] = gload<uint8_t>(vsp, vrow * static_cast<uint32_t>(a.c.vs_sr) + vch * (D / 4) / 32);
+        }
+      }
+    };
+
+    float m = -kInf, lsum = 0.f;
+    f32x4 o[ET];
+#pragma unroll
+    for (int t = 0; t < ET; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    auto block = [&](int v, const Pages& pg, const DecBlk<D, BITS>& r) {
+      const int key0 = sp.key_block(v) * 32;
+      // every key is seen by every row
+      const bool full = key0 + 31 <= pos_lo && key0 + 32 <= a.reach &&
+                        (key0 > pos_hi - a.window || key0 + 31 < a.sinks) && (pg.p[0] | pg.p[1]) >= 0;
+      // keys that no row sees: their values count as zero
+      auto gone = [&](int at, int p) {
+        const int key = key0 + at;
+        return p < 0 || key > pos_hi || key >= a.reach || (key >= a.sinks && key <= pos_lo - a.window);
+      };
+      // values -> this wave's tile, rows of keys
+      if constexpr (BITS == 16) {
+#pragma unroll
+        for (int j = 0; j < C::VL; ++j) {
+          u32x4 x = r.v[j];
+          const int at = j * C::RPI + vrow;
+          if (!full && gone(at, pg.p[j / (C::VL / 2)])) x = u32x4{0u, 0u, 0u, 0u};
+          *reinterpret_cast<u32x4*>(vt + at * C::VROW + vch * 16) = x;
+        }
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int at = 16 * h + vrow;
+          const bool dead = !full && gone(at, pg.p[h]);
+          const float sc = dead ? 0.f : e8m0(r.vs[h]);
+#pragma unroll
+          for (int i = 0; i < KS; ++i)
+            *reinterpret_cast<u32x4*>(vt + at * C::VROW + vch * (D / 2) + i * 16) = fp4_row8<T>(dead ? 0u : r.v[h][i], sc);
+        }
+      }
+      // S^T: keys key0 + 16 h + 4 g + i (accumulator i), row col
+      f32x4 sc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          u32x4 kk;
+          if constexpr (BITS == 16)
+            kk = r.k[h * KS + s];
+          else
+            kk = fp4_row8<T>(r.k[h][s], e8m0(r.ks[h]));
+          sc[h] = mfma16<T>(kk, qb[s], sc[h]);
+        }
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = sc[i >> 2][i & 3] * a.c2;
+      if (!full) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int key = key0 + 16 * (i >> 2) + 4 * g + (i & 3);
+          const bool seen = key <= pos && key < a.reach && (key > pos - a.window || key < a.sinks) && pg.p[i >> 2] >= 0;
+          x[i] = seen ? x[i] : -kInf;
+        }
+      }
+      float mx = x[0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[i]);
+      mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
+      const float mnew = fmaxf(m, mx);
+      const float ref = mnew == -kInf ? 0.f : mnew;  // scores of -inf alone weigh 0, not NaN
+      if (__builtin_amdgcn_ballot_w64(mnew > m) != 0) {  // some row's maximum grew: rare after the first blocks
+        const float alpha = fast_exp2(m - ref);
+        lsum *= alpha;
+#pragma unroll
+        for (int t = 0; t < ET; ++t) o[t] *= alpha;
+        m = mnew;
+      }
+      float p[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        p[i] = fast_exp2(x[i] - ref);
+        lsum += p[i];
+      }
+      const u32x4 pb = {pack2<T>(p[0], p[1]), pack2<T>(p[2], p[3]), pack2<T>(p[4], p[5]), pack2<T>(p[6], p[7])};
+#pragma unroll
+      for (int t = 0; t < ET; ++t) {
+        const u32x2 lo = ds_read_tr16(vt + trb + 32 * t);
+        const u32x2 hi = ds_read_tr16(vt + trb + 16 * C::VROW + 32 * t);
+        o[t] = mfma16<T>(u32x4{lo.x, lo.y, hi.x, hi.y}, pb, o[t]);
+      }
+    };
+
+    // Each wave takes every fourth block. Past its last one the loads in flight re-read that block (an L2 hit): they are
+    // issued whatever comes, so that the compiler's wait counts stay exact.
+    if (kb + w < k_end) {
+      const int v_last = kb + w + (k_end - 1 - kb - w) / 4 * 4;
+      auto bound = [&](int v) { return v < v_last ? v : v_last; };
+      DecBlk<D, BITS> r0, r1;
+      int v = kb + w;
+      Pages p0 = pages(v), p1 = pages(bound(v + 4));
+      load(v, p0, r0);
+      for (;;) {
+        load(bound(v + 4), p1, r1);
+        Pages p2 = pages(bound(v + 8));
+        block(v, p0, r0);
+        v += 4;
+        if (v >= k_end) break;
+        load(bound(v + 4), p2, r0);
+        p0 = pages(bound(v + 8));
+        block(v, p1, r1);
+        p1 = p0;
+        p0 = p2;
+        v += 4;
+        if (v >= k_end) break;
+      }
+    }
+    lsum += __shfl_xor(lsum, 16, kWave);
+    lsum += __shfl_xor(lsum, 32, kWave);
+
+    // ---- the four waves' states meet in LDS, over the value tiles
+    __syncthreads();
+    float* red = reinterpret_cast<float*>(dsm);
+    if (col < nq) {
+      float* rec = red + (w * 16 + col) * RS;
+      if (g == 0) {
+        rec[0] = m;
+        rec[1] = lsum;
+      }
+#pragma unroll
+      for (int t = 0; t < ET; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) rec[2 + 16 * t + 4 * g + i] = o[t][i];
+    }
+    __syncthreads();
+    const bool whole = todo == sp.blocks;
+    float* rec = ws + (static_cast<int64_t>(blockIdx.x) * 2 + (kb == 0 ? 1 : 0)) * 16 * RS;
+    for (int c = w; c < nq; c += 4) {
+      float mw[4], mm = -kInf, l = 0.f, acc[D / 64] = {};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        mw[i] = red[(i * 16 + c) * RS];
+        mm = fmaxf(mm, mw[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float* p = red + (i * 16 + c) * RS;
+        const float f = mw[i] == -kInf ? 0.f : fast_exp2(mw[i] - mm);
+        l += f * p[1];
+#pragma unroll
+        for (int j = 0; j < D / 64; ++j) acc[j] += f * p[2 + lane + 64 * j];
+      }
+      const int f = f0 + c, tok = f / R, hq = head * R + f % R;
+      if (pos_lo != pos_hi) {
+        // Rows at different positions share blocks of keys: 0 times a value that only some of them see is NaN where it is
+        // an infinity or a NaN. Such a row is done again, by itself.
+        bool nan = l != l;
+#pragma unroll
+        for (int j = 0; j < D / 64; ++j) nan |= acc[j] != acc[j];
+        if (__builtin_amdgcn_ballot_w64(nan) != 0) {
+          mm = -kInf;
+          l = 0.f;
+#pragma unroll
+          for (int j = 0; j < D / 64; ++j) acc[j] = 0.f;
+          const uint16_t* qr = a.q + (sp.row0 + tok) * a.q_st + hq * a.q_sh;
+          const int s1 = (k_end < sp.sb ? k_end : sp.sb) * 32;
+          if (kb < sp.sb) row_sweep<T, D, BITS>(a, seq, head, qr, sp.pos0 + tok, kb * 32, s1, mm, l, acc);
+          if (k_end > sp.sb)
+            row_sweep<T, D, BITS>(a, seq, head, qr, sp.pos0 + tok, sp.key_block(kb > sp.sb ? kb : sp.sb) * 32,
+                                  sp.key_block(k_end - 1) * 32 + 32, mm, l, acc);
+        }
+      }
+      if (whole) {
+        write_row<T, D>(a, sp.row0 + tok, hq, mm, l, acc);
+      } else {
+        if (lane == 0) {
+          rec[c * RS] = mm;
+          rec[c * RS + 1] = l;
+        }
+#pragma unroll
+        for (int j = 0; j < D / 64; ++j) rec[c * RS + 2 + lane + 64 * j] = acc[j];
+      }
+    }
+    if (kb == 0 && !whole)
+      cut = DecMeta{static_cast<int>((at + sp.blocks - 1) / per), seq, rb, head};
+    __syncthreads();  // before the next item's tiles
+
+    left -= todo;
+    at += todo;
+    kb += todo;
+    if (kb == sp.blocks && left > 0) {
+      kb = 0;
+      ++item;
+      if (item == sp.nb * hkv) {
+        item = 0;
+        do sp = plan_of<16, 32>(a, ++seq);
+        while (sp.n == 0);
+      }
+    }
+  }
+  if (tid == 0) meta[blockIdx.x] = cut;
+}
+
+// Joins a cut item's states: the workgroup that the item starts in left the first in its second record, the others up to
+// `last` theirs in their first. A wave takes every fourth row; lanes hold features.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void paged_decode_merge(PagedAttn a, const DecMeta* meta, const float* ws) {
+  constexpr int RS = 2 + D;
+  const DecMeta c = meta[blockIdx.x];
+  if (c.last < 0) return;
+  const int lane = threadIdx.x & 63;
+  const SeqPlan sp = plan_of<16, 32>(a, c.seq);
+  const int64_t rows = sp.n * static_cast<int64_t>(a.group) - 16 * static_cast<int64_t>(c.rb);
+  const int nq = rows < 16 ? static_cast<int>(rows) : 16;
+  const int nrec = c.last - static_cast<int>(blockIdx.x) + 1;
+  for (int i = wave_id(); i < nq; i += 4) {
+    auto rec = [&](int r) {
+      return ws + ((static_cast<int64_t>(blockIdx.x) + r) * 2 + (r == 0)) * 16 * RS + i * RS;
+    };
+    float mm = -kInf;
+    for (int r = lane; r < nrec; r += 64) mm = fmaxf(mm, rec(r)[0]);
+    mm = wave_max(mm);
+    float l = 0.f, acc[D / 64] = {};
+#pragma unroll 4
+    for (int r = 0; r < nrec; ++r) {
+      const float* p = rec(r);
+      const float f = p[0] == -kInf ? 0.f : fast_exp2(p[0] - mm);
+      l += f * p[1];
+#pragma unroll
+      for (int j = 0; j < D / 64; ++j) acc[j] += f * p[2 + lane + 64 * j];
+    }
+    const int f = c.rb * 16 + i;
+    write_row<T, D>(a, sp.row0 + f / a.group, c.head * a.group + f % a.group, mm, l, acc);
+  }
 }
 
 }  // namespace
@@ -136,9 +603,25 @@ __global__ __launch_bounds__(256) void paged_attn_rows(PagedAttn a) {
 
 using namespace pdh;
 
+namespace {
+
+// Rows a sequence and head that take the decode kernel: blocks of 16 flattened rows on average.
+bool few_rows(const pdh_paged_batch& b, int64_t group) { return b.rows * group <= 16 * b.seqs; }
+
+// Workgroups of the decode kernel: as many as run at once.
+int decode_grid(const pdh_paged_cache& c) {
+  const int cus = pdh_device_cus();
+  return (cus > 0 ? cus : 256) * (c.bits == 16 ? kDecWgs<16> : kDecWgs<4>);
+}
+
+}  // namespace
+
 extern "C" size_t pdh_paged_attention_workspace(const pdh_paged_cache* cache, const pdh_paged_batch* batch,
                                                 int64_t heads_q, int64_t window, int64_t sinks) {
-  (void)cache, (void)batch, (void)heads_q, (void)window, (void)sinks;
+  (void)window, (void)sinks;
+  if (!cache || !batch || cache->heads < 1 || heads_q < cache->heads) return 0;
+  if (few_rows(*batch, heads_q / cache->heads))
+    return static_cast<size_t>(decode_grid(*cache)) * (sizeof(DecMeta) + 2 * 16 * (2 + cache->features) * sizeof(float));
   return 0;
 }
 
@@ -146,12 +629,12 @@ extern "C" int pdh_paged_attention(const void* q, void* o, float* lse, int64_t h
                                    int64_t o_st, int64_t o_sh, const pdh_paged_cache* cache,
                                    const pdh_paged_batch* batch, int64_t window, int64_t sinks, float scale,
                                    int zero_rest, void* ws, size_t ws_bytes, void* stream) {
-  (void)ws, (void)ws_bytes;
   int shift = 0;
   const int rc = check_paged("pdh_paged_attention", cache, batch, &shift);
   if (rc) return rc;
   PDH_REQUIRE(heads_q >= 1 && heads_q <= 65535 && heads_q % cache->heads == 0, PDH_EINVAL,
               "pdh_paged_attention: heads_q must be a multiple of the cache's heads");
+  PDH_REQUIRE(batch->rows * heads_q <= INT32_MAX, PDH_EINVAL, "pdh_paged_attention: rows * heads_q must be < 2^31");
   PDH_REQUIRE(window >= 1 && sinks >= 0, PDH_EINVAL, "pdh_paged_attention: window >= 1 and sinks >= 0");
   PDH_REQUIRE(std::isfinite(scale) && scale > 0.f, PDH_EINVAL, "pdh_paged_attention: scale must be finite and > 0");
   if (batch->rows == 0) return PDH_OK;
@@ -164,6 +647,21 @@ extern "C" int pdh_paged_attention(const void* q, void* o, float* lse, int64_t h
               static_cast<int>(window < kMaxTokens ? window : kMaxTokens),
               static_cast<int>(sinks < kMaxTokens ? sinks : kMaxTokens), shift, zero_rest != 0,
               static_cast<int>(batch->width << shift), scale * kLog2e};
+  const size_t need = pdh_paged_attention_workspace(cache, batch, heads_q, window, sinks);
+  PDH_REQUIRE(ws_bytes >= need && (need == 0 || (ws && aligned16(ws))), PDH_EINVAL,
+              "pdh_paged_attention: workspace %zu bytes < required %zu, or not 16-byte aligned", ws_bytes, need);
+  if (few_rows(*batch, a.group)) {
+    const unsigned n = static_cast<unsigned>(decode_grid(*cache));
+    DecMeta* meta = static_cast<DecMeta*>(ws);
+    float* states = reinterpret_cast<float*>(meta + n);
+    by_kind(*cache, [&](auto t, auto d, auto bits) {
+      using T = decltype(t);
+      constexpr int D = decltype(d)::value;
+      paged_decode<T, D, decltype(bits)::value><<<n, 256, 0, as_stream(stream)>>>(a, meta, states);
+      paged_decode_merge<T, D><<<n, 256, 0, as_stream(stream)>>>(a, meta, states);
+    });
+    return check_launch("pdh_paged_attention (decode)");
+  }
   const dim3 grid(static_cast<unsigned>(batch->rows), static_cast<unsigned>((heads_q + 3) / 4));
   by_kind(*cache, [&](auto t, auto d, auto bits) {
     paged_attn_rows<decltype(t), decltype(d)::value, decltype(bits)::value><<<grid, 256, 0, as_stream(stream)>>>(a);
