@@ -3,8 +3,9 @@
 //   x(p, s) = scale q_p . k_s over the visible s: s <= p and (s < sinks or s > p - window)
 //   o = sum_s softmax(x) v_s, lse = log sum_s exp x;  a row with no visible key: o = 0, lse = -inf
 //
-// Row kernel: a wave per (row, query head), keys 64 at a time, one a lane; the online softmax's maximum and sum are the
-// wave's, o's features lie across its lanes. It touches no key that the row does not see.
+// Two kernels, by the mean number of rows of a sequence times the group of query heads on a key/value head: to 16 of them
+// the decode kernel (bytes bound it), above the prompt kernel (matrix products do). Both take any batch; a lone long prompt
+// among single tokens is merely slower in the one, a lone token in the other.
 #include "attn_common.h"
 #include "paged.h"
 
@@ -28,7 +29,9 @@ struct PagedAttn {
   float c2;   // scale * log2(e)
 };
 
-// One row's softmax state over the visible keys of [k0, k1): m in units of log2, o unnormalised, features lane + 64 j.
+// One row by one wave: keys 64 at a time, one a lane; the online softmax's maximum and sum are the wave's, o's features lie
+// across its lanes. It touches no key that the row does not see, which makes it the way out for rows that share blocks of keys
+// with values that are not finite and not theirs. The row's softmax state over the visible keys of [k0, k1): m in units of log2, o unnormalised, features lane + 64 j.
 template <typename T, int D, int BITS>
 __device__ void row_sweep(const PagedAttn& a, int seq, int hk, const uint16_t* q, int pos, int k0, int k1, float& m,
                           float& l, float (&o)[D / 64]) {
@@ -116,27 +119,6 @@ __device__ __forceinline__ void write_row(const PagedAttn& a, int row, int h, fl
 #pragma unroll
   for (int j = 0; j < D / 64; ++j) out[lane + 64 * j] = Elem<T>::from_f32(o[j] * inv);
   if (lane == 0 && a.lse) a.lse[static_cast<int64_t>(row) * a.heads_q + h] = l == 0.f ? -kInf : (m + __log2f(l)) * kLn2;
-}
-
-template <typename T, int D, int BITS>
-__global__ __launch_bounds__(256) void paged_attn_rows(PagedAttn a) {
-  const int lane = threadIdx.x & 63;
-  const int row = blockIdx.x;
-  const int h = blockIdx.y * 4 + wave_id();
-  if (h >= a.heads_q) return;
-  const int seq = seq_of_row(a.b, row);
-  Seq s{0, 0, 0};
-  bool owned = false;
-  if (seq < a.b.seqs) {
-    s = seq_at(a.b, seq);
-    owned = row >= s.row0 && row < s.row0 + s.n;
-  }
-  if (!owned && !a.zero_rest) return;
-  float m = -kInf, l = 0.f, o[D / 64] = {};
-  if (owned)
-    row_sweep<T, D, BITS>(a, seq, h / a.group, a.q + row * a.q_st + h * a.q_sh, s.len - s.n + (row - s.row0), 0,
-                          kMaxTokens, m, l, o);
-  write_row<T, D>(a, row, h, m, l, o);
 }
 
 // ------------------------------------------------------------------ few rows a sequence
@@ -598,6 +580,480 @@ __global__ __launch_bounds__(256) void paged_decode_merge(PagedAttn a, const Dec
   }
 }
 
+// ------------------------------------------------------------------ many rows a sequence
+//
+// Prompts: matrix products bound the work. Blocks of 128 flattened rows (row * group + head), 32 a wave, sweep tiles of 32
+// keys that the workgroup stages in LDS, double-buffered; the products, the swizzled tiles, the softmax with a maximum that
+// moves only when it must and the lazily read operands are the forward kernel's of flash_fwd.hip. The rows of a group lie
+// side by side, so that a block spans few positions: at a group of 4, 32 of them, and one tile in 32 keys is cut by the diagonal.
+//
+// A tile's two halves of 16 keys lie in one page each. 16 bits: direct loads into LDS through a buffer resource per half,
+// built from the half's page; keys that no row of the block sees are given an offset past the resource and read as zero.
+// 4 bits: half of the threads fetch K's codes and scales, half V's, one load each, a tile ahead in registers, and widen them
+// into the same LDS rows when the tile before is done with.
+//
+// Workgroups: a sequence's blocks come in slots starts * group / 128 + sequence onward (rounded down), which never overlap,
+// so that the grid is known without the starts; a workgroup counts the sequences at or before its slot. Late blocks, which
+// see the most keys, go first, in runs of four of alternating direction (the four shader engines of an XCD draw alike); an
+// XCD works through whole heads, whose keys its L2 holds. A grid too small for the chip cuts each block's tiles into parts
+// that paged_prompt_merge joins.
+
+template <int D>
+struct ProCfg {
+  static constexpr int BM = 128, BN = 32;
+  static constexpr int ROWB = D * 2;
+  static constexpr int CPR = D / 8;
+  static constexpr int TILEB = BN * ROWB;
+  static constexpr int KBUF = 0, VBUF = 2 * TILEB;
+  static constexpr int LDS = 4 * TILEB;
+  static constexpr int RPK = 1024 / ROWB;    // rows of a 1 KB direct load
+  static constexpr int NDMA = BN / RPK / 4;  // loads of K, and of V, a wave and tile
+  static constexpr int KS = D / 32;
+  static constexpr int FB = D / 16;
+  static constexpr int PF = 2;   // V operands in flight ahead of their product
+  static constexpr int KPF = 3;  // K operands in flight
+};
+
+constexpr float kTau = 8.0f;    // log2 of the growth of a row's maximum that is let pass
+constexpr int kPartTiles = 8;   // no part of a block's keys is shorter, but the last
+
+// A block's keys: tiles [0, sb) (the first tokens) and [wb, eb), cut into parts of `part` tiles.
+struct BlockKeys {
+  int sb, wb, tiles, part, parts;
+  __device__ __forceinline__ int tile(int v) const { return v < sb ? v : v - sb + wb; }
+};
+
+__device__ __forceinline__ BlockKeys block_keys(const PagedAttn& a, int pos_lo, int pos_hi, int nsplit) {
+  BlockKeys b;
+  const int end = pos_hi + 1 < a.reach ? pos_hi + 1 : a.reach;
+  const int eb = end > 0 ? (end + 31) / 32 : 0;
+  const int lo = pos_lo - a.window + 1;
+  b.wb = lo > 0 ? lo / 32 : 0;
+  b.wb = b.wb < eb ? b.wb : eb;
+  const int sink = a.sinks < end ? a.sinks : end;
+  b.sb = sink > 0 ? (sink + 31) / 32 : 0;
+  b.sb = b.sb < b.wb ? b.sb : b.wb;
+  b.tiles = b.sb + eb - b.wb;
+  b.part = (b.tiles + nsplit - 1) / nsplit;
+  b.part = b.part > kPartTiles ? b.part : kPartTiles;
+  b.parts = b.tiles > b.part ? (b.tiles + b.part - 1) / b.part : 1;
+  return b;
+}
+
+// The sequence of a slot (seqs: the rows behind the last one; -1: none) and the block's number in it.
+__device__ __forceinline__ int seq_of_slot(const PagedAttn& a, int slot, int& rb) {
+  const int lane = threadIdx.x & 63, rows = static_cast<int>(a.b.rows);
+  auto base = [&](int64_t i) {
+    const int r = a.b.seqs ? clamp_row(a.b.starts[i], rows) : 0;
+    return static_cast<int>(static_cast<int64_t>(r) * a.group / 128 + i);
+  };
+  int n = 0;
+  for (int64_t i = 0; i <= a.b.seqs; i += 64)
+    n += __popcll(__builtin_amdgcn_ballot_w64(i + lane <= a.b.seqs && base(i + lane) <= slot));
+  n = __builtin_amdgcn_readfirstlane(n) - 1;
+  if (n >= 0) rb = slot - __builtin_amdgcn_readfirstlane(base(n));
+  return n;
+}
+
+// Partial states of cut blocks: [nsplit][rows * heads_q] rows of o, then of (m in log2 units, l).
+struct Parts {
+  int nsplit;
+  int64_t plane;  // rows * heads_q
+  float* ws;
+  template <int D>
+  __device__ __forceinline__ float* o(int split, int64_t i) const {
+    return ws + (split * plane + i) * D;
+  }
+  template <int D>
+  __device__ __forceinline__ float* ml(int split, int64_t i) const {
+    return ws + nsplit * plane * D + (split * plane + i) * 2;
+  }
+};
+
+template <typename T, int D, int BITS>
+__global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, int nslots) {
+  using C = ProCfg<D>;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[C::LDS];
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, G = lane >> 4, w = wave_id();
+  const int R = a.group;
+
+  // ---- workgroup -> part, head, slot
+  int bid = blockIdx.x;
+  const int split = bid % pt.nsplit;
+  bid /= pt.nsplit;
+  const int per = gridDim.x / pt.nsplit >> 3;  // blocks an XCD
+  const int lin = (bid & 7) * per + (bid >> 3);
+  const int head = lin / nslots;
+  if (head >= a.c.heads) return;
+  int j = lin % nslots;
+  if ((j | 3) < nslots && (j & 4)) j ^= 3;
+  int rb = 0;
+  const int seq = seq_of_slot(a, nslots - 1 - j, rb);
+  if (seq < 0) return;
+  const SeqPlan sp = plan_of<128, 32>(a, seq);
+  if (rb < 0 || rb >= sp.nb) return;
+
+  // ---- the block's rows: lane row h of wave w is flattened row 128 rb + 32 w + 16 h + c
+  const int64_t nrow = static_cast<int64_t>(sp.n) * R;
+  const int f0 = rb * C::BM;
+  const int fend = nrow < f0 + C::BM ? static_cast<int>(nrow) : f0 + C::BM;
+  const int pos_lo = sp.pos0 + f0 / R, pos_hi = sp.pos0 + (fend - 1) / R;
+  const BlockKeys bk = block_keys(a, pos_lo, pos_hi, pt.nsplit);
+  if (split >= bk.parts) return;
+  const int v0 = split * bk.part, v1 = v0 + bk.part < bk.tiles ? v0 + bk.part : bk.tiles;
+  const int fw = f0 + 32 * w;
+  const bool busy = fw < fend;  // this wave has rows
+  const int wpos_hi = busy ? sp.pos0 + ((fw + 31 < fend - 1 ? fw + 31 : fend - 1)) / R : -1;
+  int pos[2], row[2], hq[2];
+  u32x4 qreg[2][C::KS];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int f = fw + 16 * h + c;
+    const bool live = f < fend;
+    const int ff = live ? f : f0;
+    row[h] = sp.row0 + ff / R;
+    hq[h] = head * R + ff % R;
+    pos[h] = live ? sp.pos0 + ff / R : -1;
+    const uint16_t* qr = a.q + row[h] * a.q_st + hq[h] * a.q_sh;
+#pragma unroll
+    for (int ks = 0; ks < C::KS; ++ks) {
+      const u32x4 x = *reinterpret_cast<const u32x4*>(qr + ks * 32 + G * 8);
+      qreg[h][ks] = live ? x : u32x4{0u, 0u, 0u, 0u};
+    }
+    row[h] = live ? row[h] : -1;
+  }
+
+  // ---- tiles: pages of the two halves, whether every row sees every key
+  struct Tile {
+    int key0, p[2];
+  };
+  const int32_t* trow = a.b.table + seq * a.b.ld_table;
+  auto tile_at = [&](int v) {
+    Tile t;
+    t.key0 = bk.tile(v) * 32;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int e = (t.key0 + 16 * h) >> a.shift;
+      const int p = e < a.b.width ? uniform_i32(trow + e) : -1;
+      t.p[h] = static_cast<uint32_t>(p) < static_cast<uint64_t>(a.c.pages) ? p : -1;
+    }
+    return t;
+  };
+  auto is_full = [&](const Tile& t) {
+    return t.key0 + 31 <= pos_lo && t.key0 + 32 <= a.reach && (t.key0 > pos_hi - a.window || t.key0 + 31 < a.sinks) &&
+           (t.p[0] | t.p[1]) >= 0;
+  };
+  auto gone = [&](const Tile& t, int at, int p) {  // no row of the block sees the key
+    const int key = t.key0 + at;
+    return p < 0 || key > pos_hi || key >= a.reach || (key >= a.sinks && key <= pos_lo - a.window);
+  };
+  const int in_mask = (1 << a.shift) - 1;
+
+  // ---- staging, 16 bits
+  const uint32_t krow = static_cast<uint32_t>(a.c.k_sr) * 2, vrow = static_cast<uint32_t>(a.c.v_sr) * 2;
+  const int lrow = lane / C::CPR, slot = lane % C::CPR;
+  auto stage16 = [&](const Tile& t, int buf) {
+    const bool full = is_full(t);
+#pragma unroll
+    for (int i = 0; i < C::NDMA; ++i) {
+      const int blk = i * 4 + w, at0 = blk * C::RPK, h = at0 >> 4;  // its rows lie in one half
+      const int pg = h ? t.p[1] : t.p[0];
+      const int64_t p = pg < 0 ? 0 : pg;
+      const int in = (t.key0 + at0) & in_mask;
+      const uint16_t* kp = static_cast<const uint16_t*>(a.c.k) + p * a.c.k_sp + head * a.c.k_sh + in * a.c.k_sr;
+      const uint16_t* vp = static_cast<const uint16_t*>(a.c.v) + p * a.c.v_sp + head * a.c.v_sh + in * a.c.v_sr;
+      const rsrc_t kr = make_rsrc(kp, (C::RPK - 1) * krow + C::ROWB);
+      const rsrc_t vr = make_rsrc(vp, (C::RPK - 1) * vrow + C::ROWB);
+      const int at = at0 + lrow;
+      uint32_t dk = lrow * krow + ((slot ^ swz16_k<D>(at)) << 4);
+      uint32_t dv = lrow * vrow + ((slot ^ swz16_v<D>(at)) << 4);
+      if (!full && gone(t, at, pg)) dk = dv = 0x7ffffff0u;  // past the resource: zeros
+      dma16(kr, smem + C::KBUF + buf * C::TILEB + blk * 1024, dk, 0);
+      dma16(vr, smem + C::VBUF + buf * C::TILEB + blk * 1024, dv, 0);
+    }
+  };
+  // ---- staging, 4 bits: thread -> K (waves 0, 1) or V (2, 3), row, chunk of D / 4 features
+  typedef typename DecBlk<D, 4>::codes codes_t;
+  codes_t codes{};
+  float cscale = 0.f;
+  const bool isv = w >= 2;
+  const int crow = (tid & 127) >> 2, cch = tid & 3;
+  auto fetch4 = [&](const Tile& t) {
+    const int pg = crow >> 4 ? t.p[1] : t.p[0];
+    const int64_t p = pg < 0 ? 0 : pg;
+    const int in = (t.key0 + crow) & in_mask;
+    const char* base = static_cast<const char*>(isv ? a.c.v : a.c.k) +
+                       (isv ? p * a.c.v_sp + head * a.c.v_sh + in * a.c.v_sr : p * a.c.k_sp + head * a.c.k_sh + in * a.c.k_sr);
+    const uint8_t* sb = static_cast<const uint8_t*>(isv ? a.c.v_scale : a.c.k_scale) +
+                        (isv ? p * a.c.vs_sp + head * a.c.vs_sh + in * a.c.vs_sr : p * a.c.ks_sp + head * a.c.ks_sh + in * a.c.ks_sr);
+    codes = *reinterpret_cast<const codes_t*>(base + cch * (D / 8));
+    cscale = e8m0(sb[cch * (D / 4) / 32]);
+    if (!is_full(t) && gone(t, crow, pg)) {
+      codes = codes_t{};
+      cscale = 0.f;
+    }
+  };
+  auto commit4 = [&](int buf) {
+    unsigned char* dst = smem + (isv ? C::VBUF : C::KBUF) + buf * C::TILEB + crow * C::ROWB;
+    const int swz = isv ? swz16_v<D>(crow) : swz16_k<D>(crow);
+#pragma unroll
+    for (int i = 0; i < C::KS; ++i)
+      *reinterpret_cast<u32x4*>(dst + (((cch * C::KS + i) ^ swz) << 4)) = fp4_row8<T>(codes[i], cscale);
+  };
+
+  // ---- per-lane operand offsets
+  int ka[C::KS];  // K row c, chunk 4 ks + G
+#pragma unroll
+  for (int ks = 0; ks < C::KS; ++ks) ka[ks] = c * C::ROWB + (((4 * ks + G) ^ swz16_k<D>(c)) << 4);
+  int va[C::FB];  // transposed V reads: row 4 G + k4 (+ 16), features 16 fb + 4 cc .. + 3
+  {
+    const int k4 = (lane >> 2) & 3, cc = lane & 3, r = 4 * G + k4;
+#pragma unroll
+    for (int fb = 0; fb < C::FB; ++fb)
+      va[fb] = r * C::ROWB + (((2 * fb + (cc >> 1)) ^ swz16_v<D>(r)) << 4) + ((cc & 1) << 3);
+  }
+
+  float mused[2] = {-kInf, -kInf}, lsum[2] = {0.f, 0.f};  // raw scores' reference, this lane's part of the sum
+  f32x4 oacc[C::FB][2];
+#pragma unroll
+  for (int fb = 0; fb < C::FB; ++fb) oacc[fb][0] = oacc[fb][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  auto vfrag = [&](const unsigned char* vt, int fb) {
+    const u32x2 lo = ds_read_tr16(vt + va[fb]);
+    const u32x2 hi = ds_read_tr16(vt + 16 * C::ROWB + va[fb]);
+    return u32x4{lo.x, lo.y, hi.x, hi.y};
+  };
+
+  auto tile = [&](auto bufc, const Tile& t, auto cutc) __attribute__((always_inline)) {
+    constexpr bool CUT = decltype(cutc)::value;
+    constexpr int buf = decltype(bufc)::value;
+    const unsigned char* kt = smem + C::KBUF + buf * C::TILEB;
+    const unsigned char* vt = smem + C::VBUF + buf * C::TILEB;
+    f32x4 sacc[2][2];  // [key half][row half]: S^T[16 kb + 4 G + i][16 h + c]
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) sacc[kb][0] = sacc[kb][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto kfrag = [&](int n) { return *reinterpret_cast<const u32x4*>(kt + (n & 1) * 16 * C::ROWB + ka[n >> 1]); };
+    u32x4 kf[C::KPF];
+#pragma unroll
+    for (int n = 0; n < C::KPF; ++n) kf[n] = kfrag(n);
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int n = 0; n < 2 * C::KS; ++n) {
+      const u32x4 kk = kf[n % C::KPF];
+      if (n + C::KPF < 2 * C::KS) kf[n % C::KPF] = kfrag(n + C::KPF);
+      const int ks = n >> 1, kb = n & 1;
+      sacc[kb][0] = mfma16<T>(kk, qreg[0][ks], sacc[kb][0]);
+      sacc[kb][1] = mfma16<T>(kk, qreg[1][ks], sacc[kb][1]);
+    }
+    u32x4 vf[C::PF];
+#pragma unroll
+    for (int n = 0; n < C::PF; ++n) vf[n] = vfrag(vt, n);
+    __builtin_amdgcn_s_setprio(0);
+
+    if constexpr (CUT) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = t.key0 + 16 * kb + 4 * G + i;
+            const bool seen = key <= pos[h] && key < a.reach && (key > pos[h] - a.window || key < a.sinks) && t.p[kb] >= 0;
+            sacc[kb][h][i] = seen ? sacc[kb][h][i] : -kInf;
+          }
+    }
+    u32x4 p[2];
+    // what the exponentials refer to: 0 while a row's scores are all -inf, whose exponentials are then 0, not NaN
+    auto ref = [&](int h) { return mused[h] == -kInf ? 0.f : mused[h]; };
+    auto expo = [&](int h, float m) {
+      const float mc = m * a.c2;
+      float e[8];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x = sacc[kb][h][i];
+          e[4 * kb + i] = CUT ? fast_exp2((x - m) * a.c2) : fast_exp2(__builtin_fmaf(x, a.c2, -mc));
+        }
+      p[h] = u32x4{pack2<T>(e[0], e[1]), pack2<T>(e[2], e[3]), pack2<T>(e[4], e[5]), pack2<T>(e[6], e[7])};
+      return ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+    };
+    auto rowmax = [&](int h) {
+      float m = -kInf;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = fmaxf(m, sacc[kb][h][i]);
+      return max4g(m);
+    };
+    auto rescale = [&](int h, float mnew) {
+      const float alpha = mnew == mused[h] ? 1.f : fast_exp2((mused[h] - mnew) * a.c2);
+      mused[h] = mnew;
+      lsum[h] *= alpha;
+#pragma unroll
+      for (int fb = 0; fb < C::FB; ++fb) oacc[fb][h] *= alpha;
+    };
+    if constexpr (!CUT) {
+      // a reference still at -inf makes these inf or NaN: over the limit
+      float part0 = expo(0, mused[0]), part1 = expo(1, mused[1]);
+      const float lim = static_cast<float>(1 << static_cast<int>(kTau));
+      if (__builtin_amdgcn_ballot_w64(!(part0 <= lim) || !(part1 <= lim)) != 0) {
+        rescale(0, fmaxf(mused[0], rowmax(0)));
+        rescale(1, fmaxf(mused[1], rowmax(1)));
+        part0 = expo(0, ref(0));
+        part1 = expo(1, ref(1));
+      }
+      lsum[0] += part0;
+      lsum[1] += part1;
+    } else {
+      const float m0 = rowmax(0), m1 = rowmax(1);
+      if (__builtin_amdgcn_ballot_w64((m0 - mused[0]) * a.c2 > kTau || (m1 - mused[1]) * a.c2 > kTau) != 0) {
+        rescale(0, fmaxf(mused[0], m0));
+        rescale(1, fmaxf(mused[1], m1));
+      }
+      lsum[0] += expo(0, ref(0));
+      lsum[1] += expo(1, ref(1));
+    }
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int fb = 0; fb < C::FB; ++fb) {
+      const u32x4 vv = vf[fb % C::PF];
+      if (fb + C::PF < C::FB) vf[fb % C::PF] = vfrag(vt, fb + C::PF);
+      oacc[fb][0] = mfma16<T>(vv, p[0], oacc[fb][0]);
+      oacc[fb][1] = mfma16<T>(vv, p[1], oacc[fb][1]);
+    }
+    __builtin_amdgcn_s_setprio(0);
+  };
+
+  if (v0 < v1) {
+    auto bound = [&](int v) { return v < v1 ? v : v1 - 1; };
+    Tile cur = tile_at(v0), next = tile_at(bound(v0 + 1));
+    if constexpr (BITS == 16) {
+      stage16(cur, 0);
+    } else {
+      fetch4(cur);
+      commit4(0);
+    }
+    auto one = [&](int v, auto bufc) __attribute__((always_inline)) {
+      constexpr int buf = decltype(bufc)::value;
+      if constexpr (BITS == 16) wait_vmcnt0();
+      __syncthreads();
+      const bool more = v + 1 < v1;
+      if (more) {
+        if constexpr (BITS == 16)
+          stage16(next, buf ^ 1);
+        else
+          fetch4(next);
+      }
+      const Tile after = tile_at(bound(v + 2));
+      if (busy && cur.key0 <= wpos_hi) {
+        if (is_full(cur))
+          tile(bufc, cur, std::false_type{});
+        else
+          tile(bufc, cur, std::true_type{});
+      }
+      if constexpr (BITS == 4)
+        if (more) commit4(buf ^ 1);
+      cur = next;
+      next = after;
+    };
+    int v = v0;
+    for (; v + 1 < v1; v += 2) {
+      one(v, std::integral_constant<int, 0>{});
+      one(v + 1, std::integral_constant<int, 1>{});
+    }
+    if (v < v1) one(v, std::integral_constant<int, 0>{});
+  }
+
+  // ---- rows out: features 16 fb + 4 G + i of rows c, 16 + c
+  unsigned again[2];  // rows (bit c) to do by themselves
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const float l = sum4g(lsum[h]);
+    bool nan = l != l;
+#pragma unroll
+    for (int fb = 0; fb < C::FB; ++fb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) nan |= oacc[fb][h][i] != oacc[fb][h][i];
+    unsigned long long b = __builtin_amdgcn_ballot_w64(nan && row[h] >= 0);
+    b |= b >> 32;
+    again[h] = static_cast<unsigned>((b | (b >> 16)) & 0xffff);
+    if (pos_lo == pos_hi) again[h] = 0;  // rows that see the same keys
+    if (row[h] < 0 || (again[h] >> c & 1)) continue;
+    const int64_t at = static_cast<int64_t>(row[h]) * a.heads_q + hq[h];
+    if (bk.parts > 1) {
+      float* po = pt.o<D>(split, at) + 4 * G;
+#pragma unroll
+      for (int fb = 0; fb < C::FB; ++fb) *reinterpret_cast<f32x4*>(po + 16 * fb) = oacc[fb][h];
+      if (G == 0) {
+        float* ml = pt.ml<D>(split, at);
+        ml[0] = mused[h] * a.c2;
+        ml[1] = l;
+      }
+    } else {
+      const float inv = l == 0.f ? 0.f : 1.0f / l;
+      uint16_t* out = a.o + row[h] * a.o_st + hq[h] * a.o_sh + 4 * G;
+#pragma unroll
+      for (int fb = 0; fb < C::FB; ++fb) {
+        const f32x4 x = oacc[fb][h];
+        *reinterpret_cast<u32x2*>(out + 16 * fb) = u32x2{pack2<T>(x[0] * inv, x[1] * inv), pack2<T>(x[2] * inv, x[3] * inv)};
+      }
+      if (G == 0 && a.lse) a.lse[at] = l == 0.f ? -kInf : (mused[h] * a.c2 + __log2f(l)) * kLn2;
+    }
+  }
+  // Rows at different positions share tiles: 0 times a value that only some of them see is NaN where it is an infinity or a
+  // NaN. Such rows are done again, each by itself.
+#pragma unroll 1
+  for (unsigned todo = again[0] | again[1] << 16; todo; todo &= todo - 1) {
+    const int f = fw + __builtin_ctz(todo), tok = f / R, h = head * R + f % R;
+    float m = -kInf, l = 0.f, o[D / 64] = {};
+    const uint16_t* qr = a.q + (sp.row0 + tok) * a.q_st + h * a.q_sh;
+    const int s1 = (v1 < bk.sb ? v1 : bk.sb) * 32;
+    if (v0 < bk.sb) row_sweep<T, D, BITS>(a, seq, head, qr, sp.pos0 + tok, v0 * 32, s1, m, l, o);
+    if (v1 > bk.sb)
+      row_sweep<T, D, BITS>(a, seq, head, qr, sp.pos0 + tok, bk.tile(v0 > bk.sb ? v0 : bk.sb) * 32, bk.tile(v1 - 1) * 32 + 32,
+                            m, l, o);
+    if (bk.parts > 1) {
+      const int64_t at = static_cast<int64_t>(sp.row0 + tok) * a.heads_q + h;
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i) pt.o<D>(split, at)[lane + 64 * i] = o[i];
+      if (lane == 0) {
+        pt.ml<D>(split, at)[0] = m;
+        pt.ml<D>(split, at)[1] = l;
+      }
+    } else {
+      write_row<T, D>(a, sp.row0 + tok, h, m, l, o);
+    }
+  }
+}
+
+// Joins the parts of blocks that were cut: a wave a row and query head.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void paged_prompt_merge(PagedAttn a, Parts pt) {
+  const int lane = threadIdx.x & 63, row = blockIdx.x, h = blockIdx.y * 4 + wave_id();
+  const int seq = seq_of_row(a.b, row);
+  if (h >= a.heads_q || seq >= a.b.seqs) return;
+  const SeqPlan sp = plan_of<128, 32>(a, seq);
+  if (row < sp.row0 || row >= sp.row0 + sp.n) return;
+  const int f0 = static_cast<int>(((row - sp.row0) * static_cast<int64_t>(a.group) + h % a.group) / 128 * 128);
+  const int64_t nrow = static_cast<int64_t>(sp.n) * a.group;
+  const int fend = nrow < f0 + 128 ? static_cast<int>(nrow) : f0 + 128;
+  const BlockKeys bk = block_keys(a, sp.pos0 + f0 / a.group, sp.pos0 + (fend - 1) / a.group, pt.nsplit);
+  if (bk.parts <= 1) return;
+  const int64_t at = static_cast<int64_t>(row) * a.heads_q + h;
+  float mm = -kInf, l = 0.f, o[D / 64] = {};
+  for (int s = 0; s < bk.parts; ++s) mm = fmaxf(mm, pt.ml<D>(s, at)[0]);
+#pragma unroll 4
+  for (int s = 0; s < bk.parts; ++s) {
+    const float* ml = pt.ml<D>(s, at);
+    const float f = ml[0] == -kInf ? 0.f : fast_exp2(ml[0] - mm);
+    l += f * ml[1];
+#pragma unroll
+    for (int j = 0; j < D / 64; ++j) o[j] += f * pt.o<D>(s, at)[lane + 64 * j];
+  }
+  write_row<T, D>(a, row, h, mm, l, o);
+}
+
 }  // namespace
 }  // namespace pdh
 
@@ -614,15 +1070,28 @@ int decode_grid(const pdh_paged_cache& c) {
   return (cus > 0 ? cus : 256) * (c.bits == 16 ? kDecWgs<16> : kDecWgs<4>);
 }
 
+// Parts that the prompt kernel cuts a block's keys into: enough for two workgroups a compute unit, of at least 512 keys of
+// what the table can hold (the lengths are not known here; a block of fewer keys makes fewer parts).
+int prompt_splits(const pdh_paged_cache& c, const pdh_paged_batch& b, int64_t group, int64_t window, int64_t sinks) {
+  const int cus = pdh_device_cus();
+  const int64_t blocks = (b.rows * group / 128 + 1) * c.heads;
+  int64_t keys = b.width * c.page_rows;
+  if (window < keys) keys = keys < window + sinks + 128 ? keys : window + sinks + 128;
+  int64_t n = 2 * (cus > 0 ? cus : 256) / blocks;
+  n = n < keys / 512 ? n : keys / 512;
+  return static_cast<int>(n < 1 ? 1 : (n < 32 ? n : 32));
+}
+
 }  // namespace
 
 extern "C" size_t pdh_paged_attention_workspace(const pdh_paged_cache* cache, const pdh_paged_batch* batch,
                                                 int64_t heads_q, int64_t window, int64_t sinks) {
-  (void)window, (void)sinks;
   if (!cache || !batch || cache->heads < 1 || heads_q < cache->heads) return 0;
   if (few_rows(*batch, heads_q / cache->heads))
     return static_cast<size_t>(decode_grid(*cache)) * (sizeof(DecMeta) + 2 * 16 * (2 + cache->features) * sizeof(float));
-  return 0;
+  const int nsplit = prompt_splits(*cache, *batch, heads_q / cache->heads, window, sinks);
+  if (nsplit == 1) return 0;
+  return static_cast<size_t>(nsplit) * batch->rows * heads_q * (2 + cache->features) * sizeof(float);
 }
 
 extern "C" int pdh_paged_attention(const void* q, void* o, float* lse, int64_t heads_q, int64_t q_st, int64_t q_sh,
@@ -662,9 +1131,20 @@ extern "C" int pdh_paged_attention(const void* q, void* o, float* lse, int64_t h
     });
     return check_launch("pdh_paged_attention (decode)");
   }
-  const dim3 grid(static_cast<unsigned>(batch->rows), static_cast<unsigned>((heads_q + 3) / 4));
+  const int nsplit = prompt_splits(*cache, *batch, a.group, window, sinks);
+  const int64_t nslots = batch->rows * a.group / 128 + batch->seqs + 1;
+  const int64_t blocks = (nslots * cache->heads + 7) / 8 * 8 * nsplit;
+  PDH_REQUIRE(blocks <= INT32_MAX, PDH_EINVAL, "pdh_paged_attention: grid too large");
+  const Parts parts{nsplit, batch->rows * heads_q, static_cast<float*>(ws)};
   by_kind(*cache, [&](auto t, auto d, auto bits) {
-    paged_attn_rows<decltype(t), decltype(d)::value, decltype(bits)::value><<<grid, 256, 0, as_stream(stream)>>>(a);
+    using T = decltype(t);
+    constexpr int D = decltype(d)::value;
+    paged_prompt<T, D, decltype(bits)::value>
+        <<<static_cast<unsigned>(blocks), 256, 0, as_stream(stream)>>>(a, parts, static_cast<int>(nslots));
+    if (nsplit > 1) {
+      const dim3 grid(static_cast<unsigned>(batch->rows), static_cast<unsigned>((heads_q + 3) / 4));
+      paged_prompt_merge<T, D><<<grid, 256, 0, as_stream(stream)>>>(a, parts);
+    }
   });
-  return check_launch("pdh_paged_attention");
+  return check_launch("pdh_paged_attention (prompt)");
 }
