@@ -185,6 +185,8 @@ struct SeqPlan {
   __device__ __forceinline__ int key_block(int v) const { return v < sb ? v : v - sb + wb; }
 };
 
+__device__ __forceinline__ int scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
 template <int ROWS, int KEYS>
 __device__ __forceinline__ SeqPlan plan_of(const PagedAttn& a, int i) {
   Seq s{0, 0, 0};
@@ -210,6 +212,13 @@ __device__ __forceinline__ SeqPlan plan_of(const PagedAttn& a, int i) {
   p.blocks = p.blocks > 0 ? p.blocks : 1;  // one that sees nothing
   p.nb = static_cast<int>((static_cast<int64_t>(s.n) * a.group + ROWS - 1) / ROWS);
   return p;
+}
+
+// The plan of a wave-uniform sequence, held in scalar registers.
+template <int ROWS, int KEYS>
+__device__ __forceinline__ SeqPlan uniform_plan(const PagedAttn& a, int i) {
+  const SeqPlan p = plan_of<ROWS, KEYS>(a, i);
+  return SeqPlan{scalar(p.row0), scalar(p.n), scalar(p.pos0), scalar(p.nb), scalar(p.sb), scalar(p.wb), scalar(p.blocks)};
 }
 
 struct DecMeta {
@@ -270,7 +279,7 @@ __global__ __launch_bounds__(256, kDecWgs<BITS>) void paged_decode(PagedAttn a, 
   int64_t in_seq = scan[1];
   SeqPlan sp;
   for (;; ++seq) {
-    sp = plan_of<16, 32>(a, seq);
+    sp = uniform_plan<16, 32>(a, seq);
     const int64_t cost = static_cast<int64_t>(sp.nb) * sp.blocks * hkv;
     if (in_seq < cost) break;
     in_seq -= cost;
@@ -287,17 +296,15 @@ __global__ __launch_bounds__(256, kDecWgs<BITS>) void paged_decode(PagedAttn a, 
   const int vrow = BITS == 16 ? lane / C::CPR : lane / 4, vch = BITS == 16 ? lane % C::CPR : lane % 4;
 
   while (left > 0) {
-    const int rb = item % sp.nb, head = item / sp.nb;
-    const int todo = static_cast<int>(sp.blocks - kb < left ? sp.blocks - kb : left);
+    const int rb = scalar(item % sp.nb), head = scalar(item / sp.nb);
+    const int todo = scalar(static_cast<int>(sp.blocks - kb < left ? sp.blocks - kb : left));
     const int k_end = kb + todo;
 
     // ---- the block's rows: column c is flattened row 16 rb + c
-    const int nq = sp.n * static_cast<int64_t>(R) - 16 * static_cast<int64_t>(rb) < 16
-                       ? static_cast<int>(sp.n * static_cast<int64_t>(R) - 16 * static_cast<int64_t>(rb))
-                       : 16;
-    const int f0 = rb * 16, fc = f0 + (col < nq ? col : 0);
+    const int f0 = rb * 16, nq = sp.n * R - f0 < 16 ? sp.n * R - f0 : 16;  // rows x heads_q < 2^31
+    const int fc = f0 + (col < nq ? col : 0);
     const int pos = sp.pos0 + fc / R;
-    const int pos_lo = sp.pos0 + f0 / R, pos_hi = sp.pos0 + (f0 + nq - 1) / R;
+    const int pos_lo = scalar(sp.pos0 + f0 / R), pos_hi = scalar(sp.pos0 + (f0 + nq - 1) / R);
     u32x4 qb[KS];
     {
       const uint16_t* qr = a.q + (sp.row0 + fc / R) * a.q_st + (head * R + fc % R) * a.q_sh;
@@ -539,7 +546,7 @@ __global__ __launch_bounds__(256, kDecWgs<BITS>) void paged_decode(PagedAttn a, 
       ++item;
       if (item == sp.nb * hkv) {
         item = 0;
-        do sp = plan_of<16, 32>(a, ++seq);
+        do sp = uniform_plan<16, 32>(a, ++seq);
         while (sp.n == 0);
       }
     }
@@ -635,9 +642,17 @@ __device__ __forceinline__ BlockKeys block_keys(const PagedAttn& a, int pos_lo, 
   b.sb = b.sb < b.wb ? b.sb : b.wb;
   b.tiles = b.sb + eb - b.wb;
   b.part = (b.tiles + nsplit - 1) / nsplit;
-  b.part = b.part > kPartTiles ? b.part : kPartTiles;
-  b.parts = b.tiles > b.part ? (b.tiles + b.part - 1) / b.part : 1;
+  b.part = scalar(b.part > kPartTiles ? b.part : kPartTiles);
+  b.parts = scalar(b.tiles > b.part ? (b.tiles + b.part - 1) / b.part : 1);
   return b;
+}
+
+// A resource over wave-uniform memory whose address the compiler may hold in vector registers.
+__device__ __forceinline__ rsrc_t uniform_rsrc(const void* base, uint32_t bytes) {
+  const uint64_t u = reinterpret_cast<uintptr_t>(base);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(u));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(u >> 32));
+  return make_rsrc(reinterpret_cast<const void*>(static_cast<uint64_t>(hi) << 32 | lo), __builtin_amdgcn_readfirstlane(bytes));
 }
 
 // The sequence of a slot (seqs: the rows behind the last one; -1: none) and the block's number in it.
@@ -679,97 +694,94 @@ __global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, in
 
   // ---- workgroup -> part, head, slot
   int bid = blockIdx.x;
-  const int split = bid % pt.nsplit;
-  bid /= pt.nsplit;
-  const int per = gridDim.x / pt.nsplit >> 3;  // blocks an XCD
+  const int split = scalar(bid % pt.nsplit);
+  bid = scalar(bid / pt.nsplit);
+  const int per = scalar(gridDim.x / pt.nsplit >> 3);  // blocks an XCD
   const int lin = (bid & 7) * per + (bid >> 3);
-  const int head = lin / nslots;
+  const int head = scalar(lin / nslots);
   if (head >= a.c.heads) return;
-  int j = lin % nslots;
+  int j = scalar(lin % nslots);
   if ((j | 3) < nslots && (j & 4)) j ^= 3;
   int rb = 0;
   const int seq = seq_of_slot(a, nslots - 1 - j, rb);
   if (seq < 0) return;
-  const SeqPlan sp = plan_of<128, 32>(a, seq);
+  const SeqPlan sp = uniform_plan<128, 32>(a, seq);
   if (rb < 0 || rb >= sp.nb) return;
 
   // ---- the block's rows: lane row h of wave w is flattened row 128 rb + 32 w + 16 h + c
-  const int64_t nrow = static_cast<int64_t>(sp.n) * R;
   const int f0 = rb * C::BM;
-  const int fend = nrow < f0 + C::BM ? static_cast<int>(nrow) : f0 + C::BM;
-  const int pos_lo = sp.pos0 + f0 / R, pos_hi = sp.pos0 + (fend - 1) / R;
+  const int fend = sp.n * R - f0 < C::BM ? sp.n * R : f0 + C::BM;  // rows x heads_q < 2^31
+  const int pos_lo = scalar(sp.pos0 + f0 / R), pos_hi = scalar(sp.pos0 + (fend - 1) / R);
   const BlockKeys bk = block_keys(a, pos_lo, pos_hi, pt.nsplit);
   if (split >= bk.parts) return;
   const int v0 = split * bk.part, v1 = v0 + bk.part < bk.tiles ? v0 + bk.part : bk.tiles;
   const int fw = f0 + 32 * w;
   const bool busy = fw < fend;  // this wave has rows
-  const int wpos_hi = busy ? sp.pos0 + ((fw + 31 < fend - 1 ? fw + 31 : fend - 1)) / R : -1;
-  int pos[2], row[2], hq[2];
+  const int wpos_hi = scalar(busy ? sp.pos0 + (fw + 31 < fend - 1 ? fw + 31 : fend - 1) / R : -1);
+  int pos[2];
   u32x4 qreg[2][C::KS];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int f = fw + 16 * h + c;
     const bool live = f < fend;
     const int ff = live ? f : f0;
-    row[h] = sp.row0 + ff / R;
-    hq[h] = head * R + ff % R;
     pos[h] = live ? sp.pos0 + ff / R : -1;
-    const uint16_t* qr = a.q + row[h] * a.q_st + hq[h] * a.q_sh;
+    const uint16_t* qr = a.q + (sp.row0 + ff / R) * a.q_st + (head * R + ff % R) * a.q_sh;
 #pragma unroll
     for (int ks = 0; ks < C::KS; ++ks) {
       const u32x4 x = *reinterpret_cast<const u32x4*>(qr + ks * 32 + G * 8);
       qreg[h][ks] = live ? x : u32x4{0u, 0u, 0u, 0u};
     }
-    row[h] = live ? row[h] : -1;
   }
 
-  // ---- tiles: pages of the two halves, whether every row sees every key
+  // ---- tiles: the pages of their two halves
   struct Tile {
     int key0, p[2];
   };
   const int32_t* trow = a.b.table + seq * a.b.ld_table;
   auto tile_at = [&](int v) {
     Tile t;
-    t.key0 = bk.tile(v) * 32;
+    t.key0 = scalar(bk.tile(v) * 32);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int e = (t.key0 + 16 * h) >> a.shift;
+      const int e = scalar((t.key0 + 16 * h) >> a.shift);
       const int p = e < a.b.width ? uniform_i32(trow + e) : -1;
-      t.p[h] = static_cast<uint32_t>(p) < static_cast<uint64_t>(a.c.pages) ? p : -1;
+      t.p[h] = scalar(static_cast<uint32_t>(p) < static_cast<uint64_t>(a.c.pages) ? p : -1);
     }
     return t;
-  };
-  auto is_full = [&](const Tile& t) {
-    return t.key0 + 31 <= pos_lo && t.key0 + 32 <= a.reach && (t.key0 > pos_hi - a.window || t.key0 + 31 < a.sinks) &&
-           (t.p[0] | t.p[1]) >= 0;
   };
   auto gone = [&](const Tile& t, int at, int p) {  // no row of the block sees the key
     const int key = t.key0 + at;
     return p < 0 || key > pos_hi || key >= a.reach || (key >= a.sinks && key <= pos_lo - a.window);
   };
   const int in_mask = (1 << a.shift) - 1;
+  bool lost = false;  // a tile that every row should see whole lacks a page
 
   // ---- staging, 16 bits
   const uint32_t krow = static_cast<uint32_t>(a.c.k_sr) * 2, vrow = static_cast<uint32_t>(a.c.v_sr) * 2;
   const int lrow = lane / C::CPR, slot = lane % C::CPR;
-  auto stage16 = [&](const Tile& t, int buf) {
-    const bool full = is_full(t);
+  const uint16_t* const kpool = static_cast<const uint16_t*>(a.c.k) + head * a.c.k_sh;
+  const uint16_t* const vpool = static_cast<const uint16_t*>(a.c.v) + head * a.c.v_sh;
+  uint32_t dk[C::NDMA], dv[C::NDMA];
+#pragma unroll
+  for (int i = 0; i < C::NDMA; ++i) {
+    const int at = (i * 4 + w) * C::RPK + lrow;
+    dk[i] = lrow * krow + ((slot ^ swz16_k<D>(at)) << 4);
+    dv[i] = lrow * vrow + ((slot ^ swz16_v<D>(at)) << 4);
+  }
+  auto stage16 = [&](const Tile& t, int buf, bool cut) {
 #pragma unroll
     for (int i = 0; i < C::NDMA; ++i) {
       const int blk = i * 4 + w, at0 = blk * C::RPK, h = at0 >> 4;  // its rows lie in one half
       const int pg = h ? t.p[1] : t.p[0];
       const int64_t p = pg < 0 ? 0 : pg;
       const int in = (t.key0 + at0) & in_mask;
-      const uint16_t* kp = static_cast<const uint16_t*>(a.c.k) + p * a.c.k_sp + head * a.c.k_sh + in * a.c.k_sr;
-      const uint16_t* vp = static_cast<const uint16_t*>(a.c.v) + p * a.c.v_sp + head * a.c.v_sh + in * a.c.v_sr;
-      const rsrc_t kr = make_rsrc(kp, (C::RPK - 1) * krow + C::ROWB);
-      const rsrc_t vr = make_rsrc(vp, (C::RPK - 1) * vrow + C::ROWB);
-      const int at = at0 + lrow;
-      uint32_t dk = lrow * krow + ((slot ^ swz16_k<D>(at)) << 4);
-      uint32_t dv = lrow * vrow + ((slot ^ swz16_v<D>(at)) << 4);
-      if (!full && gone(t, at, pg)) dk = dv = 0x7ffffff0u;  // past the resource: zeros
-      dma16(kr, smem + C::KBUF + buf * C::TILEB + blk * 1024, dk, 0);
-      dma16(vr, smem + C::VBUF + buf * C::TILEB + blk * 1024, dv, 0);
+      const rsrc_t kr = uniform_rsrc(kpool + p * a.c.k_sp + in * a.c.k_sr, (C::RPK - 1) * krow + C::ROWB);
+      const rsrc_t vr = uniform_rsrc(vpool + p * a.c.v_sp + in * a.c.v_sr, (C::RPK - 1) * vrow + C::ROWB);
+      uint32_t ok = dk[i], ov = dv[i];
+      if (cut && gone(t, at0 + lrow, pg)) ok = ov = 0x7ffffff0u;  // past the resource: zeros
+      dma16(kr, smem + C::KBUF + buf * C::TILEB + blk * 1024, ok, 0);
+      dma16(vr, smem + C::VBUF + buf * C::TILEB + blk * 1024, ov, 0);
     }
   };
   // ---- staging, 4 bits: thread -> K (waves 0, 1) or V (2, 3), row, chunk of D / 4 features
@@ -778,17 +790,19 @@ __global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, in
   float cscale = 0.f;
   const bool isv = w >= 2;
   const int crow = (tid & 127) >> 2, cch = tid & 3;
-  auto fetch4 = [&](const Tile& t) {
+  const char* const cpool = isv ? static_cast<const char*>(a.c.v) + head * a.c.v_sh + cch * (D / 8)
+                                : static_cast<const char*>(a.c.k) + head * a.c.k_sh + cch * (D / 8);
+  const uint8_t* const spool = isv ? static_cast<const uint8_t*>(a.c.v_scale) + head * a.c.vs_sh + cch * (D / 4) / 32
+                                   : static_cast<const uint8_t*>(a.c.k_scale) + head * a.c.ks_sh + cch * (D / 4) / 32;
+  const int64_t c_sp = isv ? a.c.v_sp : a.c.k_sp, s_sp = isv ? a.c.vs_sp : a.c.ks_sp;
+  const int64_t c_sr = isv ? a.c.v_sr : a.c.k_sr, s_sr = isv ? a.c.vs_sr : a.c.ks_sr;
+  auto fetch4 = [&](const Tile& t, bool cut) {
     const int pg = crow >> 4 ? t.p[1] : t.p[0];
     const int64_t p = pg < 0 ? 0 : pg;
     const int in = (t.key0 + crow) & in_mask;
-    const char* base = static_cast<const char*>(isv ? a.c.v : a.c.k) +
-                       (isv ? p * a.c.v_sp + head * a.c.v_sh + in * a.c.v_sr : p * a.c.k_sp + head * a.c.k_sh + in * a.c.k_sr);
-    const uint8_t* sb = static_cast<const uint8_t*>(isv ? a.c.v_scale : a.c.k_scale) +
-                        (isv ? p * a.c.vs_sp + head * a.c.vs_sh + in * a.c.vs_sr : p * a.c.ks_sp + head * a.c.ks_sh + in * a.c.ks_sr);
-    codes = *reinterpret_cast<const codes_t*>(base + cch * (D / 8));
-    cscale = e8m0(sb[cch * (D / 4) / 32]);
-    if (!is_full(t) && gone(t, crow, pg)) {
+    codes = *reinterpret_cast<const codes_t*>(cpool + p * c_sp + in * c_sr);
+    cscale = e8m0(spool[p * s_sp + in * s_sr]);
+    if (cut && gone(t, crow, pg)) {
       codes = codes_t{};
       cscale = 0.f;
     }
@@ -824,9 +838,9 @@ __global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, in
     return u32x4{lo.x, lo.y, hi.x, hi.y};
   };
 
-  auto tile = [&](auto bufc, const Tile& t, auto cutc) __attribute__((always_inline)) {
+  // buf: a constant where the tile is whole, so that every operand read is a lane's offset and an immediate
+  auto tile = [&](auto buf, const Tile& t, auto cutc) __attribute__((always_inline)) {
     constexpr bool CUT = decltype(cutc)::value;
-    constexpr int buf = decltype(bufc)::value;
     const unsigned char* kt = smem + C::KBUF + buf * C::TILEB;
     const unsigned char* vt = smem + C::VBUF + buf * C::TILEB;
     f32x4 sacc[2][2];  // [key half][row half]: S^T[16 kb + 4 G + i][16 h + c]
@@ -850,17 +864,23 @@ __global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, in
     for (int n = 0; n < C::PF; ++n) vf[n] = vfrag(vt, n);
     __builtin_amdgcn_s_setprio(0);
 
-    if constexpr (CUT) {
+    if constexpr (CUT) {  // key of accumulator (kb, i): key0 + 4 G + 16 kb + i
+      const int kl = t.key0 + 4 * G;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h) {
+        const int last = (pos[h] < a.reach ? pos[h] : a.reach - 1) - kl, first = pos[h] - a.window + 1 - kl;
+        const int kept = a.sinks - kl;
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int kb = 0; kb < 2; ++kb) {
+          const int end = t.p[kb] < 0 ? -1 - kMaxTokens : last;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int key = t.key0 + 16 * kb + 4 * G + i;
-            const bool seen = key <= pos[h] && key < a.reach && (key > pos[h] - a.window || key < a.sinks) && t.p[kb] >= 0;
+            const int cc = 16 * kb + i;
+            const bool seen = (cc <= end) & ((cc >= first) | (cc < kept));
             sacc[kb][h][i] = seen ? sacc[kb][h][i] : -kInf;
           }
+        }
+      }
     }
     u32x4 p[2];
     // what the exponentials refer to: 0 while a row's scores are all -inf, whose exponentials are then 0, not NaN
@@ -925,62 +945,88 @@ __global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, in
     __builtin_amdgcn_s_setprio(0);
   };
 
+  // Tiles [c0, c1) are whole for every row of the block; before them lie the first tokens and the window's left edge,
+  // behind them the diagonal.
+  int c0, c1;
+  {
+    const int edge = pos_hi - a.window + 1;
+    const int first = edge > 0 ? (edge + 31) / 32 : 0, last = (pos_lo + 1 < a.reach ? pos_lo + 1 : a.reach) >> 5;
+    c0 = bk.sb + (first > bk.wb ? first - bk.wb : 0);
+    c1 = bk.sb + (last > bk.wb ? last - bk.wb : 0);
+    if (c0 >= c1) c0 = c1 = bk.tiles;
+    c0 = c0 < v0 ? v0 : (c0 > v1 ? v1 : c0);
+    c1 = c1 < v0 ? v0 : (c1 > v1 ? v1 : c1);
+  }
   if (v0 < v1) {
     auto bound = [&](int v) { return v < v1 ? v : v1 - 1; };
+    auto is_cut = [&](int v) { return v < c0 || v >= c1; };
     Tile cur = tile_at(v0), next = tile_at(bound(v0 + 1));
+    const int odd = c0 & 1;  // tile v lies in buffer (v ^ odd) & 1: the whole ones start in buffer 0
     if constexpr (BITS == 16) {
-      stage16(cur, 0);
+      stage16(cur, (v0 ^ odd) & 1, is_cut(v0));
     } else {
-      fetch4(cur);
-      commit4(0);
+      fetch4(cur, is_cut(v0));
+      commit4((v0 ^ odd) & 1);
     }
-    auto one = [&](int v, auto bufc) __attribute__((always_inline)) {
-      constexpr int buf = decltype(bufc)::value;
+    auto one = [&](int v, auto buf, auto cutc) __attribute__((always_inline)) {
       if constexpr (BITS == 16) wait_vmcnt0();
       __syncthreads();
       const bool more = v + 1 < v1;
       if (more) {
         if constexpr (BITS == 16)
-          stage16(next, buf ^ 1);
+          stage16(next, buf ^ 1, is_cut(v + 1));
         else
-          fetch4(next);
+          fetch4(next, is_cut(v + 1));
       }
       const Tile after = tile_at(bound(v + 2));
-      if (busy && cur.key0 <= wpos_hi) {
-        if (is_full(cur))
-          tile(bufc, cur, std::false_type{});
-        else
-          tile(bufc, cur, std::true_type{});
+      if constexpr (decltype(cutc)::value) {
+        if (cur.key0 <= wpos_hi) tile(buf, cur, cutc);
+      } else {
+        lost |= (cur.p[0] | cur.p[1]) < 0;
+        if (busy) tile(buf, cur, cutc);
       }
       if constexpr (BITS == 4)
         if (more) commit4(buf ^ 1);
       cur = next;
       next = after;
     };
-    int v = v0;
-    for (; v + 1 < v1; v += 2) {
-      one(v, std::integral_constant<int, 0>{});
-      one(v + 1, std::integral_constant<int, 1>{});
+    const int pairs = c0 + ((c1 - c0) & ~1);  // whole tiles go in pairs; a last single one goes with the cut ones
+#pragma unroll 1
+    for (int v = v0; v < v1;) {
+#pragma unroll 1
+      for (; v >= c0 && v < pairs; v += 2) {
+        one(v, std::integral_constant<int, 0>{}, std::false_type{});
+        one(v + 1, std::integral_constant<int, 1>{}, std::false_type{});
+      }
+      if (v < v1) {
+        one(v, (v ^ odd) & 1, std::true_type{});
+        ++v;
+      }
     }
-    if (v < v1) one(v, std::integral_constant<int, 0>{});
   }
 
   // ---- rows out: features 16 fb + 4 G + i of rows c, 16 + c
   unsigned again[2];  // rows (bit c) to do by themselves
+  int fo = fw + c;
+  asm volatile("" : "+v"(fo));  // rows and heads are found again here, not held through the sweep
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
+    const int f = fo + 16 * h;
+    const bool live = f < fend;
+    const int row = sp.row0 + f / R, hq = head * R + f % R;
     const float l = sum4g(lsum[h]);
     bool nan = l != l;
 #pragma unroll
     for (int fb = 0; fb < C::FB; ++fb)
 #pragma unroll
       for (int i = 0; i < 4; ++i) nan |= oacc[fb][h][i] != oacc[fb][h][i];
-    unsigned long long b = __builtin_amdgcn_ballot_w64(nan && row[h] >= 0);
+    unsigned long long b = __builtin_amdgcn_ballot_w64(nan && live);
     b |= b >> 32;
     again[h] = static_cast<unsigned>((b | (b >> 16)) & 0xffff);
     if (pos_lo == pos_hi) again[h] = 0;  // rows that see the same keys
-    if (row[h] < 0 || (again[h] >> c & 1)) continue;
-    const int64_t at = static_cast<int64_t>(row[h]) * a.heads_q + hq[h];
+    if (lost) again[h] = fw + 16 * h < fend ? (fend - fw - 16 * h < 16 ? (1u << (fend - fw - 16 * h)) - 1 : 0xffff) : 0;
+    if (!live || (again[h] >> c & 1)) continue;
+    const int64_t at = static_cast<int64_t>(row) * a.heads_q + hq;
     if (bk.parts > 1) {
       float* po = pt.o<D>(split, at) + 4 * G;
 #pragma unroll
@@ -992,7 +1038,7 @@ __global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, in
       }
     } else {
       const float inv = l == 0.f ? 0.f : 1.0f / l;
-      uint16_t* out = a.o + row[h] * a.o_st + hq[h] * a.o_sh + 4 * G;
+      uint16_t* out = a.o + row * a.o_st + hq * a.o_sh + 4 * G;
 #pragma unroll
       for (int fb = 0; fb < C::FB; ++fb) {
         const f32x4 x = oacc[fb][h];
@@ -1002,7 +1048,7 @@ __global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, in
     }
   }
   // Rows at different positions share tiles: 0 times a value that only some of them see is NaN where it is an infinity or a
-  // NaN. Such rows are done again, each by itself.
+  // NaN. Such rows are done again, each by itself; all of them where a page is missing among tiles taken for whole.
 #pragma unroll 1
   for (unsigned todo = again[0] | again[1] << 16; todo; todo &= todo - 1) {
     const int f = fw + __builtin_ctz(todo), tok = f / R, h = head * R + f % R;
