@@ -331,9 +331,9 @@ typedef struct pdh_paged_cache {
   void *k, *v;
   void *k_scale, *v_scale;                 /* bits 4: [pages][heads][page_rows][features / 32]; else unused */
   int64_t pages, heads, page_rows, features;
-  int64_t k_sp, k_sh, k_sr;                /* strides of a page, a head, a row: elements (bits 4: bytes), multiples */
-  int64_t v_sp, v_sh, v_sr;                /* of 16 bytes; rows less than 2^16 apart */
-  int64_t ks_sp, ks_sh, ks_sr, vs_sp, vs_sh, vs_sr; /* the scales', bytes */
+  int64_t sp, sh, sr;    /* both pools' strides of a page, a head, a row: elements (bits 4: bytes), multiples of 16
+                          * bytes; pages less than 2^35 bytes apart, rows less than 2^16 units */
+  int64_t ssp, ssh, ssr; /* both scales', bytes; pages less than 2^31 apart */
   int32_t dtype, bits;
 } pdh_paged_cache;
 

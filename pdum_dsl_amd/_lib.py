@@ -97,7 +97,7 @@ class PagedCacheC(C.Structure):
         (n, C.c_int64)
         for n in (
             "pages heads page_rows features "
-            "k_sp k_sh k_sr v_sp v_sh v_sr ks_sp ks_sh ks_sr vs_sp vs_sh vs_sr"
+            "sp sh sr ssp ssh ssr"
         ).split()
     ] + [("dtype", C.c_int32), ("bits", C.c_int32)]
 

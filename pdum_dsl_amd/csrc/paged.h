@@ -50,6 +50,19 @@ __device__ __forceinline__ int page_of(const pdh_paged_batch& b, const pdh_paged
   return static_cast<uint32_t>(p) < static_cast<uint64_t>(c.pages) ? p : -1;
 }
 
+// Where a row of a page lies in either pool, from a head's first row: units of the pools (16-bit elements, bytes), and
+// bytes of the scales. A page's distance is a 32-bit number of 16 bytes (the pools') or bytes (the scales').
+template <int BITS>
+__device__ __forceinline__ int64_t pool_at(const pdh_paged_cache& c, int page, int in_page) {
+  constexpr int unit = BITS == 16 ? 8 : 16;
+  return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(page)) * static_cast<uint32_t>(c.sp / unit)) * unit +
+         in_page * static_cast<int>(c.sr);
+}
+__device__ __forceinline__ int64_t scale_at(const pdh_paged_cache& c, int page, int in_page) {
+  return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(page)) * static_cast<uint32_t>(c.ssp)) +
+         in_page * static_cast<int>(c.ssr);
+}
+
 // ---- 4 bits: e2m1 codes (sign, two bits of exponent, one of mantissa: 0 .5 1 1.5 2 3 4 6), two a byte, the even feature
 // in the low half; 32 features share the scale 2^(byte - 127), byte 255: NaN. gfx950 converts pairs of them, scaled, in
 // one instruction (byte 255 gives NaN for every code, byte 0 is 2^-127).
@@ -88,17 +101,17 @@ inline int check_paged(const char* fn, const pdh_paged_cache* c, const pdh_paged
   PDH_REQUIRE(c->k && c->v && aligned16(c->k) && aligned16(c->v), PDH_EINVAL, "%s: pools must be 16-byte aligned", fn);
   const int64_t unit = c->bits == 4 ? 16 : 8;  // 16 bytes
   const int64_t row = c->bits == 4 ? c->features / 2 : c->features;
-  for (int64_t s : {c->k_sp, c->k_sh, c->k_sr, c->v_sp, c->v_sh, c->v_sr})
+  for (int64_t s : {c->sp, c->sh, c->sr})
     PDH_REQUIRE(s >= 0 && s % unit == 0, PDH_EINVAL, "%s: the pools' strides must be multiples of 16 bytes, >= 0", fn);
-  PDH_REQUIRE(c->k_sr >= row && c->v_sr >= row && c->k_sr < (1 << 16) && c->v_sr < (1 << 16), PDH_EINVAL,
-              "%s: the pools' rows overlap or lie 2^16 or more apart", fn);
+  PDH_REQUIRE(c->sr >= row && c->sr < (1 << 16), PDH_EINVAL, "%s: the pools' rows overlap or lie 2^16 or more apart", fn);
+  PDH_REQUIRE(c->sp / unit < INT32_MAX && c->sh < INT64_MAX / 65536 / 2, PDH_EINVAL,
+              "%s: the pools' pages lie 2^35 bytes or more apart", fn);
   if (c->bits == 4) {
     PDH_REQUIRE(c->k_scale && c->v_scale, PDH_EINVAL, "%s: a 4-bit cache needs its scales", fn);
-    for (int64_t s : {c->ks_sp, c->ks_sh, c->ks_sr, c->vs_sp, c->vs_sh, c->vs_sr})
-      PDH_REQUIRE(s >= 0, PDH_EINVAL, "%s: the scales' strides must be >= 0", fn);
-    PDH_REQUIRE(c->ks_sr >= c->features / 32 && c->vs_sr >= c->features / 32 && c->ks_sr < (1 << 16) &&
-                    c->vs_sr < (1 << 16),
-                PDH_EINVAL, "%s: the scales' rows overlap or lie 2^16 or more apart", fn);
+    PDH_REQUIRE(c->ssp >= 0 && c->ssh >= 0 && c->ssp <= INT32_MAX, PDH_EINVAL,
+                "%s: the scales' strides must be >= 0, pages less than 2^31 bytes apart", fn);
+    PDH_REQUIRE(c->ssr >= c->features / 32 && c->ssr < (1 << 16), PDH_EINVAL,
+                "%s: the scales' rows overlap or lie 2^16 or more apart", fn);
   }
   PDH_REQUIRE(b->seqs >= 0 && b->seqs <= (1 << 20) && b->rows >= 0 && b->rows < (1 << 24), PDH_EINVAL,
               "%s: at most 2^20 sequences and 2^24 - 1 rows", fn);

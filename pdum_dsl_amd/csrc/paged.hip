@@ -145,8 +145,7 @@ __global__ __launch_bounds__(256) void paged_append(AppendArgs a) {
     return;
   }
   const int in_page = pos & ((1 << a.shift) - 1);
-  const int64_t place = kind == 1 ? page * a.c.k_sp + h * a.c.k_sh + in_page * a.c.k_sr
-                                  : page * a.c.v_sp + h * a.c.v_sh + in_page * a.c.v_sr;
+  const int64_t place = pool_at<BITS>(a.c, page, in_page) + h * a.c.sh;
   if constexpr (BITS == 16) {
     *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(kind == 1 ? a.c.k : a.c.v) + place + f0) = out;
   } else {
@@ -154,8 +153,7 @@ __global__ __launch_bounds__(256) void paged_append(AppendArgs a) {
     const uint32_t codes = fp4_codes<T>(y, byte);
     *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(kind == 1 ? a.c.k : a.c.v) + place + f0 / 2) = codes;
     if ((f0 & 31) == 0) {
-      const int64_t sp = kind == 1 ? page * a.c.ks_sp + h * a.c.ks_sh + in_page * a.c.ks_sr
-                                   : page * a.c.vs_sp + h * a.c.vs_sh + in_page * a.c.vs_sr;
+      const int64_t sp = scale_at(a.c, page, in_page) + h * a.c.ssh;
       static_cast<uint8_t*>(kind == 1 ? a.c.k_scale : a.c.v_scale)[sp + f0 / 32] = static_cast<uint8_t>(byte);
     }
   }
@@ -192,13 +190,11 @@ __global__ __launch_bounds__(256) void paged_rows(RowsArgs a) {
   u32x4 x = {0u, 0u, 0u, 0u};
   if (page >= 0) {
     const int in_page = pos & ((1 << a.shift) - 1);
-    const int64_t place = isk ? page * a.c.k_sp + h * a.c.k_sh + in_page * a.c.k_sr
-                              : page * a.c.v_sp + h * a.c.v_sh + in_page * a.c.v_sr;
+    const int64_t place = pool_at<BITS>(a.c, page, in_page) + h * a.c.sh;
     if constexpr (BITS == 16) {
       x = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(isk ? a.c.k : a.c.v) + place + f0);
     } else {
-      const int64_t sp = isk ? page * a.c.ks_sp + h * a.c.ks_sh + in_page * a.c.ks_sr
-                             : page * a.c.vs_sp + h * a.c.vs_sh + in_page * a.c.vs_sr;
+      const int64_t sp = scale_at(a.c, page, in_page) + h * a.c.ssh;
       const uint32_t codes =
           *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(isk ? a.c.k : a.c.v) + place + f0 / 2);
       x = fp4_row8<T>(codes, e8m0(static_cast<const uint8_t*>(isk ? a.c.k_scale : a.c.v_scale)[sp + f0 / 32]));

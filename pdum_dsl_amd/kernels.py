@@ -788,7 +788,7 @@ class PagedCache:
     table names, wherever those are in the pool.
 
     16 bits: ``k`` and ``v`` are [pages, heads, page_rows, features], bf16 or
-    f16, any strides that are multiples of 8 elements, features contiguous.
+    f16, any strides, equal in both, that are multiples of 8 elements, features contiguous.
     4 bits: ``k`` and ``v`` are uint8 [pages, heads, page_rows, features / 2]
     (strides multiples of 16) and ``k_scale`` / ``v_scale`` uint8 [pages,
     heads, page_rows, features / 32]: e2m1 codes, the even feature in the low
@@ -824,21 +824,24 @@ class PagedCache:
         if (bits == 4) != (ks is not None) or (bits == 4) != (vs is not None):
             raise ValueError("PagedCache: a 4-bit cache has k_scale and v_scale, a 16-bit one neither")
 
-        def apart(t):  # the strides of pages, heads and rows; those of a single one count for nothing
-            return [st if n > 1 else 0 for st, n in zip(t.stride()[:3], t.shape[:3])]
+        def apart(nm, x, y):  # the strides of pages, heads and rows; those of a single one count for nothing
+            st, other = ([n_st if n > 1 else 0 for n_st, n in zip(t.stride()[:3], x.shape)] for t in (x, y))
+            if st != other:
+                raise ValueError(f"PagedCache: {nm} must have the same strides (got {x.stride()}, {y.stride()})")
+            return st
 
-        scales = [0] * 6
+        scales = [0] * 3
         if bits == 4:
             want = (pages, heads, rows, d // 32)
             for nm, t in (("k_scale", ks), ("v_scale", vs)):
                 if t.dtype != torch.uint8 or tuple(t.shape) != want or t.stride(3) != 1:
                     raise ValueError(f"PagedCache: {nm} must be uint8 {want} with contiguous groups")
-            scales = apart(ks) + apart(vs)
+            scales = apart("k_scale and v_scale", ks, vs)
         devices = {t.device for t in (k, v, ks, vs) if t is not None}
         if len(devices) != 1:
             raise ValueError("PagedCache: the tensors must be on one device")
-        return _lib.PagedCacheC(_ptr(k), _ptr(v), _ptr(ks), _ptr(vs), pages, heads, rows, d, *apart(k), *apart(v),
-                                *scales, _DT[dtype], bits)
+        return _lib.PagedCacheC(_ptr(k), _ptr(v), _ptr(ks), _ptr(vs), pages, heads, rows, d,
+                                *apart("k and v", k, v), *scales, _DT[dtype], bits)
 
     @functools.cached_property
     def _call(self):

@@ -392,13 +392,12 @@ def test_pools_of_any_strides(K, new):
 
 
 def test_pages_past_32_bits(K):
-    """Pages of a pool over 2^32 bytes apart, and keys whose place in it passes 2^31 elements."""
+    """Pages whose place in the pool passes 2^32 bytes."""
     pr, d, hkv, hq = 16, 64, 1, 4
-    far = (1 << 32) // 2 // 4 + 8 * 1024  # elements from page to page: the pool spans 4 of these, over 8 GB
-    store = torch.zeros(far * 4 + pr * d, dtype=torch.bfloat16, device="cuda")
+    far = (1 << 32) // 2 // 4 + 8 * 1024  # elements from page to page: a pool spans 4 of these, over 4 GB
     rng = np.random.default_rng(10)
-    k = store.as_strided((5, hkv, pr, d), (far, pr * d, d, 1))
-    v = torch.zeros_like(k)
+    k, v = (torch.zeros(far * 4 + pr * d, dtype=torch.bfloat16, device="cuda").as_strided((5, hkv, pr, d), (far, pr * d, d, 1))
+            for _ in range(2))
     cache = K.PagedCache(k, v)
     lengths, new = [70, 33], [1, 33]
     table = np.array([[4, 0, 3, 1, 2], [2, 4, 1, 0, 3]], dtype=np.int32)[:, :5]

@@ -63,8 +63,7 @@ FAKE = 256  # a pointer that is never dereferenced: every call below is refused 
 def _structs(cache=None, batch=None):
     from pdum_dsl_amd import _lib
 
-    c = _lib.PagedCacheC(FAKE, FAKE, None, None, 4, 2, 16, 64, 2048, 1024, 64, 2048, 1024, 64, 0, 0, 0, 0, 0, 0,
-                         _lib.PDH_BF16, 16)
+    c = _lib.PagedCacheC(FAKE, FAKE, None, None, 4, 2, 16, 64, 2048, 1024, 64, 0, 0, 0, _lib.PDH_BF16, 16)
     b = _lib.PagedBatch(FAKE, FAKE, FAKE, 3, 5, 4, 4)
     for st, changes in ((c, cache), (b, batch)):
         for n, v in (changes or {}).items():
@@ -73,7 +72,7 @@ def _structs(cache=None, batch=None):
 
 
 def _four_bits(**kw):
-    return dict(bits=4, k_scale=FAKE, v_scale=FAKE, ks_sr=2, vs_sr=2, k_sr=32, v_sr=32, **kw)
+    return dict(bits=4, k_scale=FAKE, v_scale=FAKE, ssr=2, sr=32, **kw)
 
 
 def _calls(c, b):
@@ -98,14 +97,16 @@ def _calls(c, b):
     (dict(heads=0), None, "number of pages or heads", "E"),
     (dict(k=None), None, "pools", "E"),
     (dict(v=FAKE + 8), None, "16-byte aligned", "E"),
-    (dict(k_sp=-8), None, "strides", "E"),
-    (dict(v_sh=1028), None, "multiples of 16 bytes", "E"),
-    (dict(k_sr=56), None, "rows overlap", "E"),
-    (dict(v_sr=1 << 16), None, "2^16", "E"),
-    (_four_bits(k_sp=8), None, "multiples of 16 bytes", "E"),
+    (dict(sp=-8), None, "strides", "E"),
+    (dict(sh=1028), None, "multiples of 16 bytes", "E"),
+    (dict(sr=56), None, "rows overlap", "E"),
+    (dict(sr=1 << 16), None, "2^16", "E"),
+    (_four_bits(sp=8), None, "multiples of 16 bytes", "E"),
     (dict(_four_bits(), k_scale=None), None, "needs its scales", "E"),
-    (dict(_four_bits(), vs_sr=1), None, "scales' rows", "E"),
-    (dict(_four_bits(), ks_sp=-1), None, "scales' strides", "E"),
+    (dict(_four_bits(), ssr=1), None, "scales' rows", "E"),
+    (dict(sp=1 << 34), None, "2^35 bytes", "E"),
+    (_four_bits(ssp=1 << 31), None, "2^31 bytes", "E"),
+    (dict(_four_bits(), ssp=-1), None, "scales' strides", "E"),
     (None, dict(rows=1 << 24), "rows", "E"),
     (None, dict(rows=-1), "rows", "E"),
     (None, dict(seqs=(1 << 20) + 1), "sequences", "E"),
@@ -171,6 +172,7 @@ def test_wrapper_refusals():
         (K.PagedCache(z(2, 2, 16, 64), z(2, 1, 16, 64)), "page_rows, features"),
         (K.PagedCache(z(0, 2, 16, 64), z(0, 2, 16, 64)), "not empty"),
         (K.PagedCache(z(2, 2, 64, 16).transpose(2, 3), z(2, 2, 16, 64)), "contiguous"),
+        (K.PagedCache(z(2, 2, 16, 64), z(2, 16, 2, 64).transpose(1, 2)), "same strides"),
         (K.PagedCache(z(2, 2, 16, 32, dt=u8), z(2, 2, 16, 32, dt=u8)), "k_scale and v_scale"),
         (K.PagedCache(z(2, 2, 16, 64), z(2, 2, 16, 64), z(2, 2, 16, 2, dt=u8), None), "k_scale and v_scale"),
         (K.PagedCache(z(2, 2, 16, 32, dt=u8), z(2, 2, 16, 32, dt=u8), z(2, 2, 16, 1, dt=u8), z(2, 2, 16, 2, dt=u8)),
