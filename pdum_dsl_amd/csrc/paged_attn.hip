@@ -27,6 +27,13 @@ struct PagedAttn {
   int shift, zero_rest;
   int reach;  // keys that the table has pages for
   float c2;   // scale * log2(e)
+  // The page of an entry is read without a branch, entries past the table's as its last (their keys are past reach and
+  // seen by no row), and looked at only when it is needed, so that the load is not waited for before.
+  const int32_t* table;  // some memory where the table has no entry
+  int last_entry, pages;
+  __device__ __forceinline__ bool has(int page) const {
+    return static_cast<uint32_t>(page) < static_cast<uint32_t>(pages);
+  }
 };
 
 // One row by one wave: keys 64 at a time, one a lane; the online softmax's maximum and sum are the wave's, o's features lie
@@ -154,6 +161,7 @@ struct DecCfg {
   static constexpr int RS = 2 + D;  // floats of a row's state: m, l, o
   static constexpr int RED = 4 * 16 * RS * 4;
   static constexpr int LDS = 4 * VTILE > RED ? 4 * VTILE : RED;
+  static constexpr int NB = 2;  // blocks of keys in registers: one computed, the others in flight
   // The unit of work is a block of keys. An item costs ITEM more, so that the short ones of a batch of many are not all one
   // workgroup's; a share is at least LEAST.
   static constexpr int ITEM = 4, LEAST = 8;
@@ -173,6 +181,25 @@ struct DecBlk<D, 4> {
   uint32_t ks[2], vs[2];  // scale bytes
 };
 
+// A resource over wave-uniform memory whose address the compiler may hold in vector registers.
+__device__ __forceinline__ rsrc_t uniform_rsrc(const void* base, uint32_t bytes) {
+  const uint64_t u = reinterpret_cast<uintptr_t>(base);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(u));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(u >> 32));
+  return make_rsrc(reinterpret_cast<const void*>(static_cast<uint64_t>(hi) << 32 | lo), __builtin_amdgcn_readfirstlane(bytes));
+}
+
+__device__ __forceinline__ uint32_t bload8(rsrc_t r, uint32_t voff) {
+  return __builtin_amdgcn_raw_buffer_load_b8(r, voff, 0, 0);
+}
+template <int D>
+__device__ __forceinline__ typename DecBlk<D, 4>::codes bload_codes(rsrc_t r, uint32_t voff) {
+  if constexpr (D == 128)
+    return bload128(r, voff, 0);
+  else
+    return bload64(r, voff, 0);
+}
+
 // Device memory that no kernel in flight writes, read through the scalar cache where the address is uniform.
 __device__ __forceinline__ int32_t uniform_i32(const int32_t* p) {
   typedef const __attribute__((address_space(4))) int32_t c_i32;
@@ -187,6 +214,11 @@ struct SeqPlan {
 };
 
 __device__ __forceinline__ int scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+__device__ __forceinline__ int64_t scalar64(int64_t x) {
+  return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(scalar(static_cast<int>(x >> 32)))) << 32 |
+                              static_cast<uint32_t>(scalar(static_cast<int>(x))));
+}
 
 template <int ROWS, int KEYS>
 __device__ __forceinline__ SeqPlan plan_of(const PagedAttn& a, int i) {
@@ -271,7 +303,8 @@ __global__ __launch_bounds__(256, (dec_wgs<D, BITS>())) void paged_decode(PagedA
     before += i < w ? scan[i] : 0;
     total += scan[i];
   }
-  int64_t per = (total + gridDim.x - 1) / gridDim.x;
+  total = scalar64(total);
+  int64_t per = scalar64((total + gridDim.x - 1) / gridDim.x);
   per = per > C::LEAST ? (per + 3) / 4 * 4 : C::LEAST;  // whole rounds of the four waves
   int64_t at = per * blockIdx.x;
   int64_t left = total - at < per ? total - at : per;
@@ -323,46 +356,43 @@ __global__ __launch_bounds__(256, (dec_wgs<D, BITS>())) void paged_decode(PagedA
     }
 
     struct Pages {
-      int p[2];  // of the two halves of a block; -1: none
+      int p[2];  // the entries of a block's two halves, as they stand in the table
     };
-    const int32_t* trow = a.b.table + seq * a.b.ld_table;
+    const int32_t* trow = a.table + seq * a.b.ld_table;
     auto pages = [&](int v) {
-      Pages r;
       const int key0 = scalar(sp.key_block(v) * 32);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int e = scalar((key0 + 16 * h) >> a.shift);
-        const int p = e < a.b.width ? uniform_i32(trow + e) : -1;
-        r.p[h] = scalar(static_cast<uint32_t>(p) < static_cast<uint64_t>(a.c.pages) ? p : -1);
-      }
-      return r;
+      const int e0 = key0 >> a.shift, e1 = (key0 + 16) >> a.shift;
+      return Pages{{uniform_i32(trow + (e0 < a.last_entry ? e0 : a.last_entry)),
+                    uniform_i32(trow + (e1 < a.last_entry ? e1 : a.last_entry))}};
     };
     const char* const kpool = static_cast<const char*>(a.c.k) + head * a.c.sh * ES;
     const char* const vpool = static_cast<const char*>(a.c.v) + head * a.c.sh * ES;
     const char* const kspool = static_cast<const char*>(a.c.k_scale) + head * a.c.ssh;
     const char* const vspool = static_cast<const char*>(a.c.v_scale) + head * a.c.ssh;
-    // A half without a page reads page 0: what it holds is masked.
+    // Through a buffer resource a half and pool: a lane's address is one 32-bit offset. A half without a page reads page 0:
+    // what it holds is masked.
     auto load = [&](int v, const Pages& pg, DecBlk<D, BITS>& r) {
       const int key0 = scalar(sp.key_block(v) * 32);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int p = pg.p[h] < 0 ? 0 : pg.p[h];
+        const int p = a.has(pg.p[h]) ? pg.p[h] : 0;
         const int in = (key0 + 16 * h) & ((1 << a.shift) - 1);
         const int64_t at = pool_at<BITS>(a.c, p, in) * ES;
-        const char *kp = kpool + at, *vp = vpool + at;
+        const uint32_t span = 15 * rst + D * BITS / 8;
+        const rsrc_t kr = uniform_rsrc(kpool + at, span), vr = uniform_rsrc(vpool + at, span);
         if constexpr (BITS == 16) {
 #pragma unroll
-          for (int s = 0; s < KS; ++s) r.k[h * KS + s] = gload<u32x4>(kp, col * rst + g * 16 + s * 64);
+          for (int s = 0; s < KS; ++s) r.k[h * KS + s] = bload128(kr, col * rst + g * 16 + s * 64, 0);
 #pragma unroll
-          for (int j = 0; j < C::VL / 2; ++j)
-            r.v[h * (C::VL / 2) + j] = gload<u32x4>(vp, (j * C::RPI + vrow) * rst + vch * 16);
+          for (int j = 0; j < C::VL / 2; ++j) r.v[h * (C::VL / 2) + j] = bload128(vr, vrow * rst + vch * 16, j * C::RPI * rst);
         } else {
-          typedef typename DecBlk<D, 4>::codes codes;
           const int64_t sat = scale_at(a.c, p, in);
-          r.k[h] = gload<codes>(kp, col * rst + g * (D / 8));
-          r.ks[h] = gload<uint8_t>(kspool + sat, col * srst + g * (D / 4) / 32);
-          r.v[h] = gload<codes>(vp, vrow * rst + vch * (D / 8));
-          r.vs[h] = gload<uint8_t>(vspool + sat, vrow * srst + vch * (D / 4) / 32);
+          const uint32_t sspan = 15 * srst + D / 32;
+          const rsrc_t ksr = uniform_rsrc(kspool + sat, sspan), vsr = uniform_rsrc(vspool + sat, sspan);
+          r.k[h] = bload_codes<D>(kr, col * rst + g * (D / 8));
+          r.ks[h] = bload8(ksr, col * srst + g * (D / 4) / 32);
+          r.v[h] = bload_codes<D>(vr, vrow * rst + vch * (D / 8));
+          r.vs[h] = bload8(vsr, vrow * srst + vch * (D / 4) / 32);
         }
       }
     };
@@ -376,11 +406,11 @@ __global__ __launch_bounds__(256, (dec_wgs<D, BITS>())) void paged_decode(PagedA
       const int key0 = scalar(sp.key_block(v) * 32);
       // every key is seen by every row
       const bool full = (key0 + 31 <= pos_lo) & (key0 + 32 <= a.reach) &
-                        ((key0 > pos_hi - a.window) | (key0 + 31 < a.sinks)) & ((pg.p[0] | pg.p[1]) >= 0);
+                        ((key0 > pos_hi - a.window) | (key0 + 31 < a.sinks)) & a.has(pg.p[0]) & a.has(pg.p[1]);
       if (!full) {  // keys that no row sees: their values count as zero
         const int last = (pos_hi < a.reach ? pos_hi : a.reach - 1) - key0, first = pos_lo - a.window + 1 - key0;
         const int kept = a.sinks - key0;
-        auto gone = [&](int at, int p) { return (p < 0) | (at > last) | ((at >= kept) & (at < first)); };
+        auto gone = [&](int at, int p) { return !a.has(p) | (at > last) | ((at >= kept) & (at < first)); };
         if constexpr (BITS == 16) {
 #pragma unroll
           for (int j = 0; j < C::VL; ++j)
@@ -425,7 +455,7 @@ __global__ __launch_bounds__(256, (dec_wgs<D, BITS>())) void paged_decode(PagedA
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int cc = 16 * (i >> 2) + (i & 3);
-          const int end = pg.p[i >> 2] < 0 ? -1 - kMaxTokens : last;
+          const int end = a.has(pg.p[i >> 2]) ? last : -1 - kMaxTokens;
           const bool seen = (cc <= end) & ((cc >= first) | (cc < kept));
           sc[i >> 2][i & 3] = seen ? sc[i >> 2][i & 3] : -kInf;
         }
@@ -469,23 +499,32 @@ __global__ __launch_bounds__(256, (dec_wgs<D, BITS>())) void paged_decode(PagedA
     if (kb + w < k_end) {
       const int v_last = kb + w + (k_end - 1 - kb - w) / 4 * 4;
       auto bound = [&](int v) { return v < v_last ? v : v_last; };
-      DecBlk<D, BITS> r0, r1;
-      int v = kb + w;
-      Pages p0 = pages(v), p1 = pages(bound(v + 4));
-      load(v, p0, r0);
+      constexpr int NB = C::NB;
+      DecBlk<D, BITS> r[NB];
+      Pages pg[NB], next = pages(kb + w);
+      int v = kb + w, ahead = v;
+      auto fetch = [&](int i) __attribute__((always_inline)) {
+        load(ahead, next, r[i]);
+        pg[i] = next;
+        ahead = bound(ahead + 4);
+        next = pages(ahead);
+      };
+#pragma unroll
+      for (int i = 0; i < NB - 1; ++i) fetch(i);
+      auto step = [&](auto ic) __attribute__((always_inline)) {
+        constexpr int i = decltype(ic)::value;
+        fetch((i + NB - 1) % NB);
+        block(v, pg[i], r[i]);
+        v += 4;
+        return v < k_end;
+      };
       for (;;) {
-        load(bound(v + 4), p1, r1);
-        Pages p2 = pages(bound(v + 8));
-        block(v, p0, r0);
-        v += 4;
-        if (v >= k_end) break;
-        load(bound(v + 4), p2, r0);
-        p0 = pages(bound(v + 8));
-        block(v, p1, r1);
-        p1 = p0;
-        p0 = p2;
-        v += 4;
-        if (v >= k_end) break;
+        if (!step(std::integral_constant<int, 0>{})) break;
+        if (!step(std::integral_constant<int, 1>{})) break;
+        if constexpr (NB > 2)
+          if (!step(std::integral_constant<int, (NB > 2 ? 2 : 0)>{})) break;
+        if constexpr (NB > 3)
+          if (!step(std::integral_constant<int, (NB > 3 ? 3 : 0)>{})) break;
       }
     }
     lsum = sum4g(lsum);
@@ -712,14 +751,6 @@ __device__ __forceinline__ BlockKeys block_keys(const PagedAttn& a, int pos_lo, 
   return b;
 }
 
-// A resource over wave-uniform memory whose address the compiler may hold in vector registers.
-__device__ __forceinline__ rsrc_t uniform_rsrc(const void* base, uint32_t bytes) {
-  const uint64_t u = reinterpret_cast<uintptr_t>(base);
-  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(u));
-  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(u >> 32));
-  return make_rsrc(reinterpret_cast<const void*>(static_cast<uint64_t>(hi) << 32 | lo), __builtin_amdgcn_readfirstlane(bytes));
-}
-
 // The sequence of a slot (seqs: the rows behind the last one; -1: none) and the block's number in it.
 __device__ __forceinline__ int seq_of_slot(const PagedAttn& a, int slot, int& rb) {
   const int lane = threadIdx.x & 63, rows = static_cast<int>(a.b.rows);
@@ -801,23 +832,17 @@ __global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, in
 
   // ---- tiles: the pages of their two halves
   struct Tile {
-    int key0, p[2];
+    int key0, p[2];  // the pages as they stand in the table
   };
-  const int32_t* trow = a.b.table + seq * a.b.ld_table;
+  const int32_t* trow = a.table + seq * a.b.ld_table;
   auto tile_at = [&](int v) {
-    Tile t;
-    t.key0 = scalar(bk.tile(v) * 32);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int e = scalar((t.key0 + 16 * h) >> a.shift);
-      const int p = e < a.b.width ? uniform_i32(trow + e) : -1;
-      t.p[h] = scalar(static_cast<uint32_t>(p) < static_cast<uint64_t>(a.c.pages) ? p : -1);
-    }
-    return t;
+    const int key0 = scalar(bk.tile(v) * 32), e0 = key0 >> a.shift, e1 = (key0 + 16) >> a.shift;
+    return Tile{key0, {uniform_i32(trow + (e0 < a.last_entry ? e0 : a.last_entry)),
+                       uniform_i32(trow + (e1 < a.last_entry ? e1 : a.last_entry))}};
   };
   auto gone = [&](const Tile& t, int at, int p) {  // no row of the block sees the key
     const int key = t.key0 + at;
-    return p < 0 || key > pos_hi || key >= a.reach || (key >= a.sinks && key <= pos_lo - a.window);
+    return !a.has(p) | (key > pos_hi) | (key >= a.reach) | ((key >= a.sinks) & (key <= pos_lo - a.window));
   };
   const int in_mask = (1 << a.shift) - 1;
   bool lost = false;  // a tile that every row should see whole lacks a page
@@ -839,7 +864,7 @@ __global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, in
     for (int i = 0; i < C::NDMA; ++i) {
       const int blk = i * 4 + w, at0 = blk * C::RPK, h = at0 >> 4;  // its rows lie in one half
       const int pg = h ? t.p[1] : t.p[0];
-      const int64_t first = pool_at<16>(a.c, pg < 0 ? 0 : pg, (t.key0 + at0) & in_mask);
+      const int64_t first = pool_at<16>(a.c, a.has(pg) ? pg : 0, (t.key0 + at0) & in_mask);
       const rsrc_t kr = uniform_rsrc(kpool + first, (C::RPK - 1) * grow + C::ROWB);
       const rsrc_t vr = uniform_rsrc(vpool + first, (C::RPK - 1) * grow + C::ROWB);
       uint32_t ok = dk[i], ov = dv[i];
@@ -858,7 +883,7 @@ __global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, in
   const uint8_t* const spool = static_cast<const uint8_t*>(isv ? a.c.v_scale : a.c.k_scale) + head * a.c.ssh + cch * (D / 4) / 32;
   auto fetch4 = [&](const Tile& t, bool cut) {
     const int pg = crow >> 4 ? t.p[1] : t.p[0];
-    const int p = pg < 0 ? 0 : pg, in = (t.key0 + crow) & in_mask;
+    const int p = a.has(pg) ? pg : 0, in = (t.key0 + crow) & in_mask;
     codes = *reinterpret_cast<const codes_t*>(cpool + pool_at<4>(a.c, p, in));
     cscale = e8m0(spool[scale_at(a.c, p, in)]);
     if (cut && gone(t, crow, pg)) {
@@ -931,7 +956,7 @@ __global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, in
         const int kept = a.sinks - kl;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
-          const int end = t.p[kb] < 0 ? -1 - kMaxTokens : last;
+          const int end = a.has(t.p[kb]) ? last : -1 - kMaxTokens;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int cc = 16 * kb + i;
@@ -1041,7 +1066,7 @@ __global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, in
       if constexpr (decltype(cutc)::value) {
         if (cur.key0 <= wpos_hi) tile(buf, cur, cutc);
       } else {
-        lost |= (cur.p[0] | cur.p[1]) < 0;
+        lost |= !(a.has(cur.p[0]) & a.has(cur.p[1]));
         if (busy) tile(buf, cur, cutc);
       }
       if constexpr (BITS == 4)
@@ -1224,7 +1249,10 @@ extern "C" int pdh_paged_attention(const void* q, void* o, float* lse, int64_t h
               static_cast<int>(heads_q), static_cast<int>(heads_q / cache->heads),
               static_cast<int>(window < kMaxTokens ? window : kMaxTokens),
               static_cast<int>(sinks < kMaxTokens ? sinks : kMaxTokens), shift, zero_rest != 0,
-              static_cast<int>(batch->width << shift), scale * kLog2e};
+              static_cast<int>(batch->width << shift), scale * kLog2e,
+              batch->width > 0 ? batch->table : batch->starts, static_cast<int>(batch->width > 0 ? batch->width - 1 : 0),
+              static_cast<int>(cache->pages)};
+  if (batch->width == 0) a.b.ld_table = 0;
   const size_t need = pdh_paged_attention_workspace(cache, batch, heads_q, window, sinks);
   PDH_REQUIRE(ws_bytes >= need && (need == 0 || (ws && aligned16(ws))), PDH_EINVAL,
               "pdh_paged_attention: workspace %zu bytes < required %zu, or not 16-byte aligned", ws_bytes, need);
