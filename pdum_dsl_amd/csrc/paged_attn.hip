@@ -189,15 +189,15 @@ __device__ __forceinline__ rsrc_t uniform_rsrc(const void* base, uint32_t bytes)
   return make_rsrc(reinterpret_cast<const void*>(static_cast<uint64_t>(hi) << 32 | lo), __builtin_amdgcn_readfirstlane(bytes));
 }
 
-__device__ __forceinline__ uint32_t bload8(rsrc_t r, uint32_t voff) {
-  return __builtin_amdgcn_raw_buffer_load_b8(r, voff, 0, 0);
+__device__ __forceinline__ uint32_t bload8(rsrc_t r, uint32_t voff, uint32_t soff) {
+  return __builtin_amdgcn_raw_buffer_load_b8(r, voff, soff, 0);
 }
 template <int D>
-__device__ __forceinline__ typename DecBlk<D, 4>::codes bload_codes(rsrc_t r, uint32_t voff) {
+__device__ __forceinline__ typename DecBlk<D, 4>::codes bload_codes(rsrc_t r, uint32_t voff, uint32_t soff) {
   if constexpr (D == 128)
-    return bload128(r, voff, 0);
+    return bload128(r, voff, soff);
   else
-    return bload64(r, voff, 0);
+    return bload64(r, voff, soff);
 }
 
 // Device memory that no kernel in flight writes, read through the scalar cache where the address is uniform.
@@ -260,7 +260,8 @@ struct DecMeta {
   int last, row0, rows, f0, head, pad;
 };
 
-template <typename T, int D, int BITS>
+// FAR: a pool reaches past 32-bit offsets.
+template <typename T, int D, int BITS, bool FAR>
 __global__ __launch_bounds__(256, (dec_wgs<D, BITS>())) void paged_decode(PagedAttn a, DecMeta* meta, float* ws) {
   using C = DecCfg<D, BITS>;
   constexpr int KS = C::KS, ET = C::ET, RS = C::RS;
@@ -327,11 +328,14 @@ __global__ __launch_bounds__(256, (dec_wgs<D, BITS>())) void paged_decode(PagedA
   DecMeta cut{-1, 0, 0, 0, 0, 0};
 
   unsigned char* vt = dsm + w * C::VTILE;
-  // transposed value reads: lane 4k + c of group g addresses row 4 g + k, features 4 c .. +3 (+ 16 t)
-  const int trb = (4 * g + (col >> 2)) * C::VROW + (col & 3) * 8;
+  // Value rows in LDS: the 16-byte slot of chunk c is c ^ ((row >> 2) & 1), which spreads the 4-bit writes (four chunks of
+  // a row 64 bytes apart) over all banks. Transposed reads: lane 4k + c of group g addresses row 4 g + k, features 4 c .. +3
+  // (+ 16 t).
+  const int trb = (4 * g + (col >> 2)) * C::VROW + ((((col >> 1) & 1) ^ (g & 1)) << 4) + (col & 1) * 8;
   constexpr int ES = BITS == 16 ? 2 : 1;  // bytes of a stride's unit
   const uint32_t rst = static_cast<uint32_t>(a.c.sr) * ES, srst = static_cast<uint32_t>(a.c.ssr);
   const int vrow = BITS == 16 ? lane / C::CPR : lane / 4, vch = BITS == 16 ? lane % C::CPR : lane % 4;
+  const int vflip = (vrow >> 2) & 1;  // of row 16 h + vrow; of j * RPI + vrow together with j * RPI's
 
   while (left > 0) {
     const int rb = scalar(item % sp.nb), head = scalar(item / sp.nb);
@@ -369,33 +373,58 @@ __global__ __launch_bounds__(256, (dec_wgs<D, BITS>())) void paged_decode(PagedA
     const char* const vpool = static_cast<const char*>(a.c.v) + head * a.c.sh * ES;
     const char* const kspool = static_cast<const char*>(a.c.k_scale) + head * a.c.ssh;
     const char* const vspool = static_cast<const char*>(a.c.v_scale) + head * a.c.ssh;
-    // Through a buffer resource a half and pool: a lane's address is one 32-bit offset. A half without a page reads page 0:
-    // what it holds is masked.
+    // Through buffer resources, a lane's address one 32-bit offset: one resource a pool and a page's place as the scalar
+    // offset, or FAR, a resource a page. A half without a page reads page 0: what it holds is masked.
+    const int in_last = (1 << a.shift) - 1;
+    const uint32_t whole_span = (a.pages - 1) * (static_cast<uint32_t>(a.c.sp) * ES) + in_last * rst + D * BITS / 8;
+    const uint32_t whole_sspan = (a.pages - 1) * static_cast<uint32_t>(a.c.ssp) + in_last * srst + D / 32;
+    rsrc_t krs = make_rsrc(kpool, whole_span), vrs = make_rsrc(vpool, whole_span);
+    rsrc_t ksrs = make_rsrc(kspool, whole_sspan), vsrs = make_rsrc(vspool, whole_sspan);
     auto load = [&](int v, const Pages& pg, DecBlk<D, BITS>& r) {
       const int key0 = scalar(sp.key_block(v) * 32);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int p = a.has(pg.p[h]) ? pg.p[h] : 0;
-        const int in = (key0 + 16 * h) & ((1 << a.shift) - 1);
-        const int64_t at = pool_at<BITS>(a.c, p, in) * ES;
-        const uint32_t span = 15 * rst + D * BITS / 8;
-        const rsrc_t kr = uniform_rsrc(kpool + at, span), vr = uniform_rsrc(vpool + at, span);
+        const int in = (key0 + 16 * h) & in_last;
+        uint32_t so = 0, sso = 0;
+        if constexpr (FAR) {
+          const int64_t at = pool_at<BITS>(a.c, p, in) * ES;
+          const uint32_t span = 15 * rst + D * BITS / 8;
+          krs = uniform_rsrc(kpool + at, span);
+          vrs = uniform_rsrc(vpool + at, span);
+          if constexpr (BITS == 4) {
+            const int64_t sat = scale_at(a.c, p, in);
+            const uint32_t sspan = 15 * srst + D / 32;
+            ksrs = uniform_rsrc(kspool + sat, sspan);
+            vsrs = uniform_rsrc(vspool + sat, sspan);
+          }
+        } else {
+          so = p * (static_cast<uint32_t>(a.c.sp) * ES) + in * rst;
+          if constexpr (BITS == 4) sso = p * static_cast<uint32_t>(a.c.ssp) + in * srst;
+        }
         if constexpr (BITS == 16) {
 #pragma unroll
-          for (int s = 0; s < KS; ++s) r.k[h * KS + s] = bload128(kr, col * rst + g * 16 + s * 64, 0);
+          for (int s = 0; s < KS; ++s) r.k[h * KS + s] = bload128(krs, col * rst + g * 16 + s * 64, so);
 #pragma unroll
-          for (int j = 0; j < C::VL / 2; ++j) r.v[h * (C::VL / 2) + j] = bload128(vr, vrow * rst + vch * 16, j * C::RPI * rst);
+          for (int j = 0; j < C::VL / 2; ++j)
+            r.v[h * (C::VL / 2) + j] = bload128(vrs, vrow * rst + vch * 16, so + j * C::RPI * rst);
         } else {
-          const int64_t sat = scale_at(a.c, p, in);
-          const uint32_t sspan = 15 * srst + D / 32;
-          const rsrc_t ksr = uniform_rsrc(kspool + sat, sspan), vsr = uniform_rsrc(vspool + sat, sspan);
-          r.k[h] = bload_codes<D>(kr, col * rst + g * (D / 8));
-          r.ks[h] = bload8(ksr, col * srst + g * (D / 4) / 32);
-          r.v[h] = bload_codes<D>(vr, vrow * rst + vch * (D / 8));
-          r.vs[h] = bload8(vsr, vrow * srst + vch * (D / 4) / 32);
+          r.k[h] = bload_codes<D>(krs, col * rst + g * (D / 8), so);
+          r.ks[h] = bload8(ksrs, col * srst + g * (D / 4) / 32, sso);
+          r.v[h] = bload_codes<D>(vrs, vrow * rst + vch * (D / 8), so);
+          r.vs[h] = bload8(vsrs, vrow * srst + vch * (D / 4) / 32, sso);
         }
       }
     };
+
+    // blocks [c0, c1) are seen whole by every row, as far as their pages are there
+    int c0, c1;
+    {
+      const int edge = pos_hi - a.window + 1;
+      const int first = edge > 0 ? (edge + 31) / 32 : 0, last = (pos_lo + 1 < a.reach ? pos_lo + 1 : a.reach) >> 5;
+      c0 = sp.sb + (first > sp.wb ? first - sp.wb : 0);
+      c1 = sp.sb + (last > sp.wb ? last - sp.wb : 0);
+    }
 
     float m = -kInf, lsum = 0.f;  // the raw scores' reference, this lane's part of the sum
     f32x4 o[ET];
@@ -404,9 +433,7 @@ __global__ __launch_bounds__(256, (dec_wgs<D, BITS>())) void paged_decode(PagedA
 
     auto block = [&](int v, const Pages& pg, DecBlk<D, BITS>& r) __attribute__((always_inline)) {
       const int key0 = scalar(sp.key_block(v) * 32);
-      // every key is seen by every row
-      const bool full = (key0 + 31 <= pos_lo) & (key0 + 32 <= a.reach) &
-                        ((key0 > pos_hi - a.window) | (key0 + 31 < a.sinks)) & a.has(pg.p[0]) & a.has(pg.p[1]);
+      const bool full = (v >= c0) & (v < c1) & a.has(pg.p[0]) & a.has(pg.p[1]);  // every row sees every key
       if (!full) {  // keys that no row sees: their values count as zero
         const int last = (pos_hi < a.reach ? pos_hi : a.reach - 1) - key0, first = pos_lo - a.window + 1 - key0;
         const int kept = a.sinks - key0;
@@ -427,13 +454,14 @@ __global__ __launch_bounds__(256, (dec_wgs<D, BITS>())) void paged_decode(PagedA
       // values -> this wave's tile, rows of keys
       if constexpr (BITS == 16) {
 #pragma unroll
-        for (int j = 0; j < C::VL; ++j) *reinterpret_cast<u32x4*>(vt + (j * C::RPI + vrow) * C::VROW + vch * 16) = r.v[j];
+        for (int j = 0; j < C::VL; ++j)
+          *reinterpret_cast<u32x4*>(vt + (j * C::RPI + vrow) * C::VROW + ((vch ^ vflip ^ (j * C::RPI >> 2 & 1)) << 4)) = r.v[j];
       } else {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int i = 0; i < KS; ++i)
-            *reinterpret_cast<u32x4*>(vt + (16 * h + vrow) * C::VROW + vch * (D / 2) + i * 16) =
+            *reinterpret_cast<u32x4*>(vt + (16 * h + vrow) * C::VROW + vch * (D / 2) + ((i ^ vflip) << 4)) =
                 fp4_row8<T>(r.v[h][i], e8m0(r.vs[h]));
       }
       // S^T: keys key0 + 16 h + 4 g + i (accumulator i), row col
@@ -511,20 +539,15 @@ __global__ __launch_bounds__(256, (dec_wgs<D, BITS>())) void paged_decode(PagedA
       };
 #pragma unroll
       for (int i = 0; i < NB - 1; ++i) fetch(i);
-      auto step = [&](auto ic) __attribute__((always_inline)) {
-        constexpr int i = decltype(ic)::value;
-        fetch((i + NB - 1) % NB);
-        block(v, pg[i], r[i]);
-        v += 4;
-        return v < k_end;
-      };
-      for (;;) {
-        if (!step(std::integral_constant<int, 0>{})) break;
-        if (!step(std::integral_constant<int, 1>{})) break;
-        if constexpr (NB > 2)
-          if (!step(std::integral_constant<int, (NB > 2 ? 2 : 0)>{})) break;
-        if constexpr (NB > 3)
-          if (!step(std::integral_constant<int, (NB > 3 ? 3 : 0)>{})) break;
+      // (not left in the middle of a round: the accumulators would be held twice)
+#pragma unroll 1
+      for (; v < k_end; v += 4 * NB) {
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+          if (i == 0 || v + 4 * i < k_end) {
+            fetch((i + NB - 1) % NB);
+            block(v + 4 * i, pg[i], r[i]);
+          }
       }
     }
     lsum = sum4g(lsum);
@@ -1263,7 +1286,14 @@ extern "C" int pdh_paged_attention(const void* q, void* o, float* lse, int64_t h
     by_kind(*cache, [&](auto t, auto d, auto bits) {
       using T = decltype(t);
       constexpr int D = decltype(d)::value;
-      paged_decode<T, D, decltype(bits)::value><<<n, 256, 0, as_stream(stream)>>>(a, meta, states);
+      constexpr int B = decltype(bits)::value;
+      // what a 32-bit offset from a head's first row has to reach, in bytes
+      const int64_t pool = ((cache->pages - 1) * cache->sp + cache->page_rows * cache->sr) * (B == 16 ? 2 : 1);
+      const int64_t scales = B == 4 ? (cache->pages - 1) * cache->ssp + cache->page_rows * cache->ssr : 0;
+      if (pool < (int64_t{1} << 32) && scales < (int64_t{1} << 32))
+        paged_decode<T, D, B, false><<<n, 256, 0, as_stream(stream)>>>(a, meta, states);
+      else
+        paged_decode<T, D, B, true><<<n, 256, 0, as_stream(stream)>>>(a, meta, states);
       paged_decode_merge<T, D><<<n, 1024, 0, as_stream(stream)>>>(a, meta, states);
     });
     return check_launch("pdh_paged_attention (decode)");
