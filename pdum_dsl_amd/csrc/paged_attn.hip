@@ -260,7 +260,7 @@ struct DecMeta {
   int last, row0, rows, f0, head, pad;
 };
 
-// FAR: a pool reaches past 32-bit offsets.
+// FAR: a pool reaches past the offsets of one buffer resource (2^31 bytes).
 template <typename T, int D, int BITS, bool FAR>
 __global__ __launch_bounds__(256, (dec_wgs<D, BITS>())) void paged_decode(PagedAttn a, DecMeta* meta, float* ws) {
   using C = DecCfg<D, BITS>;
@@ -804,7 +804,7 @@ struct Parts {
   }
 };
 
-template <typename T, int D, int BITS>
+template <typename T, int D, int BITS, bool FAR>
 __global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, int nslots) {
   using C = ProCfg<D>;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[C::LDS];
@@ -870,53 +870,74 @@ __global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, in
   const int in_mask = (1 << a.shift) - 1;
   bool lost = false;  // a tile that every row should see whole lacks a page
 
-  // ---- staging, 16 bits
-  const uint32_t grow = static_cast<uint32_t>(a.c.sr) * 2;
+  // ---- staging. A wave's part of a tile lies in one half, in one page: one buffer resource a pool with the page's place as
+  // the scalar offset, or FAR, a resource a page; a lane's address is one offset that does not change.
+  constexpr int ES = BITS == 16 ? 2 : 1;
+  const uint32_t rst = static_cast<uint32_t>(a.c.sr) * ES, srst = static_cast<uint32_t>(a.c.ssr);
+  const uint32_t whole_span = (a.pages - 1) * (static_cast<uint32_t>(a.c.sp) * ES) + in_mask * rst + D * BITS / 8;
+  auto page_place = [&](int pg, int in, const char* pool, rsrc_t& r) {  // units of bytes
+    if constexpr (FAR) {
+      r = uniform_rsrc(pool + pool_at<BITS>(a.c, a.has(pg) ? pg : 0, in) * ES, 15 * rst + D * BITS / 8);
+      return 0u;
+    } else {
+      return static_cast<uint32_t>(scalar((a.has(pg) ? pg : 0) * (static_cast<uint32_t>(a.c.sp) * ES) + in * rst));
+    }
+  };
+  // 16 bits
+  const char* const kpool = static_cast<const char*>(a.c.k) + head * a.c.sh * ES;
+  const char* const vpool = static_cast<const char*>(a.c.v) + head * a.c.sh * ES;
+  rsrc_t krs = uniform_rsrc(kpool, whole_span), vrs = uniform_rsrc(vpool, whole_span);
   const int lrow = lane / C::CPR, slot = lane % C::CPR;
-  const uint16_t* const kpool = static_cast<const uint16_t*>(a.c.k) + head * a.c.sh;
-  const uint16_t* const vpool = static_cast<const uint16_t*>(a.c.v) + head * a.c.sh;
   uint32_t dk[C::NDMA], dv[C::NDMA];
 #pragma unroll
   for (int i = 0; i < C::NDMA; ++i) {
     const int at = (i * 4 + w) * C::RPK + lrow;
-    dk[i] = lrow * grow + ((slot ^ swz16_k<D>(at)) << 4);
-    dv[i] = lrow * grow + ((slot ^ swz16_v<D>(at)) << 4);
+    dk[i] = lrow * rst + ((slot ^ swz16_k<D>(at)) << 4);
+    dv[i] = lrow * rst + ((slot ^ swz16_v<D>(at)) << 4);
   }
   auto stage16 = [&](const Tile& t, int buf, bool cut) {
 #pragma unroll
     for (int i = 0; i < C::NDMA; ++i) {
       const int blk = i * 4 + w, at0 = blk * C::RPK, h = at0 >> 4;  // its rows lie in one half
-      const int pg = h ? t.p[1] : t.p[0];
-      const int64_t first = pool_at<16>(a.c, a.has(pg) ? pg : 0, (t.key0 + at0) & in_mask);
-      const rsrc_t kr = uniform_rsrc(kpool + first, (C::RPK - 1) * grow + C::ROWB);
-      const rsrc_t vr = uniform_rsrc(vpool + first, (C::RPK - 1) * grow + C::ROWB);
+      const int pg = h ? t.p[1] : t.p[0], in = (t.key0 + at0) & in_mask;
+      const uint32_t so = page_place(pg, in, kpool, krs);
+      if constexpr (FAR) page_place(pg, in, vpool, vrs);
       uint32_t ok = dk[i], ov = dv[i];
       if (cut && gone(t, at0 + lrow, pg)) ok = ov = 0x7ffffff0u;  // past the resource: zeros
-      dma16(kr, smem + C::KBUF + buf * C::TILEB + blk * 1024, ok, 0);
-      dma16(vr, smem + C::VBUF + buf * C::TILEB + blk * 1024, ov, 0);
+      dma16(krs, smem + C::KBUF + buf * C::TILEB + blk * 1024, ok, so);
+      dma16(vrs, smem + C::VBUF + buf * C::TILEB + blk * 1024, ov, so);
     }
   };
-  // ---- staging, 4 bits: thread -> K (waves 0, 1) or V (2, 3), row, chunk of D / 4 features
+  // 4 bits: waves 0 and 1 take K's halves, 2 and 3 V's; a lane a row and a chunk of D / 4 features
   typedef typename DecBlk<D, 4>::codes codes_t;
   codes_t codes{};
-  float cscale = 0.f;
+  uint32_t cbyte = 0;
   const bool isv = w >= 2;
-  const int crow = (tid & 127) >> 2, cch = tid & 3;
-  const char* const cpool = static_cast<const char*>(isv ? a.c.v : a.c.k) + head * a.c.sh + cch * (D / 8);
-  const uint8_t* const spool = static_cast<const uint8_t*>(isv ? a.c.v_scale : a.c.k_scale) + head * a.c.ssh + cch * (D / 4) / 32;
+  const int crow = 16 * (w & 1) + (lane >> 2), cch = lane & 3;
+  const char* const cpool = isv ? vpool : kpool;
+  const char* const spool = static_cast<const char*>(isv ? a.c.v_scale : a.c.k_scale) + head * a.c.ssh;
+  rsrc_t crs = uniform_rsrc(cpool, whole_span);
+  rsrc_t srs = uniform_rsrc(spool, (a.pages - 1) * static_cast<uint32_t>(a.c.ssp) + in_mask * srst + D / 32);
+  const uint32_t coff = (lane >> 2) * rst + cch * (D / 8), soff = (lane >> 2) * srst + cch * (D / 4) / 32;
   auto fetch4 = [&](const Tile& t, bool cut) {
-    const int pg = crow >> 4 ? t.p[1] : t.p[0];
-    const int p = a.has(pg) ? pg : 0, in = (t.key0 + crow) & in_mask;
-    codes = *reinterpret_cast<const codes_t*>(cpool + pool_at<4>(a.c, p, in));
-    cscale = e8m0(spool[scale_at(a.c, p, in)]);
+    const int pg = (w & 1) ? t.p[1] : t.p[0], in = (t.key0 + 16 * (w & 1)) & in_mask;
+    const uint32_t so = page_place(pg, in, cpool, crs);
+    uint32_t sso = 0;
+    if constexpr (FAR)
+      srs = uniform_rsrc(spool + scale_at(a.c, a.has(pg) ? pg : 0, in), 15 * srst + D / 32);
+    else
+      sso = scalar((a.has(pg) ? pg : 0) * static_cast<uint32_t>(a.c.ssp) + in * srst);
+    codes = bload_codes<D>(crs, coff, so);
+    cbyte = bload8(srs, soff, sso);
     if (cut && gone(t, crow, pg)) {
       codes = codes_t{};
-      cscale = 0.f;
+      cbyte = 0;
     }
   };
   auto commit4 = [&](int buf) {
     unsigned char* dst = smem + (isv ? C::VBUF : C::KBUF) + buf * C::TILEB + crow * C::ROWB;
     const int swz = isv ? swz16_v<D>(crow) : swz16_k<D>(crow);
+    const float cscale = e8m0(cbyte);
 #pragma unroll
     for (int i = 0; i < C::KS; ++i)
       *reinterpret_cast<u32x4*>(dst + (((cch * C::KS + i) ^ swz) << 4)) = fp4_row8<T>(codes[i], cscale);
@@ -1279,6 +1300,11 @@ extern "C" int pdh_paged_attention(const void* q, void* o, float* lse, int64_t h
   const size_t need = pdh_paged_attention_workspace(cache, batch, heads_q, window, sinks);
   PDH_REQUIRE(ws_bytes >= need && (need == 0 || (ws && aligned16(ws))), PDH_EINVAL,
               "pdh_paged_attention: workspace %zu bytes < required %zu, or not 16-byte aligned", ws_bytes, need);
+  // what an offset from a head's first row has to reach, in bytes; to 2^31, so that 0x7ffffff0 lies past every resource and
+  // no sum of two offsets wraps
+  const int64_t pool = ((cache->pages - 1) * cache->sp + cache->page_rows * cache->sr) * (cache->bits == 16 ? 2 : 1);
+  const int64_t scales = cache->bits == 4 ? (cache->pages - 1) * cache->ssp + cache->page_rows * cache->ssr : 0;
+  const bool far = pool >= 0x7fff0000 || scales >= 0x7fff0000;
   if (few_rows(*batch, a.group)) {
     const unsigned n = static_cast<unsigned>(decode_grid(*cache));
     DecMeta* meta = static_cast<DecMeta*>(ws);
@@ -1287,10 +1313,7 @@ extern "C" int pdh_paged_attention(const void* q, void* o, float* lse, int64_t h
       using T = decltype(t);
       constexpr int D = decltype(d)::value;
       constexpr int B = decltype(bits)::value;
-      // what a 32-bit offset from a head's first row has to reach, in bytes
-      const int64_t pool = ((cache->pages - 1) * cache->sp + cache->page_rows * cache->sr) * (B == 16 ? 2 : 1);
-      const int64_t scales = B == 4 ? (cache->pages - 1) * cache->ssp + cache->page_rows * cache->ssr : 0;
-      if (pool < (int64_t{1} << 32) && scales < (int64_t{1} << 32))
+      if (!far)
         paged_decode<T, D, B, false><<<n, 256, 0, as_stream(stream)>>>(a, meta, states);
       else
         paged_decode<T, D, B, true><<<n, 256, 0, as_stream(stream)>>>(a, meta, states);
@@ -1306,8 +1329,12 @@ extern "C" int pdh_paged_attention(const void* q, void* o, float* lse, int64_t h
   by_kind(*cache, [&](auto t, auto d, auto bits) {
     using T = decltype(t);
     constexpr int D = decltype(d)::value;
-    paged_prompt<T, D, decltype(bits)::value>
-        <<<static_cast<unsigned>(blocks), 256, 0, as_stream(stream)>>>(a, parts, static_cast<int>(nslots));
+    constexpr int B = decltype(bits)::value;
+    const unsigned n = static_cast<unsigned>(blocks);
+    if (!far)
+      paged_prompt<T, D, B, false><<<n, 256, 0, as_stream(stream)>>>(a, parts, static_cast<int>(nslots));
+    else
+      paged_prompt<T, D, B, true><<<n, 256, 0, as_stream(stream)>>>(a, parts, static_cast<int>(nslots));
     if (nsplit > 1) {
       const dim3 grid(static_cast<unsigned>(batch->rows), static_cast<unsigned>((heads_q + 3) / 4));
       paged_prompt_merge<T, D><<<grid, 256, 0, as_stream(stream)>>>(a, parts);
