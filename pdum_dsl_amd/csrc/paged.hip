@@ -58,15 +58,13 @@ __device__ __forceinline__ uint32_t fp4_codes(const float (&y)[8], uint32_t& byt
   e = e < 1 ? 1 : (e < kMost ? e : kMost);
   const bool finite = top < 0x7f800000u;
   byte = finite ? e : 255;
-  const float inv = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+  // v_cvt_scalef32_pk_fp4_f32: two values over 2^(e - 127) to the nearest codes, ties to even ones, past 6 to 6
+  const float scale = e8m0(e);
   uint32_t codes = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {  // ties go to the even code
-    const float a = __builtin_fabsf(y[i]) * inv;
-    uint32_t c = (a > 0.25f) + (a >= 0.75f) + (a > 1.25f) + (a >= 1.75f) + (a > 2.5f) + (a >= 3.5f) + (a > 5.0f);
-    c |= (__float_as_uint(y[i]) >> 31) << 3;
-    codes |= c << (4 * i);
-  }
+  codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, y[0], y[1], scale, 0);
+  codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, y[2], y[3], scale, 1);
+  codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, y[4], y[5], scale, 2);
+  codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, y[6], y[7], scale, 3);
   return codes;
 }
 

@@ -9,6 +9,7 @@
 #include "attn_common.h"
 #include "paged.h"
 
+#include <atomic>
 #include <cmath>
 namespace pdh {
 namespace {
@@ -732,7 +733,7 @@ __global__ __launch_bounds__(1024) void paged_decode_merge(PagedAttn a, const De
 // XCD works through whole heads, whose keys its L2 holds. A grid too small for the chip cuts each block's tiles into parts
 // that paged_prompt_merge joins.
 
-template <int D>
+template <int D, int BITS>
 struct ProCfg {
   static constexpr int BM = 128, BN = 32;
   static constexpr int ROWB = D * 2;
@@ -744,8 +745,10 @@ struct ProCfg {
   static constexpr int NDMA = BN / RPK / 4;  // loads of K, and of V, a wave and tile
   static constexpr int KS = D / 32;
   static constexpr int FB = D / 16;
-  static constexpr int PF = 2;   // V operands in flight ahead of their product
-  static constexpr int KPF = 3;  // K operands in flight
+  static constexpr int PF = 1;  // V operands in flight ahead of their product
+  // K operands in flight: as many as the registers hold without spills (4 bits, D = 128: the codes take theirs). 2 x 4096
+  // tokens, 32/8 heads of 128: 256 us, with two and three 258; 4 bits 272, with one and three 290, two and three 295
+  static constexpr int KPF = BITS == 4 && D == 128 ? 1 : 2;
 };
 
 constexpr float kTau = 8.0f;    // log2 of the growth of a row's maximum that is let pass
@@ -806,7 +809,7 @@ struct Parts {
 
 template <typename T, int D, int BITS, bool FAR>
 __global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, int nslots) {
-  using C = ProCfg<D>;
+  using C = ProCfg<D, BITS>;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[C::LDS];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, G = lane >> 4, w = wave_id();
   const int R = a.group;
@@ -1201,31 +1204,35 @@ __global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, in
   }
 }
 
-// Joins the parts of blocks that were cut: a wave a row and query head.
+// Joins the parts of blocks that were cut: a workgroup a row and eight query heads, a wave two of them.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void paged_prompt_merge(PagedAttn a, Parts pt) {
-  const int lane = threadIdx.x & 63, row = blockIdx.x, h = blockIdx.y * 4 + wave_id();
+  const int lane = threadIdx.x & 63, row = blockIdx.x;
   const int seq = seq_of_row(a.b, row);
-  if (h >= a.heads_q || seq >= a.b.seqs) return;
-  const SeqPlan sp = plan_of<128, 32>(a, seq);
+  if (seq >= a.b.seqs) return;
+  const SeqPlan sp = uniform_plan<128, 32>(a, seq);
   if (row < sp.row0 || row >= sp.row0 + sp.n) return;
-  const int f0 = static_cast<int>(((row - sp.row0) * static_cast<int64_t>(a.group) + h % a.group) / 128 * 128);
-  const int64_t nrow = static_cast<int64_t>(sp.n) * a.group;
-  const int fend = nrow < f0 + 128 ? static_cast<int>(nrow) : f0 + 128;
-  const BlockKeys bk = block_keys(a, sp.pos0 + f0 / a.group, sp.pos0 + (fend - 1) / a.group, pt.nsplit);
-  if (bk.parts <= 1) return;
-  const int64_t at = static_cast<int64_t>(row) * a.heads_q + h;
-  float mm = -kInf, l = 0.f, o[D / 64] = {};
-  for (int s = 0; s < bk.parts; ++s) mm = fmaxf(mm, pt.ml<D>(s, at)[0]);
+  const int R = a.group;
+  const int h_end = blockIdx.y * 8 + 8 < a.heads_q ? blockIdx.y * 8 + 8 : a.heads_q;
+  for (int h = blockIdx.y * 8 + wave_id(); h < h_end; h += 4) {
+    const int f0 = ((row - sp.row0) * R + h % R) / 128 * 128;
+    const int fend = sp.n * R - f0 < 128 ? sp.n * R : f0 + 128;
+    const BlockKeys bk = block_keys(a, scalar(sp.pos0 + f0 / R), scalar(sp.pos0 + (fend - 1) / R), pt.nsplit);
+    if (bk.parts <= 1) continue;
+    const int64_t at = static_cast<int64_t>(row) * a.heads_q + h;
+    float mm = -kInf, l = 0.f, o[D / 64] = {};
 #pragma unroll 4
-  for (int s = 0; s < bk.parts; ++s) {
-    const float* ml = pt.ml<D>(s, at);
-    const float f = ml[0] == -kInf ? 0.f : fast_exp2(ml[0] - mm);
-    l += f * ml[1];
+    for (int s = 0; s < bk.parts; ++s) {
+      const float* ml = pt.ml<D>(s, at);
+      const float mnew = fmaxf(mm, ml[0]);
+      const float was = mm == -kInf ? 0.f : fast_exp2(mm - mnew), f = ml[0] == -kInf ? 0.f : fast_exp2(ml[0] - mnew);
+      l = l * was + f * ml[1];
 #pragma unroll
-    for (int j = 0; j < D / 64; ++j) o[j] += f * pt.o<D>(s, at)[lane + 64 * j];
+      for (int j = 0; j < D / 64; ++j) o[j] = o[j] * was + f * pt.o<D>(s, at)[lane + 64 * j];
+      mm = mnew;
+    }
+    write_row<T, D>(a, row, h, mm, l, o);
   }
-  write_row<T, D>(a, row, h, mm, l, o);
 }
 
 }  // namespace
@@ -1235,14 +1242,27 @@ using namespace pdh;
 
 namespace {
 
+// The current device's compute units; asked for once a device (two runtime calls, 1 us, otherwise in every call).
+int64_t compute_units() {
+  static std::atomic<int> known[64];
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+  int n = known[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    n = pdh_device_cus();
+    n = n > 0 ? n : 256;
+    known[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
 // Rows a sequence and head that take the decode kernel: blocks of 16 flattened rows on average.
 bool few_rows(const pdh_paged_batch& b, int64_t group) { return b.rows * group <= 16 * b.seqs; }
 
 // Workgroups of the decode kernel: as many as run at once.
 int decode_grid(const pdh_paged_cache& c) {
-  const int cus = pdh_device_cus();
-  return (cus > 0 ? cus : 256) * (c.features == 128 ? (c.bits == 16 ? dec_wgs<128, 16>() : dec_wgs<128, 4>())
-                                                    : (c.bits == 16 ? dec_wgs<64, 16>() : dec_wgs<64, 4>()));
+  return static_cast<int>(compute_units()) * (c.features == 128 ? (c.bits == 16 ? dec_wgs<128, 16>() : dec_wgs<128, 4>())
+                                                                : (c.bits == 16 ? dec_wgs<64, 16>() : dec_wgs<64, 4>()));
 }
 
 // Parts that the prompt kernel cuts a block's keys into: as many as bring the grid nearest to two workgroups a compute unit,
@@ -1251,11 +1271,10 @@ int decode_grid(const pdh_paged_cache& c) {
 // ragged over 7001 230 / 179, 8 x 64 over 8192 235 / 78; a prompt of 1024 tokens 38 / 48 (two parts of 512), of 2048 under a
 // window of 1024 56 / 101 (two parts): those stay whole.
 int prompt_splits(const pdh_paged_cache& c, const pdh_paged_batch& b, int64_t group, int64_t window, int64_t sinks) {
-  const int cus = pdh_device_cus();
   const int64_t blocks = (b.rows * group / 128 + 1) * c.heads;
   int64_t keys = b.width * c.page_rows;
   if (window < keys) keys = keys < window + sinks + 128 ? keys : window + sinks + 128;
-  int64_t n = (4 * (cus > 0 ? cus : 256) + blocks) / (2 * blocks);
+  int64_t n = (4 * compute_units() + blocks) / (2 * blocks);
   n = n < keys / 1024 ? n : keys / 1024;
   return static_cast<int>(n < 1 ? 1 : (n < 32 ? n : 32));
 }
@@ -1336,7 +1355,7 @@ extern "C" int pdh_paged_attention(const void* q, void* o, float* lse, int64_t h
     else
       paged_prompt<T, D, B, true><<<n, 256, 0, as_stream(stream)>>>(a, parts, static_cast<int>(nslots));
     if (nsplit > 1) {
-      const dim3 grid(static_cast<unsigned>(batch->rows), static_cast<unsigned>((heads_q + 3) / 4));
+      const dim3 grid(static_cast<unsigned>(batch->rows), static_cast<unsigned>((heads_q + 7) / 8));
       paged_prompt_merge<T, D><<<grid, 256, 0, as_stream(stream)>>>(a, parts);
     }
   });

@@ -845,10 +845,10 @@ class PagedCache:
 
     @functools.cached_property
     def _call(self):
-        """What a call needs of the cache: the struct, device, value type, heads, features."""
+        """What a call needs of the cache: the struct, device, value type, heads, features, what a workspace goes by."""
         c = self.c
         return (C.byref(c), self.k.get_device(), torch.bfloat16 if c.dtype == PDH_BF16 else torch.float16, c.heads,
-                c.features)
+                c.features, (self.k.get_device(), c.bits, c.features, c.heads, c.page_rows))
 
 
 def paged_cache(pages: int, heads: int, page_rows: int, features: int, dtype: torch.dtype = torch.bfloat16, *,
@@ -949,7 +949,7 @@ def paged_append(
     Rows of no sequence are stored nowhere; their rows of the result are zero,
     or stay as they are in ``out`` (which may be q itself). Two tokens with one
     place leave either of them, or parts of both, there."""
-    cc, _, dtype, heads, d = cache._call
+    cc, _, dtype, heads, d, _ = cache._call
     rows = k.shape[0] if k.dim() == 3 else 0
     b = _paged("paged_append", cache, table, starts, lengths, rows, (k, v, q, rotary, out, bad))
     ks = _tokens("paged_append", "k", k, dtype, heads, d)
@@ -996,7 +996,7 @@ def paged_rows(
     16-bit type, of the tokens that :func:`paged_append` stores for the same
     ``table``, ``starts`` and ``lengths`` (starts that ascend by the lengths:
     everything). Tokens without a place and rows of no sequence are zero."""
-    cc, _, dtype, heads, d = cache._call
+    cc, _, dtype, heads, d, _ = cache._call
     if rows < 0:
         raise ValueError("paged_rows: rows must be >= 0")
     b = _paged("paged_rows", cache, table, starts, lengths, int(rows), ())
@@ -1004,6 +1004,15 @@ def paged_rows(
     v = torch.empty_like(k)
     _lib.call("pdh_paged_rows", k.data_ptr(), v.data_ptr(), heads * d, d, heads * d, d, cc, C.byref(b), 1, _stream())
     return k, v
+
+
+@functools.lru_cache(maxsize=4096)
+def _paged_workspace(cache: tuple, rows: int, seqs: int, width: int, hq: int, window: int, sinks: int) -> int:
+    """pdh_paged_attention_workspace by all that it looks at (of the device, which is the current one, the compute units)."""
+    _, bits, features, heads, page_rows = cache
+    c = _lib.PagedCacheC(bits=bits, features=features, heads=heads, page_rows=page_rows)
+    b = _lib.PagedBatch(rows=rows, seqs=seqs, width=width)
+    return _lib.lib().pdh_paged_attention_workspace(C.byref(c), C.byref(b), hq, window, sinks)
 
 
 def paged_attention(
@@ -1034,7 +1043,7 @@ def paged_attention(
     that sees nothing (or only scores of -inf) has o = 0 and lse = -inf. Rows
     of no sequence likewise; ``out`` (q's shape and type) they leave as it is.
     The 4 bits are exact in the 16-bit type but for f16 under 2^-24."""
-    cc, _, dtype, heads, d = cache._call
+    cc, _, dtype, heads, d, _ = cache._call
     b = _paged("paged_attention", cache, table, starts, lengths, q.shape[0] if q.dim() == 3 else 0, (q, out))
     qs = _tokens("paged_attention", "q", q, dtype, None, d)
     rows, hq = q.shape[:2]
@@ -1050,7 +1059,7 @@ def paged_attention(
     if not zero:
         _written("paged_attention", "out", o)
     lse = q.new_empty((rows, hq), dtype=torch.float32) if want_lse else None
-    need = _lib.lib().pdh_paged_attention_workspace(cc, C.byref(b), hq, window, int(sinks))
+    need = _paged_workspace(cache._call[5], rows, b.seqs, b.width, hq, window, int(sinks))
     ws = q.new_empty((need + 3) // 4, dtype=torch.float32) if need else None
     _lib.call("pdh_paged_attention", q.data_ptr(), o.data_ptr(), _ptr(lse), hq, *qs, *os, cc, C.byref(b), window,
               int(sinks), sc, int(zero), _ptr(ws), need, _stream())
