@@ -339,7 +339,7 @@ typedef struct pdh_paged_cache {
 
 /* The sequences of one call, device memory that the kernels read when they
  * run: sequence i's new tokens are rows starts[i] .. starts[i + 1] - 1 (starts
- * ascend) and the last of its lengths[i] tokens: row r has position
+ * ascend from 0) and the last of its lengths[i] tokens: row r has position
  * lengths[i] - (starts[i + 1] - r). Values out of range reach no memory: a
  * row outside [0, rows) is not there, a token before 0, past the table or on a
  * page outside the pool has no place. */

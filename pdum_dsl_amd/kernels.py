@@ -934,8 +934,8 @@ def paged_append(
 
     Sequence i's new tokens are rows starts[i] .. starts[i + 1] - 1 and the
     last of its lengths[i] tokens (these counted), at the places that row i
-    of ``table`` [sequences, pages] names; ``starts`` ascend; all three are int32 on the
-    device, read when the kernel runs. ``rotary`` (:func:`rotary_table`, fp32
+    of ``table`` [sequences, pages] names; ``starts`` ascend from 0; all three
+    are int32 on the device, read when the kernel runs. ``rotary`` (:func:`rotary_table`, fp32
     [positions, rotated], rotated a multiple of 16) turns features i and i +
     rotated / 2, or 2 i and 2 i + 1 where ``interleaved``; the rest stay as
     they are. fp32 arithmetic, rounded once to the cache's type or to its 4
@@ -962,7 +962,7 @@ def paged_append(
             raise ValueError("paged_append: q has no heads")
         zero = out is None
         if zero:
-            out = q.new_empty(q.shape)
+            out = _like(q)
         os = _tokens("paged_append", "out", out, dtype, hq, d, rows)
         if not zero:
             _written("paged_append", "out", out)
@@ -995,7 +995,7 @@ def paged_rows(
     """What the cache holds: keys and values [rows, heads, features], in its
     16-bit type, of the tokens that :func:`paged_append` stores for the same
     ``table``, ``starts`` and ``lengths`` (starts that ascend by the lengths:
-    everything). Tokens without a place and rows of no sequence are zero."""
+    all that the sequences hold). Tokens without a place and rows of no sequence are zero."""
     cc, _, dtype, heads, d, _ = cache._call
     if rows < 0:
         raise ValueError("paged_rows: rows must be >= 0")
@@ -1054,7 +1054,7 @@ def paged_attention(
         raise ValueError(f"paged_attention: window >= 1 and sinks >= 0 (got {window}, {sinks})")
     sc = 1.0 / math.sqrt(d) if scale is None else float(scale)
     zero = out is None
-    o = q.new_empty(q.shape) if zero else out
+    o = _like(q) if zero else out
     os = _tokens("paged_attention", "out", o, dtype, hq, d, rows)
     if not zero:
         _written("paged_attention", "out", o)
