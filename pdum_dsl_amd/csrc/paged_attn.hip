@@ -730,7 +730,7 @@ __global__ __launch_bounds__(1024) void paged_decode_merge(PagedAttn a, const De
 // Workgroups: a sequence's blocks come in slots starts * group / 128 + sequence onward (rounded down), which never overlap,
 // so that the grid is known without the starts; a workgroup counts the sequences at or before its slot. Late blocks, which
 // see the most keys, go first, in runs of four of alternating direction (the four shader engines of an XCD draw alike); an
-// XCD works through whole heads, whose keys its L2 holds. A grid too small for the chip cuts each block's tiles into parts
+// XCD works through few heads at a time, whose keys its L2 holds (SlotMap). A grid too small for the chip cuts each block's tiles into parts
 // that paged_prompt_merge joins.
 
 template <int D, int BITS>
@@ -807,8 +807,19 @@ struct Parts {
   }
 };
 
+// Which workgroup takes which head and slot. Workgroups go round the eight XCDs; XCD x takes units x `units` and onward, a
+// unit being every `shares`-th slot of a head (1 where the heads divide by eight), up to kHeadsRun of them at a time, the late
+// slots of all of those first. Against whole heads one after the other, us, bf16: 2 x 4096 tokens, 12 heads of 64, 130 -> 88;
+// 16 heads on one, 128 -> 104; 4 x 4096, 16 of 64, 192 -> 182; 2 x 4096, 32/8 of 128, 262 -> 261. One unit at a time: 107,
+// 104, 189, 266; eight: as three. Sequences in turn as well (two, four at a time): 80, 104, 174, 261, but 8 x 512 rows over
+// 7001 keys 439 -> 478 and 459, their keys no longer in L2.
+constexpr int kHeadsRun = 3;
+struct SlotMap {
+  int units, shares, unit_slots;
+};
+
 template <typename T, int D, int BITS, bool FAR>
-__global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, int nslots) {
+__global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, SlotMap mp, int nslots) {
   using C = ProCfg<D, BITS>;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[C::LDS];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, G = lane >> 4, w = wave_id();
@@ -818,12 +829,16 @@ __global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, in
   int bid = blockIdx.x;
   const int split = scalar(bid % pt.nsplit);
   bid = scalar(bid / pt.nsplit);
-  const int per = scalar(gridDim.x / pt.nsplit >> 3);  // blocks an XCD
-  const int lin = (bid & 7) * per + (bid >> 3);
-  const int head = scalar(lin / nslots);
-  if (head >= a.c.heads) return;
-  int j = scalar(lin % nslots);
-  if ((j | 3) < nslots && (j & 4)) j ^= 3;
+  const int r = bid >> 3, per_run = kHeadsRun * mp.unit_slots;  // of this XCD's workgroups
+  const int first = scalar(r / per_run) * kHeadsRun, in_run = scalar(r % per_run);
+  const int n = mp.units - first < kHeadsRun ? mp.units - first : kHeadsRun;
+  if (n <= 0) return;
+  const int unit = (bid & 7) * mp.units + first + scalar(in_run % n);
+  const int head = scalar(unit / mp.shares);
+  int j = scalar(in_run / n);
+  if ((j | 3) < mp.unit_slots && (j & 4)) j ^= 3;
+  j = j * mp.shares + scalar(unit % mp.shares);
+  if (j >= nslots) return;
   int rb = 0;
   const int seq = seq_of_slot(a, nslots - 1 - j, rb);
   if (seq < 0) return;
@@ -1342,7 +1357,11 @@ extern "C" int pdh_paged_attention(const void* q, void* o, float* lse, int64_t h
   }
   const int nsplit = prompt_splits(*cache, *batch, a.group, window, sinks);
   const int64_t nslots = batch->rows * a.group / 128 + batch->seqs + 1;
-  const int64_t blocks = (nslots * cache->heads + 7) / 8 * 8 * nsplit;
+  SlotMap mp{0, 1, 0};
+  while (cache->heads * mp.shares % 8 != 0) mp.shares *= 2;
+  mp.units = static_cast<int>(cache->heads * mp.shares / 8);
+  mp.unit_slots = static_cast<int>((nslots + mp.shares - 1) / mp.shares);
+  const int64_t blocks = int64_t{8} * mp.units * mp.unit_slots * nsplit;
   PDH_REQUIRE(blocks <= INT32_MAX, PDH_EINVAL, "pdh_paged_attention: grid too large");
   const Parts parts{nsplit, batch->rows * heads_q, static_cast<float*>(ws)};
   by_kind(*cache, [&](auto t, auto d, auto bits) {
@@ -1351,9 +1370,9 @@ extern "C" int pdh_paged_attention(const void* q, void* o, float* lse, int64_t h
     constexpr int B = decltype(bits)::value;
     const unsigned n = static_cast<unsigned>(blocks);
     if (!far)
-      paged_prompt<T, D, B, false><<<n, 256, 0, as_stream(stream)>>>(a, parts, static_cast<int>(nslots));
+      paged_prompt<T, D, B, false><<<n, 256, 0, as_stream(stream)>>>(a, parts, mp, static_cast<int>(nslots));
     else
-      paged_prompt<T, D, B, true><<<n, 256, 0, as_stream(stream)>>>(a, parts, static_cast<int>(nslots));
+      paged_prompt<T, D, B, true><<<n, 256, 0, as_stream(stream)>>>(a, parts, mp, static_cast<int>(nslots));
     if (nsplit > 1) {
       const dim3 grid(static_cast<unsigned>(batch->rows), static_cast<unsigned>((heads_q + 7) / 8));
       paged_prompt_merge<T, D><<<grid, 256, 0, as_stream(stream)>>>(a, parts);

@@ -143,3 +143,31 @@ def test_any_starts_and_lengths_stay_in_range():
                 r0, n, *_ = _plan(starts, lengths, seq, rows, group, 64, LIMIT, 0, 128)
                 if 0 <= rb < -(-n * group // 128):
                     assert r0 + (rb * 128) // group < rows
+
+
+def _head_slot(bid, heads, nslots):
+    """The prompt kernel's workgroup -> (head, slot), None where it has none; and the grid."""
+    shares = 1
+    while heads * shares % 8:
+        shares *= 2
+    units, unit_slots, run_of = heads * shares // 8, -(-nslots // shares), 3
+    grid = 8 * units * unit_slots
+    r, per_run = bid >> 3, run_of * unit_slots
+    first, in_run = r // per_run * run_of, r % per_run
+    n = min(units - first, run_of)
+    if n <= 0:
+        return None, grid
+    unit = (bid & 7) * units + first + in_run % n
+    j = in_run // n
+    if (j | 3) < unit_slots and j & 4:
+        j ^= 3
+    j = j * shares + unit % shares
+    return ((unit // shares, nslots - 1 - j) if j < nslots else None), grid
+
+
+@pytest.mark.parametrize("heads", [1, 2, 3, 5, 8, 12, 16, 32, 40])
+@pytest.mark.parametrize("nslots", [1, 2, 7, 67, 131])
+def test_every_head_and_slot_has_one_workgroup(heads, nslots):
+    grid = _head_slot(0, heads, nslots)[1]
+    got = [x for x in (_head_slot(b, heads, nslots)[0] for b in range(grid)) if x is not None]
+    assert sorted(got) == [(h, s) for h in range(heads) for s in range(nslots)]
