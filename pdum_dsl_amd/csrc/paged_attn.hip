@@ -11,6 +11,7 @@
 
 #include <atomic>
 #include <cmath>
+
 namespace pdh {
 namespace {
 
@@ -39,7 +40,8 @@ struct PagedAttn {
 
 // One row by one wave: keys 64 at a time, one a lane; the online softmax's maximum and sum are the wave's, o's features lie
 // across its lanes. It touches no key that the row does not see, which makes it the way out for rows that share blocks of keys
-// with values that are not finite and not theirs. The row's softmax state over the visible keys of [k0, k1): m in units of log2, o unnormalised, features lane + 64 j.
+// with values that are not finite and not theirs. The row's softmax state over the visible keys of [k0, k1): m in units of
+// log2, o unnormalised, features lane + 64 j.
 template <typename T, int D, int BITS>
 __device__ void row_sweep(const PagedAttn& a, int seq, int hk, const uint16_t* q, int pos, int k0, int k1, float& m,
                           float& l, float (&o)[D / 64]) {
@@ -221,7 +223,7 @@ __device__ __forceinline__ int64_t scalar64(int64_t x) {
                               static_cast<uint32_t>(scalar(static_cast<int>(x))));
 }
 
-template <int ROWS, int KEYS>
+template <int ROWS>
 __device__ __forceinline__ SeqPlan plan_of(const PagedAttn& a, int i) {
   Seq s{0, 0, 0};
   if (i < a.b.seqs) {
@@ -235,12 +237,12 @@ __device__ __forceinline__ SeqPlan plan_of(const PagedAttn& a, int i) {
   p.n = s.n;
   p.pos0 = s.len - s.n;
   const int end = s.len < a.reach ? s.len : a.reach;
-  const int eb = (end + KEYS - 1) / KEYS;
+  const int eb = (end + 31) / 32;
   const int lo = p.pos0 - a.window + 1;
-  p.wb = lo > 0 ? lo / KEYS : 0;
+  p.wb = lo > 0 ? lo / 32 : 0;
   p.wb = p.wb < eb ? p.wb : eb;
   const int sink = a.sinks < end ? a.sinks : end;
-  p.sb = (sink + KEYS - 1) / KEYS;
+  p.sb = (sink + 31) / 32;
   p.sb = p.sb < p.wb ? p.sb : p.wb;
   p.blocks = p.sb + eb - p.wb;
   p.blocks = p.blocks > 0 ? p.blocks : 1;  // one that sees nothing
@@ -249,16 +251,16 @@ __device__ __forceinline__ SeqPlan plan_of(const PagedAttn& a, int i) {
 }
 
 // The plan of a wave-uniform sequence, held in scalar registers.
-template <int ROWS, int KEYS>
+template <int ROWS>
 __device__ __forceinline__ SeqPlan uniform_plan(const PagedAttn& a, int i) {
-  const SeqPlan p = plan_of<ROWS, KEYS>(a, i);
+  const SeqPlan p = plan_of<ROWS>(a, i);
   return SeqPlan{scalar(p.row0), scalar(p.n), scalar(p.pos0), scalar(p.nb), scalar(p.sb), scalar(p.wb), scalar(p.blocks)};
 }
 
 // An item that starts in a workgroup's share and ends in another's (last; -1: none): its first row, rows, number of
 // flattened rows before it, head.
 struct DecMeta {
-  int last, row0, rows, f0, head, pad;
+  int last, row0, rows, f0, head;
 };
 
 // FAR: a pool reaches past the offsets of one buffer resource (2^31 bytes).
@@ -286,7 +288,7 @@ __global__ __launch_bounds__(256, (dec_wgs<D, BITS>())) void paged_decode(PagedA
   for (int j = 0; j < each; ++j) {
     const int i = tid * each + j;
     if (i < nseq) {
-      mp = plan_of<16, 32>(a, i);
+      mp = plan_of<16>(a, i);
       mine += cost(mp);
     }
   }
@@ -311,14 +313,14 @@ __global__ __launch_bounds__(256, (dec_wgs<D, BITS>())) void paged_decode(PagedA
   int64_t at = per * blockIdx.x;
   int64_t left = total - at < per ? total - at : per;
   if (left <= 0) {
-    if (tid == 0) meta[blockIdx.x] = DecMeta{-1, 0, 0, 0, 0, 0};
+    if (tid == 0) meta[blockIdx.x] = DecMeta{-1, 0, 0, 0, 0};
     return;
   }
   if (before <= at && at < before + mine) {  // the share starts in one of this thread's sequences
     int64_t in = at - before;
     int i = tid * each;
     if (each > 1)
-      for (mp = plan_of<16, 32>(a, i); in >= cost(mp); mp = plan_of<16, 32>(a, ++i)) in -= cost(mp);
+      for (mp = plan_of<16>(a, i); in >= cost(mp); mp = plan_of<16>(a, ++i)) in -= cost(mp);
     const int units = mp.blocks + C::ITEM;
     first = Start{mp, i, static_cast<int>(in / units), static_cast<int>(in % units)};
   }
@@ -326,17 +328,14 @@ __global__ __launch_bounds__(256, (dec_wgs<D, BITS>())) void paged_decode(PagedA
   SeqPlan sp{scalar(first.sp.row0), scalar(first.sp.n),  scalar(first.sp.pos0),  scalar(first.sp.nb),
              scalar(first.sp.sb),   scalar(first.sp.wb), scalar(first.sp.blocks)};
   int seq = scalar(first.seq), item = scalar(first.item), unit = scalar(first.unit);  // heads x row blocks < 2^31 (host)
-  DecMeta cut{-1, 0, 0, 0, 0, 0};
+  DecMeta cut{-1, 0, 0, 0, 0};
 
   unsigned char* vt = dsm + w * C::VTILE;
-  // Value rows in LDS: the 16-byte slot of chunk c is c ^ ((row >> 2) & 1), which spreads the 4-bit writes (four chunks of
-  // a row 64 bytes apart) over all banks. Transposed reads: lane 4k + c of group g addresses row 4 g + k, features 4 c .. +3
-  // (+ 16 t).
-  const int trb = (4 * g + (col >> 2)) * C::VROW + ((((col >> 1) & 1) ^ (g & 1)) << 4) + (col & 1) * 8;
+  // transposed value reads: lane 4k + c of group g addresses row 4 g + k, features 4 c .. +3 (+ 16 t)
+  const int trb = (4 * g + (col >> 2)) * C::VROW + (col & 3) * 8;
   constexpr int ES = BITS == 16 ? 2 : 1;  // bytes of a stride's unit
   const uint32_t rst = static_cast<uint32_t>(a.c.sr) * ES, srst = static_cast<uint32_t>(a.c.ssr);
   const int vrow = BITS == 16 ? lane / C::CPR : lane / 4, vch = BITS == 16 ? lane % C::CPR : lane % 4;
-  const int vflip = (vrow >> 2) & 1;  // of row 16 h + vrow; of j * RPI + vrow together with j * RPI's
 
   while (left > 0) {
     const int rb = scalar(item % sp.nb), head = scalar(item / sp.nb);
@@ -455,14 +454,13 @@ __global__ __launch_bounds__(256, (dec_wgs<D, BITS>())) void paged_decode(PagedA
       // values -> this wave's tile, rows of keys
       if constexpr (BITS == 16) {
 #pragma unroll
-        for (int j = 0; j < C::VL; ++j)
-          *reinterpret_cast<u32x4*>(vt + (j * C::RPI + vrow) * C::VROW + ((vch ^ vflip ^ (j * C::RPI >> 2 & 1)) << 4)) = r.v[j];
+        for (int j = 0; j < C::VL; ++j) *reinterpret_cast<u32x4*>(vt + (j * C::RPI + vrow) * C::VROW + vch * 16) = r.v[j];
       } else {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int i = 0; i < KS; ++i)
-            *reinterpret_cast<u32x4*>(vt + (16 * h + vrow) * C::VROW + vch * (D / 2) + ((i ^ vflip) << 4)) =
+            *reinterpret_cast<u32x4*>(vt + (16 * h + vrow) * C::VROW + vch * (D / 2) + i * 16) =
                 fp4_row8<T>(r.v[h][i], e8m0(r.vs[h]));
       }
       // S^T: keys key0 + 16 h + 4 g + i (accumulator i), row col
@@ -617,7 +615,7 @@ __global__ __launch_bounds__(256, (dec_wgs<D, BITS>())) void paged_decode(PagedA
       }
     }
     if (kb == 0 && !whole)
-      cut = DecMeta{static_cast<int>((at + units - 1) / per), sp.row0, nq, f0, head, 0};
+      cut = DecMeta{static_cast<int>((at + units - 1) / per), sp.row0, nq, f0, head};
     __syncthreads();  // before the next item's tiles
 
     left -= take;
@@ -628,7 +626,7 @@ __global__ __launch_bounds__(256, (dec_wgs<D, BITS>())) void paged_decode(PagedA
       ++item;
       if (item == sp.nb * hkv) {
         item = 0;
-        do sp = uniform_plan<16, 32>(a, ++seq);
+        do sp = uniform_plan<16>(a, ++seq);
         while (sp.n == 0);
       }
     }
@@ -655,12 +653,16 @@ __global__ __launch_bounds__(1024) void paged_decode_merge(PagedAttn a, const De
           float rm[8], rl[8], ro[8][DL];
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const int r = r0 + 4 * j < nrec ? r0 + 4 * j : r0;
+            const bool in = r0 + 4 * j < nrec;  // one that is not there reads another's place, and counts as empty
+            const int r = in ? r0 + 4 * j : r0;
             const float* p = ws + ((static_cast<int64_t>(blockIdx.x) + r) * 2 + (r == 0)) * 16 * RS + i * RS;
-            rm[j] = r0 + 4 * j < nrec ? p[0] : -kInf;
-            rl[j] = p[1];
+            rm[j] = in ? p[0] : -kInf;
+            rl[j] = in ? p[1] : 0.f;
 #pragma unroll
-            for (int d = 0; d < DL; ++d) ro[j][d] = p[2 + lane + 64 * d];
+            for (int d = 0; d < DL; ++d) {
+              const float x = p[2 + lane + 64 * d];
+              ro[j][d] = in ? x : 0.f;
+            }
           }
           float mm = m;
 #pragma unroll
@@ -842,7 +844,7 @@ __global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, Sl
   int rb = 0;
   const int seq = seq_of_slot(a, nslots - 1 - j, rb);
   if (seq < 0) return;
-  const SeqPlan sp = uniform_plan<128, 32>(a, seq);
+  const SeqPlan sp = uniform_plan<128>(a, seq);
   if (rb < 0 || rb >= sp.nb) return;
 
   // ---- the block's rows: lane row h of wave w is flattened row 128 rb + 32 w + 16 h + c
@@ -1225,7 +1227,7 @@ __global__ __launch_bounds__(256) void paged_prompt_merge(PagedAttn a, Parts pt)
   const int lane = threadIdx.x & 63, row = blockIdx.x;
   const int seq = seq_of_row(a.b, row);
   if (seq >= a.b.seqs) return;
-  const SeqPlan sp = uniform_plan<128, 32>(a, seq);
+  const SeqPlan sp = uniform_plan<128>(a, seq);
   if (row < sp.row0 || row >= sp.row0 + sp.n) return;
   const int R = a.group;
   const int h_end = blockIdx.y * 8 + 8 < a.heads_q ? blockIdx.y * 8 + 8 : a.heads_q;
@@ -1288,7 +1290,7 @@ int decode_grid(const pdh_paged_cache& c) {
 int prompt_splits(const pdh_paged_cache& c, const pdh_paged_batch& b, int64_t group, int64_t window, int64_t sinks) {
   const int64_t blocks = (b.rows * group / 128 + 1) * c.heads;
   int64_t keys = b.width * c.page_rows;
-  if (window < keys) keys = keys < window + sinks + 128 ? keys : window + sinks + 128;
+  if (window < keys && sinks < keys) keys = keys < window + sinks + 128 ? keys : window + sinks + 128;
   int64_t n = (4 * compute_units() + blocks) / (2 * blocks);
   n = n < keys / 1024 ? n : keys / 1024;
   return static_cast<int>(n < 1 ? 1 : (n < 32 ? n : 32));
@@ -1317,7 +1319,7 @@ extern "C" int pdh_paged_attention(const void* q, void* o, float* lse, int64_t h
               "pdh_paged_attention: heads_q must be a multiple of the cache's heads");
   PDH_REQUIRE(batch->rows * heads_q <= INT32_MAX, PDH_EINVAL, "pdh_paged_attention: rows * heads_q must be < 2^31");
   PDH_REQUIRE(window >= 1 && sinks >= 0, PDH_EINVAL, "pdh_paged_attention: window >= 1 and sinks >= 0");
-  PDH_REQUIRE(std::isfinite(scale) && scale > 0.f, PDH_EINVAL, "pdh_paged_attention: scale must be finite and > 0");
+  PDH_REQUIRE(std::isfinite(scale * kLog2e) && scale > 0.f, PDH_EINVAL, "pdh_paged_attention: scale must be finite and > 0");
   if (batch->rows == 0) return PDH_OK;
   PDH_REQUIRE(q && o && aligned16(q) && aligned16(o), PDH_EINVAL,
               "pdh_paged_attention: q and o must be 16-byte aligned");
@@ -1362,7 +1364,8 @@ extern "C" int pdh_paged_attention(const void* q, void* o, float* lse, int64_t h
   mp.units = static_cast<int>(cache->heads * mp.shares / 8);
   mp.unit_slots = static_cast<int>((nslots + mp.shares - 1) / mp.shares);
   const int64_t blocks = int64_t{8} * mp.units * mp.unit_slots * nsplit;
-  PDH_REQUIRE(blocks <= INT32_MAX, PDH_EINVAL, "pdh_paged_attention: grid too large");
+  PDH_REQUIRE(blocks < (1 << 24), PDH_EINVAL, "pdh_paged_attention: too many rows and heads: %lld workgroups, at most 2^24 - 1",
+              (long long)blocks);  // of 256 threads: a launch counts threads in 32 bits
   const Parts parts{nsplit, batch->rows * heads_q, static_cast<float*>(ws)};
   by_kind(*cache, [&](auto t, auto d, auto bits) {
     using T = decltype(t);

@@ -972,16 +972,17 @@ def paged_append(
         raise ValueError("paged_append: out is q's, and there is no q")
     else:
         zero = False
-    positions, rotated, ldr = 0, 0, 0
+    positions, rotated, ldr, tab = 0, 0, 0, None
     if rotary is not None:
         if rotary.dtype != torch.float32 or rotary.dim() != 2 or rotary.stride(1) != 1:
             raise ValueError("paged_append: rotary must be fp32 [positions, rotated] with contiguous rows")
         positions, rotated = rotary.shape
         ldr = rotary.stride(0) if positions > 1 else rotated
+        tab = rotary.data_ptr() or starts.data_ptr()  # a table of no positions, which is not read, has no address
     if bad is not None and (bad.dtype != torch.int32 or bad.numel() < 1):
         raise ValueError("paged_append: bad is an int32 device scalar")
     _lib.call("pdh_paged_append", k.data_ptr(), v.data_ptr(), _ptr(q), _ptr(out), hq, *ks, *vs, *qs, *os, cc, C.byref(b),
-              _ptr(rotary), positions, rotated, ldr, int(interleaved), int(zero), _ptr(bad), _stream())
+              tab, positions, rotated, ldr, int(interleaved), int(zero), _ptr(bad), _stream())
     return out
 
 
@@ -1041,7 +1042,8 @@ def paged_attention(
     What a row does not see has no part in it, whatever the cache holds there;
     tokens on pages outside the pool or past the table are not seen. A row
     that sees nothing (or only scores of -inf) has o = 0 and lse = -inf. Rows
-    of no sequence likewise; ``out`` (q's shape and type) they leave as it is.
+    of no sequence likewise; ``out`` (q's shape and type, or q itself) they
+    leave as it is.
     The 4 bits are exact in the 16-bit type but for f16 under 2^-24."""
     cc, _, dtype, heads, d, _ = cache._call
     b = _paged("paged_attention", cache, table, starts, lengths, q.shape[0] if q.dim() == 3 else 0, (q, out))
@@ -1058,7 +1060,11 @@ def paged_attention(
     os = _tokens("paged_attention", "out", o, dtype, hq, d, rows)
     if not zero:
         _written("paged_attention", "out", o)
-    lse = q.new_empty((rows, hq), dtype=torch.float32) if want_lse else None
+        if o.data_ptr() == q.data_ptr() and os != qs:
+            raise ValueError("paged_attention: out in q's place must have q's strides")
+    lse = None
+    if want_lse:  # the call leaves rows of no sequence alone in both results, or in neither
+        lse = q.new_empty((rows, hq), dtype=torch.float32) if zero else q.new_full((rows, hq), -math.inf, dtype=torch.float32)
     need = _paged_workspace(cache._call[5], rows, b.seqs, b.width, hq, window, int(sinks))
     ws = q.new_empty((need + 3) // 4, dtype=torch.float32) if need else None
     _lib.call("pdh_paged_attention", q.data_ptr(), o.data_ptr(), _ptr(lse), hq, *qs, *os, cc, C.byref(b), window,

@@ -265,3 +265,46 @@ def test_tensors_of_another_device_are_refused(K, monkeypatch):
                  lambda: K.paged_attention(x, cache, *t)):
         with pytest.raises(ValueError, match="current device"):
             call()
+
+
+@pytest.mark.parametrize("new", [1, 3, 130])
+def test_an_infinite_value_is_its_rows_sum(K, new):
+    """A value of +inf that a row sees: +inf in that feature, whatever parts the row's keys were cut into; nothing elsewhere."""
+    rng = np.random.default_rng(31)
+    pr, d, hq, hkv, n, key = 16, 64, 8, 2, 6000, 3
+    table, starts, lens, rows, pages = batch(rng, [n], [new], pr)
+    cache, pk, pv = _pools(rng, K, "bf16", 16, pages, hkv, pr, d)
+    q = torch.as_tensor(rng.standard_normal((rows, hq, d))).bfloat16().cuda()
+    want = op.attention(_host(q), pk, pv, table, starts, lens, scale=d**-0.5, every=max(1, new // 25))
+    cache.v[table[0, 0], :, key, 5] = float("inf")
+    o, lse = K.paged_attention(q, cache, *_ints(table, starts, lens))
+    assert torch.isposinf(o[:, :, 5]).all()
+    o = _host(o)
+    o[:, :, 5] = want[0][:, :, 5]
+    check_attention(o, _host(lse), want, "bf16", d, f"{new} rows")
+
+
+@pytest.mark.parametrize("lengths,new", [([700, 90, 5], [1, 1, 1]), ([700, 90], [3, 2]), ([300, 200], [300, 40]), ([6000], [130])])
+def test_attention_in_the_place_of_q(K, lengths, new):
+    rng = np.random.default_rng(32)
+    pr, d, hq, hkv = 16, 64, 8, 2
+    table, starts, lens, rows, pages = batch(rng, lengths, new, pr, pad=3)
+    cache, _, _ = _pools(rng, K, "bf16", 16, pages, hkv, pr, d)
+    qkv = torch.as_tensor(rng.standard_normal((rows, hq + 2 * hkv, d))).bfloat16().cuda()
+    q, held = qkv[:, :hq], qkv.clone()
+    want, lse = K.paged_attention(q, cache, *_ints(table, starts, lens))
+    got, lse2 = K.paged_attention(q, cache, *_ints(table, starts, lens), out=q)
+    live = rows - 3
+    assert got is q and torch.equal(q[:live], want[:live])
+    assert torch.equal(lse, lse2) and torch.isneginf(lse[live:]).all()
+    assert torch.equal(q[live:], held[live:, :hq]) and torch.equal(qkv[:, hq:], held[:, hq:])
+    with pytest.raises(ValueError, match="q's strides"):
+        K.paged_attention(q, cache, *_ints(table, starts, lens), out=q.as_strided((rows, hq, d), (hq * d, d, 1)))
+
+
+def test_a_rotary_table_of_no_positions_has_room_for_no_token(K):
+    cache = K.paged_cache(2, 2, 16, 64)
+    x = torch.ones((3, 4, 64), dtype=torch.bfloat16, device="cuda")
+    bad = torch.zeros(1, dtype=torch.int32, device="cuda")
+    got = K.paged_append(x[:, :2], x[:, 2:], cache, *_ints([[0]], [0, 3], [3]), q=x, rotary=K.rotary_table(0, 32), bad=bad)
+    assert (got == 0).all() and (cache.k == 0).all() and (cache.v == 0).all() and int(bad) == 3

@@ -211,3 +211,21 @@ def test_wrapper_refusals():
     with pytest.raises(ValueError, match="overlap"):
         K._written("f", "out", z(1, 2, 64).expand(3, 2, 64))
     K._written("f", "out", z(2, 3, 64).transpose(0, 1))
+
+
+def test_sizes_past_a_launch_and_sums_past_64_bits():
+    from pdum_dsl_amd import _lib
+
+    lib, p = _lib.lib(), C.c_void_p(FAKE)
+    c, b = _structs(dict(heads=64, sp=64 * 16 * 64), dict(seqs=1 << 20, rows=(1 << 24) - 1))
+
+    def attend(window=5, sinks=0, scale=1.0):
+        return lib.pdh_paged_attention(p, p, None, 128, 128 * 64, 64, 128 * 64, 64, C.byref(c), C.byref(b), window, sinks,
+                                       scale, 1, p, 1 << 40, None)
+
+    assert attend() == _lib.PDH_EINVAL and "workgroups" in _lib.last_error(), _lib.last_error()
+    assert attend(scale=3.0e38) == _lib.PDH_EINVAL and "scale" in _lib.last_error()  # scale log2 e is past fp32
+    most = (1 << 63) - 1
+    c, b = _structs(None, dict(rows=200, seqs=1, width=1 << 20))
+    size = lambda window, sinks: lib.pdh_paged_attention_workspace(C.byref(c), C.byref(b), 4, window, sinks)  # noqa: E731
+    assert size(most, 0) == size(1, most) == size(most, most) > size(5, 0)
