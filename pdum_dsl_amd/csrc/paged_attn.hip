@@ -146,10 +146,11 @@ __device__ __forceinline__ void write_row(const PagedAttn& a, int row, int h, fl
 // is loaded as codes: a lane takes features D/4 g .. + D/4 of its row (one load, one scale), which k-step s contracts by
 // eights, and q is laid out to match; V is widened to 16 bits on its way into LDS.
 
-// Workgroups a compute unit holds at once, by registers.
+// Workgroups a compute unit holds at once: what keeps memory busy, no more. 64 sequences of 8192 tokens, 32/8 heads, us with
+// two / three: 4 bits, D = 128, 126 / 130, D = 64 59 / 64; 16 bits, 16 heads of 64, 378 / 376; D = 128 has registers for two.
 template <int D, int BITS>
 __host__ __device__ constexpr int dec_wgs() {
-  return BITS == 16 && D == 128 ? 2 : 3;
+  return BITS == 16 && D == 64 ? 3 : 2;
 }
 
 template <int D, int BITS>
@@ -635,26 +636,27 @@ __global__ __launch_bounds__(256, (dec_wgs<D, BITS>())) void paged_decode(PagedA
 }
 
 // Joins a cut item's states: the workgroup that the item starts in left the first in its second record, the others up to
-// `last` theirs in their first. Sixteen waves: four rows at a time, a quarter of the records each, eight of them in flight;
-// the quarters meet in LDS. Then the rows behind the last sequence, spread over the grid.
+// `last` theirs in their first. Eight waves: four rows at a time, half of the records each, eight of them in flight; the
+// halves meet in LDS. Then the rows behind the last sequence, spread over the grid. 5 us at 64 x 8192 tokens (as many
+// workgroups as the decode kernel's, which 1024 threads each would run in two rounds: 8).
 template <typename T, int D>
-__global__ __launch_bounds__(1024) void paged_decode_merge(PagedAttn a, const DecMeta* meta, const float* ws) {
+__global__ __launch_bounds__(512) void paged_decode_merge(PagedAttn a, const DecMeta* meta, const float* ws) {
   constexpr int RS = 2 + D, DL = D / 64;
-  __shared__ float part[16][RS];
+  __shared__ float part[8][RS];
   const DecMeta c = meta[blockIdx.x];
   const int lane = threadIdx.x & 63, w = wave_id();
   if (c.last >= 0) {
     const int nrec = c.last - static_cast<int>(blockIdx.x) + 1;
     for (int i0 = 0; i0 < c.rows; i0 += 4) {
-      const int i = i0 + (w >> 2);
+      const int i = i0 + (w >> 1);
       float m = -kInf, l = 0.f, o[DL] = {};
       if (i < c.rows) {
-        for (int r0 = w & 3; r0 < nrec; r0 += 32) {
+        for (int r0 = w & 1; r0 < nrec; r0 += 16) {
           float rm[8], rl[8], ro[8][DL];
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const bool in = r0 + 4 * j < nrec;  // one that is not there reads another's place, and counts as empty
-            const int r = in ? r0 + 4 * j : r0;
+            const bool in = r0 + 2 * j < nrec;  // one that is not there reads another's place, and counts as empty
+            const int r = in ? r0 + 2 * j : r0;
             const float* p = ws + ((static_cast<int64_t>(blockIdx.x) + r) * 2 + (r == 0)) * 16 * RS + i * RS;
             rm[j] = in ? p[0] : -kInf;
             rl[j] = in ? p[1] : 0.f;
@@ -688,14 +690,13 @@ __global__ __launch_bounds__(1024) void paged_decode_merge(PagedAttn a, const De
 #pragma unroll
       for (int d = 0; d < DL; ++d) part[w][2 + lane + 64 * d] = o[d];
       __syncthreads();
-      if ((w & 3) == 0 && i < c.rows) {
-#pragma unroll
-        for (int q = 1; q < 4; ++q) m = fmaxf(m, part[w + q][0]);
+      if ((w & 1) == 0 && i < c.rows) {
+        m = fmaxf(m, part[w + 1][0]);
         l = 0.f;
 #pragma unroll
         for (int d = 0; d < DL; ++d) o[d] = 0.f;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
+        for (int q = 0; q < 2; ++q) {
           const float* p = part[w + q];
           const float f = p[0] == -kInf ? 0.f : fast_exp2(p[0] - m);
           l += f * p[1];
@@ -711,8 +712,8 @@ __global__ __launch_bounds__(1024) void paged_decode_merge(PagedAttn a, const De
   if (a.zero_rest) {
     const int tail = a.b.seqs ? clamp_row(a.b.starts[a.b.seqs], static_cast<int>(a.b.rows)) : 0;
     const float none[DL] = {};
-    for (int64_t x = tail * static_cast<int64_t>(a.heads_q) + blockIdx.x * 16 + w; x < a.b.rows * a.heads_q;
-         x += gridDim.x * 16)
+    for (int64_t x = tail * static_cast<int64_t>(a.heads_q) + blockIdx.x * 8 + w; x < a.b.rows * a.heads_q;
+         x += gridDim.x * 8)
       write_row<T, D>(a, static_cast<int>(x / a.heads_q), static_cast<int>(x % a.heads_q), -kInf, 0.f, none);
   }
 }
@@ -774,8 +775,8 @@ __device__ __forceinline__ BlockKeys block_keys(const PagedAttn& a, int pos_lo, 
   b.sb = b.sb < b.wb ? b.sb : b.wb;
   b.tiles = b.sb + eb - b.wb;
   b.part = (b.tiles + nsplit - 1) / nsplit;
-  b.part = scalar(b.part > kPartTiles ? b.part : kPartTiles);
-  b.parts = scalar(b.tiles > b.part ? (b.tiles + b.part - 1) / b.part : 1);
+  b.part = b.part > kPartTiles ? b.part : kPartTiles;
+  b.parts = b.tiles > b.part ? (b.tiles + b.part - 1) / b.part : 1;
   return b;
 }
 
@@ -851,7 +852,9 @@ __global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, Sl
   const int f0 = rb * C::BM;
   const int fend = sp.n * R - f0 < C::BM ? sp.n * R : f0 + C::BM;  // rows x heads_q < 2^31
   const int pos_lo = scalar(sp.pos0 + f0 / R), pos_hi = scalar(sp.pos0 + (fend - 1) / R);
-  const BlockKeys bk = block_keys(a, pos_lo, pos_hi, pt.nsplit);
+  BlockKeys bk = block_keys(a, pos_lo, pos_hi, pt.nsplit);
+  bk.part = scalar(bk.part);
+  bk.parts = scalar(bk.parts);
   if (split >= bk.parts) return;
   const int v0 = split * bk.part, v1 = v0 + bk.part < bk.tiles ? v0 + bk.part : bk.tiles;
   const int fw = f0 + 32 * w;
@@ -1221,35 +1224,38 @@ __global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, Sl
   }
 }
 
-// Joins the parts of blocks that were cut: a workgroup a row and eight query heads, a wave two of them.
+// Joins the parts of blocks that were cut. A lane takes four features, so that a wave has two rows' heads of 128 at once (four
+// of 64): what a row's sequence and parts are is looked up once for all, and the loads of a wave's heads go together.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void paged_prompt_merge(PagedAttn a, Parts pt) {
-  const int lane = threadIdx.x & 63, row = blockIdx.x;
+  constexpr int LPH = D / 4, HEADS = 256 / LPH;  // lanes a head, heads a workgroup
+  const int row = blockIdx.x, h = blockIdx.y * HEADS + threadIdx.x / LPH, e = threadIdx.x % LPH * 4;
   const int seq = seq_of_row(a.b, row);
-  if (seq >= a.b.seqs) return;
+  if (seq >= a.b.seqs || h >= a.heads_q) return;
   const SeqPlan sp = uniform_plan<128>(a, seq);
   if (row < sp.row0 || row >= sp.row0 + sp.n) return;
   const int R = a.group;
-  const int h_end = blockIdx.y * 8 + 8 < a.heads_q ? blockIdx.y * 8 + 8 : a.heads_q;
-  for (int h = blockIdx.y * 8 + wave_id(); h < h_end; h += 4) {
-    const int f0 = ((row - sp.row0) * R + h % R) / 128 * 128;
-    const int fend = sp.n * R - f0 < 128 ? sp.n * R : f0 + 128;
-    const BlockKeys bk = block_keys(a, scalar(sp.pos0 + f0 / R), scalar(sp.pos0 + (fend - 1) / R), pt.nsplit);
-    if (bk.parts <= 1) continue;
-    const int64_t at = static_cast<int64_t>(row) * a.heads_q + h;
-    float mm = -kInf, l = 0.f, o[D / 64] = {};
+  const int f0 = ((row - sp.row0) * R + h % R) / 128 * 128;
+  const int fend = sp.n * R - f0 < 128 ? sp.n * R : f0 + 128;
+  const int parts = block_keys(a, sp.pos0 + f0 / R, sp.pos0 + (fend - 1) / R, pt.nsplit).parts;
+  if (parts <= 1) return;
+  const int64_t at = static_cast<int64_t>(row) * a.heads_q + h;
+  float m = -kInf, l = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int s = 0; s < bk.parts; ++s) {
-      const float* ml = pt.ml<D>(s, at);
-      const float mnew = fmaxf(mm, ml[0]);
-      const float was = mm == -kInf ? 0.f : fast_exp2(mm - mnew), f = ml[0] == -kInf ? 0.f : fast_exp2(ml[0] - mnew);
-      l = l * was + f * ml[1];
-#pragma unroll
-      for (int j = 0; j < D / 64; ++j) o[j] = o[j] * was + f * pt.o<D>(s, at)[lane + 64 * j];
-      mm = mnew;
-    }
-    write_row<T, D>(a, row, h, mm, l, o);
+  for (int s = 0; s < parts; ++s) {
+    const float2 ml = *reinterpret_cast<const float2*>(pt.ml<D>(s, at));
+    const f32x4 x = *reinterpret_cast<const f32x4*>(pt.o<D>(s, at) + e);
+    const float mnew = fmaxf(m, ml.x);
+    const float was = m == -kInf ? 0.f : fast_exp2(m - mnew), f = ml.x == -kInf ? 0.f : fast_exp2(ml.x - mnew);
+    l = l * was + f * ml.y;
+    o = o * was + x * f;
+    m = mnew;
   }
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  *reinterpret_cast<u32x2*>(a.o + row * a.o_st + h * a.o_sh + e) =
+      u32x2{pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv)};
+  if (e == 0 && a.lse) a.lse[at] = l == 0.f ? -kInf : (m + __log2f(l)) * kLn2;
 }
 
 }  // namespace
@@ -1353,7 +1359,7 @@ extern "C" int pdh_paged_attention(const void* q, void* o, float* lse, int64_t h
         paged_decode<T, D, B, false><<<n, 256, 0, as_stream(stream)>>>(a, meta, states);
       else
         paged_decode<T, D, B, true><<<n, 256, 0, as_stream(stream)>>>(a, meta, states);
-      paged_decode_merge<T, D><<<n, 1024, 0, as_stream(stream)>>>(a, meta, states);
+      paged_decode_merge<T, D><<<n, 512, 0, as_stream(stream)>>>(a, meta, states);
     });
     return check_launch("pdh_paged_attention (decode)");
   }
@@ -1377,7 +1383,7 @@ extern "C" int pdh_paged_attention(const void* q, void* o, float* lse, int64_t h
     else
       paged_prompt<T, D, B, true><<<n, 256, 0, as_stream(stream)>>>(a, parts, mp, static_cast<int>(nslots));
     if (nsplit > 1) {
-      const dim3 grid(static_cast<unsigned>(batch->rows), static_cast<unsigned>((heads_q + 7) / 8));
+      const dim3 grid(static_cast<unsigned>(batch->rows), static_cast<unsigned>((heads_q * D / 4 + 255) / 256));
       paged_prompt_merge<T, D><<<grid, 256, 0, as_stream(stream)>>>(a, parts);
     }
   });
