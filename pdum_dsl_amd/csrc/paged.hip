@@ -216,9 +216,9 @@ extern "C" int pdh_paged_append(const void* k, const void* v, const void* q, voi
   const int rc = check_paged("pdh_paged_append", cache, batch, &shift);
   if (rc) return rc;
   PDH_REQUIRE(heads_q >= 0 && heads_q <= 65535, PDH_EINVAL, "pdh_paged_append: bad number of query heads");
+  if (batch->rows == 0) return PDH_OK;
   PDH_REQUIRE((q == nullptr) == (heads_q == 0) && (q_out == nullptr) == (heads_q == 0), PDH_EINVAL,
               "pdh_paged_append: q and q_out come together, with heads_q >= 1");
-  if (batch->rows == 0) return PDH_OK;
   PDH_REQUIRE(k && v && aligned16(k) && aligned16(v) && aligned16(q) && aligned16(q_out), PDH_EINVAL,
               "pdh_paged_append: k, v, q and q_out must be 16-byte aligned");
   for (int64_t s : {k_st, k_sh, v_st, v_sh, q_st, q_sh, qo_st, qo_sh})

@@ -875,34 +875,40 @@ def rotary_table(positions: int, rotated: int, base: float = 10000.0, *,
 
 
 def _paged(name, cache, table, starts, lengths, rows, others):
-    """The checked batch of a call on a paged cache."""
-    dev = torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -1
-    if cache._call[1] != dev or dev < 0:
+    """The checked batch of a call on a paged cache. (This and _tokens are most of a small call's time on the host: a shape
+    or stride is asked for once.)"""
+    dev = cache._call[1]
+    if dev < 0 or torch._C._cuda_getDevice() != dev:
         _one_device(cache.k)
-    _one_device(table, starts, lengths, *others)
+    for t in (table, starts, lengths, *others):
+        if t is not None and t.get_device() != dev:
+            _one_device(t)
     if table.dtype != torch.int32 or starts.dtype != torch.int32 or lengths.dtype != torch.int32:
         raise ValueError(f"{name}: table, starts and lengths are int32")
-    seqs = lengths.shape[0] if lengths.dim() == 1 else -1
-    if seqs < 0 or starts.shape != (seqs + 1,) or table.dim() != 2 or table.shape[0] != seqs:
+    ts, ss, ls = table.shape, starts.shape, lengths.shape
+    if len(ts) != 2 or len(ss) != 1 or len(ls) != 1 or ts[0] != ls[0] or ss[0] != ls[0] + 1:
         raise ValueError(f"{name}: table [sequences, pages], starts [sequences + 1], lengths [sequences] (got "
-                         f"{tuple(table.shape)}, {tuple(starts.shape)}, {tuple(lengths.shape)})")
-    width = table.shape[1]
-    if not (starts.is_contiguous() and lengths.is_contiguous()) or (width > 1 and table.stride(1) != 1):
+                         f"{tuple(ts)}, {tuple(ss)}, {tuple(ls)})")
+    seqs, width = ts
+    ld, inner = table.stride()
+    if not (starts.is_contiguous() and lengths.is_contiguous()) or (width > 1 and inner != 1):
         raise ValueError(f"{name}: starts, lengths and the table's rows must be contiguous")
     return _lib.PagedBatch(table.data_ptr(), starts.data_ptr(), lengths.data_ptr(), seqs, rows, width,
-                           table.stride(0) if seqs > 1 else width)
+                           ld if seqs > 1 else width)
 
 
 def _tokens(name, nm, t, dtype, heads, features, rows=None):
     """A [rows, heads, features] tensor's row and head strides, checked."""
-    if t.dtype != dtype or t.dim() != 3 or t.shape[2] != features or (heads is not None and t.shape[1] != heads) or (
-            rows is not None and t.shape[0] != rows):
-        raise ValueError(f"{name}: {nm} must be {dtype} [{'rows' if rows is None else rows}, "
-                         f"{'heads' if heads is None else heads}, {features}] (got {t.dtype} {tuple(t.shape)})")
-    st = t.stride()
-    if st[2] != 1:
-        raise ValueError(f"{name}: {nm}'s features must be contiguous")
-    return (st[0] if t.shape[0] > 1 else 0), (st[1] if t.shape[1] > 1 else 0)
+    shape = t.shape
+    if len(shape) == 3 and t.dtype == dtype:
+        n, h, f = shape
+        if f == features and (heads is None or h == heads) and (rows is None or n == rows):
+            sn, sh, sf = t.stride()
+            if sf != 1:
+                raise ValueError(f"{name}: {nm}'s features must be contiguous")
+            return (sn if n > 1 else 0), (sh if h > 1 else 0)
+    raise ValueError(f"{name}: {nm} must be {dtype} [{'rows' if rows is None else rows}, "
+                     f"{'heads' if heads is None else heads}, {features}] (got {t.dtype} {tuple(shape)})")
 
 
 def _written(name, nm, t):
@@ -962,9 +968,9 @@ def paged_append(
             raise ValueError("paged_append: q has no heads")
         zero = out is None
         if zero:
-            out = _like(q)
-        os = _tokens("paged_append", "out", out, dtype, hq, d, rows)
-        if not zero:
+            out, os = _like(q), (hq * d, d)
+        else:
+            os = _tokens("paged_append", "out", out, dtype, hq, d, rows)
             _written("paged_append", "out", out)
             if out.data_ptr() == q.data_ptr() and os != qs:
                 raise ValueError("paged_append: out in q's place must have q's strides")
@@ -1056,9 +1062,10 @@ def paged_attention(
         raise ValueError(f"paged_attention: window >= 1 and sinks >= 0 (got {window}, {sinks})")
     sc = 1.0 / math.sqrt(d) if scale is None else float(scale)
     zero = out is None
-    o = _like(q) if zero else out
-    os = _tokens("paged_attention", "out", o, dtype, hq, d, rows)
-    if not zero:
+    if zero:
+        o, os = _like(q), (hq * d, d)
+    else:
+        o, os = out, _tokens("paged_attention", "out", out, dtype, hq, d, rows)
         _written("paged_attention", "out", o)
         if o.data_ptr() == q.data_ptr() and os != qs:
             raise ValueError("paged_attention: out in q's place must have q's strides")

@@ -308,3 +308,10 @@ def test_a_rotary_table_of_no_positions_has_room_for_no_token(K):
     bad = torch.zeros(1, dtype=torch.int32, device="cuda")
     got = K.paged_append(x[:, :2], x[:, 2:], cache, *_ints([[0]], [0, 3], [3]), q=x, rotary=K.rotary_table(0, 32), bad=bad)
     assert (got == 0).all() and (cache.k == 0).all() and (cache.v == 0).all() and int(bad) == 3
+
+
+def test_no_rows_to_append(K):
+    cache = K.paged_cache(2, 2, 16, 64)
+    x = torch.empty((0, 8, 64), dtype=torch.bfloat16, device="cuda")
+    got = K.paged_append(x[:, 4:6], x[:, 6:], cache, *_ints([[0]], [0, 0], [7]), q=x[:, :4], rotary=K.rotary_table(9, 64))
+    assert got.shape == (0, 4, 64) and (cache.k == 0).all()
