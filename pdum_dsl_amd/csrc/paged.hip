@@ -5,7 +5,9 @@
 // brought. y = x cos -+ partner sin in fp32, each product and the sum rounded (no fma): the same two roundings for both of a
 // pair, and what elementary fp32 operations give. Then one rounding to the type, or to 4 bits: four neighbouring threads
 // hold a scale's 32 features, so its maximum takes two exchanges. Bytes bound it: each input is read and each output
-// written once.
+// written once. 8 x 1024 tokens, 32/8 heads of 128: 39 us, 202 MB (5.2 TB/s, as a copy of that size from memory); to 4 bits
+// 41 us, 181 MB (4.4; VALU half busy with the rotation and the scales). 64 single tokens: 3.7 us, a launch. A workgroup
+// takes chunks of one row, whose sequence is looked up once.
 #include "paged.h"
 
 namespace pdh {
@@ -165,6 +167,7 @@ struct RowsArgs {
   int shift, zero_rest;
 };
 
+// A chunk of 8 features a thread, as above: 8 x 1024 tokens of 4 bits 12.4 us, 55 MB (4.4 TB/s).
 template <typename T, int D, int BITS>
 __global__ __launch_bounds__(256) void paged_rows(RowsArgs a) {
   constexpr int CPH = D / 8;

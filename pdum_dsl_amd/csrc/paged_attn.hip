@@ -4,8 +4,9 @@
 //   o = sum_s softmax(x) v_s, lse = log sum_s exp x;  a row with no visible key: o = 0, lse = -inf
 //
 // Two kernels, by the mean number of rows of a sequence times the group of query heads on a key/value head: to 16 of them
-// the decode kernel (bytes bound it), above the prompt kernel (matrix products do). Both take any batch; a lone long prompt
-// among single tokens is merely slower in the one, a lone token in the other.
+// the decode kernel (bytes bound it), above the prompt kernel (matrix products do). 64 sequences of 8192 tokens, 32/8 heads
+// of 128, us by the one / the other: 4 rows each 367 / 403 (4 bits 128 / 222), 5 rows, two blocks, 711 / 421 (239 / 233). Both
+// take any batch; a lone long prompt among single tokens is merely slower in the one, a lone token in the other.
 #include "attn_common.h"
 #include "paged.h"
 
@@ -134,7 +135,12 @@ __device__ __forceinline__ void write_row(const PagedAttn& a, int row, int h, fl
 // Decode: the work is reading the caches once. A sequence's rows times the group of query heads that share a key/value head,
 // flattened (row * group + head), are cut into blocks of 16, the columns of v_mfma_f32_16x16x32: every cached byte that a
 // block reads serves all of them. Keys go by blocks of 32 on the absolute grid, so that a block lies in at most two pages,
-// whose numbers are wave-uniform scalars, fetched two blocks ahead.
+// whose numbers are wave-uniform scalars, fetched a block before its loads are issued.
+//
+// Memory bounds it. 64 x 8192 tokens, 32/8 heads of 128: 16 bits 360 us, 2154 MB fetched (6.0 TB/s), 4 bits 107 us, 607 MB
+// (5.7; 36 MB of them lines of scales that a page of 16 rows fills by half); with every sequence on the same pages, which L2
+// then holds, 4 bits take 71. A copy of such sizes moves 5.1 to 5.4 TB/s. 24 ragged sequences of up to 30000 under a window:
+// 75 us, 411 MB. Short calls are latency: 1 x 1000 tokens 9.4 us, of which two rounds of blocks are half.
 //
 // Shares. Sequences differ in length, and the lengths are device memory. Every workgroup sums up all sequences' work (blocks of
 // keys x blocks of rows x heads), takes the same share of the line they form, and sweeps what lies in it: a part of one
@@ -165,10 +171,16 @@ struct DecCfg {
   static constexpr int RS = 2 + D;  // floats of a row's state: m, l, o
   static constexpr int RED = 4 * 16 * RS * 4;
   static constexpr int LDS = 4 * VTILE > RED ? 4 * VTILE : RED;
-  static constexpr int NB = 2;  // blocks of keys in registers: one computed, the others in flight
-  // The unit of work is a block of keys. An item costs ITEM more, so that the short ones of a batch of many are not all one
-  // workgroup's; a share is at least LEAST.
-  static constexpr int ITEM = 4, LEAST = 8;
+  // Blocks of keys in registers: one computed, the others in flight. Three and four, 4 bits, 64 x 8192, heads of 128: 128 and
+  // 130 us against 126; one, refilled when its keys are used, 125, but heads of 64 64 against 59.
+  static constexpr int NB = 2;
+  // The unit of work is a block of keys. An item costs ITEM more (what its q, its state and their join take), so that the
+  // short ones of a batch of many are not all one workgroup's; a share is at least LEAST, two rounds of the four waves, and
+  // ITEM as much, so that no short share sweeps keys of two items, one after the other. us at ITEM 0 / 4 / 8 / 12: 7 x 4 tokens over
+  // 5003 (4 bits, heads of 64) 17.7 / 17.5 / 16.4 / 16.1, 1 over 5000 16.2 / 14.1 / 12.9 / 12.9, 4 over 300 15.2 / 13.1 / 11.8 /
+  // 11.9, 512 ragged over 100 64.5 / 56.0 / 57.5 / 58.5, 24 over 30000 under a window 82 / 80 / 80 / 83; at LEAST 4 / 8 / 16,
+  // 1 over 1000 11.2 / 11.7 / 15.7, 1 over 5000 15.3 / 12.9 / 16.2.
+  static constexpr int ITEM = 8, LEAST = 8;
 };
 
 // One block of 32 keys in flight.
@@ -264,7 +276,8 @@ struct DecMeta {
   int last, row0, rows, f0, head;
 };
 
-// FAR: a pool reaches past the offsets of one buffer resource (2^31 bytes).
+// FAR: a pool reaches past the offsets of one buffer resource (2^31 bytes), and each page gets its own: 64 x 8192 tokens of 16
+// bits take as long so (376 us), but 2 x 4096 tokens of a prompt 264 instead of 260.
 template <typename T, int D, int BITS, bool FAR>
 __global__ __launch_bounds__(256, (dec_wgs<D, BITS>())) void paged_decode(PagedAttn a, DecMeta* meta, float* ws) {
   using C = DecCfg<D, BITS>;
@@ -733,8 +746,13 @@ __global__ __launch_bounds__(512) void paged_decode_merge(PagedAttn a, const Dec
 // Workgroups: a sequence's blocks come in slots starts * group / 128 + sequence onward (rounded down), which never overlap,
 // so that the grid is known without the starts; a workgroup counts the sequences at or before its slot. Late blocks, which
 // see the most keys, go first, in runs of four of alternating direction (the four shader engines of an XCD draw alike); an
-// XCD works through few heads at a time, whose keys its L2 holds (SlotMap). A grid too small for the chip cuts each block's tiles into parts
-// that paged_prompt_merge joins.
+// XCD works through few heads at a time, whose keys its L2 holds (SlotMap). A grid too small for the chip cuts each block's
+// tiles into parts that paged_prompt_merge joins.
+//
+// The matrix pipe and the softmax's VALU share the clock that the part's power leaves: 2 x 4096 tokens, 32/8 heads of 128,
+// 266-279 us (990 to 1030 TFLOP/s; a library product of 8192^3 has 1200), matrix pipe 48% busy, VALU 50%, 2.0 GHz. 8192 under
+// a window of 1024: 151-160 us (860), of 35 tiles a block one in ten is cut or outside. 4 bits, 4 x 500 ragged rows over 7001:
+// 148 us and 12 of joining (750), 33% busy: a tile's codes are widened between the products of two.
 
 template <int D, int BITS>
 struct ProCfg {
@@ -1224,8 +1242,9 @@ __global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, Sl
   }
 }
 
-// Joins the parts of blocks that were cut. A lane takes four features, so that a wave has two rows' heads of 128 at once (four
-// of 64): what a row's sequence and parts are is looked up once for all, and the loads of a wave's heads go together.
+// Joins the parts of blocks that were cut. A lane takes four features, so that a wave has two heads of 128 at once (four of
+// 64): a row's sequence and parts are looked up once for all of them, and their loads go together. Latency and bytes: 12 us
+// for 42 MB of parts (4 x 500 ragged rows, two parts; one head a wave after another: 20).
 template <typename T, int D>
 __global__ __launch_bounds__(256) void paged_prompt_merge(PagedAttn a, Parts pt) {
   constexpr int LPH = D / 4, HEADS = 256 / LPH;  // lanes a head, heads a workgroup
@@ -1290,9 +1309,9 @@ int decode_grid(const pdh_paged_cache& c) {
 
 // Parts that the prompt kernel cuts a block's keys into: as many as bring the grid nearest to two workgroups a compute unit,
 // of at least 1024 keys of what the table can hold (the lengths are not known here; a block of fewer keys makes fewer
-// parts). Measured, bf16, 32/8 heads of 128, us uncut / cut: 512 rows over 8192 keys 237 / 98, 128 over 8192 236 / 46, 4 x 500
-// ragged over 7001 230 / 179, 8 x 64 over 8192 235 / 78; a prompt of 1024 tokens 38 / 48 (two parts of 512), of 2048 under a
-// window of 1024 56 / 101 (two parts): those stay whole.
+// parts). Measured, bf16, 32/8 heads of 128, us uncut / cut: 512 rows over 8192 keys 191 / 92, 128 over 8192 190 / 41, 4 x
+// 500 ragged over 7001 188 / 150 (4 bits 212 / 165), 8 x 64 over 8192 197 / 100. Shorter parts lost: a prompt of 1024
+// tokens in two 26% longer, of 2048 under a window of 1024 80%: those stay whole.
 int prompt_splits(const pdh_paged_cache& c, const pdh_paged_batch& b, int64_t group, int64_t window, int64_t sinks) {
   const int64_t blocks = (b.rows * group / 128 + 1) * c.heads;
   int64_t keys = b.width * c.page_rows;
