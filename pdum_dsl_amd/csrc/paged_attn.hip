@@ -772,6 +772,17 @@ struct ProCfg {
   static constexpr int KPF = BITS == 4 && D == 128 ? 1 : 2;
 };
 
+// The 16-byte slot of chunk c of a tile's row is c ^ this. Key rows are read as rows, 16 a load, value rows by the transposing
+// 8-byte reads; both are conflict-free so, as in the forward kernel, whose layout this is.
+template <int D>
+__device__ __forceinline__ int key_swizzle(int row) {
+  return D == 128 ? (row & 15) : (4 * (((row >> 1) ^ (row >> 3)) & 1) | 2 * ((row >> 2) & 1));
+}
+template <int D>
+__device__ __forceinline__ int value_swizzle(int row) {
+  return D == 128 ? 2 * (row & 7) : 2 * ((row & 3) ^ ((row >> 2) & 1));
+}
+
 constexpr float kTau = 8.0f;    // log2 of the growth of a row's maximum that is let pass
 constexpr int kPartTiles = 8;   // no part of a block's keys is shorter, but the last
 
@@ -933,8 +944,8 @@ __global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, Sl
 #pragma unroll
   for (int i = 0; i < C::NDMA; ++i) {
     const int at = (i * 4 + w) * C::RPK + lrow;
-    dk[i] = lrow * rst + ((slot ^ swz16_k<D>(at)) << 4);
-    dv[i] = lrow * rst + ((slot ^ swz16_v<D>(at)) << 4);
+    dk[i] = lrow * rst + ((slot ^ key_swizzle<D>(at)) << 4);
+    dv[i] = lrow * rst + ((slot ^ value_swizzle<D>(at)) << 4);
   }
   auto stage16 = [&](const Tile& t, int buf, bool cut) {
 #pragma unroll
@@ -977,7 +988,7 @@ __global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, Sl
   };
   auto commit4 = [&](int buf) {
     unsigned char* dst = smem + (isv ? C::VBUF : C::KBUF) + buf * C::TILEB + crow * C::ROWB;
-    const int swz = isv ? swz16_v<D>(crow) : swz16_k<D>(crow);
+    const int swz = isv ? value_swizzle<D>(crow) : key_swizzle<D>(crow);
     const float cscale = e8m0(cbyte);
 #pragma unroll
     for (int i = 0; i < C::KS; ++i)
@@ -987,13 +998,13 @@ __global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, Sl
   // ---- per-lane operand offsets
   int ka[C::KS];  // K row c, chunk 4 ks + G
 #pragma unroll
-  for (int ks = 0; ks < C::KS; ++ks) ka[ks] = c * C::ROWB + (((4 * ks + G) ^ swz16_k<D>(c)) << 4);
+  for (int ks = 0; ks < C::KS; ++ks) ka[ks] = c * C::ROWB + (((4 * ks + G) ^ key_swizzle<D>(c)) << 4);
   int va[C::FB];  // transposed V reads: row 4 G + k4 (+ 16), features 16 fb + 4 cc .. + 3
   {
     const int k4 = (lane >> 2) & 3, cc = lane & 3, r = 4 * G + k4;
 #pragma unroll
     for (int fb = 0; fb < C::FB; ++fb)
-      va[fb] = r * C::ROWB + (((2 * fb + (cc >> 1)) ^ swz16_v<D>(r)) << 4) + ((cc & 1) << 3);
+      va[fb] = r * C::ROWB + (((2 * fb + (cc >> 1)) ^ value_swizzle<D>(r)) << 4) + ((cc & 1) << 3);
   }
 
   float mused[2] = {-kInf, -kInf}, lsum[2] = {0.f, 0.f};  // raw scores' reference, this lane's part of the sum

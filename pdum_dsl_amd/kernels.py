@@ -1050,7 +1050,8 @@ def paged_attention(
     that sees nothing (or only scores of -inf) has o = 0 and lse = -inf. Rows
     of no sequence likewise; ``out`` (q's shape and type, or q itself) they
     leave as it is.
-    The 4 bits are exact in the 16-bit type but for f16 under 2^-24."""
+    The 4 bits are exact in bf16; in f16 they round under scales of 2^-23,
+    and pass 65504 in caches that :func:`paged_append` did not fill."""
     cc, _, dtype, heads, d, _ = cache._call
     b = _paged("paged_attention", cache, table, starts, lengths, q.shape[0] if q.dim() == 3 else 0, (q, out))
     qs = _tokens("paged_attention", "q", q, dtype, None, d)

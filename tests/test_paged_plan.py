@@ -4,6 +4,9 @@ states where the merge reads them; the prompt kernel's slots belong to one
 block of one sequence each; starts and lengths of any values reach no row, page
 or state out of range."""
 
+import re
+from pathlib import Path
+
 import numpy as np
 import pytest
 
@@ -171,3 +174,14 @@ def test_every_head_and_slot_has_one_workgroup(heads, nslots):
     grid = _head_slot(0, heads, nslots)[1]
     got = [x for x in (_head_slot(b, heads, nslots)[0] for b in range(grid)) if x is not None]
     assert sorted(got) == [(h, s) for h in range(heads) for s in range(nslots)]
+
+
+def test_prompt_tiles_are_laid_out_as_the_forward_kernels():
+    """The swizzles of the prompt kernel's tiles are the forward kernel's, whose reads other tests hold to no bank conflicts."""
+    src = Path(__file__).resolve().parents[1] / "pdum_dsl_amd" / "csrc"
+
+    def body(name, file):
+        return re.search(r"int %s\(int row\) \{\s*return (.*?);\s*\}" % name, (src / file).read_text(), re.S).group(1)
+
+    for paged, dense in (("key_swizzle", "swz16_k"), ("value_swizzle", "swz16_v")):
+        assert body(paged, "paged_attn.hip") == body(dense, "flash_fwd.hip")
