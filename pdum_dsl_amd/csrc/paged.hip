@@ -1,17 +1,22 @@
 // A paged cache's rows: appending keys and values with their positions' rotation on the way, and reading them back.
 //
-// Append. A row's (heads_q + 2 heads_kv) heads are cut into chunks of 8 features, one a thread; a chunk's partner in the
-// rotation (features f and f + rotated / 2) is read by its own thread too, from the cache line that the neighbours have
-// brought. y = x cos -+ partner sin in fp32, each product and the sum rounded (no fma): the same two roundings for both of a
-// pair, and what elementary fp32 operations give. Then one rounding to the type, or to 4 bits: four neighbouring threads
-// hold a scale's 32 features, so its maximum takes two exchanges. Bytes bound it: each input is read and each output
-// written once. 8 x 1024 tokens, 32/8 heads of 128: 39 us, 202 MB (5.2 TB/s, as a copy of that size from memory); to 4 bits
-// 41 us, 181 MB (4.4; VALU half busy with the rotation and the scales). 64 single tokens: 3.7 us, a launch. A workgroup
-// takes chunks of one row, whose sequence is looked up once.
+// Append. A row's (heads_q + 2 heads_kv) heads are cut into chunks of 8 features, one or four a thread, whose features are
+// alike; a chunk's partner in the rotation (features f and f + rotated / 2) is read by its own thread too, from the cache
+// line that the neighbours have brought. y = x cos -+ partner sin in fp32, each product and the sum rounded (no fma): the
+// same two roundings for both of a pair, and what elementary fp32 operations give. Then one rounding to the type, or to 4
+// bits: four neighbouring threads hold a scale's 32 features, so its maximum takes two exchanges.
+//
+// Bytes bound it, each input read and each output written once, and before them the chain of loads to a token's place
+// (starts, lengths, page), which is why a thread asks for all of its chunks first. 8 x 1024 tokens, 32/8 heads of 128, inputs
+// in turn: 44.5 us, 202 MB (4.5 TB/s; 34 where they are in the last-level cache), with 1 / 2 / 3 / 6 chunks a thread 50 / 48 /
+// 44 / 47; to 4 bits 35 there, 181 MB, with one chunk 41. Short calls have too few threads so: 64 single tokens 3.3 us with
+// one, 4.0 with four (a launch).
 #include "paged.h"
 
 namespace pdh {
 namespace {
+
+constexpr int64_t kManyItems = 1024 * 256;  // us with one / four a thread: 49000 3.3 / 4.0, 110000 6.3 / 6.9, 390000 5.4 / 4.9
 
 struct AppendArgs {
   const uint16_t *k, *v, *q;
@@ -70,28 +75,31 @@ __device__ __forceinline__ uint32_t fp4_codes(const float (&y)[8], uint32_t& byt
   return codes;
 }
 
-template <typename T, int D, int BITS>
+template <typename T, int D, int BITS, int NC>
 __global__ __launch_bounds__(256) void paged_append(AppendArgs a) {
   constexpr int CPH = D / 8;  // chunks a head
   const int row = blockIdx.x;
-  const int item = blockIdx.y * 256 + threadIdx.x;
+  const int item0 = blockIdx.y * (256 * NC) + threadIdx.x;  // q's heads, then k's, then v's
   const int hkv = static_cast<int>(a.c.heads);
-  const int head = item / CPH, f0 = item % CPH * 8;  // q's heads, then k's, then v's
-  const bool live = head < a.heads_q + 2 * hkv;      // alike for four neighbours
-  const int kind = head < a.heads_q ? 0 : (head < a.heads_q + hkv ? 1 : 2);
-  const int h = kind == 0 ? head : (kind == 1 ? head - a.heads_q : head - a.heads_q - hkv);
-  const uint16_t* src = kind == 0   ? a.q + row * a.q_st + h * a.q_sh
-                        : kind == 1 ? a.k + row * a.k_st + h * a.k_sh
-                                    : a.v + row * a.v_st + h * a.v_sh;
-  const bool turn = kind < 2 && a.rotary && f0 < a.rotated;
-  const int half = a.rotated >> 1;
-  const bool upper = f0 >= half;  // of a pair of halves
-  u32x4 x = {0u, 0u, 0u, 0u}, px = {0u, 0u, 0u, 0u};
-  if (live) x = *reinterpret_cast<const u32x4*>(src + f0);
-  if (live && turn && !a.interleaved) px = *reinterpret_cast<const u32x4*>(src + (upper ? f0 - half : f0 + half));
+  const int heads = a.heads_q + 2 * hkv, half = a.rotated >> 1;
+  const int f0 = item0 % CPH * 8;  // alike for all chunks of a thread
+  const bool upper = f0 >= half;   // of a pair of halves
+  auto head_of = [&](int j) { return (item0 + 256 * j) / CPH; };  // alike for four neighbours
+  auto turned = [&](int head) { return head < a.heads_q + hkv && a.rotary && f0 < a.rotated; };
+  u32x4 x[NC], px[NC];
+#pragma unroll
+  for (int j = 0; j < NC; ++j) {
+    const int head = head_of(j);
+    x[j] = px[j] = u32x4{0u, 0u, 0u, 0u};
+    if (head >= heads) continue;
+    const uint16_t* src = head < a.heads_q         ? a.q + row * a.q_st + head * a.q_sh
+                          : head < a.heads_q + hkv ? a.k + row * a.k_st + (head - a.heads_q) * a.k_sh
+                                                   : a.v + row * a.v_st + (head - a.heads_q - hkv) * a.v_sh;
+    x[j] = *reinterpret_cast<const u32x4*>(src + f0);
+    if (turned(head) && !a.interleaved) px[j] = *reinterpret_cast<const u32x4*>(src + (upper ? f0 - half : f0 + half));
+  }
 
   const int seq = seq_of_row(a.b, row);
-  if (!live) return;
   int pos = -1, page = -1;
   bool owned = false;
   if (seq < a.b.seqs) {
@@ -101,60 +109,69 @@ __global__ __launch_bounds__(256) void paged_append(AppendArgs a) {
     if (owned && (!a.rotary || pos < a.positions)) page = page_of(a.b, a.c, a.shift, seq, pos);
   }
   if (!owned && !a.zero_rest) return;
-  if (owned && page < 0 && item == 0 && a.bad) atomicAdd(a.bad, 1);
-  uint16_t* qo = a.qo + row * a.qo_st + h * a.qo_sh + f0;
-  if (page < 0) {  // of no sequence, or a token without a place
-    if (kind == 0) *reinterpret_cast<u32x4*>(qo) = u32x4{0u, 0u, 0u, 0u};
-    return;
+  if (owned && page < 0 && item0 == 0 && a.bad) atomicAdd(a.bad, 1);
+  const bool nowhere = page < 0;  // of no sequence, or a token without a place
+  const int in_page = pos & ((1 << a.shift) - 1);
+  const int64_t place = nowhere ? 0 : pool_at<BITS>(a.c, page, in_page);
+  const float* cs = a.rotary + pos * a.ld_rotary;
+  f32x4u c[2], sn[2];  // of this thread's features: pairs (four of each), or halves (eight)
+  if (!nowhere && a.rotary && f0 < a.rotated) {
+    const int at = a.interleaved ? f0 >> 1 : (upper ? f0 - half : f0);
+    c[0] = *reinterpret_cast<const f32x4u*>(cs + at);
+    sn[0] = *reinterpret_cast<const f32x4u*>(cs + half + at);
+    if (!a.interleaved) {
+      c[1] = *reinterpret_cast<const f32x4u*>(cs + at + 4);
+      sn[1] = *reinterpret_cast<const f32x4u*>(cs + half + at + 4);
+    }
   }
-
-  u32x4 out = x;
-  float y[8];
-  unpack8<T>(x, y);
-  if (turn) {
+#pragma unroll
+  for (int j = 0; j < NC; ++j) {
+    const int head = head_of(j);
+    if (head >= heads) break;
+    const int kind = head < a.heads_q ? 0 : (head < a.heads_q + hkv ? 1 : 2);
+    if (nowhere) {
+      if (kind == 0) *reinterpret_cast<u32x4*>(a.qo + row * a.qo_st + head * a.qo_sh + f0) = u32x4{0u, 0u, 0u, 0u};
+      continue;
+    }
+    u32x4 out = x[j];
+    float y[8];
+    unpack8<T>(x[j], y);
+    if (turned(head)) {
 #pragma clang fp contract(off)
-    const float* cs = a.rotary + pos * a.ld_rotary;
-    if (a.interleaved) {
-      const f32x4u c = *reinterpret_cast<const f32x4u*>(cs + (f0 >> 1));
-      const f32x4u s = *reinterpret_cast<const f32x4u*>(cs + half + (f0 >> 1));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float u = y[2 * i], w = y[2 * i + 1];
-        y[2 * i] = u * c[i] - w * s[i];
-        y[2 * i + 1] = w * c[i] + u * s[i];
-      }
-    } else {
-      float p[8];
-      unpack8<T>(px, p);
-      const int at = upper ? f0 - half : f0;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const f32x4u c = *reinterpret_cast<const f32x4u*>(cs + at + 4 * j);
-        const f32x4u s = *reinterpret_cast<const f32x4u*>(cs + half + at + 4 * j);
+      if (a.interleaved) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float yc = y[4 * j + i] * c[i], ps = p[4 * j + i] * s[i];
-          y[4 * j + i] = upper ? yc + ps : yc - ps;
+          const float u = y[2 * i], w = y[2 * i + 1];
+          y[2 * i] = u * c[0][i] - w * sn[0][i];
+          y[2 * i + 1] = w * c[0][i] + u * sn[0][i];
+        }
+      } else {
+        float p[8];
+        unpack8<T>(px[j], p);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float yc = y[i] * c[i >> 2][i & 3], ps = p[i] * sn[i >> 2][i & 3];
+          y[i] = upper ? yc + ps : yc - ps;
         }
       }
+      out = pack8<T>(y);
     }
-    out = pack8<T>(y);
-  }
-  if (kind == 0) {
-    *reinterpret_cast<u32x4*>(qo) = out;
-    return;
-  }
-  const int in_page = pos & ((1 << a.shift) - 1);
-  const int64_t place = pool_at<BITS>(a.c, page, in_page) + h * a.c.sh;
-  if constexpr (BITS == 16) {
-    *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(kind == 1 ? a.c.k : a.c.v) + place + f0) = out;
-  } else {
-    uint32_t byte;
-    const uint32_t codes = fp4_codes<T>(y, byte);
-    *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(kind == 1 ? a.c.k : a.c.v) + place + f0 / 2) = codes;
-    if ((f0 & 31) == 0) {
-      const int64_t sp = scale_at(a.c, page, in_page) + h * a.c.ssh;
-      static_cast<uint8_t*>(kind == 1 ? a.c.k_scale : a.c.v_scale)[sp + f0 / 32] = static_cast<uint8_t>(byte);
+    if (kind == 0) {
+      *reinterpret_cast<u32x4*>(a.qo + row * a.qo_st + head * a.qo_sh + f0) = out;
+      continue;
+    }
+    const int h = kind == 1 ? head - a.heads_q : head - a.heads_q - hkv;
+    const int64_t at = place + h * a.c.sh;
+    if constexpr (BITS == 16) {
+      *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(kind == 1 ? a.c.k : a.c.v) + at + f0) = out;
+    } else {
+      uint32_t byte;
+      const uint32_t codes = fp4_codes<T>(y, byte);
+      *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(kind == 1 ? a.c.k : a.c.v) + at + f0 / 2) = codes;
+      if ((f0 & 31) == 0) {
+        const int64_t sp = scale_at(a.c, page, in_page) + h * a.c.ssh;
+        static_cast<uint8_t*>(kind == 1 ? a.c.k_scale : a.c.v_scale)[sp + f0 / 32] = static_cast<uint8_t>(byte);
+      }
     }
   }
 }
@@ -167,7 +184,7 @@ struct RowsArgs {
   int shift, zero_rest;
 };
 
-// A chunk of 8 features a thread, as above: 8 x 1024 tokens of 4 bits 12.4 us, 55 MB (4.4 TB/s).
+// A chunk of 8 features a thread: 8 x 1024 tokens of 4 bits, 8 heads of 128, 12.5 us, 55 MB (4.4 TB/s); four, 13.9.
 template <typename T, int D, int BITS>
 __global__ __launch_bounds__(256) void paged_rows(RowsArgs a) {
   constexpr int CPH = D / 8;
@@ -205,6 +222,15 @@ __global__ __launch_bounds__(256) void paged_rows(RowsArgs a) {
   *reinterpret_cast<u32x4*>(out + f0) = x;
 }
 
+// f(chunks a thread): four where they fill the chip all the same, one where a call is short.
+template <typename F>
+void by_chunks(int64_t rows, int64_t items, F f) {
+  if (rows * items > kManyItems)
+    f(std::integral_constant<int, 4>{});
+  else
+    f(std::integral_constant<int, 1>{});
+}
+
 }  // namespace
 }  // namespace pdh
 
@@ -236,9 +262,12 @@ extern "C" int pdh_paged_append(const void* k, const void* v, const void* q, voi
                      rotary, ld_rotary, positions, static_cast<int>(rotary ? rotated : 0), interleaved != 0,
                      static_cast<int>(heads_q), shift, zero_rest != 0, bad};
   const int64_t items = (heads_q + 2 * cache->heads) * (cache->features / 8);
-  const dim3 grid(static_cast<unsigned>(batch->rows), static_cast<unsigned>((items + 255) / 256));
-  by_kind(*cache, [&](auto t, auto d, auto bits) {
-    paged_append<decltype(t), decltype(d)::value, decltype(bits)::value><<<grid, 256, 0, as_stream(stream)>>>(a);
+  by_chunks(batch->rows, items, [&](auto nc) {
+    constexpr int NC = decltype(nc)::value;
+    const dim3 grid(static_cast<unsigned>(batch->rows), static_cast<unsigned>((items + 256 * NC - 1) / (256 * NC)));
+    by_kind(*cache, [&](auto t, auto d, auto bits) {
+      paged_append<decltype(t), decltype(d)::value, decltype(bits)::value, NC><<<grid, 256, 0, as_stream(stream)>>>(a);
+    });
   });
   return check_launch("pdh_paged_append");
 }
