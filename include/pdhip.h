@@ -340,7 +340,8 @@ typedef struct pdh_paged_cache {
 /* The sequences of one call, device memory that the kernels read when they
  * run: sequence i's new tokens are rows starts[i] .. starts[i + 1] - 1 (starts
  * ascend from 0) and the last of its lengths[i] tokens: row r has position
- * lengths[i] - (starts[i + 1] - r). Values out of range reach no memory: a
+ * lengths[i] - (starts[i + 1] - r). At most 2^20 sequences and 2^24 - 1 rows
+ * a call. Values out of range reach no memory: a
  * row outside [0, rows) is not there, a token before 0, past the table or on a
  * page outside the pool has no place. */
 typedef struct pdh_paged_batch {
@@ -388,7 +389,7 @@ int pdh_paged_rows(void* k_out, void* v_out, int64_t ko_st, int64_t ko_sh, int64
  * factors. Tokens that a row does not see count for nothing in it whatever the
  * pools hold. A row that sees nothing, or scores of -inf alone: o = 0, lse =
  * -inf; rows of no sequence likewise where zero_rest != 0, else they are not
- * written. ws, 16-byte aligned, holds pdh_paged_attention_workspace bytes for
+ * written. o may be q, with q's strides. ws, 16-byte aligned, holds pdh_paged_attention_workspace bytes for
  * the same sizes (partial states of rows whose keys several workgroups share).
  * Nothing is atomic: results repeat bit for bit. No counterpart in the
  * reference. */

@@ -781,7 +781,7 @@ def attn_decode_static(
 # ------------------------------------------------------------- paged caches
 
 
-@dataclass(frozen=True)
+@dataclass(frozen=True, eq=False)
 class PagedCache:
     """Keys and values of many sequences in pages of ``page_rows`` tokens
     (a power of two, 16 to 4096): a sequence's tokens lie in the pages that its row of a

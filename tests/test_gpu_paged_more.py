@@ -315,3 +315,39 @@ def test_no_rows_to_append(K):
     x = torch.empty((0, 8, 64), dtype=torch.bfloat16, device="cuda")
     got = K.paged_append(x[:, 4:6], x[:, 6:], cache, *_ints([[0]], [0, 0], [7]), q=x[:, :4], rotary=K.rotary_table(9, 64))
     assert got.shape == (0, 4, 64) and (cache.k == 0).all()
+
+
+@pytest.mark.parametrize("dtype,bits,hq,hkv,d,rotated,pairs", [
+    ("bf16", 16, 32, 8, 128, 128, False), ("f16", 4, 32, 8, 128, 64, True), ("bf16", 4, 13, 13, 64, 64, False),
+    ("f16", 16, 7, 3, 64, 16, True), ("bf16", 16, 0, 40, 128, 0, False),
+])
+def test_a_large_batch_is_its_small_ones(K, dtype, bits, hq, hkv, d, rotated, pairs):
+    """Rows enough for several chunks a thread (over 2^18 of 8 features in all): the bits of the same rows appended a few at a time."""
+    rng = np.random.default_rng(33)
+    lengths, pr = [3001, 40, 1500, 0, 777], 32
+    new = [int(min(n, m)) for n, m in zip(lengths, [2900, 40, 1499, 0, 500])]
+    table, starts, lens, rows, pages = batch(rng, lengths, new, pr, pad=17)
+    assert rows * (hq + 2 * hkv) * (d // 8) > 1 << 18
+    table[2, 5] = pages  # a page outside the pool: its tokens are dropped
+    caches = [K.paged_cache(pages, hkv, pr, d, DT[dtype], bits=bits) for _ in range(2)]
+    x = torch.as_tensor(rng.standard_normal((rows, max(hq, 1) + 2 * hkv, d))).to(DT[dtype]).cuda()
+    q, k, v = (x[:, :hq] if hq else None), x[:, -2 * hkv : -hkv], x[:, -hkv:]
+    rot = K.rotary_table(3000, rotated) if rotated else None  # the first sequence's last token lies past it
+    bad = torch.zeros(2, dtype=torch.int32, device="cuda")
+    got = K.paged_append(k, v, caches[0], *_ints(table, starts, lens), q=q, rotary=rot, interleaved=pairs, bad=bad[:1])
+    for i in range(len(lens)):
+        for r in range(starts[i], starts[i + 1], 150):
+            n = min(150, starts[i + 1] - r)
+            t = _ints(table[i : i + 1], [0, n], [lens[i] - (starts[i + 1] - r) + n])
+            part = K.paged_append(k[r : r + n], v[r : r + n], caches[1], *t, q=q[r : r + n] if hq else None, rotary=rot,
+                                  interleaved=pairs, bad=bad[1:])
+            assert not hq or torch.equal(part, got[r : r + n])
+    assert not hq or (got[starts[-1] :] == 0).all()
+    assert int(bad[0]) == int(bad[1]) == 32 + bool(rotated)
+    for a, b in ((getattr(c, n) for c in caches) for n in ("k", "v", "k_scale", "v_scale") if bits == 4 or len(n) == 1):
+        assert torch.equal(a, b)
+    if hq:  # in q's place
+        turned = x.clone()
+        at = turned[:, :hq]
+        K.paged_append(k, v, caches[1], *_ints(table, starts, lens), q=at, rotary=rot, interleaved=pairs, out=at)
+        assert torch.equal(at[: starts[-1]], got[: starts[-1]]) and torch.equal(turned[starts[-1] :], x[starts[-1] :])
