@@ -11,6 +11,8 @@ import numpy as np
 import pytest
 
 LIMIT = 1 << 30
+SOURCES = Path(__file__).resolve().parents[1] / "pdum_dsl_amd" / "csrc"
+ITEM, LEAST = map(int, re.search(r"ITEM = (\d+), LEAST = (\d+);", (SOURCES / "paged_attn.hip").read_text()).groups())
 
 
 def _seq(starts, lengths, i, rows):
@@ -29,7 +31,7 @@ def _plan(starts, lengths, i, rows, group, reach, window, sinks, per_block, keys
     return r0, n, pos0, -(-n * group // per_block), sb, wb, max(sb + eb - wb, 1)
 
 
-def _shares(plans, heads, grid, item_cost=4, least=8):
+def _shares(plans, heads, grid, item_cost=ITEM, least=LEAST):
     """What each workgroup sweeps: (workgroup, sequence, item, first block, end block, its record or None, cut's last)."""
     cost = [p[3] * (p[6] + item_cost) * heads for p in plans]
     total = sum(cost)
@@ -178,10 +180,8 @@ def test_every_head_and_slot_has_one_workgroup(heads, nslots):
 
 def test_prompt_tiles_are_laid_out_as_the_forward_kernels():
     """The swizzles of the prompt kernel's tiles are the forward kernel's, whose reads other tests hold to no bank conflicts."""
-    src = Path(__file__).resolve().parents[1] / "pdum_dsl_amd" / "csrc"
-
     def body(name, file):
-        return re.search(r"int %s\(int row\) \{\s*return (.*?);\s*\}" % name, (src / file).read_text(), re.S).group(1)
+        return re.search(r"int %s\(int row\) \{\s*return (.*?);\s*\}" % name, (SOURCES / file).read_text(), re.S).group(1)
 
     for paged, dense in (("key_swizzle", "swz16_k"), ("value_swizzle", "swz16_v")):
         assert body(paged, "paged_attn.hip") == body(dense, "flash_fwd.hip")
