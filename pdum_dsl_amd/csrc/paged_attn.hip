@@ -921,7 +921,7 @@ __global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, Sl
     return !a.has(p) | (key > pos_hi) | (key >= a.reach) | ((key >= a.sinks) & (key <= pos_lo - a.window));
   };
   const int in_mask = (1 << a.shift) - 1;
-  bool lost = false;  // a tile that every row should see whole lacks a page
+  bool lost = false;  // a tile of a pair that every row should see whole lacks a page
 
   // ---- staging. A wave's part of a tile lies in one half, in one page: one buffer resource a pool with the page's place as
   // the scalar offset, or FAR, a resource a page; a lane's address is one offset that does not change.
@@ -1126,8 +1126,8 @@ __global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, Sl
     __builtin_amdgcn_s_setprio(0);
   };
 
-  // Tiles [c0, c1) are whole for every row of the block; before them lie the first tokens and the window's left edge,
-  // behind them the diagonal.
+  // Tiles [c0, c1) are whole for every row of the block, as far as their pages are there; before them lie the first tokens
+  // and the window's left edge, behind them the diagonal.
   int c0, c1;
   {
     const int edge = pos_hi - a.window + 1;
@@ -1140,7 +1140,10 @@ __global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, Sl
   }
   if (v0 < v1) {
     auto bound = [&](int v) { return v < v1 ? v : v1 - 1; };
-    auto is_cut = [&](int v) { return v < c0 || v >= c1; };
+    // Whole tiles go in pairs; a last single one is computed, and therefore staged, with the cut ones: a half without a page
+    // is zeros there, and a page of somebody else's, looked at afterwards (`lost`), in a pair alone.
+    const int pairs = c0 + ((c1 - c0) & ~1);
+    auto is_cut = [&](int v) { return v < c0 || v >= pairs; };
     Tile cur = tile_at(v0), next = tile_at(bound(v0 + 1));
     const int odd = c0 & 1;  // tile v lies in buffer (v ^ odd) & 1: the whole ones start in buffer 0
     if constexpr (BITS == 16) {
@@ -1171,7 +1174,6 @@ __global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, Sl
       cur = next;
       next = after;
     };
-    const int pairs = c0 + ((c1 - c0) & ~1);  // whole tiles go in pairs; a last single one goes with the cut ones
 #pragma unroll 1
     for (int v = v0; v < v1;) {
 #pragma unroll 1
