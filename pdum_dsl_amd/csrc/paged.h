@@ -3,7 +3,8 @@
 // Cache: pools [pages][heads][page_rows][features]; token s of sequence i lies in page table[i][s / page_rows], row
 // s % page_rows. Batch: sequence i's new tokens are rows starts[i] .. starts[i + 1] - 1 of the call's tensors and the last
 // of its lengths[i] tokens. starts, lengths and the table are device memory that no host code has seen, so every kernel
-// clamps what it derives from them: rows to [0, rows), positions to the table's reach, page numbers to the pool.
+// clamps what it derives from them: rows to [0, rows), keys to the table's reach, page numbers to the pool. A row's position
+// goes by starts as it stands, lengths[i] - (starts[i + 1] - row), whether or not the rows behind it are there.
 #pragma once
 
 #include "common.h"
@@ -14,20 +15,24 @@
 namespace pdh {
 
 constexpr int kMaxTokens = 1 << 30;  // a table's reach: positions and keys are 32-bit
+// Lengths count as no more: the positions of up to 2^24 rows that end there are all past every table, and a window from
+// them, another 2^30 back, is still a 32-bit number.
+constexpr int kMaxLength = kMaxTokens + (1 << 24);
 
 // One sequence's part of a batch.
 struct Seq {
   int row0, n;  // its first row and number of new tokens
-  int len;      // tokens in the cache, the new ones included, in [0, kMaxTokens]
+  int len;      // tokens in the cache up to its last row that is there, in [0, kMaxLength]; 0 where all rows lie before it
 };
 
 __device__ __forceinline__ int clamp_row(int r, int rows) { return r < 0 ? 0 : (r < rows ? r : rows); }
 
 __device__ __forceinline__ Seq seq_at(const pdh_paged_batch& b, int i) {
   const int rows = static_cast<int>(b.rows);
-  const int r0 = clamp_row(b.starts[i], rows), r1 = clamp_row(b.starts[i + 1], rows);
-  const int len = b.lengths[i];
-  return Seq{r0, r1 > r0 ? r1 - r0 : 0, len < 0 ? 0 : (len < kMaxTokens ? len : kMaxTokens)};
+  const int end = b.starts[i + 1], r0 = clamp_row(b.starts[i], rows), r1 = clamp_row(end, rows);
+  const int held = b.lengths[i];
+  const int len = (held > 0 ? held : 0) - (end > rows ? end - rows : 0);  // less the tokens whose rows are not there
+  return Seq{r0, r1 > r0 ? r1 - r0 : 0, len < 0 ? 0 : (len < kMaxLength ? len : kMaxLength)};
 }
 
 // The sequence that owns a row: the number of sequences that end at or before it (seqs: none owns it). One wave, every

@@ -1366,7 +1366,7 @@ extern "C" int pdh_paged_attention(const void* q, void* o, float* lse, int64_t h
     PDH_REQUIRE(s >= 0 && s % 8 == 0, PDH_EINVAL, "pdh_paged_attention: strides must be multiples of 8 elements, >= 0");
   PagedAttn a{static_cast<const uint16_t*>(q), static_cast<uint16_t*>(o), lse, q_st, q_sh, o_st, o_sh, *cache, *batch,
               static_cast<int>(heads_q), static_cast<int>(heads_q / cache->heads),
-              static_cast<int>(window < kMaxTokens ? window : kMaxTokens),
+              static_cast<int>(window < kMaxTokens ? window : kMaxLength),  // of 2^30 and more: every position's whole past
               static_cast<int>(sinks < kMaxTokens ? sinks : kMaxTokens), shift, zero_rest != 0,
               static_cast<int>(batch->width << shift), scale * kLog2e,
               batch->width > 0 ? batch->table : batch->starts, static_cast<int>(batch->width > 0 ? batch->width - 1 : 0),

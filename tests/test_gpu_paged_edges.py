@@ -49,3 +49,85 @@ def test_a_missing_page_is_not_another_ones(K, dtype, bits, missing, half, windo
     o, lse = K.paged_attention(q, cache, *_ints(table, starts, lens), window=window, sinks=2)
     want = op.attention(_host(q), pk, pv, table, starts, lens, scale=d**-0.5, window=window, sinks=2)
     check_attention(_host(o), _host(lse), want, dtype, d, f"missing {missing}, half {half}")
+
+
+@pytest.mark.parametrize("starts,lengths,rows", [
+    ([0, 8], [8], 5), ([0, 3, 12], [20, 30], 7), ([0, 90], [150], 61), ([0, 1, 200, 300], [40, 210, 100], 130),
+    ([0, 2**31 - 1], [2**31 - 1], 8), ([0, 2**31 - 1], [2**31 - 1], 40), ([0, 2**31 - 1], [30], 40),
+])
+@pytest.mark.parametrize("bits", [16, 4])
+def test_sequences_that_go_on_behind_the_rows(K, starts, lengths, rows, bits):
+    """A call of fewer rows than starts describes: the rows that are there have the positions that they would have."""
+    rng = np.random.default_rng(41)
+    pr, d, hq, hkv = 16, 64, 4, 2
+    n, width = len(lengths), 14
+    pages = n * width
+    table = rng.permutation(pages).reshape(n, width).astype(np.int32)
+    cache = K.paged_cache(pages, hkv, pr, d, bits=bits)
+    whole, *_ = _pools(rng, K, "bf16", bits, pages, hkv, pr, d)
+    for a, b in ((cache.k, whole.k), (cache.v, whole.v), (cache.k_scale, whole.k_scale), (cache.v_scale, whole.v_scale)):
+        if a is not None:
+            a.copy_(b)
+    x = torch.as_tensor(rng.standard_normal((rows, hq + 2 * hkv, d))).bfloat16().cuda()
+    tab = op.rotary_table(300, d)
+    bad = torch.zeros(1, dtype=torch.int32, device="cuda")
+    t = _ints(table, starts, lengths)
+    q = K.paged_append(x[:, hq : hq + hkv], x[:, hq + hkv :], cache, *t, q=x[:, :hq], rotary=torch.as_tensor(tab).cuda(), bad=bad)
+    gk, gv = K.paged_rows(cache, *t, rows)
+    want_q, dropped = np.zeros((rows, hq, d)), 0
+    owned = np.zeros((pages, pr), dtype=bool)
+    for r, i, pos in op.tokens(starts, lengths, rows):
+        w = op.place(table, i, pos, pr, pages)
+        if w is None:
+            dropped += 1
+            assert (gk[r] == 0).all() and (gv[r] == 0).all()
+            continue
+        owned[w] = True
+        want_q[r] = torch.as_tensor(op.rotate(x[r, :hq].float().cpu().numpy(), tab[pos], False)).bfloat16().double().numpy()
+        if bits == 16:
+            assert torch.equal(cache.v[w[0], :, w[1]], x[r, hq + hkv :])
+            assert torch.equal(gk[r], cache.k[w[0], :, w[1]]) and torch.equal(gv[r], x[r, hq + hkv :])
+        else:
+            codes, scale = op.fp4(_host(x[r, hq + hkv :]), 125)
+            np.testing.assert_array_equal(_host(gv[r]), op.fp4_values(codes, scale))
+    assert int(bad) == dropped
+    np.testing.assert_array_equal(_host(q), want_q)
+    for a, b in ((cache.k, whole.k), (cache.v, whole.v)):  # and nothing else is stored
+        same = (a == b).all(-1).all(1).cpu().numpy()
+        assert same[~owned].all()
+    full = torch.arange(0, n * width * pr + 1, width * pr)
+    kk, vv = (_host(y).reshape(pages, pr, hkv, d).transpose(0, 2, 1, 3) for y in K.paged_rows(
+        cache, torch.arange(pages, dtype=torch.int32, device="cuda").view(n, width), *_ints(full, [width * pr] * n), pages * pr))
+    for window, sinks in ((None, 0), (50, 3)):
+        o, lse = K.paged_attention(q, cache, *t, window=window, sinks=sinks)
+        want = op.attention(_host(q), kk, vv, table, starts, lengths, scale=d**-0.5, window=window, sinks=sinks)
+        check_attention(_host(o), _host(lse), want, "bf16", d, f"{starts} {window}")
+
+
+@pytest.mark.parametrize("rows", [5, 60])
+def test_lengths_past_the_longest_table(K, rows):
+    """A table of 2^30 tokens and lengths over that: tokens past it have no place, those before it keep theirs, and a window
+    goes by the positions as they are."""
+    rng = np.random.default_rng(42)
+    pr, d, hq, hkv, reach = 4096, 64, 4, 2, 1 << 30
+    table = torch.full((1, reach // pr), -1, dtype=torch.int32, device="cuda")
+    table[0, -1] = 1
+    cache, pk, pv = _pools(rng, K, "bf16", 16, 3, hkv, pr, d)
+    x = torch.as_tensor(rng.standard_normal((rows, hq + 2 * hkv, d))).bfloat16().cuda()
+    q, v = x[:, :hq], x[:, hq + hkv :]
+    past = rows - 2
+    for length, fits in ((reach + past, 2), (reach + 3 * rows, 0), (2**31 - 1, 0)):
+        before = cache.v.clone()
+        bad = torch.zeros(1, dtype=torch.int32, device="cuda")
+        t = (table, *_ints([0, rows], [length]))
+        K.paged_append(x[:, hq : hq + hkv], v, cache, *t, bad=bad)
+        assert int(bad) == rows - fits
+        want = before.clone()
+        for r in range(fits):
+            want[1, :, pr - fits + r] = v[r]
+        assert torch.equal(cache.v, want)
+        # the same by a table of the last page alone, with all positions 2^30 - 4096 earlier
+        o, lse = K.paged_attention(q, cache, *t, window=500)
+        near = [[1]], [0, rows], [min(length - reach + pr, 9000)]
+        ref = op.attention(_host(q), _host(cache.k), _host(cache.v), np.array(near[0]), near[1], near[2], scale=d**-0.5, window=500)
+        check_attention(_host(o), _host(lse), ref, "bf16", d, str(length))
