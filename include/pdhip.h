@@ -339,12 +339,12 @@ typedef struct pdh_paged_cache {
 
 /* The sequences of one call, device memory that the kernels read when they
  * run: sequence i's new tokens are rows starts[i] .. starts[i + 1] - 1 (starts
- * ascend from 0) and the last of its lengths[i] tokens: row r has position
- * lengths[i] - (starts[i + 1] - r). At most 2^20 sequences and 2^24 - 1 rows
- * a call. Values out of range reach no memory: a
- * row outside [0, rows) is not there (those that are keep their positions), a
- * token before 0, past the table or on a page outside the pool has no place;
- * lengths over 2^30 + 2^24 count as that. */
+ * ascend; rows before the first and behind the last are of no sequence) and the
+ * last of its lengths[i] tokens: row r has position lengths[i] - (starts[i + 1]
+ * - r). At most 2^20 sequences and 2^24 - 1 rows a call. Values out of range
+ * reach no memory: a row outside [0, rows) is not there (those that are keep
+ * their positions), a token before 0, past the table or on a page outside the
+ * pool has no place; lengths over 2^30 + 2^24 count as that. */
 typedef struct pdh_paged_batch {
   const int32_t* table;   /* [seqs][width], rows ld_table apart; width * page_rows <= 2^30 */
   const int32_t* starts;  /* [seqs + 1] */

@@ -651,8 +651,8 @@ __global__ __launch_bounds__(256, (dec_wgs<D, BITS>())) void paged_decode(PagedA
 
 // Joins a cut item's states: the workgroup that the item starts in left the first in its second record, the others up to
 // `last` theirs in their first. Eight waves: four rows at a time, half of the records each, eight of them in flight; the
-// halves meet in LDS. Then the rows behind the last sequence, spread over the grid. 5 us at 64 x 8192 tokens (as many
-// workgroups as the decode kernel's, which 1024 threads each would run in two rounds: 8).
+// halves meet in LDS. Then the rows of no sequence, before the first and behind the last, spread over the grid. 5 us at 64 x
+// 8192 tokens (as many workgroups as the decode kernel's, which 1024 threads each would run in two rounds: 8).
 template <typename T, int D>
 __global__ __launch_bounds__(512) void paged_decode_merge(PagedAttn a, const DecMeta* meta, const float* ws) {
   constexpr int RS = 2 + D, DL = D / 64;
@@ -724,11 +724,14 @@ __global__ __launch_bounds__(512) void paged_decode_merge(PagedAttn a, const Dec
     }
   }
   if (a.zero_rest) {
-    const int tail = a.b.seqs ? clamp_row(a.b.starts[a.b.seqs], static_cast<int>(a.b.rows)) : 0;
+    const int rows = static_cast<int>(a.b.rows);
+    const int before = clamp_row(a.b.starts[0], rows), tail = clamp_row(a.b.starts[a.b.seqs], rows);
+    const int64_t end = (before + static_cast<int64_t>(rows) - tail) * a.heads_q;
     const float none[DL] = {};
-    for (int64_t x = tail * static_cast<int64_t>(a.heads_q) + blockIdx.x * 8 + w; x < a.b.rows * a.heads_q;
-         x += gridDim.x * 8)
-      write_row<T, D>(a, static_cast<int>(x / a.heads_q), static_cast<int>(x % a.heads_q), -kInf, 0.f, none);
+    for (int64_t x = blockIdx.x * 8 + w; x < end; x += gridDim.x * 8) {
+      const int i = static_cast<int>(x / a.heads_q);
+      write_row<T, D>(a, i < before ? i : i - before + tail, static_cast<int>(x % a.heads_q), -kInf, 0.f, none);
+    }
   }
 }
 
@@ -810,16 +813,16 @@ __device__ __forceinline__ BlockKeys block_keys(const PagedAttn& a, int pos_lo, 
   return b;
 }
 
-// The sequence of a slot (seqs: the rows behind the last one; -1: none) and the block's number in it.
-__device__ __forceinline__ int seq_of_slot(const PagedAttn& a, int slot, int& rb) {
+// The sequence of a slot (seqs: the rows behind the last one; -1: none), the block's number in it, and the number of rows
+// before the first sequence.
+__device__ __forceinline__ int seq_of_slot(const PagedAttn& a, int slot, int& rb, int& before) {
   const int lane = threadIdx.x & 63, rows = static_cast<int>(a.b.rows);
-  auto base = [&](int64_t i) {
-    const int r = a.b.seqs ? clamp_row(a.b.starts[i], rows) : 0;
-    return static_cast<int>(static_cast<int64_t>(r) * a.group / 128 + i);
-  };
+  auto start = [&](int64_t i) { return a.b.seqs ? clamp_row(a.b.starts[i], rows) : 0; };
+  auto base = [&](int64_t i) { return static_cast<int>(static_cast<int64_t>(start(i)) * a.group / 128 + i); };
   int n = 0;
   for (int64_t i = 0; i <= a.b.seqs; i += 64)
     n += __popcll(__builtin_amdgcn_ballot_w64(i + lane <= a.b.seqs && base(i + lane) <= slot));
+  before = __builtin_amdgcn_readfirstlane(start(0));
   n = __builtin_amdgcn_readfirstlane(n) - 1;
   if (n >= 0) rb = slot - __builtin_amdgcn_readfirstlane(base(n));
   return n;
@@ -872,8 +875,14 @@ __global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, Sl
   if ((j | 3) < mp.unit_slots && (j & 4)) j ^= 3;
   j = j * mp.shares + scalar(unit % mp.shares);
   if (j >= nslots) return;
-  int rb = 0;
-  const int seq = seq_of_slot(a, nslots - 1 - j, rb);
+  int rb = 0, before;
+  const int seq = seq_of_slot(a, nslots - 1 - j, rb, before);
+  if (before > 0 && a.zero_rest && split == 0) {  // rows before the first sequence, spread over the heads' slots
+    const float none[D / 64] = {};
+    const int64_t end = static_cast<int64_t>(before) * a.heads_q;
+    for (int64_t x = (static_cast<int64_t>(head) * nslots + j) * 4 + w; x < end; x += a.c.heads * nslots * 4)
+      write_row<T, D>(a, static_cast<int>(x / a.heads_q), static_cast<int>(x % a.heads_q), -kInf, 0.f, none);
+  }
   if (seq < 0) return;
   const SeqPlan sp = uniform_plan<128>(a, seq);
   if (rb < 0 || rb >= sp.nb) return;

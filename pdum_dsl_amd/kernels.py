@@ -940,7 +940,7 @@ def paged_append(
 
     Sequence i's new tokens are rows starts[i] .. starts[i + 1] - 1 and the
     last of its lengths[i] tokens (these counted), at the places that row i
-    of ``table`` [sequences, pages] names; ``starts`` ascend from 0; all three
+    of ``table`` [sequences, pages] names; ``starts`` ascend (rows before and behind them are of no sequence); all three
     are int32 on the device, read when the kernel runs. Rows that ``starts`` names behind the call's last
     are not there, and the others have their positions all the same. ``rotary`` (:func:`rotary_table`, fp32
     [positions, rotated], rotated a multiple of 16) turns features i and i +

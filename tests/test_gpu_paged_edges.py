@@ -1,6 +1,8 @@
 """The paged-cache operators on the GPU where a table, starts or lengths are not what a call means: pages that are missing,
 rows that no sequence owns, sequences that go on behind the call's rows, lengths past every table."""
 
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -131,3 +133,34 @@ def test_lengths_past_the_longest_table(K, rows):
         near = [[1]], [0, rows], [min(length - reach + pr, 9000)]
         ref = op.attention(_host(q), _host(cache.k), _host(cache.v), np.array(near[0]), near[1], near[2], scale=d**-0.5, window=500)
         check_attention(_host(o), _host(lse), ref, "bf16", d, str(length))
+
+
+@pytest.mark.parametrize("new", [[1, 2, 1], [2, 70, 130]])
+@pytest.mark.parametrize("first", [1, 5, 70])
+def test_rows_before_the_first_sequence_are_of_no_sequence(K, new, first):
+    from pdum_dsl_amd import _lib
+
+    rng = np.random.default_rng(43)
+    pr, d, hq, hkv = 16, 64, 8, 2
+    table, starts, lens, rows, pages = batch(rng, [90, 80, 200], new, pr, pad=2)
+    starts, rows = starts + first, rows + first
+    cache, pk, pv = _pools(rng, K, "bf16", 16, pages, hkv, pr, d)
+    q = torch.as_tensor(rng.standard_normal((rows, hq, d))).bfloat16().cuda()
+    t = _ints(table, starts, lens)
+    want = op.attention(_host(q), pk, pv, table, starts, lens, scale=d**-0.5)
+    o, lse = K.paged_attention(q, cache, *t)
+    check_attention(_host(o), _host(lse), want, "bf16", d, "starts that begin later")
+    b = _lib.PagedBatch(t[0].data_ptr(), t[1].data_ptr(), t[2].data_ptr(), 3, rows, table.shape[1], table.shape[1])
+    need = _lib.lib().pdh_paged_attention_workspace(C.byref(cache.c), C.byref(b), hq, 1 << 40, 0)
+    ws = torch.full((need // 4 + 4,), float("nan"), device="cuda")
+    owned = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    owned[first:-2] = True
+    for rest in (1, 0):
+        o2, l2 = torch.full_like(q, 9.0), torch.full((rows, hq), 9.0, device="cuda")
+        _lib.call("pdh_paged_attention", q.data_ptr(), o2.data_ptr(), l2.data_ptr(), hq, hq * d, d, hq * d, d, C.byref(cache.c),
+                  C.byref(b), 1 << 40, 0, d**-0.5, rest, ws.data_ptr(), need, K._stream())
+        assert torch.equal(o2[owned], o[owned]) and torch.equal(l2[owned], lse[owned])
+        if rest:
+            assert (o2[~owned] == 0).all() and torch.isneginf(l2[~owned]).all()
+        else:
+            assert (o2[~owned] == 9.0).all() and (l2[~owned] == 9.0).all()
