@@ -366,8 +366,10 @@ typedef struct pdh_paged_batch {
  * A token without a place, or past the rotary's positions, is stored nowhere,
  * its row of q_out is zero, and it adds 1 to *bad (device int, may be NULL).
  * Rows of no sequence are written zero to q_out where zero_rest != 0, else
- * not at all. Tokens that share a place leave any of them, or a mixture. No
- * counterpart in the reference. */
+ * not at all. Tokens that share a place leave any of them, or a mixture;
+ * pools whose rows overlap (a stride of 0, keys in the values' memory) are
+ * refused here, though not where they are read. No counterpart in the
+ * reference. */
 int pdh_paged_append(const void* k, const void* v, const void* q, void* q_out, int64_t heads_q, int64_t k_st,
                      int64_t k_sh, int64_t v_st, int64_t v_sh, int64_t q_st, int64_t q_sh, int64_t qo_st,
                      int64_t qo_sh, const pdh_paged_cache* cache, const pdh_paged_batch* batch, const float* rotary,

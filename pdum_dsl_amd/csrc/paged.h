@@ -8,6 +8,7 @@
 #pragma once
 
 #include "common.h"
+#include "spans.h"
 
 #include <initializer_list>
 #include <type_traits>
@@ -126,6 +127,20 @@ inline int check_paged(const char* fn, const pdh_paged_cache* c, const pdh_paged
     PDH_REQUIRE((b->table || b->width == 0) && b->starts && b->lengths, PDH_EINVAL, "%s: null table, starts or lengths", fn);
   *shift = __builtin_ctzll(static_cast<unsigned long long>(p));
   return PDH_OK;
+}
+
+// Whether no two rows of a cache's pools, and of its scales, share a byte: an append stores several otherwise in one place,
+// and which of them stays goes by the order of the workgroups. Keys and values are one array more, two entries long: they
+// may lie in one tensor.
+inline bool pools_apart(const pdh_paged_cache& c) {
+  auto apart = [&](const void* k, const void* v, int64_t row, int64_t page, int64_t head, int64_t in_page) {
+    const intptr_t between = reinterpret_cast<intptr_t>(v) - reinterpret_cast<intptr_t>(k);
+    return Spans(k, row, {{c.pages, page}, {c.heads, head}, {c.page_rows, in_page}, {2, between < 0 ? -between : between}})
+        .apart();
+  };
+  if (c.bits == 16) return apart(c.k, c.v, c.features * 2, c.sp * 2, c.sh * 2, c.sr * 2);
+  return apart(c.k, c.v, c.features / 2, c.sp, c.sh, c.sr) &&
+         apart(c.k_scale, c.v_scale, c.features / 32, c.ssp, c.ssh, c.ssr);
 }
 
 // f(element type, features, bits) of a cache.

@@ -252,6 +252,8 @@ extern "C" int pdh_paged_append(const void* k, const void* v, const void* q, voi
               "pdh_paged_append: k, v, q and q_out must be 16-byte aligned");
   for (int64_t s : {k_st, k_sh, v_st, v_sh, q_st, q_sh, qo_st, qo_sh})
     PDH_REQUIRE(s >= 0 && s % 8 == 0, PDH_EINVAL, "pdh_paged_append: strides must be multiples of 8 elements, >= 0");
+  PDH_REQUIRE(pools_apart(*cache), PDH_EINVAL,
+              "pdh_paged_append: rows of the cache's pools or scales overlap, or keys and values do");
   if (rotary) {
     PDH_REQUIRE(rotated >= 16 && rotated % 16 == 0 && rotated <= cache->features, PDH_EUNSUPPORTED,
                 "pdh_paged_append: rotated must be a multiple of 16 in [16, features] (got %lld)", (long long)rotated);

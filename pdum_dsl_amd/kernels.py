@@ -955,7 +955,8 @@ def paged_append(
     is zero, and it counts in ``bad`` (an int32 device scalar) when given.
     Rows of no sequence are stored nowhere; their rows of the result are zero,
     or stay as they are in ``out`` (which may be q itself). Two tokens with one
-    place leave either of them, or parts of both, there."""
+    place leave either of them, or parts of both, there; a cache whose rows lie
+    in one another (an expanded pool, one tensor for keys and values) is refused."""
     cc, _, dtype, heads, d, _ = cache._call
     rows = k.shape[0] if k.dim() == 3 else 0
     b = _paged("paged_append", cache, table, starts, lengths, rows, (k, v, q, rotary, out, bad))

@@ -164,3 +164,63 @@ def test_rows_before_the_first_sequence_are_of_no_sequence(K, new, first):
             assert (o2[~owned] == 0).all() and torch.isneginf(l2[~owned]).all()
         else:
             assert (o2[~owned] == 9.0).all() and (l2[~owned] == 9.0).all()
+
+
+def _layouts(pages, hkv, pr, d):
+    """Keys' and values' views of one tensor, and of two, in the orders that programs hold them in; d: bytes or features."""
+    def make(*shape):
+        return torch.zeros(shape, dtype=torch.uint8, device="cuda")
+
+    both = make(pages, 2, hkv, pr, d)
+    yield both[:, 0], both[:, 1]
+    yield both[:, 1], both[:, 0]  # the values before the keys
+    both = make(2, pages, hkv, pr, d)
+    yield both[0], both[1]
+    both = make(pages, pr, hkv, 2 * d)
+    yield both[..., :d].transpose(1, 2), both[..., d:].transpose(1, 2)
+    both = make(pages, pr, 2 * hkv, d).transpose(1, 2)
+    yield both[:, :hkv], both[:, hkv:]
+    yield both[:, ::2], both[:, 1::2]
+    both = make(2 * pages, hkv, pr, d)
+    yield both[::2], both[1::2]
+    yield make(pages, hkv, pr, d), make(pages, hkv, pr, d)
+    both = make(hkv, pages + 3, pr, d).transpose(0, 1)
+    yield both[:pages], make(hkv, pages + 3, pr, d).transpose(0, 1)[3:]
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("hkv", [1, 2])
+def test_an_append_to_pools_in_one_tensor(K, bits, hkv):
+    """Pools that lie in one another without sharing memory take the same bits as pools of their own; those that share it
+    are refused, and may still be read."""
+    from pdum_dsl_amd import _lib
+
+    rng = np.random.default_rng(44)
+    pr, d = 16, 64
+    table, starts, lens, rows, pages = batch(rng, [40, 33], [40, 3], pr)
+    x = torch.as_tensor(rng.standard_normal((rows, 2 * hkv, d))).bfloat16().cuda()
+    k, v = x[:, :hkv], x[:, hkv:]
+    t = _ints(table, starts, lens)
+    own = K.paged_cache(pages, hkv, pr, d, bits=bits)
+    K.paged_append(k, v, own, *t)
+    for pk, pv in _layouts(pages, hkv, pr, 2 * d if bits == 16 else d // 2):
+        if bits == 16:
+            cache = K.PagedCache(pk.view(torch.bfloat16), pv.view(torch.bfloat16))
+        else:
+            scales = torch.zeros((pages, 2, hkv, pr, d // 32), dtype=torch.uint8, device="cuda")
+            cache = K.PagedCache(pk, pv, scales[:, 0], scales[:, 1])
+        K.paged_append(k, v, cache, *t)
+        for a, b in ((cache.k, own.k), (cache.v, own.v), (cache.k_scale, own.k_scale), (cache.v_scale, own.v_scale)):
+            assert a is None or torch.equal(a, b)
+    if bits == 4:
+        shared = (K.PagedCache(own.k, own.v, own.k_scale, own.k_scale), K.PagedCache(own.k, own.k, own.k_scale, own.v_scale))
+    else:
+        shared = (K.PagedCache(own.k, own.k), K.PagedCache(own.k[:1].expand(3, -1, -1, -1), own.v[:1].expand(3, -1, -1, -1)))
+    for cache in shared:
+        held = [p.clone() for p in (own.k, own.v)]
+        with pytest.raises(_lib.PdhError, match="overlap"):
+            K.paged_append(k, v, cache, *t)
+        assert torch.equal(own.k, held[0]) and torch.equal(own.v, held[1])
+        K.paged_rows(cache, *t, rows)
+        o, _ = K.paged_attention(k, cache, *t)
+        assert torch.isfinite(o.float()).all()

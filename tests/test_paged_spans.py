@@ -1,0 +1,112 @@
+"""What the paged-cache calls refuse to write: the host's arithmetic on strided rows, compiled from its header and held
+against every byte of small arrays, and the refusals of the C entry points (each fires before any HIP call)."""
+
+import ctypes as C
+import random
+import subprocess
+from pathlib import Path
+
+import pytest
+
+from tests.test_paged_ops import FAKE, _four_bits, _structs
+
+CSRC = Path(__file__).resolve().parents[1] / "pdum_dsl_amd" / "csrc"
+
+MAIN = """
+#include "spans.h"
+#include <cstdio>
+using pdh::Spans;
+static bool read(Spans& s) {
+  long long at, width, n[4], st[4];
+  if (scanf("%lld %lld", &at, &width) != 2) return false;
+  for (int i = 0; i < 4; ++i) scanf("%lld %lld", &n[i], &st[i]);
+  s = Spans(reinterpret_cast<const void*>(at), width, {{n[0], st[0]}, {n[1], st[1]}, {n[2], st[2]}, {n[3], st[3]}});
+  return true;
+}
+int main() {
+  Spans a(nullptr, 1, {});
+  while (read(a)) printf("%d\\n", a.apart());
+}
+"""
+
+
+def _run(tmp_path, main, arrays):
+    (tmp_path / "spans.cpp").write_text(main)
+    exe = tmp_path / "spans"
+    subprocess.run(["g++", "-std=c++17", "-O1", "-I", str(CSRC), str(tmp_path / "spans.cpp"), "-o", str(exe)], check=True)
+    text = "\n".join(" ".join(map(str, (at, width, *[x for axis in axes for x in axis]))) for at, width, axes in arrays)
+    out = subprocess.run([str(exe)], input=text, check=True, capture_output=True, text=True).stdout
+    return [bool(int(line)) for line in out.split()]
+
+
+def _rows(at, axes):
+    starts = [at]
+    for n, step in axes:
+        starts = [s + i * step for s in starts for i in range(n)]
+    return starts
+
+
+def _draw(rng):
+    """Axes of a few entries, half of the time each stepping over the ones before it, by little or much."""
+    width, axes = rng.choice([4, 8, 64]), []
+    extent = width
+    for _ in range(4):
+        n = rng.choice([1, 1, 2, 3, 5])
+        step = extent * rng.choice([1, 1, 2, 3]) + rng.choice([0, 0, 4]) if rng.random() < 0.8 else rng.randrange(0, 300)
+        axes.append((n, step))
+        extent = max(extent, (n - 1) * step + extent)
+    rng.shuffle(axes)
+    return rng.randrange(0, 400), width, axes
+
+
+def test_no_array_that_overlaps_is_taken_for_apart(tmp_path):
+    rng = random.Random(1)
+    arrays = [_draw(rng) for _ in range(3000)]
+    got = _run(tmp_path, MAIN, arrays)
+    right = 0
+    for (at, width, axes), apart in zip(arrays, got):
+        starts = sorted(_rows(at, axes))
+        truth = all(b - a >= width for a, b in zip(starts, starts[1:]))
+        assert truth or not apart, (at, width, axes)
+        ordered, extent = sorted((s, n) for n, s in axes if n > 1), width
+        nested = True
+        for s, n in ordered:
+            nested &= s >= extent
+            extent += (n - 1) * s
+        assert apart == nested, (at, width, axes)  # nothing that nests is refused
+        right += truth and apart
+    assert right > 1000
+
+
+FAR = 1 << 24  # the values' pool, past the end of the keys'
+
+
+def _append(cache, batch=None):
+    from pdum_dsl_amd import _lib
+
+    c, b = _structs(cache, batch)
+    q = C.c_void_p(FAKE)
+    rc = _lib.lib().pdh_paged_append(C.c_void_p(FAR), C.c_void_p(2 * FAR), q, q, 4, 256, 64, 256, 64, 256, 64, 256, 64, C.byref(c),
+                                     C.byref(b), None, 0, 0, 0, 0, 1, None, None)
+    return rc, _lib.last_error()
+
+
+@pytest.mark.parametrize("cache", [
+    dict(),  # keys and values in one tensor
+    dict(v=FAKE + 64),  # values between keys
+    dict(v=FAKE + 4 * 2048 * 2 - 128),  # the values' first row is the keys' last
+    dict(v=FAR, sh=0),  # heads in one place
+    dict(v=FAR, sp=0),  # pages in one place
+    dict(v=FAR, sh=512),  # heads inside one another
+    dict(v=FAR, sp=1024),  # a page starts in the one before
+    dict(_four_bits(v=FAR), sp=1024, sh=512, ssp=64, ssh=32),  # scales of keys and values in one tensor
+    dict(_four_bits(v=FAR), sp=1024, sh=512, v_scale=FAR // 2, ssp=32, ssh=32),  # scales' pages in one another
+    dict(_four_bits(v=FAR), sp=1024, sh=512, v_scale=FAR // 2, ssp=64, ssh=0),
+    dict(_four_bits(), sp=1024, sh=512, v_scale=FAR // 2, ssp=64, ssh=32),  # codes of keys and values in one tensor
+])
+def test_an_append_to_rows_that_overlap_is_refused(cache):
+    from pdum_dsl_amd import _lib
+
+    rc, text = _append(cache)
+    assert rc == _lib.PDH_EINVAL and "overlap" in text, (rc, text)
+    assert _append(cache, dict(rows=0))[0] == _lib.PDH_OK  # nothing to store
