@@ -354,8 +354,8 @@ typedef struct pdh_paged_batch {
 
 /* Store k and v [rows][heads][features] (strides *_st of a row, *_sh of a
  * head, multiples of 8 elements, 16-byte aligned) at their tokens' places, and
- * write q [rows][heads_q][features] to q_out (which may be q; both NULL with
- * heads_q = 0). Where rotary (fp32 [positions][rotated], rows ld_rotary apart;
+ * write q [rows][heads_q][features] to q_out (which may be q, with its strides,
+ * and overlaps no input otherwise; both NULL with heads_q = 0). Where rotary (fp32 [positions][rotated], rows ld_rotary apart;
  * cosines, then sines) is given, k and q are turned by their positions first:
  * for i < rotated / 2 with (a, b) = features (i, i + rotated / 2), or (2 i, 2 i
  * + 1) if interleaved, (a cos - b sin, b cos + a sin), in fp32, every product
@@ -392,7 +392,8 @@ int pdh_paged_rows(void* k_out, void* v_out, int64_t ko_st, int64_t ko_sh, int64
  * factors. Tokens that a row does not see count for nothing in it whatever the
  * pools hold. A row that sees nothing, or scores of -inf alone: o = 0, lse =
  * -inf; rows of no sequence likewise where zero_rest != 0, else they are not
- * written. o may be q, with q's strides. ws, 16-byte aligned, holds pdh_paged_attention_workspace bytes for
+ * written. o may be q, with q's strides, and does not overlap it otherwise. ws, 16-byte
+ * aligned, holds pdh_paged_attention_workspace bytes for
  * the same sizes (partial states of rows whose keys several workgroups share).
  * Nothing is atomic: results repeat bit for bit. No counterpart in the
  * reference. */

@@ -143,6 +143,16 @@ inline bool pools_apart(const pdh_paged_cache& c) {
          apart(c.k_scale, c.v_scale, c.features / 32, c.ssp, c.ssh, c.ssr);
 }
 
+// A [rows][heads][features] tensor of 16-bit elements.
+struct Tokens {
+  const void* p;
+  int64_t rows, heads, features, st, sh;
+  Spans spans() const { return Spans(p, features * 2, {{rows, st * 2}, {heads, sh * 2}}); }
+  bool in_place_of(const Tokens& o) const {  // of the same sizes
+    return p == o.p && (rows <= 1 || st == o.st) && (heads <= 1 || sh == o.sh);
+  }
+};
+
 // f(element type, features, bits) of a cache.
 template <typename F>
 void by_kind(const pdh_paged_cache& c, F f) {

@@ -252,6 +252,16 @@ extern "C" int pdh_paged_append(const void* k, const void* v, const void* q, voi
               "pdh_paged_append: k, v, q and q_out must be 16-byte aligned");
   for (int64_t s : {k_st, k_sh, v_st, v_sh, q_st, q_sh, qo_st, qo_sh})
     PDH_REQUIRE(s >= 0 && s % 8 == 0, PDH_EINVAL, "pdh_paged_append: strides must be multiples of 8 elements, >= 0");
+  if (heads_q > 0) {  // chunks are read by other workgroups than write them, but where q_out is q
+    const int64_t n = batch->rows, d = cache->features;
+    const Tokens out{q_out, n, heads_q, d, qo_st, qo_sh}, in{q, n, heads_q, d, q_st, q_sh};
+    const Spans o = out.spans();
+    PDH_REQUIRE(o.apart(), PDH_EINVAL, "pdh_paged_append: q_out's rows overlap");
+    PDH_REQUIRE((out.in_place_of(in) || o.apart_from(in.spans())) &&
+                    o.apart_from(Tokens{k, n, cache->heads, d, k_st, k_sh}.spans()) &&
+                    o.apart_from(Tokens{v, n, cache->heads, d, v_st, v_sh}.spans()),
+                PDH_EINVAL, "pdh_paged_append: q_out overlaps k, v or q (it may be q, with q's strides)");
+  }
   PDH_REQUIRE(pools_apart(*cache), PDH_EINVAL,
               "pdh_paged_append: rows of the cache's pools or scales overlap, or keys and values do");
   if (rotary) {
@@ -284,6 +294,9 @@ extern "C" int pdh_paged_rows(void* k_out, void* v_out, int64_t ko_st, int64_t k
               "pdh_paged_rows: the outputs must be 16-byte aligned");
   for (int64_t s : {ko_st, ko_sh, vo_st, vo_sh})
     PDH_REQUIRE(s >= 0 && s % 8 == 0, PDH_EINVAL, "pdh_paged_rows: strides must be multiples of 8 elements, >= 0");
+  const Spans ko = Tokens{k_out, batch->rows, cache->heads, cache->features, ko_st, ko_sh}.spans();
+  const Spans vo = Tokens{v_out, batch->rows, cache->heads, cache->features, vo_st, vo_sh}.spans();
+  PDH_REQUIRE(ko.apart() && vo.apart() && ko.apart_from(vo), PDH_EINVAL, "pdh_paged_rows: rows of the outputs overlap");
   const RowsArgs a{static_cast<uint16_t*>(k_out), static_cast<uint16_t*>(v_out), ko_st, ko_sh, vo_st, vo_sh, *cache,
                    *batch, shift, zero_rest != 0};
   const int64_t items = 2 * cache->heads * (cache->features / 8);

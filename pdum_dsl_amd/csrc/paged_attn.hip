@@ -1373,6 +1373,10 @@ extern "C" int pdh_paged_attention(const void* q, void* o, float* lse, int64_t h
               "pdh_paged_attention: q and o must be 16-byte aligned");
   for (int64_t s : {q_st, q_sh, o_st, o_sh})
     PDH_REQUIRE(s >= 0 && s % 8 == 0, PDH_EINVAL, "pdh_paged_attention: strides must be multiples of 8 elements, >= 0");
+  const Tokens out{o, batch->rows, heads_q, cache->features, o_st, o_sh}, in{q, batch->rows, heads_q, cache->features, q_st, q_sh};
+  PDH_REQUIRE(out.spans().apart(), PDH_EINVAL, "pdh_paged_attention: o's rows overlap");
+  PDH_REQUIRE(out.in_place_of(in) || out.spans().apart_from(in.spans()), PDH_EINVAL,
+              "pdh_paged_attention: o overlaps q (it may be q, with q's strides)");
   PagedAttn a{static_cast<const uint16_t*>(q), static_cast<uint16_t*>(o), lse, q_st, q_sh, o_st, o_sh, *cache, *batch,
               static_cast<int>(heads_q), static_cast<int>(heads_q / cache->heads),
               static_cast<int>(window < kMaxTokens ? window : kMaxLength),  // of 2^30 and more: every position's whole past

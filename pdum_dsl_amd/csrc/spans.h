@@ -37,6 +37,24 @@ struct Spans {
       if (axis[i].step < extent(i)) return false;
     return true;
   }
+
+  // No row of the first `count` axes shares a byte with one of b's first `bcount`, whose first lies `between` bytes behind.
+  // What both step over by the longest step, S, is taken off: rests that span no more than S can meet at two distances
+  // alone, their own modulo S and S less. (Arrays that this does not tell apart count as overlapping.)
+  bool apart_from(int count, const Spans& b, int bcount, __int128 between) const {
+    const __int128 ea = extent(count), eb = b.extent(bcount);
+    if (between >= ea || -between >= eb) return true;
+    const int64_t sa = count > 0 ? axis[count - 1].step : 0, sb = bcount > 0 ? b.axis[bcount - 1].step : 0;
+    const int64_t step = sa > sb ? sa : sb;
+    if (step == 0) return false;
+    const int ca = sa == step ? count - 1 : count, cb = sb == step ? bcount - 1 : bcount;
+    if (extent(ca) > step || b.extent(cb) > step) return false;
+    const __int128 rest = (between % step + step) % step;
+    return apart_from(ca, b, cb, rest) && apart_from(ca, b, cb, rest - step);
+  }
+  bool apart_from(const Spans& b) const {
+    return apart_from(axes, b, b.axes, static_cast<__int128>(b.at) - static_cast<__int128>(at));
+  }
 };
 
 }  // namespace pdh

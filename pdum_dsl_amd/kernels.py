@@ -954,7 +954,8 @@ def paged_append(
     page table, or a page outside the pool) is dropped, its row of the result
     is zero, and it counts in ``bad`` (an int32 device scalar) when given.
     Rows of no sequence are stored nowhere; their rows of the result are zero,
-    or stay as they are in ``out`` (which may be q itself). Two tokens with one
+    or stay as they are in ``out`` (which may be q itself, and does not overlap
+    q, k or v otherwise). Two tokens with one
     place leave either of them, or parts of both, there; a cache whose rows lie
     in one another (an expanded pool, one tensor for keys and values) is refused."""
     cc, _, dtype, heads, d, _ = cache._call

@@ -224,3 +224,41 @@ def test_an_append_to_pools_in_one_tensor(K, bits, hkv):
         K.paged_rows(cache, *t, rows)
         o, _ = K.paged_attention(k, cache, *t)
         assert torch.isfinite(o.float()).all()
+
+
+def test_results_in_one_tensor_with_inputs(K):
+    """q's place, and other heads of the tensor that holds q, k and v, rows first and heads first; a part of q is refused."""
+    from pdum_dsl_amd import _lib
+
+    rng = np.random.default_rng(45)
+    pr, d, hq, hkv = 16, 64, 4, 2
+    for lengths, new in (([40, 33], [2, 1]), ([90, 33], [70, 3])):
+        table, starts, lens, rows, pages = batch(rng, lengths, new, pr)
+        t, tab = _ints(table, starts, lens), K.rotary_table(100, d)
+        x = torch.as_tensor(rng.standard_normal((rows, 2 * hq + 2 * hkv, d))).bfloat16().cuda()
+        for turned in (x, x.transpose(0, 1).contiguous().transpose(0, 1)):
+            q, k, v, rest = turned[:, :hq], turned[:, hq : hq + hkv], turned[:, hq + hkv : hq + 2 * hkv], turned[:, hq + 2 * hkv :]
+            want = None
+            for place in (None, rest, q):
+                cache, held = K.paged_cache(pages, hkv, pr, d), turned.clone()
+                got = K.paged_append(k, v, cache, *t, q=q, rotary=tab, out=place).clone()
+                o = K.paged_attention(q, cache, *t, out=place)[0].clone()  # (of q as it now is)
+                assert want is None or torch.equal(got, want)
+                want = got
+                if place is None:
+                    plain = o
+                    assert torch.equal(turned, held)
+                elif place is rest:
+                    assert torch.equal(o, plain) and torch.equal(turned[:, : hq + 2 * hkv], held[:, : hq + 2 * hkv])
+                else:
+                    assert torch.equal(turned[:, hq:], held[:, hq:])
+            turned.copy_(held)  # q as it was
+        wide = torch.zeros((rows + 1, hq, d), dtype=torch.bfloat16, device="cuda")
+        kv = torch.zeros((rows, hkv, d), dtype=torch.bfloat16, device="cuda")
+        for q, out in ((wide[1:], wide[:-1]), (wide[:-1], wide[1:])):
+            with pytest.raises(_lib.PdhError, match="overlap"):
+                K.paged_append(kv, kv, cache, *t, q=q, out=out)
+            with pytest.raises(_lib.PdhError, match="overlap"):
+                K.paged_attention(q, cache, *t, out=out)
+        with pytest.raises(_lib.PdhError, match="overlap"):
+            K.paged_append(kv, wide[1:, :hkv], cache, *t, q=torch.zeros_like(wide[1:]), out=wide[1:])

@@ -29,6 +29,13 @@ int main() {
 }
 """
 
+PAIRS = MAIN.split("int main()")[0] + """
+int main() {
+  Spans a(nullptr, 1, {}), b = a;
+  while (read(a) && read(b)) printf("%d\\n", a.apart_from(b) ? b.apart_from(a) : b.apart_from(a) ? 2 : 0);
+}
+"""
+
 
 def _run(tmp_path, main, arrays):
     (tmp_path / "spans.cpp").write_text(main)
@@ -78,6 +85,37 @@ def test_no_array_that_overlaps_is_taken_for_apart(tmp_path):
     assert right > 1000
 
 
+def test_no_two_arrays_that_overlap_are_taken_for_apart(tmp_path):
+    """Drawn pairs, half of them cut from one tensor as a projection's q, k and v are, those of which are always told apart."""
+    rng = random.Random(2)
+    arrays, views = [], []
+    for _ in range(4000):
+        if rng.random() < 0.5:
+            arrays += [_draw(rng), _draw(rng)]
+            views.append(False)
+            continue
+        rows, d, gap = rng.choice([1, 2, 7]), rng.choice([4, 16]), rng.choice([0, 0, 4])
+        parts = [rng.choice([1, 2, 5]) for _ in range(3)]
+        heads = sum(parts)
+        if rng.random() < 0.5:  # rows of heads, or heads of rows
+            st, sh = heads * d + gap, d
+        else:
+            st, sh = d, rows * d + gap
+        at = rng.randrange(0, 4) * 64
+        both = rng.sample(range(3), 2)
+        arrays += [(at + sum(parts[:i]) * sh, d, [(rows, st), (parts[i], sh), (1, 0), (1, 0)]) for i in both]
+        views.append(True)
+    got = _run(tmp_path, PAIRS, arrays)
+    assert len(got) == len(views)
+    seen = 0
+    for a, b, apart, view in zip(arrays[::2], arrays[1::2], got, views):
+        truth = all(x + a[1] <= y or y + b[1] <= x for x in _rows(a[0], a[2]) for y in _rows(b[0], b[2]))
+        assert truth or not apart, (a, b)
+        assert apart or not view, (a, b)
+        seen += truth and apart and max(_rows(a[0], a[2])) > min(_rows(b[0], b[2]))
+    assert seen > 1000
+
+
 FAR = 1 << 24  # the values' pool, past the end of the keys'
 
 
@@ -110,3 +148,37 @@ def test_an_append_to_rows_that_overlap_is_refused(cache):
     rc, text = _append(cache)
     assert rc == _lib.PDH_EINVAL and "overlap" in text, (rc, text)
     assert _append(cache, dict(rows=0))[0] == _lib.PDH_OK  # nothing to store
+
+
+@pytest.mark.parametrize("out,st,sh", [
+    (FAKE + 512, 256, 64),  # q, a row on
+    (FAKE + 128, 256, 64),  # a head on
+    (FAKE, 512, 64),  # q's place, with other strides
+    (FAKE, 256, 128),
+    (FAR, 256, 64),  # k
+    (2 * FAR + 64, 256, 64),  # v
+    (FAR - 256, 256, 64),  # its end lies in k
+    (4 * FAR, 64, 64), (4 * FAR, 0, 64),  # rows in one another
+])
+def test_results_that_overlap_inputs_are_refused(out, st, sh):
+    from pdum_dsl_amd import _lib
+
+    lib, q = _lib.lib(), C.c_void_p(FAKE)
+    c, b = _structs(dict(k=8 * FAR, v=16 * FAR))
+    rc = lib.pdh_paged_append(C.c_void_p(FAR), C.c_void_p(2 * FAR), q, C.c_void_p(out), 4, 256, 64, 256, 64, 256, 64, st, sh,
+                              C.byref(c), C.byref(b), None, 0, 0, 0, 0, 1, None, None)
+    assert rc == _lib.PDH_EINVAL and "overlap" in _lib.last_error(), (rc, _lib.last_error())
+    if FAR - 256 <= out < 4 * FAR:
+        return
+    rc = lib.pdh_paged_attention(q, C.c_void_p(out), None, 4, 256, 64, st, sh, C.byref(c), C.byref(b), 5, 0, 1.0, 1,
+                                 C.c_void_p(32 * FAR), 1 << 40, None)
+    assert rc == _lib.PDH_EINVAL and "overlap" in _lib.last_error(), (rc, _lib.last_error())
+
+
+@pytest.mark.parametrize("v,st,sh", [(FAR, 128, 64), (FAR + 64, 128, 64), (FAR - 1024, 128, 64), (2 * FAR, 64, 64), (2 * FAR, 128, 0)])
+def test_read_back_rows_that_overlap_are_refused(v, st, sh):
+    from pdum_dsl_amd import _lib
+
+    c, b = _structs()
+    rc = _lib.lib().pdh_paged_rows(C.c_void_p(FAR), C.c_void_p(v), 128, 64, st, sh, C.byref(c), C.byref(b), 1, None)
+    assert rc == _lib.PDH_EINVAL and "overlap" in _lib.last_error(), (rc, _lib.last_error())
