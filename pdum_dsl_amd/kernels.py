@@ -795,8 +795,8 @@ class PagedCache:
     half of a byte, times 2^(scale - 127) (255: NaN). ``dtype`` is the 16-bit
     type that they are computed with. features 64 or 128.
 
-    The object describes the tensors, whose contents the calls read and write;
-    they stay in place while it lives."""
+    The object describes the tensors as they are at its first call, and the calls read and
+    write their contents; given other memory since (``set_``, ``.data``, a resized storage) they are refused."""
 
     k: torch.Tensor
     v: torch.Tensor
@@ -844,11 +844,19 @@ class PagedCache:
                                 *apart("k and v", k, v), *scales, _DT[dtype], bits)
 
     @functools.cached_property
-    def _call(self):
-        """What a call needs of the cache: the struct, device, value type, heads, features, what a workspace goes by."""
+    def _described(self):
         c = self.c
         return (C.byref(c), self.k.get_device(), torch.bfloat16 if c.dtype == PDH_BF16 else torch.float16, c.heads,
-                c.features, (self.k.get_device(), c.bits, c.features, c.heads, c.page_rows))
+                c.features, (self.k.get_device(), c.bits, c.features, c.heads, c.page_rows)), (c.k, c.v, c.k_scale, c.v_scale)
+
+    @property
+    def _call(self):
+        """What a call needs of the cache: the struct, device, value type, heads, features, what a workspace goes by."""
+        call, (k, v, ks, vs) = self._described
+        if self.k.data_ptr() != k or self.v.data_ptr() != v or (
+                ks is not None and (self.k_scale.data_ptr() != ks or self.v_scale.data_ptr() != vs)):
+            raise ValueError("PagedCache: its tensors have moved to other memory; they take a PagedCache of their own")
+        return call
 
 
 def paged_cache(pages: int, heads: int, page_rows: int, features: int, dtype: torch.dtype = torch.bfloat16, *,
