@@ -389,7 +389,8 @@ int pdh_paged_rows(void* k_out, void* v_out, int64_t ko_st, int64_t ko_sh, int64
  * all):
  *   x = scale q . k_s, o = sum softmax(x) v_s, lse = log sum exp x   (scale > 0)
  * fp32 scores, statistics and sums; the weights are rounded to dtype as
- * factors. Tokens that a row does not see count for nothing in it whatever the
+ * factors (half a step of each; of PDH_F16 those under 2^-32 of the largest
+ * are lost). Tokens that a row does not see count for nothing in it whatever the
  * pools hold. A row that sees nothing, or scores of -inf alone: o = 0, lse =
  * -inf; rows of no sequence likewise where zero_rest != 0, else they are not
  * written. o may be q, with q's strides, and does not overlap it otherwise. ws, 16-byte

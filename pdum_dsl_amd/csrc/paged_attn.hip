@@ -19,6 +19,12 @@ namespace {
 
 constexpr float kInf = __builtin_inff();
 
+// Softmax weights are factors of a 16-bit matrix product, rounded to the type (half a step of each; their sum is of the fp32
+// ones). f16 ends at 2^-24: there they are taken 2^kLift larger, o and the sum with them, so that the largest is 2^7 to 2^15
+// and what is lost lies under 2^-32 of it: 2^20 keys of that come to 2^-12. States are (m, l, o) with m - kLift for m.
+template <typename T>
+constexpr float kLift = std::is_same_v<T, _Float16> ? 7.0f : 0.0f;
+
 struct PagedAttn {
   const uint16_t* q;
   uint16_t* o;
@@ -502,19 +508,20 @@ __global__ __launch_bounds__(256, (dec_wgs<D, BITS>())) void paged_decode(PagedA
           sc[i >> 2][i & 3] = seen ? sc[i >> 2][i & 3] : -kInf;
         }
       }
-      // The exponentials refer to a maximum that moves only when they leave (0, 2^8], or are not numbers (a maximum of
+      // The exponentials refer to a maximum that moves only when they leave (0, 2^(8 + kLift)], or are not numbers (a maximum of
       // -inf: the first block): then the block's maximum is found and everything rescaled.
       u32x4 pb;
       auto expo = [&](float ref) {
-        const float mc = ref * a.c2;
+        const float mc = ref * a.c2 - kLift<T>;
         float p[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) p[i] = fast_exp2(__builtin_fmaf(sc[i >> 2][i & 3], a.c2, -mc));
         pb = u32x4{pack2<T>(p[0], p[1]), pack2<T>(p[2], p[3]), pack2<T>(p[4], p[5]), pack2<T>(p[6], p[7])};
         return ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
       };
+      constexpr float kLimit = kLift<T> > 0.f ? 32768.f : 256.f;
       float part = expo(m);
-      if (__builtin_amdgcn_ballot_w64(!(part <= 256.f)) != 0) {
+      if (__builtin_amdgcn_ballot_w64(!(part <= kLimit)) != 0) {
         float mx = sc[0][0];
 #pragma unroll
         for (int i = 1; i < 8; ++i) mx = fmaxf(mx, sc[i >> 2][i & 3]);
@@ -572,7 +579,7 @@ __global__ __launch_bounds__(256, (dec_wgs<D, BITS>())) void paged_decode(PagedA
     if (col < nq) {
       float* rec = red + (w * 16 + col) * RS;
       if (g == 0) {
-        rec[0] = m * a.c2;  // log2 units
+        rec[0] = m * a.c2 - kLift<T>;  // log2 units
         rec[1] = lsum;
       }
 #pragma unroll
@@ -1076,14 +1083,19 @@ __global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, Sl
     // what the exponentials refer to: 0 while a row's scores are all -inf, whose exponentials are then 0, not NaN
     auto ref = [&](int h) { return mused[h] == -kInf ? 0.f : mused[h]; };
     auto expo = [&](int h, float m) {
-      const float mc = m * a.c2;
+      const float mc = m * a.c2 - kLift<T>;
       float e[8];
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float x = sacc[kb][h][i];
-          e[4 * kb + i] = CUT ? fast_exp2((x - m) * a.c2) : fast_exp2(__builtin_fmaf(x, a.c2, -mc));
+          if constexpr (!CUT)
+            e[4 * kb + i] = fast_exp2(__builtin_fmaf(x, a.c2, -mc));
+          else if constexpr (kLift<T> > 0.f)
+            e[4 * kb + i] = fast_exp2(__builtin_fmaf(x - m, a.c2, kLift<T>));
+          else
+            e[4 * kb + i] = fast_exp2((x - m) * a.c2);
         }
       p[h] = u32x4{pack2<T>(e[0], e[1]), pack2<T>(e[2], e[3]), pack2<T>(e[4], e[5]), pack2<T>(e[6], e[7])};
       return ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
@@ -1106,7 +1118,7 @@ __global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, Sl
     if constexpr (!CUT) {
       // a reference still at -inf makes these inf or NaN: over the limit
       float part0 = expo(0, mused[0]), part1 = expo(1, mused[1]);
-      const float lim = static_cast<float>(1 << static_cast<int>(kTau));
+      const float lim = static_cast<float>(1 << static_cast<int>(kTau + kLift<T>));
       if (__builtin_amdgcn_ballot_w64(!(part0 <= lim) || !(part1 <= lim)) != 0) {
         rescale(0, fmaxf(mused[0], rowmax(0)));
         rescale(1, fmaxf(mused[1], rowmax(1)));
@@ -1225,7 +1237,7 @@ __global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, Sl
       for (int fb = 0; fb < C::FB; ++fb) *reinterpret_cast<f32x4*>(po + 16 * fb) = oacc[fb][h];
       if (G == 0) {
         float* ml = pt.ml<D>(split, at);
-        ml[0] = mused[h] * a.c2;
+        ml[0] = mused[h] * a.c2 - kLift<T>;
         ml[1] = l;
       }
     } else {
@@ -1236,7 +1248,7 @@ __global__ __launch_bounds__(256, 3) void paged_prompt(PagedAttn a, Parts pt, Sl
         const f32x4 x = oacc[fb][h];
         *reinterpret_cast<u32x2*>(out + 16 * fb) = u32x2{pack2<T>(x[0] * inv, x[1] * inv), pack2<T>(x[2] * inv, x[3] * inv)};
       }
-      if (G == 0 && a.lse) a.lse[at] = l == 0.f ? -kInf : (mused[h] * a.c2 + __log2f(l)) * kLn2;
+      if (G == 0 && a.lse) a.lse[at] = l == 0.f ? -kInf : (mused[h] * a.c2 - kLift<T> + __log2f(l)) * kLn2;
     }
   }
   // Rows at different positions share tiles: 0 times a value that only some of them see is NaN where it is an infinity or a

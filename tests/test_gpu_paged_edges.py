@@ -262,3 +262,39 @@ def test_results_in_one_tensor_with_inputs(K):
                 K.paged_attention(q, cache, *t, out=out)
         with pytest.raises(_lib.PdhError, match="overlap"):
             K.paged_append(kv, wide[1:, :hkv], cache, *t, q=torch.zeros_like(wide[1:]), out=wide[1:])
+
+
+@pytest.mark.parametrize("bits,gap", [(16, 14), (16, 16), (16, 17), (16, 19), (4, 16)])
+@pytest.mark.parametrize("n,new,sinks,window", [(6000, 1, 0, None), (6000, 3, 0, None), (6000, 130, 0, None), (9000, 1, 1, 5000),
+                                                (9000, 200, 1, 5000)])
+def test_f16_weights_far_under_the_largest_still_count(K, bits, gap, n, new, sinks, window):
+    """A first token takes nearly all of each row's weight, and its value is 0: the result is what thousands of weights of
+    e^-gap come to. f16 has numbers down to 2^-24, and e^-17 lies under 2^-24.5."""
+    rng = np.random.default_rng(46)
+    pr, d, hq, hkv = 16, 64, 8, 2
+    table, starts, lens, rows, pages = batch(rng, [n], [new], pr)
+    x = torch.zeros((n, 2, hkv, d), dtype=torch.float16, device="cuda")
+    x[0, 0, :, 0] = gap / d**-0.5  # a key whose score is gap; all others' are 0
+    x[1:, 1] = torch.as_tensor(rng.choice([0.5, 1.0, 1.5, 2.0], (n - 1, hkv, d))).half()
+    cache = K.paged_cache(pages, hkv, pr, d, torch.float16, bits=bits)
+    K.paged_append(x[:, 0], x[:, 1], cache, *_ints(table, [0, n], lens))
+    kk, vv = (_host(t) for t in K.paged_rows(cache, *_ints(table, [0, n], lens), n))
+    assert (kk == _host(x[:, 0])).all() and (vv == _host(x[:, 1])).all()  # 4 bits hold these
+    q = torch.zeros((rows, hq, d), dtype=torch.float16, device="cuda")
+    q[:, :, 0] = 1.0
+    o, lse = K.paged_attention(q, cache, *_ints(table, starts, lens), window=window, sinks=sinks)
+    o, lse = _host(o), _host(lse)
+    for r in range(rows):
+        pos = n - new + r
+        lo = 1 if window is None else pos - window + 1
+        v = vv[lo : pos + 1].repeat(hq // hkv, axis=1)
+        w = np.exp(-float(gap))
+        den = 1 + len(v) * w
+        want = w * v.sum(0) / den
+        # each weight is rounded by half a step: 2^-11 of it, or of 2^-14 2^-7 where the largest is 2^7; the exponential by
+        # 2^-21 and 2^-23 gap, sums by 2^-24 an addition, the result by 2^-11 or 2^-25
+        part = 2.0**-11 + 2.0**-20 + gap * 2.0**-22 + len(v) * 2.0**-23
+        bound = part * want + 2.0**-32 * v.sum(0)
+        bound = bound + 2.0**-11 * (want + bound) + 2.0**-25
+        assert (np.abs(o[r] - want) <= bound).all(), (r, np.abs(o[r] - want).max(), want.max())
+        assert np.abs(lse[r] - (gap + np.log(den))).max() <= 2.0**-20 + gap * 2.0**-21 + len(v) * 2.0**-23
