@@ -390,14 +390,15 @@ int pdh_paged_rows(void* k_out, void* v_out, int64_t ko_st, int64_t ko_sh, int64
  *   x = scale q . k_s, o = sum softmax(x) v_s, lse = log sum exp x   (scale > 0)
  * fp32 scores, statistics and sums; the weights are rounded to dtype as
  * factors (half a step of each; of PDH_F16 those under 2^-32 of the largest
- * are lost). Tokens that a row does not see count for nothing in it whatever the
- * pools hold. A row that sees nothing, or scores of -inf alone: o = 0, lse =
- * -inf; rows of no sequence likewise where zero_rest != 0, else they are not
- * written. o may be q, with q's strides, and does not overlap it otherwise. ws, 16-byte
- * aligned, holds pdh_paged_attention_workspace bytes for
- * the same sizes (partial states of rows whose keys several workgroups share).
- * Nothing is atomic: results repeat bit for bit. No counterpart in the
- * reference. */
+ * are lost). Tokens that a row does not see count for nothing in it whatever
+ * the pools hold. A row that sees nothing, or scores of -inf alone: o = 0, lse
+ * = -inf; rows of no sequence likewise where zero_rest != 0, else they are not
+ * written. o may be q, with q's strides, and does not overlap it otherwise.
+ * ws, 16-byte aligned, holds pdh_paged_attention_workspace bytes for the same
+ * sizes (partial states of rows whose keys several workgroups share). seqs x
+ * rows x heads_q x width x page_rows is under 2^71 where rows x heads_q / heads
+ * <= 16 seqs. Nothing is atomic: results repeat bit for bit. No counterpart in
+ * the reference. */
 size_t pdh_paged_attention_workspace(const pdh_paged_cache* cache, const pdh_paged_batch* batch, int64_t heads_q,
                                      int64_t window, int64_t sinks);
 int pdh_paged_attention(const void* q, void* o, float* lse, int64_t heads_q, int64_t q_st, int64_t q_sh, int64_t o_st,

@@ -1406,6 +1406,11 @@ extern "C" int pdh_paged_attention(const void* q, void* o, float* lse, int64_t h
   const int64_t scales = cache->bits == 4 ? (cache->pages - 1) * cache->ssp + cache->page_rows * cache->ssr : 0;
   const bool far = pool >= 0x7fff0000 || scales >= 0x7fff0000;
   if (few_rows(*batch, a.group)) {
+    // The kernel sums up the work of all sequences, which starts that do not ascend may give all rows each, in 64 bits.
+    const double most = static_cast<double>(batch->seqs) * static_cast<double>((batch->rows * a.group / 16 + 1) * cache->heads) *
+                        static_cast<double>(a.reach / 32 + 1 + DecCfg<64, 16>::ITEM);
+    PDH_REQUIRE(most < 4.6e18, PDH_EINVAL,
+                "pdh_paged_attention: too many sequences, rows and tokens of the table: %g blocks of work, 2^62 at most", most);
     const unsigned n = static_cast<unsigned>(decode_grid(*cache));
     DecMeta* meta = static_cast<DecMeta*>(ws);
     float* states = reinterpret_cast<float*>(meta + n);

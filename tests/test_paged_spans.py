@@ -182,3 +182,20 @@ def test_read_back_rows_that_overlap_are_refused(v, st, sh):
     c, b = _structs()
     rc = _lib.lib().pdh_paged_rows(C.c_void_p(FAR), C.c_void_p(v), 128, 64, st, sh, C.byref(c), C.byref(b), 1, None)
     assert rc == _lib.PDH_EINVAL and "overlap" in _lib.last_error(), (rc, _lib.last_error())
+
+
+@pytest.mark.parametrize("width,heads,group", [(1 << 18, 64, 2), (1 << 18, 1, 4), (1 << 12, 64, 2)])
+def test_work_that_could_pass_a_64_bit_sum_is_refused(width, heads, group):
+    """The decode kernel sums up all sequences' work before it looks for its own. Starts that do not ascend can give every
+    sequence all rows, and the sum then passes 2^63: no share of it would be found."""
+    from pdum_dsl_amd import _lib
+
+    rows, seqs, page = (1 << 24) // group, 1 << 20, 4096
+    work = seqs * (rows * group // 16) * heads * (width * page // 32)  # of 2^20 sequences of all rows
+    assert work > 1 << 63
+    c, b = _structs(dict(heads=heads, sp=heads * page * 64, sh=page * 64, page_rows=page, v=FAR),
+                    dict(seqs=seqs, rows=rows - 1, width=width, ld_table=0))
+    hq, q = heads * group, C.c_void_p(2 * FAR)
+    rc = _lib.lib().pdh_paged_attention(q, q, None, hq, hq * 64, 64, hq * 64, 64, C.byref(c), C.byref(b), 1 << 40, 0, 1.0, 1, q,
+                                        1 << 40, None)
+    assert rc == _lib.PDH_EINVAL and "work" in _lib.last_error(), (rc, _lib.last_error())
