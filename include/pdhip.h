@@ -355,7 +355,7 @@ typedef struct pdh_paged_batch {
 /* Store k and v [rows][heads][features] (strides *_st of a row, *_sh of a
  * head, multiples of 8 elements, 16-byte aligned) at their tokens' places, and
  * write q [rows][heads_q][features] to q_out (which may be q, with its strides,
- * and overlaps no input otherwise; both NULL with heads_q = 0). Where rotary (fp32 [positions][rotated], rows ld_rotary apart;
+ * and overlaps no input nor the cache otherwise; both NULL with heads_q = 0). Where rotary (fp32 [positions][rotated], rows ld_rotary apart;
  * cosines, then sines) is given, k and q are turned by their positions first:
  * for i < rotated / 2 with (a, b) = features (i, i + rotated / 2), or (2 i, 2 i
  * + 1) if interleaved, (a cos - b sin, b cos + a sin), in fp32, every product
@@ -377,8 +377,8 @@ int pdh_paged_append(const void* k, const void* v, const void* q, void* q_out, i
                      void* stream);
 
 /* The values that the cache holds of the batch's tokens, in dtype, to k_out
- * and v_out [rows][heads][features]; tokens without a place are zero, rows of
- * no sequence too where zero_rest != 0. No counterpart in the reference. */
+ * and v_out [rows][heads][features], in memory of their own; tokens without a
+ * place are zero, rows of no sequence too where zero_rest != 0. No counterpart in the reference. */
 int pdh_paged_rows(void* k_out, void* v_out, int64_t ko_st, int64_t ko_sh, int64_t vo_st, int64_t vo_sh,
                    const pdh_paged_cache* cache, const pdh_paged_batch* batch, int zero_rest, void* stream);
 
@@ -393,7 +393,7 @@ int pdh_paged_rows(void* k_out, void* v_out, int64_t ko_st, int64_t ko_sh, int64
  * are lost). Tokens that a row does not see count for nothing in it whatever
  * the pools hold. A row that sees nothing, or scores of -inf alone: o = 0, lse
  * = -inf; rows of no sequence likewise where zero_rest != 0, else they are not
- * written. o may be q, with q's strides, and does not overlap it otherwise.
+ * written. o may be q, with q's strides, and overlaps neither it nor the cache.
  * ws, 16-byte aligned, holds pdh_paged_attention_workspace bytes for the same
  * sizes (partial states of rows whose keys several workgroups share). seqs x
  * rows x heads_q x width x page_rows is under 2^71 where rows x heads_q / heads

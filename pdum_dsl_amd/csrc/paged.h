@@ -143,6 +143,20 @@ inline bool pools_apart(const pdh_paged_cache& c) {
          apart(c.k_scale, c.v_scale, c.features / 32, c.ssp, c.ssh, c.ssr);
 }
 
+// Whether an output shares no byte with the cache's pools and scales, which other workgroups read.
+inline bool clear_of_cache(const Spans& out, const pdh_paged_cache& c) {
+  auto clear = [&](const void* p, int64_t row, int64_t page, int64_t head, int64_t in_page) {
+    return out.apart_from(Spans(p, row, {{c.pages, page}, {c.heads, head}, {c.page_rows, in_page}}));
+  };
+  const int64_t es = c.bits == 16 ? 2 : 1, row = c.features * c.bits / 8;
+  for (const void* p : {c.k, c.v})
+    if (!clear(p, row, c.sp * es, c.sh * es, c.sr * es)) return false;
+  if (c.bits == 4)
+    for (const void* p : {c.k_scale, c.v_scale})
+      if (!clear(p, c.features / 32, c.ssp, c.ssh, c.ssr)) return false;
+  return true;
+}
+
 // A [rows][heads][features] tensor of 16-bit elements.
 struct Tokens {
   const void* p;

@@ -261,6 +261,7 @@ extern "C" int pdh_paged_append(const void* k, const void* v, const void* q, voi
                     o.apart_from(Tokens{k, n, cache->heads, d, k_st, k_sh}.spans()) &&
                     o.apart_from(Tokens{v, n, cache->heads, d, v_st, v_sh}.spans()),
                 PDH_EINVAL, "pdh_paged_append: q_out overlaps k, v or q (it may be q, with q's strides)");
+    PDH_REQUIRE(clear_of_cache(o, *cache), PDH_EINVAL, "pdh_paged_append: q_out overlaps the cache");
   }
   PDH_REQUIRE(pools_apart(*cache), PDH_EINVAL,
               "pdh_paged_append: rows of the cache's pools or scales overlap, or keys and values do");
@@ -297,6 +298,8 @@ extern "C" int pdh_paged_rows(void* k_out, void* v_out, int64_t ko_st, int64_t k
   const Spans ko = Tokens{k_out, batch->rows, cache->heads, cache->features, ko_st, ko_sh}.spans();
   const Spans vo = Tokens{v_out, batch->rows, cache->heads, cache->features, vo_st, vo_sh}.spans();
   PDH_REQUIRE(ko.apart() && vo.apart() && ko.apart_from(vo), PDH_EINVAL, "pdh_paged_rows: rows of the outputs overlap");
+  PDH_REQUIRE(clear_of_cache(ko, *cache) && clear_of_cache(vo, *cache), PDH_EINVAL,
+              "pdh_paged_rows: the outputs overlap the cache");
   const RowsArgs a{static_cast<uint16_t*>(k_out), static_cast<uint16_t*>(v_out), ko_st, ko_sh, vo_st, vo_sh, *cache,
                    *batch, shift, zero_rest != 0};
   const int64_t items = 2 * cache->heads * (cache->features / 8);

@@ -1405,12 +1405,14 @@ extern "C" int pdh_paged_attention(const void* q, void* o, float* lse, int64_t h
   const int64_t pool = ((cache->pages - 1) * cache->sp + cache->page_rows * cache->sr) * (cache->bits == 16 ? 2 : 1);
   const int64_t scales = cache->bits == 4 ? (cache->pages - 1) * cache->ssp + cache->page_rows * cache->ssr : 0;
   const bool far = pool >= 0x7fff0000 || scales >= 0x7fff0000;
+  const bool clear = clear_of_cache(out.spans(), *cache);
   if (few_rows(*batch, a.group)) {
     // The kernel sums up the work of all sequences, which starts that do not ascend may give all rows each, in 64 bits.
     const double most = static_cast<double>(batch->seqs) * static_cast<double>((batch->rows * a.group / 16 + 1) * cache->heads) *
                         static_cast<double>(a.reach / 32 + 1 + DecCfg<64, 16>::ITEM);
     PDH_REQUIRE(most < 4.6e18, PDH_EINVAL,
                 "pdh_paged_attention: too many sequences, rows and tokens of the table: %g blocks of work, 2^62 at most", most);
+    PDH_REQUIRE(clear, PDH_EINVAL, "pdh_paged_attention: o overlaps the cache");
     const unsigned n = static_cast<unsigned>(decode_grid(*cache));
     DecMeta* meta = static_cast<DecMeta*>(ws);
     float* states = reinterpret_cast<float*>(meta + n);
@@ -1435,6 +1437,7 @@ extern "C" int pdh_paged_attention(const void* q, void* o, float* lse, int64_t h
   const int64_t blocks = int64_t{8} * mp.units * mp.unit_slots * nsplit;
   PDH_REQUIRE(blocks < (1 << 24), PDH_EINVAL, "pdh_paged_attention: too many rows and heads: %lld workgroups, at most 2^24 - 1",
               (long long)blocks);  // of 256 threads: a launch counts threads in 32 bits
+  PDH_REQUIRE(clear, PDH_EINVAL, "pdh_paged_attention: o overlaps the cache");
   const Parts parts{nsplit, batch->rows * heads_q, static_cast<float*>(ws)};
   by_kind(*cache, [&](auto t, auto d, auto bits) {
     using T = decltype(t);

@@ -4,6 +4,7 @@
 #include <algorithm>
 #include <cstdint>
 #include <initializer_list>
+#include <utility>
 
 namespace pdh {
 
@@ -23,10 +24,11 @@ struct Spans {
     std::sort(axis, axis + axes, [](const Axis& a, const Axis& b) { return a.step < b.step; });
   }
 
-  // Bytes from the first row's start to the last one's end, of the first `count` axes.
-  __int128 extent(int count) const {
+  // Bytes from the first row's start to the last one's end, of some of the axes (bits of `some`).
+  __int128 extent(unsigned some) const {
     __int128 e = width;
-    for (int i = 0; i < count; ++i) e += static_cast<__int128>(axis[i].n - 1) * axis[i].step;
+    for (int i = 0; i < axes; ++i)
+      if (some >> i & 1) e += static_cast<__int128>(axis[i].n - 1) * axis[i].step;
     return e;
   }
 
@@ -34,26 +36,33 @@ struct Spans {
   // without lying inside one another are refused with the overlapping ones.)
   bool apart() const {
     for (int i = 0; i < axes; ++i)
-      if (axis[i].step < extent(i)) return false;
+      if (axis[i].step < extent((1u << i) - 1)) return false;
     return true;
   }
 
-  // No row of the first `count` axes shares a byte with one of b's first `bcount`, whose first lies `between` bytes behind.
-  // What both step over by the longest step, S, is taken off: rests that span no more than S can meet at two distances
-  // alone, their own modulo S and S less. (Arrays that this does not tell apart count as overlapping.)
-  bool apart_from(int count, const Spans& b, int bcount, __int128 between) const {
-    const __int128 ea = extent(count), eb = b.extent(bcount);
-    if (between >= ea || -between >= eb) return true;
-    const int64_t sa = count > 0 ? axis[count - 1].step : 0, sb = bcount > 0 ? b.axis[bcount - 1].step : 0;
-    const int64_t step = sa > sb ? sa : sb;
-    if (step == 0) return false;
-    const int ca = sa == step ? count - 1 : count, cb = sb == step ? bcount - 1 : bcount;
-    if (extent(ca) > step || b.extent(cb) > step) return false;
-    const __int128 rest = (between % step + step) % step;
-    return apart_from(ca, b, cb, rest) && apart_from(ca, b, cb, rest - step);
+  // No row of some of the axes shares a byte with one of b's, whose first lies `between` bytes behind. Any step S of theirs
+  // that tells it will do: without the axes that step by multiples of S, blocks that span no more than S can meet at two
+  // distances alone, their own modulo S and S less. (Arrays that no step tells apart count as overlapping.)
+  bool apart_from(unsigned some, const Spans& b, unsigned of_b, __int128 between) const {
+    if (between >= extent(some) || -between >= b.extent(of_b)) return true;
+    auto rest = [](const Spans& s, unsigned m, int64_t step) {
+      for (int i = 0; i < s.axes; ++i)
+        if (s.axis[i].step % step == 0) m &= ~(1u << i);
+      return m;
+    };
+    for (const auto& [s, m] : {std::pair{this, some}, std::pair{&b, of_b}})
+      for (int i = s->axes - 1; i >= 0; --i) {
+        const int64_t step = s->axis[i].step;
+        if (!(m >> i & 1) || step == 0) continue;
+        const unsigned ra = rest(*this, some, step), rb = rest(b, of_b, step);
+        if (extent(ra) > step || b.extent(rb) > step) continue;
+        const __int128 at0 = (between % step + step) % step;
+        if (apart_from(ra, b, rb, at0) && apart_from(ra, b, rb, at0 - step)) return true;
+      }
+    return false;
   }
   bool apart_from(const Spans& b) const {
-    return apart_from(axes, b, b.axes, static_cast<__int128>(b.at) - static_cast<__int128>(at));
+    return apart_from((1u << axes) - 1, b, (1u << b.axes) - 1, static_cast<__int128>(b.at) - static_cast<__int128>(at));
   }
 };
 

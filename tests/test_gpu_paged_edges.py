@@ -298,3 +298,29 @@ def test_f16_weights_far_under_the_largest_still_count(K, bits, gap, n, new, sin
         bound = bound + 2.0**-11 * (want + bound) + 2.0**-25
         assert (np.abs(o[r] - want) <= bound).all(), (r, np.abs(o[r] - want).max(), want.max())
         assert np.abs(lse[r] - (gap + np.log(den))).max() <= 2.0**-20 + gap * 2.0**-21 + len(v) * 2.0**-23
+
+
+def test_results_between_the_pools_rows(K):
+    """One tensor that holds the cache's rows and, beside them, room for results: taken, where no byte is shared."""
+    from pdum_dsl_amd import _lib
+
+    rng = np.random.default_rng(47)
+    pr, d, hq, hkv, pages = 16, 64, 4, 2, 8
+    table, starts, lens, rows, _ = batch(rng, [40, 33], [9, 1], pr, spare=pages - 6)
+    x = torch.as_tensor(rng.standard_normal((rows, hq + 2 * hkv, d))).bfloat16().cuda()
+    t = _ints(table, starts, lens)
+    own = K.paged_cache(pages, hkv, pr, d)
+    want = K.paged_append(x[:, hq : hq + hkv], x[:, hq + hkv :], own, *t, q=x[:, :hq])
+    o, lse = K.paged_attention(want, own, *t)
+    wide = torch.zeros((pages, hkv, pr, 3 * d), dtype=torch.bfloat16, device="cuda")
+    cache = K.PagedCache(wide[..., :d], wide[..., d : 2 * d])
+    free = wide.view(pages * hkv * pr // hq, hq, 3 * d)[:rows, :, 2 * d :]
+    got = K.paged_append(x[:, hq : hq + hkv], x[:, hq + hkv :], cache, *t, q=x[:, :hq], out=free)
+    assert torch.equal(got, want) and torch.equal(cache.k, own.k) and torch.equal(cache.v, own.v)
+    o2, lse2 = K.paged_attention(want, cache, *t, out=free)
+    assert torch.equal(o2, o) and torch.equal(lse2, lse)
+    for out in (own.k.view(-1, hq, d)[:rows], own.v.view(-1, hq, d)[-rows:]):
+        with pytest.raises(_lib.PdhError, match="overlap"):
+            K.paged_attention(want, own, *t, out=out)
+        with pytest.raises(_lib.PdhError, match="overlap"):
+            K.paged_append(x[:, :hkv], x[:, :hkv], own, *t, q=want, out=out)

@@ -184,6 +184,28 @@ def test_read_back_rows_that_overlap_are_refused(v, st, sh):
     assert rc == _lib.PDH_EINVAL and "overlap" in _lib.last_error(), (rc, _lib.last_error())
 
 
+@pytest.mark.parametrize("bits,at", [(16, FAR), (16, 2 * FAR), (16, FAR + 6144), (16, 2 * FAR - 1024), (4, FAR), (4, 2 * FAR + 2048),
+                                     (4, 3 * FAR), (4, 4 * FAR + 64)])
+def test_results_in_the_cache_are_refused(bits, at):
+    from pdum_dsl_amd import _lib
+
+    lib, far = _lib.lib(), C.c_void_p(32 * FAR)
+    kind = dict() if bits == 16 else dict(bits=4, sp=1024, sh=512, sr=32, ssp=64, ssh=32, ssr=2, k_scale=3 * FAR, v_scale=4 * FAR)
+    c, b = _structs(dict(k=FAR, v=2 * FAR, **kind))
+    out, more, other = C.c_void_p(at), C.c_void_p(33 * FAR), C.c_void_p(34 * FAR)
+    for call in (
+        lambda: lib.pdh_paged_append(more, more, far, out, 4, 256, 64, 256, 64, 256, 64, 256, 64, C.byref(c), C.byref(b), None, 0, 0,
+                                     0, 0, 1, None, None),
+        lambda: lib.pdh_paged_rows(out, far, 128, 64, 128, 64, C.byref(c), C.byref(b), 1, None),
+        lambda: lib.pdh_paged_rows(far, out, 128, 64, 128, 64, C.byref(c), C.byref(b), 1, None),
+        lambda: lib.pdh_paged_attention(far, out, None, 4, 256, 64, 256, 64, C.byref(c), C.byref(b), 5, 0, 1.0, 1, other, 1 << 40,
+                                        None),
+        lambda: lib.pdh_paged_attention(far, out, None, 32, 32 * 64, 64, 32 * 64, 64, C.byref(c), C.byref(b), 5, 0, 1.0, 1, other,
+                                        1 << 40, None),
+    ):
+        assert call() == _lib.PDH_EINVAL and "overlap" in _lib.last_error(), _lib.last_error()
+
+
 @pytest.mark.parametrize("width,heads,group", [(1 << 18, 64, 2), (1 << 18, 1, 4), (1 << 12, 64, 2)])
 def test_work_that_could_pass_a_64_bit_sum_is_refused(width, heads, group):
     """The decode kernel sums up all sequences' work before it looks for its own. Starts that do not ascend can give every
