@@ -222,10 +222,13 @@ __global__ __launch_bounds__(256) void paged_rows(RowsArgs a) {
   *reinterpret_cast<u32x4*>(out + f0) = x;
 }
 
-// f(chunks a thread): four where they fill the chip all the same, one where a call is short.
+// f(chunks a thread): four where they fill the chip all the same, one where a call is short, or a row no more chunks than a
+// workgroup has threads, which then take none but their first: 16/4 heads of 64, 192 chunks, us with one / four: 2000 rows
+// 6.0 / 6.5, 8192 16.2 / 17.5, 16384 28.1 / 31.0 (4 bits 29.7 / 33.4); 12/12 heads of 64, 288 chunks: 1000 rows 5.5 / 4.9, 8192
+// 26.6 / 19.4, 16384 48.5 / 34.0 (51.4 / 38.4).
 template <typename F>
 void by_chunks(int64_t rows, int64_t items, F f) {
-  if (rows * items > kManyItems)
+  if (items > 256 && rows * items > kManyItems)
     f(std::integral_constant<int, 4>{});
   else
     f(std::integral_constant<int, 1>{});
