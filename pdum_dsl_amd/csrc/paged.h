@@ -37,7 +37,8 @@ __device__ __forceinline__ Seq seq_at(const pdh_paged_batch& b, int i) {
 }
 
 // The sequence that owns a row: the number of sequences that end at or before it (seqs: none owns it). One wave, every
-// lane the same row; 64 sequences a load.
+// lane the same row; 64 sequences a load. Every wave of a call reads them all: an append of single tokens, 4/2 heads of 64, takes
+// 3.1 / 5.1 / 32 / 419 us for 64 / 700 / 4096 / 16384 sequences.
 __device__ __forceinline__ int seq_of_row(const pdh_paged_batch& b, int row) {
   const int lane = threadIdx.x & 63;
   int n = 0;

@@ -5,9 +5,12 @@
 //
 // Two kernels, by the mean number of rows of a sequence times the group of query heads on a key/value head: to 16 of them
 // the decode kernel (bytes bound it), above the prompt kernel (matrix products do). 64 sequences of 8192 tokens, 32/8 heads
-// of 128, us by the one / the other: 4 rows each 367 / 403 (4 bits 128 / 222), 5 rows, two blocks, 711 / 421 (239 / 233). Both
-// take any batch; single tokens in the prompt kernel, which a prompt among them brings there, cost what they read in 16 bits
-// (64 of 8192 tokens and a prompt of 2048: 421 together, 361 + 64 apart), more in 4 (282, 105 + 69).
+// of 128, us by the one / the other: 4 rows each 367 / 403 (4 bits 128 / 222), 5 rows, two blocks, 711 / 421 (239 / 233). The
+// switch lies where 16 bits have it; 4 bits, whose bytes take 107 us, jump there (8 rows 226, 16 275). Both take any batch, the
+// whole of it by its mean. Single tokens that a prompt brings to the prompt kernel cost what they read in 16 bits (64 of 8192
+// tokens and a prompt of 2048: 421 together, 361 + 64 apart), more in 4 (282, 105 + 69); a piece that single tokens bring to
+// the decode kernel reads its cache once for 16 of its rows times the group: 255 of 1000 tokens and 500 rows over 32768, 2403
+// together, 189 + 282 apart (4 bits 807, 59 + 286).
 #include "attn_common.h"
 #include "paged.h"
 
@@ -19,8 +22,10 @@ namespace {
 
 constexpr float kInf = __builtin_inff();
 
-// Softmax weights are factors of a 16-bit matrix product, rounded to the type (half a step of each; their sum is of the fp32
-// ones). f16 ends at 2^-24: there they are taken 2^kLift larger, o and the sum with them, so that the largest is 2^7 to 2^15
+// Softmax weights are factors of a 16-bit matrix product, which has no wider ones, rounded to the type (half a step of each;
+// their sum is of the fp32 ones). A second product by what the rounding leaves would bring o to 64 bits' own rounding: half
+// as many matrix instructions again in prompts, which they bound; in decode 4% for four drafted tokens of 4 bits and 7% for
+// heads of 64, and a visible infinity times a rest of 0 or less is not its sum. f16 ends at 2^-24: there they are taken 2^kLift larger, o and the sum with them, so that the largest is 2^7 to 2^15
 // and what is lost lies under 2^-32 of it: 2^20 keys of that come to 2^-12. States are (m, l, o) with m - kLift for m.
 template <typename T>
 constexpr float kLift = std::is_same_v<T, _Float16> ? 7.0f : 0.0f;
@@ -761,9 +766,11 @@ __global__ __launch_bounds__(512) void paged_decode_merge(PagedAttn a, const Dec
 // tiles into parts that paged_prompt_merge joins.
 //
 // The matrix pipe and the softmax's VALU share the clock that the part's power leaves: 2 x 4096 tokens, 32/8 heads of 128,
-// 266-279 us (990 to 1030 TFLOP/s; a library product of 8192^3 has 1200), matrix pipe 48% busy, VALU 50%, 2.0 GHz. 8192 under
-// a window of 1024: 151-160 us (860), of 35 tiles a block one in ten is cut or outside. 4 bits, 4 x 500 ragged rows over 7001:
-// 148 us and 12 of joining (750), 33% busy: a tile's codes are widened between the products of two.
+// 257-270 us on several cards (1020 to 1070 TFLOP/s; a library product of 8192^3 has 1200), 281 under a profiler, matrix pipe 48%
+// busy, VALU 50%, 2.0 GHz. 8192 under a window of 1024: 148-158 us (820-870); of 35 tiles a block one in ten is cut or outside,
+// and 4096 / 6144 / 8192 / 9216 / 12288 rows take 87 / 118 / 153 / 168 / 218 us: 16 us for 1000 more, 1050 TFLOP/s, and 30 us at
+// the ends of the launch, where the chip fills and drains. 4 bits, 4 x 500 ragged rows over 7001: 148 us and 12 of joining (750), 33% busy: a tile's codes are widened between
+// the products of two.
 
 template <int D, int BITS>
 struct ProCfg {
@@ -779,7 +786,8 @@ struct ProCfg {
   static constexpr int FB = D / 16;
   static constexpr int PF = 1;  // V operands in flight ahead of their product
   // K operands in flight: as many as the registers hold without spills (4 bits, D = 128: the codes take theirs). 2 x 4096
-  // tokens, 32/8 heads of 128: 256 us, with two and three 258; 4 bits 272, with one and three 290, two and three 295
+  // tokens, 32/8 heads of 128, us: one of V and two of K 256, two and three 258, no more than two cards differ; 4 bits, one
+  // and one 272, one and three 290, two and three 295
   static constexpr int KPF = BITS == 4 && D == 128 ? 1 : 2;
 };
 
@@ -853,7 +861,7 @@ struct Parts {
 // Which workgroup takes which head and slot. Workgroups go round the eight XCDs; XCD x takes units x `units` and onward, a
 // unit being every `shares`-th slot of a head (1 where the heads divide by eight), up to kHeadsRun of them at a time, the late
 // slots of all of those first. Against whole heads one after the other, us, bf16: 2 x 4096 tokens, 12 heads of 64, 130 -> 88;
-// 16 heads on one, 128 -> 104; 4 x 4096, 16 of 64, 192 -> 182; 2 x 4096, 32/8 of 128, 262 -> 261. One unit at a time: 107,
+// 16 heads on one, 128 -> 104; 4 x 4096, 16 of 64, 192 -> 182; 2 x 4096, 32/8 of 128, 262 and 261. One unit at a time: 107,
 // 104, 189, 266; eight: as three. Sequences in turn as well (two, four at a time): 80, 104, 174, 261, but 8 x 512 rows over
 // 7001 keys 439 -> 478 and 459, their keys no longer in L2.
 constexpr int kHeadsRun = 3;
@@ -1346,7 +1354,11 @@ int decode_grid(const pdh_paged_cache& c) {
 // of at least 1024 keys of what the table can hold (the lengths are not known here; a block of fewer keys makes fewer
 // parts). Measured, bf16, 32/8 heads of 128, us uncut / cut: 512 rows over 8192 keys 191 / 92, 128 over 8192 190 / 41, 4 x
 // 500 ragged over 7001 188 / 150 (4 bits 212 / 165), 8 x 64 over 8192 197 / 100. Shorter parts lost: a prompt of 1024
-// tokens in two 26% longer, of 2048 under a window of 1024 80%: those stay whole.
+// tokens in two 26% longer, of 2048 under a window of 1024 80%: those stay whole. At 128 over 8192 that is one workgroup a
+// compute unit, 2.8 times the floor. Blocks are counted by rows alone; of sequences shorter than a block there are more, cut
+// finer than the target. Counted by sequences too, us: 64 x 5 over 8192 418 -> 384 (4 bits 234 -> 245), 256 x 1 over 4096, 160/8
+// heads, 819 -> 769, 24 x 8 over 8192 167 -> 160, but 64 x 1 ragged over 16000, 160/8, 636 -> 670, 24 x 20 over 4000, 12 heads of
+// 64, 55 -> 62, 40 x 17 ragged over 9000, 16/4 of 64, 68 -> 77: neither is better throughout.
 int prompt_splits(const pdh_paged_cache& c, const pdh_paged_batch& b, int64_t group, int64_t window, int64_t sinks) {
   const int64_t blocks = (b.rows * group / 128 + 1) * c.heads;
   int64_t keys = b.width * c.page_rows;

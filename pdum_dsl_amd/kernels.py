@@ -962,8 +962,8 @@ def paged_append(
     page table, or a page outside the pool) is dropped, its row of the result
     is zero, and it counts in ``bad`` (an int32 device scalar) when given.
     Rows of no sequence are stored nowhere; their rows of the result are zero,
-    or stay as they are in ``out`` (which may be q itself, and does not overlap
-    q, k or v otherwise). Two tokens with one
+    or stay as they are in ``out`` (which may be q itself, and overlaps neither
+    q, k or v otherwise nor the cache). Two tokens with one
     place leave either of them, or parts of both, there; a cache whose rows lie
     in one another (an expanded pool, one tensor for keys and values) is refused."""
     cc, _, dtype, heads, d, _ = cache._call
@@ -1054,13 +1054,15 @@ def paged_attention(
     only the last ``window`` of those (its own counted) and the first
     ``sinks`` of the sequence. One token a sequence, a whole prompt, or both
     in one call. Returns (o, lse): q's shape and type; fp32 [rows, query
-    heads], None without ``want_lse``.
+    heads], None without ``want_lse``. A batch goes to one kernel, by its mean
+    rows a sequence: where the lengths are known, single tokens and a long
+    piece are faster as two calls (up to five times over a cache of 32768 tokens).
 
     What a row does not see has no part in it, whatever the cache holds there;
     tokens on pages outside the pool or past the table are not seen. A row
     that sees nothing (or only scores of -inf) has o = 0 and lse = -inf. Rows
-    of no sequence likewise; ``out`` (q's shape and type, or q itself) they
-    leave as it is.
+    of no sequence likewise; ``out`` (q's shape and type, or q itself; it
+    overlaps neither q otherwise nor the cache) they leave as it is.
     The 4 bits are exact in bf16; in f16 they round under scales of 2^-23,
     and pass 65504 in caches that :func:`paged_append` did not fill."""
     cc, _, dtype, heads, d, _ = cache._call
