@@ -355,8 +355,9 @@ typedef struct pdh_paged_batch {
 /* Store k and v [rows][heads][features] (strides *_st of a row, *_sh of a
  * head, multiples of 8 elements, 16-byte aligned) at their tokens' places, and
  * write q [rows][heads_q][features] to q_out (which may be q, with its strides,
- * and overlaps no input nor the cache otherwise; both NULL with heads_q = 0). Where rotary (fp32 [positions][rotated], rows ld_rotary apart;
- * cosines, then sines) is given, k and q are turned by their positions first:
+ * and overlaps no input nor the cache otherwise; both NULL with heads_q = 0).
+ * Where rotary (fp32 [positions][rotated], rows ld_rotary apart; cosines, then
+ * sines) is given, k and q are turned by their positions first:
  * for i < rotated / 2 with (a, b) = features (i, i + rotated / 2), or (2 i, 2 i
  * + 1) if interleaved, (a cos - b sin, b cos + a sin), in fp32, every product
  * and sum rounded; rotated a multiple of 16. One rounding to dtype; or to 4
@@ -378,7 +379,8 @@ int pdh_paged_append(const void* k, const void* v, const void* q, void* q_out, i
 
 /* The values that the cache holds of the batch's tokens, in dtype, to k_out
  * and v_out [rows][heads][features], in memory of their own; tokens without a
- * place are zero, rows of no sequence too where zero_rest != 0. No counterpart in the reference. */
+ * place are zero, rows of no sequence too where zero_rest != 0. No counterpart
+ * in the reference. */
 int pdh_paged_rows(void* k_out, void* v_out, int64_t ko_st, int64_t ko_sh, int64_t vo_st, int64_t vo_sh,
                    const pdh_paged_cache* cache, const pdh_paged_batch* batch, int zero_rest, void* stream);
 

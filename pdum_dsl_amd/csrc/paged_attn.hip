@@ -25,8 +25,9 @@ constexpr float kInf = __builtin_inff();
 // Softmax weights are factors of a 16-bit matrix product, which has no wider ones, rounded to the type (half a step of each;
 // their sum is of the fp32 ones). A second product by what the rounding leaves would bring o to 64 bits' own rounding: half
 // as many matrix instructions again in prompts, which they bound; in decode 4% for four drafted tokens of 4 bits and 7% for
-// heads of 64, and a visible infinity times a rest of 0 or less is not its sum. f16 ends at 2^-24: there they are taken 2^kLift larger, o and the sum with them, so that the largest is 2^7 to 2^15
-// and what is lost lies under 2^-32 of it: 2^20 keys of that come to 2^-12. States are (m, l, o) with m - kLift for m.
+// heads of 64, and a visible infinity times a rest of 0 or less is not its sum. f16 ends at 2^-24: there weights are taken
+// 2^kLift larger, o and the sum with them, so that the largest is 2^7 to 2^15 and what is lost lies under 2^-32 of it: 2^20
+// keys of that come to 2^-12. States are (m, l, o) with m - kLift for m.
 template <typename T>
 constexpr float kLift = std::is_same_v<T, _Float16> ? 7.0f : 0.0f;
 
@@ -769,8 +770,8 @@ __global__ __launch_bounds__(512) void paged_decode_merge(PagedAttn a, const Dec
 // 257-270 us on several cards (1020 to 1070 TFLOP/s; a library product of 8192^3 has 1200), 281 under a profiler, matrix pipe 48%
 // busy, VALU 50%, 2.0 GHz. 8192 under a window of 1024: 148-158 us (820-870); of 35 tiles a block one in ten is cut or outside,
 // and 4096 / 6144 / 8192 / 9216 / 12288 rows take 87 / 118 / 153 / 168 / 218 us: 16 us for 1000 more, 1050 TFLOP/s, and 30 us at
-// the ends of the launch, where the chip fills and drains. 4 bits, 4 x 500 ragged rows over 7001: 148 us and 12 of joining (750), 33% busy: a tile's codes are widened between
-// the products of two.
+// the ends of the launch, where the chip fills and drains. 4 bits, 4 x 500 ragged rows over 7001: 148 us and 12 of joining
+// (750), 33% busy: a tile's codes are widened between the products of two.
 
 template <int D, int BITS>
 struct ProCfg {
@@ -785,7 +786,7 @@ struct ProCfg {
   static constexpr int KS = D / 32;
   static constexpr int FB = D / 16;
   static constexpr int PF = 1;  // V operands in flight ahead of their product
-  // K operands in flight: as many as the registers hold without spills (4 bits, D = 128: the codes take theirs). 2 x 4096
+  // K operands in flight: as many as the registers hold (4 bits, D = 128: the codes take theirs, and ten spill). 2 x 4096
   // tokens, 32/8 heads of 128, us: one of V and two of K 256, two and three 258, no more than two cards differ; 4 bits, one
   // and one 272, one and three 290, two and three 295
   static constexpr int KPF = BITS == 4 && D == 128 ? 1 : 2;
